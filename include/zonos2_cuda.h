@@ -153,6 +153,83 @@ int zonos2cu_head_softcap(const void *W_dev, zonos2cu_dtype dtype, int rows_per_
                           int vocab, int dim, const void *hidden_dev, int batch, float softcap,
                           float *logits_dev, void *stream);
 
+/* ---- the tail of a decoder block (device pointers) ------------------------- */
+
+/* The norm of a block's output, its gate, the scaled residual sum, and the
+ * RMSNorm that follows (the next block's, or the output norm ahead of the head),
+ * in one pass over each row:
+ *     y = block * post_weight / rms(block)    (post_eps >= 0; y = block below 0)
+ *     r = resid + scale * g * y
+ *     n = r * norm_weight / rms(r),           rms(x) = sqrt(mean(x^2) + eps)
+ * in f32, r and n rounded once each to `dtype` (n from the unrounded r).
+ *   resid_dev, block_dev  [rows] rows of dim elements of `dtype`, their starts
+ *                resid_stride and block_stride elements apart (>= dim).
+ *   gate_dev     NULL (g = 1), or the value of row r, column d at element
+ *                r * gate_row_stride + d * gate_col_stride: (stride, 1) one per
+ *                element, (stride, 0) one per row, (0, 1) one per column.  With
+ *                gate_sigmoid g = 1 / (1 + exp(-gate)), else the value itself.
+ *   post_weight_dev, norm_weight_dev  [dim] f32, or NULL for 1.
+ *   resid_out_dev (r), normed_out_dev (n)  rows out_stride elements apart; one of
+ *                them may be NULL.  Either may be resid_dev or block_dev itself, at
+ *                the same row stride (out_stride); no other overlap is allowed.
+ * Replaces, for a block with these parts, the residual sum and the
+ * rms_norm_per_token behind it (src/zonos2_model.cpp:19-35, :684-685). */
+int zonos2cu_block_norm(const void *resid_dev, const void *block_dev, zonos2cu_dtype dtype,
+                        int rows, int dim, long long resid_stride, long long block_stride,
+                        const float *post_weight_dev, float post_eps, const void *gate_dev,
+                        long long gate_row_stride, int gate_col_stride, int gate_sigmoid,
+                        float scale, const float *norm_weight_dev, float norm_eps,
+                        void *resid_out_dev, void *normed_out_dev, long long out_stride,
+                        void *stream);
+
+/* ---- drafted frames against the target (device pointers) -------------------- */
+
+/* No counterpart in the reference.  A stream has up to n_draft drafted frames of
+ * n_cb codes, and the target's logits at each of their positions and at the one
+ * after them: row (s, d, c) is logits_dev[((s*(n_draft+1) + d)*n_cb + c) *
+ * row_stride .. + vocab), the head's output for n_streams * (n_draft + 1) hidden
+ * rows.  Per row, p is the distribution zonos2cu_sample_rows draws from (penalty,
+ * masks, temperature, top-k, top-p, min-p, in that order; tokens ordered by logit
+ * descending, then token ascending) and q the draft's.  With the row's uniforms
+ * u0, u1 in [0, 1):
+ *   - the drafted code t stands iff u0 * q(t) < p(t) (never outside [0, vocab));
+ *   - a refused code is drawn from max(p - q, 0), or from p where that is zero
+ *     everywhere: the first token in the order above that has weight and whose
+ *     cumulative weight reaches u1 of the total;
+ *   - a stream's first frame with a refused code is its last emitted one; if all
+ *     its drafts stand, the frame after them is drawn from p and is the last.
+ * The emitted frames then have the distribution the sampler would have given them
+ * one at a time.  Decisions are made in f64.
+ *   drafts_dev   [n_streams][n_draft][n_cb].
+ *   draft_probs_dev  q, [n_streams][n_draft][n_cb][vocab] f32, or NULL: the drafts
+ *                are certain (q(t) = 1; looked up rather than drawn).  A NaN in q
+ *                refuses the code it belongs to and gives it no weight.
+ *   n_drafts_dev [n_streams] how many of the n_draft frames each stream has
+ *                (clamped to [0, n_draft]), or NULL: all of them.
+ *   uniforms_dev [n_streams][n_draft + 1][n_cb][2]: u0, u1 (u0 of the position
+ *                after the drafts is not used).
+ *   hist_dev     [n_streams][n_cb][hist_len] ring (may be NULL when hist_len == 0)
+ *                and hist_pos_dev [n_streams], each stream's next write position
+ *                (taken mod hist_len).  Position d's penalty sees the ring with
+ *                the d frames drafted before it appended; the emitted frames are
+ *                appended and hist_pos_dev advanced by their number, mod hist_len.
+ *   allow_dev, delay_step  as in zonos2cu_sample_rows; position d counts as
+ *                delay step delay_step + d.
+ *   codes_dev    [n_streams][n_draft + 1][n_cb]: the emitted frames, -1 after them.
+ *   n_accepted_dev  [n_streams]: drafted frames that stand whole; n_accepted + 1
+ *                frames are emitted.
+ *   flags_dev    as codes_dev or NULL: ZONOS2CU_FLAG_* of each emitted code, 0 after.
+ * No two of the buffers may overlap.
+ * Limits: 1 <= vocab <= 1024, 1 <= n_cb <= 16, n_draft <= ZONOS2CU_MAX_DRAFTS. */
+#define ZONOS2CU_MAX_DRAFTS 4095
+int zonos2cu_verify_drafts(const float *logits_dev, int n_streams, int n_draft, int n_cb,
+                           int vocab, long long row_stride, const zonos2cu_sample_params *params,
+                           const int32_t *drafts_dev, const float *draft_probs_dev,
+                           const int32_t *n_drafts_dev, const float *uniforms_dev,
+                           int32_t *hist_dev, int hist_len, int32_t *hist_pos_dev,
+                           const uint32_t *allow_dev, int delay_step, int32_t *codes_dev,
+                           int32_t *n_accepted_dev, int32_t *flags_dev, void *stream);
+
 /* ---- context: device-resident state for a batch of decode streams --------- */
 
 typedef struct zonos2cu_ctx zonos2cu_ctx;

@@ -10,10 +10,12 @@
 #include <mutex>
 #include <new>
 
+#include "block_norm.cuh"
 #include "common.cuh"
 #include "head.cuh"
 #include "generate.cuh"
 #include "sampler.cuh"
+#include "verify.cuh"
 #include "zonos2_cuda.h"
 
 namespace {
@@ -363,6 +365,109 @@ int zonos2cu_head_softcap(const void *W_dev, zonos2cu_dtype dtype, int rows_per_
 {
     return launch_head(W_dev, dtype, rows_per_cb, n_cb, vocab, dim, hidden_dev, batch, softcap,
                        logits_dev, stream, false, 1.0f);
+}
+
+int zonos2cu_block_norm(const void *resid_dev, const void *block_dev, zonos2cu_dtype dtype,
+                        int rows, int dim, long long resid_stride, long long block_stride,
+                        const float *post_weight_dev, float post_eps, const void *gate_dev,
+                        long long gate_row_stride, int gate_col_stride, int gate_sigmoid,
+                        float scale, const float *norm_weight_dev, float norm_eps,
+                        void *resid_out_dev, void *normed_out_dev, long long out_stride,
+                        void *stream)
+{
+    if (dtype != ZONOS2CU_F32 && dtype != ZONOS2CU_BF16) return ZONOS2CU_EINVAL;
+    if (rows < 0 || dim < 1) return ZONOS2CU_EINVAL;
+    if (resid_stride < dim || block_stride < dim || out_stride < dim) return ZONOS2CU_EINVAL;
+    if (!isfinite(post_eps) || !isfinite(scale)) return ZONOS2CU_EINVAL;
+    if (normed_out_dev && (!(norm_eps >= 0.0f) || !isfinite(norm_eps))) return ZONOS2CU_EINVAL;
+    if (gate_dev) {
+        if (gate_col_stride != 0 && gate_col_stride != 1) return ZONOS2CU_EINVAL;
+        if (gate_row_stride < 0 ||
+            (gate_row_stride > 0 && gate_row_stride < (gate_col_stride ? dim : 1)))
+            return ZONOS2CU_EINVAL;
+    }
+    if (rows == 0) return ZONOS2CU_OK;
+    if (!resid_dev || !block_dev || (!resid_out_dev && !normed_out_dev)) return ZONOS2CU_EINVAL;
+    const uintptr_t es = dtype == ZONOS2CU_F32 ? 4 : 2;
+    if ((uintptr_t)resid_dev % es || (uintptr_t)block_dev % es || (uintptr_t)gate_dev % es ||
+        (uintptr_t)resid_out_dev % es || (uintptr_t)normed_out_dev % es ||
+        (uintptr_t)post_weight_dev % 4 || (uintptr_t)norm_weight_dev % 4)
+        return ZONOS2CU_EINVAL;
+    z2::BlockNormArgs a{};
+    a.resid = resid_dev;
+    a.block = block_dev;
+    a.resid_stride = resid_stride;
+    a.block_stride = block_stride;
+    a.rows = rows;
+    a.dim = dim;
+    a.post_norm = post_eps >= 0.0f;
+    a.post_weight = post_weight_dev;
+    a.post_eps = post_eps;
+    a.gate = gate_dev;
+    a.gate_row_stride = gate_row_stride;
+    a.gate_col_stride = gate_col_stride;
+    a.gate_sigmoid = gate_sigmoid;
+    a.scale = scale;
+    a.norm_weight = norm_weight_dev;
+    a.norm_eps = norm_eps;
+    a.resid_out = resid_out_dev;
+    a.normed_out = normed_out_dev;
+    a.out_stride = out_stride;
+    Z2_CK(z2::launch_block_norm(a, dtype == ZONOS2CU_BF16, (cudaStream_t)stream));
+    return ZONOS2CU_OK;
+}
+
+int zonos2cu_verify_drafts(const float *logits_dev, int n_streams, int n_draft, int n_cb,
+                           int vocab, long long row_stride, const zonos2cu_sample_params *params,
+                           const int32_t *drafts_dev, const float *draft_probs_dev,
+                           const int32_t *n_drafts_dev, const float *uniforms_dev,
+                           int32_t *hist_dev, int hist_len, int32_t *hist_pos_dev,
+                           const uint32_t *allow_dev, int delay_step, int32_t *codes_dev,
+                           int32_t *n_accepted_dev, int32_t *flags_dev, void *stream)
+{
+    if (n_streams < 0 || n_cb < 1 || n_cb > z2::kSamplerCbMax || vocab < 1) return ZONOS2CU_EINVAL;
+    if (n_draft < 0 || n_draft > ZONOS2CU_MAX_DRAFTS) return ZONOS2CU_EINVAL;
+    if (vocab > z2::kSamplerVocabMax) return ZONOS2CU_EUNSUPPORTED;
+    if (row_stride < vocab || hist_len < 0) return ZONOS2CU_EINVAL;
+    if (hist_len > 0 && (!hist_dev || !hist_pos_dev)) return ZONOS2CU_EINVAL;
+    const int rc = check_params(params, vocab);
+    if (rc) return rc;
+    if (n_streams == 0) return ZONOS2CU_OK;
+    if (!logits_dev || !uniforms_dev || !codes_dev || !n_accepted_dev ||
+        (n_draft > 0 && !drafts_dev))
+        return ZONOS2CU_EINVAL;
+    if ((uintptr_t)logits_dev % 4 || (uintptr_t)draft_probs_dev % 4 || (uintptr_t)uniforms_dev % 4)
+        return ZONOS2CU_EINVAL;
+    z2::VerifyArgs a{};
+    a.logits = logits_dev;
+    a.row_stride = row_stride;
+    a.n_streams = n_streams;
+    a.n_draft = n_draft;
+    a.n_cb = n_cb;
+    a.vocab = vocab;
+    a.temperature = params->temperature;
+    a.top_p = params->top_p;
+    a.min_p = params->min_p;
+    a.rho = params->repetition_penalty;
+    a.inv_rho = 1.0f / params->repetition_penalty;
+    a.inv_temp = 1.0 / (double)params->temperature;
+    a.top_k = params->top_k;
+    a.pad_id = params->pad_id;
+    a.drafts = drafts_dev;
+    a.probs = draft_probs_dev;
+    a.n_drafts = n_drafts_dev;
+    a.uniforms = uniforms_dev;
+    a.hist = hist_len > 0 ? hist_dev : nullptr;
+    a.hist_len = hist_len;
+    a.hist_pos = hist_pos_dev;
+    a.allow = allow_dev;
+    a.delay_step = delay_step;
+    a.codes = codes_dev;
+    a.n_accepted = n_accepted_dev;
+    a.flags = flags_dev;
+    a.vec_logits = (row_stride % 4 == 0) && (vocab % 4 == 0) && ((uintptr_t)logits_dev % 16 == 0);
+    Z2_CK(z2::launch_verify(a, (cudaStream_t)stream));
+    return ZONOS2CU_OK;
 }
 
 int zonos2cu_embed_frames(const float *codebook_tables_dev, const float *text_table_dev,

@@ -45,7 +45,7 @@ EXPORTS = (
     "zonos2cu_comm_unique_id", "zonos2cu_comm_create", "zonos2cu_comm_destroy",
     "zonos2cu_gather_codes", "zonos2cu_comm_create_timeout", "zonos2cu_comm_abort",
     "zonos2cu_ipc_alloc", "zonos2cu_ipc_free", "zonos2cu_ipc_open", "zonos2cu_ipc_close",
-    "zonos2cu_push_codes",
+    "zonos2cu_push_codes", "zonos2cu_block_norm", "zonos2cu_verify_drafts",
 )
 
 
@@ -138,6 +138,10 @@ def lib() -> C.CDLL:
         "zonos2cu_ipc_open": (i, [i, C.c_char_p, C.POINTER(vp)]),
         "zonos2cu_ipc_close": (i, [vp]),
         "zonos2cu_push_codes": (i, [vp, i, ll, vp, ll, vp]),
+        "zonos2cu_block_norm": (i, [vp, vp, i, i, i, ll, ll, vp, f, vp, ll, i, i, f, vp, f, vp, vp,
+                                    ll, vp]),
+        "zonos2cu_verify_drafts": (i, [vp, i, i, i, i, ll, C.POINTER(SampleParams), vp, vp, vp, vp,
+                                       vp, i, vp, vp, i, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -227,6 +231,98 @@ def head_softcap(W, dtype: int, rows_per_cb: int, n_cb: int, vocab: int, hidden,
     rc = lib().zonos2cu_head_softcap(_ptr(W), dtype, rows_per_cb, n_cb, vocab, D, _ptr(hidden), B,
                                      softcap, _ptr(out), _stream(stream))
     _check(rc, "zonos2cu_head_softcap")
+
+
+def _dtype(t) -> int:
+    """The library's type of a torch tensor's elements."""
+    import torch
+    if t.dtype == torch.bfloat16:
+        return BF16
+    if t.dtype == torch.float32:
+        return F32
+    raise TypeError(f"expected bfloat16 or float32, got {t.dtype}")
+
+
+def _launch(fn: str, on, stream, *args) -> None:
+    """Call entry point ``fn`` on the device of tensor ``on``; the stream (default: that
+    device's current one) is its last argument."""
+    import torch
+    dev = on.get_device()
+    if dev < 0:
+        raise TypeError(f"{fn}: CUDA tensors expected")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(fn, on, stream, *args)
+    rc = getattr(lib(), fn)(*args, _stream(stream))
+    if rc < 0:
+        raise Zonos2cuError(rc, fn)
+
+
+def _rows(t, what: str) -> int:
+    """The row stride of a 2-D tensor whose rows are contiguous."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: expected [rows, dim] with contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def block_norm(resid, block, resid_out, normed_out, *, post_weight=None, post_eps: float = 1e-5,
+               gate=None, gate_sigmoid: bool = False, scale: float = 1.0, norm_weight=None,
+               norm_eps: float = 1e-5, stream=None) -> None:
+    """The tail of a decoder block: r = resid + scale * g * norm(block), n = norm(r).
+
+    resid, block [rows, dim] bf16 or f32 (row strides allowed); resid_out (r) and normed_out
+    (n) likewise, one of them may be None, and may be resid or block itself; gate: None or a
+    2-D tensor that broadcasts to [rows, dim]; weights [dim] f32 or None; post_eps < 0 leaves
+    the block's output as it is."""
+    dt, (rows, dim) = _dtype(resid), resid.shape
+    outs = [t for t in (resid_out, normed_out) if t is not None]
+    for t in (block, *outs):
+        if t.shape != resid.shape or t.dtype != resid.dtype:
+            raise ValueError("block_norm: block and outputs must match resid")
+    strides = {_rows(t, "block_norm") for t in outs}
+    if len(strides) != 1:
+        raise ValueError("block_norm: the outputs need one row stride")
+    gate_row = gate_col = 0
+    if gate is not None:
+        if gate.dtype != resid.dtype or gate.dim() != 2 or any(
+                n not in (1, m) for n, m in zip(gate.shape, resid.shape)):
+            raise ValueError("block_norm: the gate must broadcast to [rows, dim]")
+        gate_row = 0 if gate.shape[0] == 1 else gate.stride(0)
+        gate_col = 0 if gate.shape[1] == 1 else gate.stride(1)
+    for w in (post_weight, norm_weight):
+        if w is not None and (w.shape != (dim,) or _dtype(w) != F32 or not w.is_contiguous()):
+            raise ValueError("block_norm: weights are [dim] f32")
+    _launch("zonos2cu_block_norm", resid, stream, resid.data_ptr(), block.data_ptr(), dt, rows, dim,
+            _rows(resid, "block_norm"), _rows(block, "block_norm"), _ptr(post_weight), post_eps,
+            _ptr(gate), gate_row, gate_col, int(gate_sigmoid), scale, _ptr(norm_weight), norm_eps,
+            _ptr(resid_out), _ptr(normed_out), strides.pop())
+
+
+def verify_drafts(logits, params: SampleParams, drafts, uniforms, codes, n_accepted, *,
+                  vocab=None, draft_probs=None, n_drafts=None, flags=None, hist=None,
+                  hist_pos=None, allow=None, delay_step=-1, stream=None) -> None:
+    """Drafted frames against the target's logits, from given random numbers.
+
+    logits f32 [S, D + 1, C, >= vocab]; drafts int32 [S, D, C]; uniforms f32 [S, D + 1, C, 2];
+    draft_probs f32 [S, D, C, vocab] or None (certain drafts); n_drafts int32 [S] or None;
+    codes and flags int32 [S, D + 1, C]; n_accepted int32 [S]; hist int32 [S, C, H] with
+    hist_pos int32 [S], both advanced; allow int32/uint32 [S, ceil(vocab/32)].  All contiguous."""
+    S, D1, Cb, stride = logits.shape
+    V = stride if vocab is None else vocab
+    H = 0 if hist is None else hist.shape[-1]
+    for t, n in ((logits, S * D1 * Cb * stride), (drafts, S * (D1 - 1) * Cb),
+                 (uniforms, 2 * S * D1 * Cb), (draft_probs, S * (D1 - 1) * Cb * V), (n_drafts, S),
+                 (codes, S * D1 * Cb), (flags, S * D1 * Cb), (n_accepted, S), (hist, S * Cb * H),
+                 (hist_pos, S), (allow, S * ((V + 31) // 32))):
+        if t is not None and (t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"verify_drafts: a contiguous tensor of {n} elements expected, got "
+                             f"{tuple(t.shape)}")
+        if t is not None and t.element_size() != 4:
+            raise TypeError("verify_drafts: f32 and int32 tensors expected")
+    _launch("zonos2cu_verify_drafts", logits, stream, logits.data_ptr(), S, D1 - 1, Cb, V, stride,
+            C.byref(params), _ptr(drafts), _ptr(draft_probs), _ptr(n_drafts), _ptr(uniforms),
+            _ptr(hist), H, _ptr(hist_pos), _ptr(allow), delay_step, _ptr(codes), _ptr(n_accepted),
+            _ptr(flags))
 
 
 def step_noalloc(W, dtype: int, rows_per_cb: int, n_cb: int, vocab: int, hidden, params,
