@@ -15,7 +15,8 @@
  *     host.
  *   - Device memory is allocated only by these calls:
  *       zonos2cu_ctx_create, zonos2cu_set_head, zonos2cu_set_allow,
- *       zonos2cu_set_out_norm, zonos2cu_set_embeddings, zonos2cu_gen_begin
+ *       zonos2cu_set_out_norm, zonos2cu_set_adapters,
+ *       zonos2cu_set_embeddings, zonos2cu_gen_begin
  *         (owned by the context, freed by zonos2cu_ctx_destroy);
  *       the first zonos2cu_ctx_sample_host / zonos2cu_ctx_step_host of a
  *         context, and a later one with larger inputs (host-path staging,
@@ -153,6 +154,32 @@ int zonos2cu_head_softcap(const void *W_dev, zonos2cu_dtype dtype, int rows_per_
                           int vocab, int dim, const void *hidden_dev, int batch, float softcap,
                           float *logits_dev, void *stream);
 
+/* ---- the output head beside low-rank adapters (device pointers) ------------- */
+
+/* zonos2cu_head_softcap with an adapter per hidden row (no counterpart in the
+ * reference): with a = adapter_dev[b],
+ *   logits[b][c][v] = softcap * tanh((W[n] . h + scale[a] * B[a][n] . (A[a] h)) / softcap)
+ * where n = c*rows_per_cb + v and h = hidden_dev[b]; rows whose a lies outside
+ * [0, n_adapters) have no adapter.  Rows may name their adapters in any order.
+ *   A_dev        [n_adapters][rank][dim], B_dev [n_adapters][n_cb*rows_per_cb][rank],
+ *                of `dtype` like W_dev and hidden_dev.
+ *   scale_dev    [n_adapters] f32 or NULL (1).
+ *   adapter_dev  [batch] i32.
+ *   work_dev     work_bytes of scratch, 16-byte aligned, at least
+ *                zonos2cu_head_adapters_work(dtype, batch, rank) (8 bytes per row and
+ *                rank always suffice).  Calls that may overlap need scratch of their own.
+ * A h is kept in f32 beside a bf16 head and in f64 beside an f32 one, whose result
+ * is rounded once.  Any dim, vocab and rank (<= ZONOS2CU_MAX_RANK); the bf16
+ * tensor-core kernel runs where dim % 8 == 0, rank % 8 == 0 and W, hidden, A and B
+ * are 16-byte aligned, a slower kernel elsewhere. */
+#define ZONOS2CU_MAX_RANK 256
+long long zonos2cu_head_adapters_work(zonos2cu_dtype dtype, int batch, int rank);
+int zonos2cu_head_adapters(const void *W_dev, zonos2cu_dtype dtype, int rows_per_cb, int n_cb,
+                           int vocab, int dim, const void *hidden_dev, int batch, float softcap,
+                           const void *A_dev, const void *B_dev, const float *scale_dev,
+                           int n_adapters, int rank, const int32_t *adapter_dev, void *work_dev,
+                           long long work_bytes, float *logits_dev, void *stream);
+
 /* ---- the tail of a decoder block (device pointers) ------------------------- */
 
 /* The norm of a block's output, its gate, the scaled residual sum, and the
@@ -284,6 +311,20 @@ int zonos2cu_set_out_norm(zonos2cu_ctx *ctx, int enable, const float *weight_hos
  * hidden states, row 2s the conditional and row 2s+1 the unconditional state
  * of stream s; logits and codes stay [n_streams][...].  enable = 0 turns it off. */
 int zonos2cu_set_cfg(zonos2cu_ctx *ctx, int enable, float scale);
+
+/* Low-rank adapters beside the head in zonos2cu_ctx_step, as in
+ * zonos2cu_head_adapters: A [n_adapters][rank][dim], B [n_adapters][n_cb*rows_per_cb]
+ * [rank] (the first vocab rows of each codebook are kept) and scale [n_adapters] f32
+ * (NULL: 1) from host memory, `dtype` the head's (a step with another head type
+ * returns ZONOS2CU_ESTATE).  Every stream starts without one;
+ * zonos2cu_set_stream_adapters gives each stream its adapter (-1: none; NULL: none
+ * anywhere).  With guidance on, both rows of a stream use it; with the output norm's
+ * weight folded into a bf16 head it is folded into A as well.  n_adapters = 0 removes
+ * them. */
+int zonos2cu_set_adapters(zonos2cu_ctx *ctx, const void *A_host, const void *B_host,
+                          const float *scale_host, int n_adapters, int rank,
+                          zonos2cu_dtype dtype, int rows_per_cb);
+int zonos2cu_set_stream_adapters(zonos2cu_ctx *ctx, const int32_t *ids_host);
 
 /* One sampling step from device logits [n_streams][n_cb][row_stride] on
  * `stream` (NULL = the legacy default stream, like every "_dev" call); the

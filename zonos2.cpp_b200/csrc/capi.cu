@@ -13,6 +13,7 @@
 #include "block_norm.cuh"
 #include "common.cuh"
 #include "head.cuh"
+#include "head_adapters.cuh"
 #include "generate.cuh"
 #include "sampler.cuh"
 #include "verify.cuh"
@@ -367,6 +368,39 @@ int zonos2cu_head_softcap(const void *W_dev, zonos2cu_dtype dtype, int rows_per_
                        logits_dev, stream, false, 1.0f);
 }
 
+long long zonos2cu_head_adapters_work(zonos2cu_dtype dtype, int batch, int rank)
+{
+    if ((dtype != ZONOS2CU_F32 && dtype != ZONOS2CU_BF16) || batch < 0 || rank < 1 ||
+        rank > ZONOS2CU_MAX_RANK)
+        return ZONOS2CU_EINVAL;
+    return (long long)z2::adapter_work_bytes(dtype == ZONOS2CU_BF16, batch, rank);
+}
+
+int zonos2cu_head_adapters(const void *W_dev, zonos2cu_dtype dtype, int rows_per_cb, int n_cb,
+                           int vocab, int dim, const void *hidden_dev, int batch, float softcap,
+                           const void *A_dev, const void *B_dev, const float *scale_dev,
+                           int n_adapters, int rank, const int32_t *adapter_dev, void *work_dev,
+                           long long work_bytes, float *logits_dev, void *stream)
+{
+    const int rc = check_head(W_dev, dtype, rows_per_cb, n_cb, vocab, dim, hidden_dev, batch,
+                              softcap, logits_dev);
+    if (rc) return rc;
+    if (n_adapters < 1 || rank < 1 || rank > ZONOS2CU_MAX_RANK) return ZONOS2CU_EINVAL;
+    if (batch == 0) return ZONOS2CU_OK;
+    if (!A_dev || !B_dev || !adapter_dev || !work_dev) return ZONOS2CU_EINVAL;
+    const uintptr_t es = dtype == ZONOS2CU_F32 ? 4 : 2;
+    if ((uintptr_t)W_dev % es || (uintptr_t)hidden_dev % es || (uintptr_t)A_dev % es ||
+        (uintptr_t)B_dev % es || (uintptr_t)scale_dev % 4 || (uintptr_t)adapter_dev % 4 ||
+        (uintptr_t)logits_dev % 4 || (uintptr_t)work_dev % 16)
+        return ZONOS2CU_EINVAL;
+    if (work_bytes < (long long)z2::adapter_work_bytes(dtype == ZONOS2CU_BF16, batch, rank))
+        return ZONOS2CU_EINVAL;
+    z2::HeadArgs h{W_dev, rows_per_cb, n_cb, vocab, dim, hidden_dev, batch, softcap, logits_dev};
+    z2::AdapterArgs ad{A_dev, B_dev, scale_dev, n_adapters, rank, adapter_dev, 1, work_dev};
+    Z2_CK(z2::launch_head_adapters(h, ad, dtype == ZONOS2CU_BF16, (cudaStream_t)stream));
+    return ZONOS2CU_OK;
+}
+
 int zonos2cu_block_norm(const void *resid_dev, const void *block_dev, zonos2cu_dtype dtype,
                         int rows, int dim, long long resid_stride, long long block_stride,
                         const float *post_weight_dev, float post_eps, const void *gate_dev,
@@ -543,6 +577,15 @@ struct zonos2cu_ctx {
     // classifier-free guidance (zonos2cu_set_cfg): steps take 2S hidden rows
     bool cfg_on = false;
     float cfg_scale = 1.0f;
+    // low-rank adapters beside the head (zonos2cu_set_adapters)
+    int n_adapters = 0, adapter_rank = 0;   // n_adapters 0: none
+    zonos2cu_dtype adapter_dtype = ZONOS2CU_F32;
+    void *adapter_a = nullptr;        // [n][rank][D]
+    void *adapter_a_folded = nullptr; // the same with the output norm's weight in its columns
+    void *adapter_b = nullptr;        // [n][C*V][rank]
+    float *adapter_scale = nullptr;   // [n]
+    int32_t *adapter_ids = nullptr;   // [S], -1: none
+    void *adapter_work = nullptr;     // for 2S hidden rows
     // generation loop state (zonos2cu_gen_begin)
     bool gen_on = false;
     int gen_max_frames = 0, gen_eoa = 1024, gen_pad = 1025, gen_text_pad = 519;
@@ -595,14 +638,33 @@ int grow(void **p, size_t *cap, size_t want)
 // are set (synchronises the context's stream).
 int refold_head(zonos2cu_ctx *c)
 {
-    if (!c->norm_on || !c->norm_has_w || !c->head || c->head_dtype != ZONOS2CU_BF16)
-        return ZONOS2CU_OK;
+    if (!c->norm_on || !c->norm_has_w) return ZONOS2CU_OK;
+    if (c->n_adapters && c->adapter_dtype == ZONOS2CU_BF16) {   // the adapters' projections too
+        const size_t n = (size_t)c->n_adapters * c->adapter_rank, D = (size_t)c->dims.dim;
+        if (!c->adapter_a_folded) Z2_CK(cudaMalloc(&c->adapter_a_folded, 2 * n * D));
+        Z2_CK(z2::launch_fold_columns(c->adapter_a, c->norm_w, (int)n, (int)D,
+                                      c->adapter_a_folded, c->stream));
+        Z2_CK(cudaStreamSynchronize(c->stream));
+    }
+    if (!c->head || c->head_dtype != ZONOS2CU_BF16) return ZONOS2CU_OK;
     const size_t rows = (size_t)c->dims.n_cb * c->dims.vocab, D = (size_t)c->dims.dim;
     if (!c->head_folded) Z2_CK(cudaMalloc(&c->head_folded, 2 * rows * D));
     Z2_CK(z2::launch_fold_columns(c->head, c->norm_w, (int)rows, (int)D, c->head_folded,
                                   c->stream));
     Z2_CK(cudaStreamSynchronize(c->stream));
     return ZONOS2CU_OK;
+}
+
+void free_adapters(zonos2cu_ctx *c)
+{
+    cudaFree(c->adapter_a);
+    cudaFree(c->adapter_a_folded);
+    cudaFree(c->adapter_b);
+    cudaFree(c->adapter_scale);
+    cudaFree(c->adapter_work);
+    c->adapter_a = c->adapter_a_folded = c->adapter_b = c->adapter_work = nullptr;
+    c->adapter_scale = nullptr;
+    c->n_adapters = 0;
 }
 
 // Small batches: the host path's codes and flags are written by the kernels
@@ -730,6 +792,8 @@ int zonos2cu_ctx_destroy(zonos2cu_ctx *c)
     cudaFree(c->normed);
     cudaFree(c->head_folded);
     cudaFree(c->row_rcp);
+    free_adapters(c);
+    cudaFree(c->adapter_ids);
     cudaFree(c->gen_frames);
     cudaFree(c->gen_count);
     cudaFree(c->gen_next);
@@ -895,6 +959,73 @@ int zonos2cu_set_cfg(zonos2cu_ctx *c, int enable, float scale)
     Z2_CK(cudaDeviceSynchronize());   // no step may still be using the state
     c->cfg_on = enable != 0;
     c->cfg_scale = scale;
+    return ZONOS2CU_OK;
+}
+
+int zonos2cu_set_adapters(zonos2cu_ctx *c, const void *A_host, const void *B_host,
+                          const float *scale_host, int n_adapters, int rank,
+                          zonos2cu_dtype dtype, int rows_per_cb)
+{
+    if (!c || n_adapters < 0) return ZONOS2CU_EINVAL;
+    if (n_adapters > 0) {
+        if (c->dims.dim < 1 || !A_host || !B_host || rank < 1 || rank > ZONOS2CU_MAX_RANK ||
+            rows_per_cb < c->dims.vocab)
+            return ZONOS2CU_EINVAL;
+        if (dtype != ZONOS2CU_F32 && dtype != ZONOS2CU_BF16) return ZONOS2CU_EINVAL;
+    }
+    DeviceGuard g(c->device);
+    Z2_CK(cudaDeviceSynchronize());   // no step may still be using the state
+    free_adapters(c);
+    if (n_adapters == 0) return ZONOS2CU_OK;
+    const size_t es = dtype == ZONOS2CU_F32 ? 4 : 2, n = (size_t)n_adapters, R = (size_t)rank;
+    const size_t V = (size_t)c->dims.vocab, C = (size_t)c->dims.n_cb, D = (size_t)c->dims.dim;
+    const size_t S = (size_t)c->dims.n_streams;
+    Z2_CK(cudaMalloc(&c->adapter_a, es * n * R * D));
+    Z2_CK(cudaMalloc(&c->adapter_b, es * n * C * V * R));
+    Z2_CK(cudaMalloc(&c->adapter_scale, sizeof(float) * n));
+    if (S) {
+        Z2_CK(cudaMalloc(&c->adapter_work,
+                         z2::adapter_work_bytes(dtype == ZONOS2CU_BF16, (int)(2 * S), rank)));
+        if (!c->adapter_ids) Z2_CK(cudaMalloc(&c->adapter_ids, sizeof(int32_t) * S));
+        Z2_CK(cudaMemsetAsync(c->adapter_ids, 0xff, sizeof(int32_t) * S, c->stream));   // -1
+    }
+    Z2_CK(cudaMemcpyAsync(c->adapter_a, A_host, es * n * R * D, cudaMemcpyHostToDevice, c->stream));
+    // the sampled rows of each codebook, as set_head keeps them
+    for (size_t k = 0; k < n * C; k++)
+        Z2_CK(cudaMemcpyAsync(static_cast<char *>(c->adapter_b) + es * k * V * R,
+                              static_cast<const char *>(B_host) + es * k * (size_t)rows_per_cb * R,
+                              es * V * R, cudaMemcpyHostToDevice, c->stream));
+    if (scale_host) {
+        Z2_CK(cudaMemcpyAsync(c->adapter_scale, scale_host, sizeof(float) * n,
+                              cudaMemcpyHostToDevice, c->stream));
+    } else {
+        const float one = 1.0f;
+        for (size_t k = 0; k < n; k++)
+            Z2_CK(cudaMemcpyAsync(c->adapter_scale + k, &one, sizeof(float),
+                                  cudaMemcpyHostToDevice, c->stream));
+    }
+    Z2_CK(cudaStreamSynchronize(c->stream));
+    c->n_adapters = n_adapters;
+    c->adapter_rank = rank;
+    c->adapter_dtype = dtype;
+    return refold_head(c);
+}
+
+int zonos2cu_set_stream_adapters(zonos2cu_ctx *c, const int32_t *ids_host)
+{
+    if (!c) return ZONOS2CU_EINVAL;
+    if (!c->n_adapters) return ZONOS2CU_ESTATE;
+    for (int s = 0; ids_host && s < c->dims.n_streams; s++)
+        if (ids_host[s] < -1 || ids_host[s] >= c->n_adapters) return ZONOS2CU_EINVAL;
+    DeviceGuard g(c->device);
+    Z2_CK(cudaDeviceSynchronize());   // no step may still be using the state
+    const size_t bytes = sizeof(int32_t) * (size_t)c->dims.n_streams;
+    if (!bytes) return ZONOS2CU_OK;
+    if (ids_host)
+        Z2_CK(cudaMemcpyAsync(c->adapter_ids, ids_host, bytes, cudaMemcpyHostToDevice, c->stream));
+    else
+        Z2_CK(cudaMemsetAsync(c->adapter_ids, 0xff, bytes, c->stream));
+    Z2_CK(cudaStreamSynchronize(c->stream));
     return ZONOS2CU_OK;
 }
 
@@ -1082,6 +1213,7 @@ int zonos2cu_ctx_step(zonos2cu_ctx *c, const void *hidden_dev, zonos2cu_dtype dt
     if (!c || !hidden_dev) return ZONOS2CU_EINVAL;
     if (!c->head) return ZONOS2CU_ESTATE;
     if (dtype != c->head_dtype) return ZONOS2CU_EINVAL;
+    if (c->n_adapters && c->adapter_dtype != c->head_dtype) return ZONOS2CU_ESTATE;
     DeviceGuard g(c->device);
     const zonos2cu_dims &d = c->dims;
     int rc = check_params(params, d.vocab);
@@ -1103,9 +1235,22 @@ int zonos2cu_ctx_step(zonos2cu_ctx *c, const void *hidden_dev, zonos2cu_dtype dt
             h = c->normed;
         }
     }
-    rc = launch_head(W, dtype, d.vocab, d.n_cb, d.vocab, d.dim, h, rows_in, 15.0f, lg, st,
-                     c->cfg_on, c->cfg_scale, row_scale);
-    if (rc) return rc;
+    if (c->n_adapters && rows_in > 0) {
+        z2::HeadArgs a{W, d.vocab, d.n_cb, d.vocab, d.dim, h, rows_in, 15.0f, lg};
+        a.cfg = c->cfg_on ? 1 : 0;
+        a.cfg_scale = c->cfg_scale;
+        a.row_scale = row_scale;
+        const void *A = c->norm_on && c->norm_has_w && dtype == ZONOS2CU_BF16
+                            ? c->adapter_a_folded : c->adapter_a;
+        const z2::AdapterArgs ad{A, c->adapter_b, c->adapter_scale, c->n_adapters,
+                                 c->adapter_rank, c->adapter_ids, c->cfg_on ? 2 : 1,
+                                 c->adapter_work};
+        Z2_CK(z2::launch_head_adapters(a, ad, dtype == ZONOS2CU_BF16, st));
+    } else {
+        rc = launch_head(W, dtype, d.vocab, d.n_cb, d.vocab, d.dim, h, rows_in, 15.0f, lg, st,
+                         c->cfg_on, c->cfg_scale, row_scale);
+        if (rc) return rc;
+    }
     return zonos2cu_ctx_sample(c, lg, d.vocab, params, delay_step, codes_dev, flags_dev, st);
 }
 

@@ -46,6 +46,8 @@ EXPORTS = (
     "zonos2cu_gather_codes", "zonos2cu_comm_create_timeout", "zonos2cu_comm_abort",
     "zonos2cu_ipc_alloc", "zonos2cu_ipc_free", "zonos2cu_ipc_open", "zonos2cu_ipc_close",
     "zonos2cu_push_codes", "zonos2cu_block_norm", "zonos2cu_verify_drafts",
+    "zonos2cu_head_adapters", "zonos2cu_head_adapters_work", "zonos2cu_set_adapters",
+    "zonos2cu_set_stream_adapters",
 )
 
 
@@ -138,6 +140,11 @@ def lib() -> C.CDLL:
         "zonos2cu_ipc_open": (i, [i, C.c_char_p, C.POINTER(vp)]),
         "zonos2cu_ipc_close": (i, [vp]),
         "zonos2cu_push_codes": (i, [vp, i, ll, vp, ll, vp]),
+        "zonos2cu_head_adapters_work": (ll, [i, i, i]),
+        "zonos2cu_head_adapters": (i, [vp, i, i, i, i, i, vp, i, f, vp, vp, vp, i, i, vp, vp, ll, vp,
+                                       vp]),
+        "zonos2cu_set_adapters": (i, [vp, vp, vp, vp, i, i, i, i]),
+        "zonos2cu_set_stream_adapters": (i, [vp, vp]),
         "zonos2cu_block_norm": (i, [vp, vp, i, i, i, ll, ll, vp, f, vp, ll, i, i, f, vp, f, vp, vp,
                                     ll, vp]),
         "zonos2cu_verify_drafts": (i, [vp, i, i, i, i, ll, C.POINTER(SampleParams), vp, vp, vp, vp,
@@ -263,6 +270,34 @@ def _rows(t, what: str) -> int:
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"{what}: expected [rows, dim] with contiguous rows")
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def head_adapters_work(dtype: int, batch: int, rank: int) -> int:
+    """Bytes of scratch that head_adapters needs."""
+    return _check(lib().zonos2cu_head_adapters_work(dtype, batch, rank),
+                  "zonos2cu_head_adapters_work")
+
+
+def head_adapters(W, dtype: int, rows_per_cb: int, n_cb: int, vocab: int, hidden, A, B, adapter,
+                  out, work, *, scale=None, softcap: float = 15.0, stream=None) -> None:
+    """head_softcap with a low-rank adapter per hidden row.
+
+    hidden [batch, dim], A [n, rank, dim], B [n, n_cb * rows_per_cb, rank] of ``dtype``;
+    adapter int32 [batch] (outside [0, n): none); scale f32 [n] or None; out f32
+    [batch, n_cb, vocab]; work: a scratch tensor of head_adapters_work() bytes."""
+    batch, dim = hidden.shape
+    n, rank, _ = A.shape
+    wide = n_cb * rows_per_cb
+    for t, size in ((W, wide * dim), (hidden, batch * dim), (A, n * rank * dim),
+                    (B, n * wide * rank), (adapter, batch), (out, batch * n_cb * vocab),
+                    (scale, n)):
+        if t is not None and (t.numel() != size or not t.is_contiguous()):
+            raise ValueError(f"head_adapters: a contiguous tensor of {size} elements expected, got "
+                             f"{tuple(t.shape)}")
+    _launch("zonos2cu_head_adapters", hidden, stream, W.data_ptr(), dtype, rows_per_cb, n_cb, vocab,
+            dim, hidden.data_ptr(), batch, softcap, A.data_ptr(), B.data_ptr(), _ptr(scale), n,
+            rank, adapter.data_ptr(), work.data_ptr(), work.numel() * work.element_size(),
+            out.data_ptr())
 
 
 def block_norm(resid, block, resid_out, normed_out, *, post_weight=None, post_eps: float = 1e-5,
@@ -503,6 +538,34 @@ class Context:
     def set_cfg(self, scale: float, enable: bool = True) -> None:
         """Guidance blend; steps then take 2 * n_streams hidden rows (2s cond, 2s+1 uncond)."""
         _check(lib().zonos2cu_set_cfg(self.h, int(enable), C.c_float(scale)), "set_cfg")
+
+    def set_adapters(self, A, B, rows_per_cb: int, dtype: int, scale=None) -> None:
+        """Low-rank adapters beside the head: A [n, rank, dim], B [n, n_cb * rows_per_cb, rank]
+        host arrays (bf16 as uint16 bits); A None removes them."""
+        if A is None:
+            _check(lib().zonos2cu_set_adapters(self.h, None, None, None, 0, 0, dtype, 0),
+                   "set_adapters")
+            return
+        A, B = np.ascontiguousarray(A), np.ascontiguousarray(B)
+        n, rank, dim = A.shape
+        if dim != self.shape.dim or B.shape != (n, self.shape.n_cb * rows_per_cb, rank):
+            raise ValueError("set_adapters: A [n, rank, dim] and B [n, n_cb * rows_per_cb, rank]")
+        if {A.itemsize, B.itemsize} != {4 if dtype == F32 else 2}:
+            raise TypeError("set_adapters: A and B must hold elements of dtype")
+        sc = None if scale is None else np.ascontiguousarray(scale, np.float32)
+        if sc is not None and sc.shape != (n,):
+            raise ValueError("set_adapters: one scale per adapter")
+        _check(lib().zonos2cu_set_adapters(self.h, A.ctypes.data, B.ctypes.data,
+                                           None if sc is None else sc.ctypes.data, n, rank, dtype,
+                                           rows_per_cb), "set_adapters")
+
+    def set_stream_adapters(self, ids) -> None:
+        """The adapter of each stream (-1: none); None: none anywhere."""
+        a = None if ids is None else np.ascontiguousarray(ids, np.int32)
+        if a is not None and a.shape != (self.shape.n_streams,):
+            raise ValueError("set_stream_adapters: one id per stream")
+        _check(lib().zonos2cu_set_stream_adapters(self.h, None if a is None else a.ctypes.data),
+               "set_stream_adapters")
 
     # ---- generation loop
     def gen_begin(self, max_frames: int, eoa_id: int = 1024, audio_pad_id: int = 1025,
