@@ -535,11 +535,12 @@ int zonos2cu_write_codes_bin(const char *path, const int32_t *frames_host, int n
 int zonos2cu_device_error(void)
 {
     Z2_CK(cudaDeviceSynchronize());
-    int v = 0, vs = 0;
+    int v = 0, vs = 0, va = 0;
     int e = z2::read_and_clear_device_error(&v);
     if (!e) e = z2::read_and_clear_sampler_error(&vs);
+    if (!e) e = z2::read_and_clear_adapter_error(&va);
     if (e) return cuda_fail((cudaError_t)e, "device error word");
-    return v ? v : vs;
+    return v ? v : vs ? vs : va;
 }
 
 }  // extern "C"

@@ -8,8 +8,9 @@
 // in f32 (f64 beside an f32 head): rounding it to bf16 would put 2^-9 of the
 // adapter's contribution into f32 logits.
 //
-// Kernels: adapter_down_kernel makes t; adapter_any_kernel, one warp per weight
-// row, takes every size and type.
+// A bf16 head runs on the tensor cores (head_adapters_tc.cu) where its sizes and
+// alignment allow.  Here: adapter_down_kernel makes t, and adapter_any_kernel, one
+// warp per weight row, takes every size and type.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -120,7 +121,9 @@ cudaError_t launch_head_adapters(const HeadArgs &h, const AdapterArgs &ad, bool 
                                  cudaStream_t stream)
 {
     if (h.batch == 0) return cudaSuccess;
-    return bf16 ? launch_any<__nv_bfloat16>(h, ad, stream) : launch_any<float>(h, ad, stream);
+    if (!bf16) return launch_any<float>(h, ad, stream);
+    const cudaError_t e = launch_head_adapters_tc(h, ad, stream);
+    return e == cudaErrorNotSupported ? launch_any<__nv_bfloat16>(h, ad, stream) : e;
 }
 
 }  // namespace z2

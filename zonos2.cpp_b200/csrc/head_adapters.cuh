@@ -24,6 +24,13 @@ struct AdapterArgs {
 // f32 for a bf16 one.
 size_t adapter_work_bytes(bool bf16, int batch, int rank);
 
+// The tcgen05 kernel (head_adapters_tc.cu), for bf16; cudaErrorNotSupported for the
+// sizes and alignments it does not take.
+cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cudaStream_t stream);
+
+// Reads and clears the device error word of its bounded waits.
+int read_and_clear_adapter_error(int *value);
+
 // HeadArgs with adapters: everything of `dtype` bf16 or f32.
 cudaError_t launch_head_adapters(const HeadArgs &h, const AdapterArgs &ad, bool bf16,
                                  cudaStream_t stream);
