@@ -114,7 +114,9 @@ cudaError_t launch_any(const HeadArgs &h, const AdapterArgs &ad, cudaStream_t st
 
 size_t adapter_work_bytes(bool bf16, int batch, int rank)
 {
-    return (size_t)batch * (size_t)rank * (bf16 ? 4 : 8);
+    const size_t t = (size_t)batch * (size_t)rank;
+    // the tensor-core path keeps two orders of the rows beside t
+    return !bf16 ? 8 * t : rank % 8 == 0 ? 4 * (t + 2 * (size_t)batch) : 4 * t;
 }
 
 cudaError_t launch_head_adapters(const HeadArgs &h, const AdapterArgs &ad, bool bf16,

@@ -20,8 +20,8 @@ struct AdapterArgs {
     void *work;            // adapter_work_bytes() bytes, 16-byte aligned
 };
 
-// Bytes of AdapterArgs::work: scale * A h per hidden row, f64 for an f32 head,
-// f32 for a bf16 one.
+// Bytes of AdapterArgs::work: scale * A h per hidden row, f64 for an f32 head, f32 for
+// a bf16 one, and an order of the rows.
 size_t adapter_work_bytes(bool bf16, int batch, int rank);
 
 // The tcgen05 kernel (head_adapters_tc.cu), for bf16; cudaErrorNotSupported for the

@@ -74,13 +74,16 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
 // error word is set, the caller winds down).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity)
 {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
+    uint64_t t0 = 0;   // the timer takes about a microsecond to read: only long waits read it
     for (uint32_t it = 1;; it++) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 255u) == 0u && globaltimer_ns() - t0 > kWaitNs) {
-            atomicCAS(&g_device_error, 0, kErrTimeout);
-            return false;
+        if ((it & 255u) == 0u) {
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > kWaitNs) {
+                atomicCAS(&g_device_error, 0, kErrTimeout);
+                return false;
+            }
         }
     }
 }
@@ -186,13 +189,16 @@ __device__ __forceinline__ bool mbar_try_wait_cl(uint32_t bar, uint32_t parity)
 }
 __device__ __forceinline__ bool mbar_wait_cl(uint32_t bar, uint32_t parity)
 {
-    if (mbar_try_wait_cl(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
+    uint64_t t0 = 0;
     for (uint32_t it = 1;; it++) {
         if (mbar_try_wait_cl(bar, parity)) return true;
-        if ((it & 255u) == 0u && globaltimer_ns() - t0 > kWaitNs) {
-            atomicCAS(&g_device_error, 0, kErrTimeout);
-            return false;
+        if ((it & 255u) == 0u) {
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > kWaitNs) {
+                atomicCAS(&g_device_error, 0, kErrTimeout);
+                return false;
+            }
         }
     }
 }
