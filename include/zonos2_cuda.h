@@ -15,8 +15,8 @@
  *     host.
  *   - Device memory is allocated only by these calls:
  *       zonos2cu_ctx_create, zonos2cu_set_head, zonos2cu_set_allow,
- *       zonos2cu_set_out_norm, zonos2cu_set_adapters,
- *       zonos2cu_set_embeddings, zonos2cu_gen_begin
+ *       zonos2cu_set_out_norm, zonos2cu_set_adapters, zonos2cu_set_cfg
+ *       (with adapters), zonos2cu_set_embeddings, zonos2cu_gen_begin
  *         (owned by the context, freed by zonos2cu_ctx_destroy);
  *       the first zonos2cu_ctx_sample_host / zonos2cu_ctx_step_host of a
  *         context, and a later one with larger inputs (host-path staging,

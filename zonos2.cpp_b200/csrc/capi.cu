@@ -587,6 +587,7 @@ struct zonos2cu_ctx {
     float *adapter_scale = nullptr;   // [n]
     int32_t *adapter_ids = nullptr;   // [S], -1: none
     void *adapter_work = nullptr;     // for 2S hidden rows
+    float *adapter_delta = nullptr;   // [2S][C*V], with guidance and a bf16 head
     // generation loop state (zonos2cu_gen_begin)
     bool gen_on = false;
     int gen_max_frames = 0, gen_eoa = 1024, gen_pad = 1025, gen_text_pad = 519;
@@ -663,9 +664,22 @@ void free_adapters(zonos2cu_ctx *c)
     cudaFree(c->adapter_b);
     cudaFree(c->adapter_scale);
     cudaFree(c->adapter_work);
+    cudaFree(c->adapter_delta);
+    c->adapter_delta = nullptr;
     c->adapter_a = c->adapter_a_folded = c->adapter_b = c->adapter_work = nullptr;
     c->adapter_scale = nullptr;
     c->n_adapters = 0;
+}
+
+// With guidance the logits' buffer holds one row per pair: the adapters' part of a bf16
+// head needs a buffer of its own.
+int ensure_adapter_delta(zonos2cu_ctx *c)
+{
+    if (!c->cfg_on || !c->n_adapters || c->adapter_dtype != ZONOS2CU_BF16 || c->adapter_delta ||
+        !n_rows(c))
+        return ZONOS2CU_OK;
+    Z2_CK(cudaMalloc(&c->adapter_delta, sizeof(float) * 2 * n_rows(c) * (size_t)c->dims.vocab));
+    return ZONOS2CU_OK;
 }
 
 // Small batches: the host path's codes and flags are written by the kernels
@@ -960,7 +974,7 @@ int zonos2cu_set_cfg(zonos2cu_ctx *c, int enable, float scale)
     Z2_CK(cudaDeviceSynchronize());   // no step may still be using the state
     c->cfg_on = enable != 0;
     c->cfg_scale = scale;
-    return ZONOS2CU_OK;
+    return ensure_adapter_delta(c);
 }
 
 int zonos2cu_set_adapters(zonos2cu_ctx *c, const void *A_host, const void *B_host,
@@ -1009,7 +1023,8 @@ int zonos2cu_set_adapters(zonos2cu_ctx *c, const void *A_host, const void *B_hos
     c->n_adapters = n_adapters;
     c->adapter_rank = rank;
     c->adapter_dtype = dtype;
-    return refold_head(c);
+    const int rc = ensure_adapter_delta(c);
+    return rc ? rc : refold_head(c);
 }
 
 int zonos2cu_set_stream_adapters(zonos2cu_ctx *c, const int32_t *ids_host)
@@ -1245,7 +1260,7 @@ int zonos2cu_ctx_step(zonos2cu_ctx *c, const void *hidden_dev, zonos2cu_dtype dt
                             ? c->adapter_a_folded : c->adapter_a;
         const z2::AdapterArgs ad{A, c->adapter_b, c->adapter_scale, c->n_adapters,
                                  c->adapter_rank, c->adapter_ids, c->cfg_on ? 2 : 1,
-                                 c->adapter_work};
+                                 c->adapter_work, c->cfg_on ? c->adapter_delta : nullptr};
         Z2_CK(z2::launch_head_adapters(a, ad, dtype == ZONOS2CU_BF16, st));
     } else {
         rc = launch_head(W, dtype, d.vocab, d.n_cb, d.vocab, d.dim, h, rows_in, 15.0f, lg, st,

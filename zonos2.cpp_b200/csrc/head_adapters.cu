@@ -115,8 +115,9 @@ cudaError_t launch_any(const HeadArgs &h, const AdapterArgs &ad, cudaStream_t st
 size_t adapter_work_bytes(bool bf16, int batch, int rank)
 {
     const size_t t = (size_t)batch * (size_t)rank;
-    // the tensor-core path keeps two orders of the rows beside t
-    return !bf16 ? 8 * t : rank % 8 == 0 ? 4 * (t + 2 * (size_t)batch) : 4 * t;
+    // beside t (a multiple of 8 ranks), the tensor-core path keeps the rows' order and its
+    // items: at most batch + 2 + 2 (batch / 8 + batch) words, 3.25 batch + 2
+    return !bf16 ? 8 * t : rank % 8 == 0 ? 4 * (t + 4 * (size_t)batch) : 4 * t;
 }
 
 cudaError_t launch_head_adapters(const HeadArgs &h, const AdapterArgs &ad, bool bf16,

@@ -18,6 +18,8 @@ struct AdapterArgs {
                            // [0, n_adapters): none
     int rows_per_id;       // 1, or 2 for guidance pairs
     void *work;            // adapter_work_bytes() bytes, 16-byte aligned
+    float *delta = nullptr;  // [batch][n_cb * vocab] scratch of a bf16 head with guidance; else
+                             // the logits' buffer serves
 };
 
 // Bytes of AdapterArgs::work: scale * A h per hidden row, f64 for an f32 head, f32 for

@@ -1,39 +1,25 @@
-// head_adapters_tc.cu -- the bf16 output head beside low-rank adapters on the
-// tcgen05 tensor cores (sm_100a).
+// head_adapters_tc.cu -- the bf16 output head beside low-rank adapters on the tensor
+// cores (sm_100a):
 //
-//     t[b]         = s_a * (A_a h[b])
-//     logits[b, n] = softcap(W[n] . h[b] + B_a[n] . t[b])
+//     t[b]         = s_a * (A_a h[b])                     adapter_down_*_kernel
+//     delta[b, n]  = B_a[n] . t[b]                        adapter_up_kernel
+//     logits[b, n] = softcap(W[n] . h[b] + delta[b, n])   adapter_head_kernel
 //
-// A small kernel (two for a large batch) makes t (f32) and orders each tile's hidden
-// rows by adapter; adapter_head_kernel is the GEMM, whose accumulators start from B_a t.
+// delta goes through the logits' own buffer: the GEMM reads an element, adds it and
+// stores the logit in its place.  The kernels are chained by programmatic dependent
+// launch, and only the GEMM's last step waits for delta, so its main loop covers the
+// small kernels of a batch that fills the SMs once.
 //
-// The GEMM's operands trade places against the plain head's: the weight rows are
-// the M of its tiles (TMEM lanes), the hidden rows the N (TMEM columns).  Few
-// streams then fill the tile (N = 16 is enough) instead of leaving most of an
-// M = 128 tile empty, and a warp's logits of one hidden row are 128 consecutive
-// bytes.
+// Everything is as good as f32: t enters its MMA as three bf16 parts, which hold all
+// of its 24 bits, and the GEMM's depth is summed in parts (kPartSteps).
 //
-// The low-rank product is made beside the main loop by four warps of their own, with
-// mma.sync on at most eight hidden rows of one adapter at a time, and stored in the
-// accumulator that the last part of the tile's depth adds to.  t enters it as three
-// bf16 parts, which hold all of its 24 bits: B t is as good as in f32.  As extra depth
-// of the main MMAs every adapter of a tile would cost a full-size step (and an
-// infinity in one adapter would reach the other rows' logits as inf * 0); on the FMA
-// pipe, t's values would have to be broadcast from shared memory (16 B per 512 B of
-// register writes), which took longer than the main loop itself.
-//
-// Warp roles (16 warps):
-//   warp 0       TMA producer of the weight and hidden tiles (128-byte swizzle);
-//   warp 1       TMEM allocation, tcgen05.mma (M = 64 or 128, or 256 over a two-SM pair);
-//   warp 2       cuts the tile's ordered rows into items (up to eight rows of one
-//                adapter).  It alone waits for the kernel that makes t and the order
-//                (griddepcontrol.wait): the GEMM's main loop overlaps that kernel;
-//   warps 4..7   B t into TMEM, an item at a time (one warp per lane quarter);
-//   warps 8..15  the sums of the parts of the depth, softcap, stores.
-// Every wait is bounded, as in head_tc.cu: a warp whose wait expires sets the error
-// word, stops waiting and copying, and the CTA winds down (copies in flight waited
-// for, TMEM freed).
-// No TMA load here uses cluster multicast.
+// Measured against keeping delta in the GEMM, for 4096 rows of 32 adapters, rank 16:
+// added in the epilogue on the FMA pipe, t broadcast from shared memory, 0.37-0.54 ms;
+// by mma.sync in four or eight warps beside the main loop into the accumulators,
+// 0.28-0.37 ms (with several adapters in every 256 rows, the warps' latency per adapter
+// exceeds the tile's MMAs); hidden rows gathered by adapter with TMA gather4, 0.54 ms
+// (a quarter of the plain copies' rate).  The separate kernel moves the logits once
+// more through memory, which the compute-bound GEMM hides.
 #include <cuda_bf16.h>
 #include <limits.h>
 #include <math.h>
@@ -48,89 +34,95 @@ int read_and_clear_adapter_error(int *value) { return take_device_error(value); 
 
 namespace {
 
+constexpr int kMaxAdapters = 4096;
+constexpr int kItem = 8;   // hidden rows per item at most: rows of one adapter
+
 // ---- the rows' order ---------------------------------------------------------
 
-constexpr int kMaxN = 256;          // hidden rows per tile (TMEM columns) at most
-constexpr int kMaxAdapters = 4096;
-constexpr uint32_t kNone = 0xffffffu;   // the key of a row without an adapter: last
+// Scratch, after t: order[batch], the rows by (adapter, row), those without one last;
+// items[], (adapter, first place in the order) each; their number.
+struct Order {
+    int32_t *rows;
+    int2 *items;
+    int32_t *n_items;
+};
 
-// The entries (key << 8) | column of a tile's rows, ascending: thread i ranks its rows
-// by counting.  *place and *group: the row's place, and the place of its key's first row.
-__device__ __forceinline__ uint32_t row_entry(const int32_t *which, int rows_per_id, int n_adapters,
-                                              int b0, int col)
+// At most this many items.
+__host__ __device__ __forceinline__ int max_items(int batch, int n_adapters)
 {
-    const int a = __ldg(which + (b0 + col) / rows_per_id);
-    return ((unsigned)a < (unsigned)n_adapters ? (uint32_t)a << 8 : kNone << 8) | (uint32_t)col;
+    return batch / kItem + min(batch, n_adapters);
 }
 
-__device__ __forceinline__ void rank_entry(const uint32_t *s_entry, int rows, uint32_t mine, int *place,
-                                           int *group)
-{
-    int n = 0, m = 0;
-    const uint32_t key = mine & ~255u;
-    for (int i = 0; i < rows; i += 4) {   // entries past the rows are all ones: none is smaller
-        const uint4 e = *reinterpret_cast<const uint4 *>(s_entry + i);
-        n += (e.x < mine) + (e.y < mine) + (e.z < mine) + (e.w < mine);
-        m += (e.x < key) + (e.y < key) + (e.z < key) + (e.w < key);
-    }
-    *place = n;
-    *group = m;
-}
-
-// One CTA per tile: list[b0 ..] = the tile's entries in order, and the rows' places in
-// the order of the whole batch by (adapter, row): order[place] = row.
 constexpr int kOrderThreads = 256;
 
+// One CTA per kOrderThreads rows: every CTA counts all rows, ranks its own by counting,
+// and the first lists the items.
 __global__ void __launch_bounds__(kOrderThreads)
-    order_rows_kernel(const int32_t *__restrict__ which, int batch, int nb, int rows_per_id,
-                      int n_adapters, uint32_t *__restrict__ list, int32_t *__restrict__ order)
+    order_rows_kernel(const int32_t *__restrict__ which, int batch, int rows_per_id, int n_adapters, Order o)
 {
-    extern __shared__ int s_count[];   // [n + 1] rows of each key (n: none), then [n + 1] before this tile
-    __shared__ int s_part[kOrderThreads / 32];
-    __shared__ __align__(16) uint32_t s_entry[kMaxN];
+    extern __shared__ int s_count[];   // [n + 1] rows of each key (n: none), then [n + 1] before this CTA's
+    __shared__ int s_part[2][kOrderThreads / 32];
+    __shared__ __align__(16) int s_key[kOrderThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = n_adapters;
-    const int b0 = (int)blockIdx.x * nb, rows = min(nb, batch - b0);
+    const int b0 = (int)blockIdx.x * kOrderThreads, rows = min(kOrderThreads, batch - b0);
     int *before = s_count + n + 1;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    auto key_of = [&](int b) {
+        const int a = __ldg(which + b / rows_per_id);
+        return (unsigned)a < (unsigned)n ? a : n;
+    };
     for (int i = tid; i < 2 * (n + 1); i += kOrderThreads) s_count[i] = 0;
-    s_entry[tid] = tid < rows ? row_entry(which, rows_per_id, n, b0, tid) : ~0u;
+    const int mine = tid < rows ? key_of(b0 + tid) : INT_MAX;
+    s_key[tid] = mine;
     __syncthreads();
 #pragma unroll 4
     for (int i = tid; i < batch; i += kOrderThreads) {
-        const int a = __ldg(which + i / rows_per_id), k = (unsigned)a < (unsigned)n ? a : n;
+        const int k = key_of(i);
         atomicAdd(&s_count[k], 1);
         if (i < b0) atomicAdd(&before[k], 1);
     }
     __syncthreads();
-    // the first place of each key in the whole order
+    // the first place and the first item of each key
     const int per = (n + kOrderThreads) / kOrderThreads;
     const int a0 = min(tid * per, n + 1), a1 = min(a0 + per, n + 1);
-    int own = 0;
-    for (int a = a0; a < a1; a++) own += s_count[a];
-    int sum = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(kFull, sum, o);
-        if (lane >= o) sum += t;
+    int own = 0, own_items = 0;
+    for (int a = a0; a < a1; a++) {
+        own += s_count[a];
+        own_items += a < n ? (s_count[a] + kItem - 1) / kItem : 0;
     }
-    if (lane == 31) s_part[warp] = sum;
+    int sum = own, sum_items = own_items;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int t = __shfl_up_sync(kFull, sum, d), u = __shfl_up_sync(kFull, sum_items, d);
+        if (lane >= d) {
+            sum += t;
+            sum_items += u;
+        }
+    }
+    if (lane == 31) {
+        s_part[0][warp] = sum;
+        s_part[1][warp] = sum_items;
+    }
     __syncthreads();
-    int base = sum - own;
-    for (int w = 0; w < warp; w++) base += s_part[w];
+    int base = sum - own, item = sum_items - own_items;
+    for (int w = 0; w < warp; w++) {
+        base += s_part[0][w];
+        item += s_part[1][w];
+    }
     for (int a = a0; a < a1; a++) {
         const int c = s_count[a];
+        if (blockIdx.x == 0 && a < n)
+            for (int i = 0; i < c; i += kItem) o.items[item++] = make_int2(a, base + i);
         s_count[a] = base;
         base += c;
     }
+    if (blockIdx.x == 0 && tid == kOrderThreads - 1) *o.n_items = item;
     __syncthreads();
-    if (tid < rows) {
-        const uint32_t mine = s_entry[tid];
-        int place, group;
-        rank_entry(s_entry, rows, mine, &place, &group);
-        list[b0 + place] = mine;
-        const int k = (mine >> 8) == kNone ? n : (int)(mine >> 8);
-        order[s_count[k] + before[k] + place - group] = b0 + tid;
+    if (tid < rows) {   // the rows with this key before this one
+        int same = 0;
+        for (int i = 0; i < tid; i++) same += s_key[i] == mine;
+        o.rows[s_count[mine] + before[mine] + same] = b0 + tid;
     }
 }
 
@@ -139,44 +131,29 @@ __global__ void __launch_bounds__(kOrderThreads)
 struct DownArgs {
     const __nv_bfloat16 *hidden, *A;
     const float *scale;
-    const int32_t *which, *order;   // order: the rows by adapter (many rows only)
+    const int32_t *which;
     int batch, dim, n_adapters, rank, rows_per_id;
     float *t;                       // [batch][rank]
-    uint32_t *list;                 // [batch] the tiles' entries (few rows only)
-    int nb, down_blocks;            // rows per tile; blocks before those that order the tiles
+    Order order;
 };
 
-// Few rows: one warp per row and four ranks, which share the row's loads; the last
-// blocks order one tile's rows each.
+// Few rows: one warp per row and four ranks, which share the row's loads.
 constexpr int kFewWarps = 4;
 constexpr long long kFewMost = 8192;   // rows x ranks
 
 __global__ void __launch_bounds__(32 * kFewWarps) adapter_down_few_kernel(const DownArgs g)
 {
-    const int lane = threadIdx.x & 31, quads = (g.rank + 3) / 4;
-    const long long i = (long long)blockIdx.x * kFewWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, quads = g.rank / 4;   // rank is a multiple of 8
+    const int i = (int)blockIdx.x * kFewWarps + (int)(threadIdx.x >> 5);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if ((int)blockIdx.x >= g.down_blocks) {
-        __shared__ __align__(16) uint32_t s_entry[kMaxN];
-        const int b0 = ((int)blockIdx.x - g.down_blocks) * g.nb, rows = min(g.nb, g.batch - b0);
-        for (int j = threadIdx.x; j < kMaxN; j += 32 * kFewWarps)
-            s_entry[j] = j < rows ? row_entry(g.which, g.rows_per_id, g.n_adapters, b0, j) : ~0u;
-        __syncthreads();
-        for (int j = threadIdx.x; j < rows; j += 32 * kFewWarps) {
-            int place, group;
-            rank_entry(s_entry, rows, s_entry[j], &place, &group);
-            g.list[b0 + place] = s_entry[j];
-        }
-        return;
-    }
-    if (i >= (long long)g.batch * quads) return;
-    const int b = (int)(i / quads), r0 = 4 * (int)(i % quads);
+    if (i >= g.batch * quads) return;
+    const int b = i / quads, r0 = 4 * (i % quads);
     const int a = __ldg(g.which + b / g.rows_per_id);
     if ((unsigned)a >= (unsigned)g.n_adapters) return;
     const uint4 *x = reinterpret_cast<const uint4 *>(g.hidden + (size_t)b * g.dim);
     const uint4 *w = reinterpret_cast<const uint4 *>(g.A + ((size_t)a * g.rank + r0) * g.dim);
-    const int n = g.dim / 8;   // rank is a multiple of 8: the four ranks exist
+    const int n = g.dim / 8;
     float acc[4] = {};
 #pragma unroll 2
     for (int k = lane; k < n; k += 32) {
@@ -232,7 +209,7 @@ __global__ void __launch_bounds__(32 * kDownWarps, 2) adapter_down_mma_kernel(co
     if (tid < kDownRows) {
         int row = -1, key = -1;
         if (p0 + tid < g.batch) {
-            row = __ldg(g.order + p0 + tid);
+            row = g.order.rows[p0 + tid];
             key = __ldg(g.which + row / g.rows_per_id);
             if ((unsigned)key >= (unsigned)g.n_adapters) key = -1;
         }
@@ -294,20 +271,130 @@ __global__ void __launch_bounds__(32 * kDownWarps, 2) adapter_down_mma_kernel(co
     }
 }
 
+// ---- delta = B_a t ----------------------------------------------------------
+
+// x = hi + mid + lo in bf16, exactly but for bits below 2^-25 of x; two values to a
+// register, the first in the low half.
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+__device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
+{
+    hi = pack_bf16(x, y);
+    x -= __uint_as_float(hi << 16);
+    y -= __uint_as_float(hi & 0xffff0000u);
+    mid = pack_bf16(x, y);
+    x -= __uint_as_float(mid << 16);
+    y -= __uint_as_float(mid & 0xffff0000u);
+    lo = pack_bf16(x, y);
+}
+
+
+struct UpArgs {
+    const __nv_bfloat16 *B;
+    const float *t;                // [batch][rank]
+    Order order;
+    int batch, n_cb, vocab, rows_per_cb, rank, n_adapters;
+    const int32_t *which;
+    int rows_per_id;
+    float *delta;                  // [batch][n_cb * vocab]
+};
+
+constexpr int kUpWarps = 4;
+constexpr int kUpRows = 64;        // weight rows per warp: four 16-row tiles
+constexpr int kUpTiles = kUpRows / 16;
+
+// CTA (i, j): item i and kUpWarps * kUpRows weight rows of one codebook; a warp takes
+// kUpRows of them.  mma.sync with the weight rows as M and the item's rows as N; ranks
+// are permuted alike for both operands, so that a lane loads four neighbours (4 k4 ..
+// 4 k4 + 3 of 16) of its rows of B and of the t of row g.
+// Bound: the store of delta (with 32 adapters, 151 MB for 4096 rows of 9 x 1024).
+__global__ void __launch_bounds__(32 * kUpWarps) adapter_up_kernel(const UpArgs a)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, k4 = lane & 3;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int items = *a.order.n_items, me = (int)blockIdx.x;
+    if (me >= items) return;
+    const int2 item = a.order.items[me];
+    const int per_cb = (a.vocab + kUpWarps * kUpRows - 1) / (kUpWarps * kUpRows);
+    const int c = (int)blockIdx.y / per_cb, v0 = ((int)blockIdx.y % per_cb) * kUpWarps * kUpRows + warp * kUpRows;
+    if (v0 >= a.vocab) return;
+    // the item's rows: those of the same adapter from its place on
+    int row = -1;
+    if (lane < kItem && item.y + lane < a.batch) {
+        row = a.order.rows[item.y + lane];
+        if (a.which[row / a.rows_per_id] != item.x) row = -1;
+    }
+    const int len = __popc(__ballot_sync(kFull, row >= 0));
+    const int row_g = __shfl_sync(kFull, row, min(g, len - 1));
+    float d[kUpTiles][4] = {};
+    const __nv_bfloat16 *base = a.B + ((size_t)item.x * a.n_cb * a.rows_per_cb + (size_t)c * a.rows_per_cb) * a.rank;
+    for (int k = 0; k < a.rank; k += 16) {
+        const bool in = k + 4 * k4 < a.rank;
+        const float4 t = in ? *reinterpret_cast<const float4 *>(a.t + (size_t)row_g * a.rank + k + 4 * k4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        uint2 w[kUpTiles][2];
+#pragma unroll
+        for (int m = 0; m < kUpTiles; m++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int v = min(v0 + 16 * m + 8 * h + g, a.vocab - 1);
+                w[m][h] = in ? __ldg(reinterpret_cast<const uint2 *>(base + (size_t)v * a.rank + k + 4 * k4)) : make_uint2(0u, 0u);
+            }
+        uint32_t h0, h1, m0, m1, l0, l1;
+        split3(t.x, t.y, h0, m0, l0);
+        split3(t.z, t.w, h1, m1, l1);
+#pragma unroll
+        for (int m = 0; m < kUpTiles; m++) {
+            float e[4] = {};   // the tensor cores add by truncation: 16 ranks at a time, then rounded
+            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, l0, l1);
+            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, m0, m1);
+            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, h0, h1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[m][i] += e[i];
+        }
+    }
+    const size_t ldo = (size_t)a.n_cb * a.vocab;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {   // this lane's two rows: 2 k4 and 2 k4 + 1
+        const int r = __shfl_sync(kFull, row, 2 * k4 + i);
+        if (2 * k4 + i >= len) continue;
+        float *to = a.delta + (size_t)r * ldo + (size_t)c * a.vocab;
+#pragma unroll
+        for (int m = 0; m < kUpTiles; m++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int v = v0 + 16 * m + 8 * h + g;
+                if (v < a.vocab) to[v] = d[m][2 * h + i];
+            }
+    }
+}
+
 // ---- the GEMM --------------------------------------------------------------
+//
+// Its operands trade places against the plain head's: the weight rows are the M of its
+// tiles (TMEM lanes), the hidden rows the N (TMEM columns).  Few streams then fill the
+// tile (N = 16 is enough) instead of leaving most of an M = 128 tile empty, and a warp's
+// logits of one hidden row are 128 consecutive bytes.
+//   warp 0       TMA producer of the weight and hidden tiles (128-byte swizzle);
+//   warp 1       TMEM allocation, tcgen05.mma (M = 64, or 256 over a two-SM pair);
+//   warps 4..11  the sums of the parts of the depth, delta, softcap, stores (two warps
+//                per TMEM lane quarter, each half of the columns).
+// Every wait is bounded, as in head_tc.cu: a warp whose wait expires sets the error
+// word, stops waiting and copying, and the CTA winds down (copies in flight waited
+// for, TMEM freed).  No TMA load here uses cluster multicast.
 
 constexpr int kBK = 64;             // bf16 elements per 128-byte swizzled row
+constexpr int kSmallN = 64, kPairN = 256;   // hidden rows per tile (TMEM columns) at most
+constexpr int kThreads = 384;       // three warps per scheduler: 168 registers
 constexpr int kSumWarps = 8;
-// With 256 hidden rows per tile a sum warp holds 128 sums per thread.  The four warp
-// groups (roles, units, sums, sums) then split the launch's 4 * 128 registers a thread as
-// 80 + 128 + 2 * 152 = 512.
-constexpr int kRoleRegs = 80, kSumRegs = 152;
-constexpr int kItem = 8;            // hidden rows per item at most
-constexpr int kGroup = 2;           // items that a unit warp works on at once
-constexpr int kPitch = 36;          // floats per column of a warp's transposition (conflict-free)
+constexpr int kKsub = 2;            // 64-deep slices per stage
 constexpr int kMaxStages = 12;
 constexpr int kMaxBufs = 4;
-constexpr int kBars = 2 * kMaxStages + 3 * kMaxBufs + 2;
+constexpr int kBars = 2 * kMaxStages + 2 * kMaxBufs;
 constexpr int kSmemMax = 232448;
 // The tensor cores add to an f32 accumulator by truncation, which costs about
 // depth * 2^-30 of the logits' size: 2e-6 over 2048.  The depth is therefore cut into
@@ -316,7 +403,7 @@ constexpr int kSmemMax = 232448;
 constexpr int kPartSteps = 48;
 
 struct GemmArgs {
-    int batch, n_cb, vocab, rows_per_cb, dim, wide;   // wide: n_cb * rows_per_cb of the caller
+    int batch, n_cb, vocab, rows_per_cb, dim;
     int tiles_b, per_cb, n_tiles;
     int nb;                     // hidden rows per tile, a multiple of 16 (32 for a pair)
     int stages, parts, bufs, buf_cols, tmem_cols;
@@ -325,10 +412,9 @@ struct GemmArgs {
     int cfg;
     float cfg_scale;
     const float *row_scale;
-    int rank;
-    const __nv_bfloat16 *B;
-    const float *t;             // [batch][rank]
-    const uint32_t *list;       // [batch] the tiles' rows in order: (adapter << 8) | column
+    const int32_t *which;
+    int rows_per_id, n_adapters;
+    const float *delta;         // rows that name an adapter; may be out
 };
 
 // cap * tanh(l / cap): an odd polynomial (Taylor to y^11) below |y| = 0.35, where its
@@ -347,11 +433,6 @@ __device__ __forceinline__ float softcap_exact(float l, float cap, float inv_cap
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
     const float large = fmaf(-2.0f * cap, r, cap);
     return fabsf(y) < 0.35f ? small : large;
-}
-
-__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v)
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *r)
@@ -382,47 +463,17 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[N])
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// x = hi + mid + lo in bf16, exactly but for bits below 2^-25 of x; two values to a
-// register, the first in the low half.
-__device__ __forceinline__ uint32_t pack_bf16(float x, float y)
-{
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint4 lds_u4(uint32_t a)
-{
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
-{
-    hi = pack_bf16(x, y);
-    x -= __uint_as_float(hi << 16);
-    y -= __uint_as_float(hi & 0xffff0000u);
-    mid = pack_bf16(x, y);
-    x -= __uint_as_float(mid << 16);
-    y -= __uint_as_float(mid & 0xffff0000u);
-    lo = pack_bf16(x, y);
-}
-
-// Threads: four role warps, UNITS unit warps, the sum warps.
-constexpr int threads_of(int units) { return 32 * (4 + units + kSumWarps); }
-
 // CTAS: 2 for a two-SM pair; BM: weight rows per CTA (TMEM lanes; 64 of them lie in the
-// first 16 lanes of each quarter); NB: hidden rows per tile at most; UNITS: unit warps
-// (4 or 8: one or two per lane quarter).
+// first 16 lanes of each quarter); NB: hidden rows per tile at most.
 // A sum warp holds NB / 2 sums per thread.  Nothing may spill: shared memory leaves the
 // L1 so little that a spilled value costs a trip to L2.
-template <int CTAS, int BM, int NB, int UNITS>
-__global__ void __launch_bounds__(threads_of(UNITS), 1)
+template <int CTAS, int BM, int NB>
+__global__ void __launch_bounds__(kThreads, 1)
     adapter_head_kernel(const __grid_constant__ CUtensorMap map_w,
                         const __grid_constant__ CUtensorMap map_h, const __grid_constant__ GemmArgs args)
 {
     constexpr bool PAIR = CTAS == 2;
     constexpr uint32_t kWBytes = BM * kBK * 2;
-    constexpr int kKsub = PAIR ? 1 : 2;                 // 64-deep slices per stage
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -431,13 +482,7 @@ __global__ void __launch_bounds__(threads_of(UNITS), 1)
     const uint32_t stage_bytes = kKsub * sub_bytes;
     const int stages = args.stages, bufs = args.bufs;
     const uint32_t smem0 = smem_u32(smem);
-    // after the stages: the tile's items (16 bytes each) and their number, the unit warps'
-    // transpositions
-    unsigned char *tail = smem + (size_t)stages * stage_bytes;
-    const uint32_t item0 = smem_u32(tail);
-    uint32_t *s_items = reinterpret_cast<uint32_t *>(tail + 16 * NB);
-    float *s_turn = reinterpret_cast<float *>(s_items + 4);   // [UNITS][kGroup * kItem][kPitch]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(s_turn + UNITS * kGroup * kItem * kPitch);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (size_t)stages * stage_bytes);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     __shared__ int s_abort;
 
@@ -449,9 +494,7 @@ __global__ void __launch_bounds__(threads_of(UNITS), 1)
     auto full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
     auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(kMaxStages + s); };
     auto done = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + b); };                  // MMA -> sums
-    auto open = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + kMaxBufs + b); };       // -> MMA
-    auto cleared = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + 2 * kMaxBufs + b); };   // sums -> units
-    const uint32_t ifull = bar0 + 8u * (uint32_t)(2 * kMaxStages + 3 * kMaxBufs), iempty = ifull + 8u;
+    auto open = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + kMaxBufs + b); };   // sums -> MMA
     auto aborted = [&]() { return *(volatile int *)&s_abort != 0; };
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -463,11 +506,8 @@ __global__ void __launch_bounds__(threads_of(UNITS), 1)
         }
         for (int b = 0; b < bufs; b++) {
             mbar_init(done(b), 1);
-            mbar_init(open(b), CTAS * UNITS);
-            mbar_init(cleared(b), kSumWarps);
+            mbar_init(open(b), CTAS * kSumWarps);
         }
-        mbar_init(ifull, 1);
-        mbar_init(iempty, UNITS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         prefetch_map(&map_w);
@@ -496,306 +536,142 @@ __global__ void __launch_bounds__(threads_of(UNITS), 1)
         v0 = (nt - c * args.per_cb) * (BM * CTAS) + (int)rank * BM;
     };
 
-    // The hidden states and W were complete before the kernel that makes t started (it
-    // waits for all work before it), so the roles below use them at once; only the adapter
-    // producer waits for t and the rows' order.
+    // The hidden states and W were complete before the kernels that make delta started
+    // (they wait for all work before them), so they are loaded at once; only the sum warps
+    // wait for delta.
     //
-    // A tile's depth is computed in `parts`, each in the next of `bufs` accumulators.  A
-    // turn (part) may start in an accumulator when the unit warps open it: the sum warps
-    // clear it first, and before a tile's last part the unit warps store B t there.
-    if (warp < 4) {
-        if constexpr (NB == kMaxN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
-        if (warp == 0) {
-            if (lane == 0) {
-                int s = 0, used = 0;
-                uint32_t ph = 0;
-                bool ok = true;
-                const uint32_t full0 = PAIR ? peer_addr(full(0), 0) : full(0);
-                for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
-                    int b0, c, v0;
-                    tile_at(tile, b0, c, v0);
-                    const int w_row = c * args.rows_per_cb + v0, h_row = b0 + (int)rank * nb_own;
-                    for (int kb = 0; kb < KB; kb++) {
-                        if (!mbar_wait(empty(s), ph ^ 1u) || aborted()) {
+    // A tile's depth is computed in `parts`, each in the next of `bufs` accumulators, which
+    // the sum warps open again once they have read it.
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, used = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            const uint32_t full0 = PAIR ? peer_addr(full(0), 0) : full(0);
+            for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
+                int b0, c, v0;
+                tile_at(tile, b0, c, v0);
+                const int w_row = c * args.rows_per_cb + v0, h_row = b0 + (int)rank * nb_own;
+                for (int kb = 0; kb < KB; kb++) {
+                    if (!mbar_wait(empty(s), ph ^ 1u) || aborted()) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t sa = smem0 + (uint32_t)s * stage_bytes, fb = full0 + 8u * (uint32_t)s;
+                    if (rank == 0) mbar_expect_tx(full(s), (uint32_t)CTAS * stage_bytes);
+#pragma unroll
+                    for (int j = 0; j < kKsub; j++) {
+                        const int kx = (kb * kKsub + j) * kBK;
+                        const uint32_t d = sa + (uint32_t)j * sub_bytes;
+                        if (PAIR) {
+                            tma_load_2d_pair(d, &map_w, kx, w_row, fb);
+                            tma_load_2d_pair(d + kWBytes, &map_h, kx, h_row, fb);
+                        } else {
+                            tma_load_2d(d, &map_w, kx, w_row, fb);
+                            tma_load_2d(d + kWBytes, &map_h, kx, h_row, fb);
+                        }
+                    }
+                    used = min(used + 1, stages);
+                    if (++s == stages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                s_abort = 1;
+                if (rank == 0)   // copies still in flight land first
+                    for (int k = 0; k < used; k++) {
+                        if (s == 0) {
+                            s = stages;
+                            ph ^= 1u;
+                        }
+                        s--;
+                        mbar_wait(full(s), ph);
+                    }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(args.nb >> 3) << 17) |
+                                   ((uint32_t)((CTAS * BM) >> 4) << 24);
+            int s = 0, buf = 0;
+            uint32_t ph = 0, bph = 0;
+            bool ok = true;
+            const uint32_t empty1 = PAIR ? peer_addr(empty(0), 1) : 0u, done1 = PAIR ? peer_addr(done(0), 1) : 0u;
+            for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
+                for (int k0 = 0; k0 < KB && ok; k0 += per_part) {   // one part of the depth
+                    const int k1 = min(k0 + per_part, KB);
+                    if (!(PAIR ? mbar_wait_cl(open(buf), bph ^ 1u) : mbar_wait(open(buf), bph ^ 1u))) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t d_tmem = tmem_base + (uint32_t)(buf * args.buf_cols);
+                        for (int kb = k0; kb < k1; kb++) {
+                        if (!(PAIR ? mbar_wait_cl(full(s), ph) : mbar_wait(full(s), ph)) || aborted()) {
                             ok = false;
                             break;
                         }
-                        const uint32_t sa = smem0 + (uint32_t)s * stage_bytes, fb = full0 + 8u * (uint32_t)s;
-                        if (rank == 0) mbar_expect_tx(full(s), (uint32_t)CTAS * stage_bytes);
+                        tc_fence_after();
+                        const uint32_t sa = smem0 + (uint32_t)s * stage_bytes;
 #pragma unroll
                         for (int j = 0; j < kKsub; j++) {
-                            const int kx = (kb * kKsub + j) * kBK;
-                            const uint32_t d = sa + (uint32_t)j * sub_bytes;
-                            if (PAIR) {
-                                tma_load_2d_pair(d, &map_w, kx, w_row, fb);
-                                tma_load_2d_pair(d + kWBytes, &map_h, kx, h_row, fb);
-                            } else {
-                                tma_load_2d(d, &map_w, kx, w_row, fb);
-                                tma_load_2d(d + kWBytes, &map_h, kx, h_row, fb);
+                            const uint64_t wd = sw128_desc(sa + (uint32_t)j * sub_bytes);
+                            const uint64_t hd = sw128_desc(sa + (uint32_t)j * sub_bytes + kWBytes);
+#pragma unroll
+                            for (int k = 0; k < kBK / 16; k++) {
+                                const uint32_t more = kb != k0 || (j | k) != 0;
+                                if (PAIR)
+                                    mma_bf16_pair(d_tmem, wd + (uint64_t)(2 * k), hd + (uint64_t)(2 * k), idesc, more);
+                                else
+                                    mma_bf16(d_tmem, wd + (uint64_t)(2 * k), hd + (uint64_t)(2 * k), idesc, more);
                             }
                         }
-                        used = min(used + 1, stages);
+                        if (PAIR) {
+                            mma_commit_pair(empty(s));
+                            mma_commit_pair(empty1 + 8u * (uint32_t)s);
+                        } else {
+                            mma_commit(empty(s));
+                        }
                         if (++s == stages) {
                             s = 0;
                             ph ^= 1u;
                         }
                     }
-                }
-                if (!ok) {
-                    s_abort = 1;
-                    if (rank == 0)   // copies still in flight land first
-                        for (int k = 0; k < used; k++) {
-                            if (s == 0) {
-                                s = stages;
-                                ph ^= 1u;
-                            }
-                            s--;
-                            mbar_wait(full(s), ph);
-                        }
-                }
-            }
-        } else if (warp == 1) {
-            if (lane == 0 && rank == 0) {
-                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(args.nb >> 3) << 17) |
-                                       ((uint32_t)((CTAS * BM) >> 4) << 24);
-                int s = 0, buf = 0;
-                uint32_t ph = 0, bph = 0;
-                bool ok = true;
-                const uint32_t empty1 = PAIR ? peer_addr(empty(0), 1) : 0u, done1 = PAIR ? peer_addr(done(0), 1) : 0u;
-                for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
-                    for (int k0 = 0; k0 < KB && ok; k0 += per_part) {   // one part of the depth
-                        const int k1 = min(k0 + per_part, KB);
-                        if (!(PAIR ? mbar_wait_cl(open(buf), bph) : mbar_wait(open(buf), bph))) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t d_tmem = tmem_base + (uint32_t)(buf * args.buf_cols);
-                        const bool onto = k1 == KB;   // the last part adds to the low-rank product
-                        for (int kb = k0; kb < k1; kb++) {
-                            if (!(PAIR ? mbar_wait_cl(full(s), ph) : mbar_wait(full(s), ph)) || aborted()) {
-                                ok = false;
-                                break;
-                            }
-                            tc_fence_after();
-                            const uint32_t sa = smem0 + (uint32_t)s * stage_bytes;
-#pragma unroll
-                            for (int j = 0; j < kKsub; j++) {
-                                const uint64_t wd = sw128_desc(sa + (uint32_t)j * sub_bytes);
-                                const uint64_t hd = sw128_desc(sa + (uint32_t)j * sub_bytes + kWBytes);
-#pragma unroll
-                                for (int k = 0; k < kBK / 16; k++) {
-                                    const uint32_t more = onto || kb != k0 || (j | k) != 0;
-                                    if (PAIR)
-                                        mma_bf16_pair(d_tmem, wd + (uint64_t)(2 * k), hd + (uint64_t)(2 * k), idesc, more);
-                                    else
-                                        mma_bf16(d_tmem, wd + (uint64_t)(2 * k), hd + (uint64_t)(2 * k), idesc, more);
-                                }
-                            }
-                            if (PAIR) {
-                                mma_commit_pair(empty(s));
-                                mma_commit_pair(empty1 + 8u * (uint32_t)s);
-                            } else {
-                                mma_commit(empty(s));
-                            }
-                            if (++s == stages) {
-                                s = 0;
-                                ph ^= 1u;
-                            }
-                        }
-                        if (ok) {
-                            if (PAIR) {
-                                mma_commit_pair(done(buf));
-                                mma_commit_pair(done1 + 8u * (uint32_t)buf);
-                            } else {
-                                mma_commit(done(buf));
-                            }
-                        }
-                        if (++buf == bufs) {
-                            buf = 0;
-                            bph ^= 1u;
+                    if (ok) {
+                        if (PAIR) {
+                            mma_commit_pair(done(buf));
+                            mma_commit_pair(done1 + 8u * (uint32_t)buf);
+                        } else {
+                            mma_commit(done(buf));
                         }
                     }
-                }
-                if (!ok) s_abort = 1;
-            }
-        } else if (warp == 2) {
-            // ---- items, 16 bytes each: adapter, rows, their columns in a byte each
-            asm volatile("griddepcontrol.wait;" ::: "memory");   // t and the order are complete
-            bool ok = true;
-            uint32_t ph = 0;
-            for (int tile = unit0; tile < args.n_tiles && ok; tile += units, ph ^= 1u) {
-                int b0, c, v0;
-                tile_at(tile, b0, c, v0);
-                const int rows = min(args.nb, args.batch - b0);
-                if (lane == 0) ok = mbar_wait(iempty, ph ^ 1u) && !aborted();
-                __syncwarp();
-                ok = __shfl_sync(kFull, ok, 0);
-                if (!ok) break;
-                int items = 0;
-                for (int p0 = 0; p0 < rows; p0 += 32) {
-                    const int p = p0 + lane, count = min(32, rows - p0);
-                    const uint32_t entry = lane < count ? args.list[b0 + p] : ~0u, key = entry >> 8;
-                    const uint32_t before = __shfl_up_sync(kFull, key, 1);
-                    const bool start = lane < count && (lane % kItem == 0 || key != before);
-                    const uint32_t starts = __ballot_sync(kFull, start);
-                    const uint32_t upto = starts & (0xffffffffu >> (31 - lane));   // starts at or before this lane
-                    const int first = 31 - __clz(upto);
-                    const uint32_t at = item0 + 16u * (uint32_t)(items + __popc(upto) - 1);
-                    if (lane < count)
-                        asm volatile("st.shared.b8 [%0], %1;" ::"r"(at + 8u + (uint32_t)(lane - first)), "r"(entry & 255u) : "memory");
-                    if (start) {
-                        const uint32_t rest = starts >> lane >> 1;
-                        const int len = rest ? __ffs(rest) : count - lane;
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(key), "r"(len) : "memory");
+                    if (++buf == bufs) {
+                        buf = 0;
+                        bph ^= 1u;
                     }
-                    items += __popc(starts);
                 }
-                if (lane == 0) *s_items = (uint32_t)items;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(ifull);
             }
-            if (!ok && lane == 0) s_abort = 1;
-            __syncwarp();
+            if (!ok) s_abort = 1;
         }
-    } else if (warp < 4 + UNITS) {
-        // ---- units: opens the turns' accumulators
+    } else if (warp >= 4) {
+        // ---- sums, softcap, stores
         const int q = warp & 3;             // the TMEM lane quarter this warp may access
-        const int g = lane >> 2, k4 = lane & 3;
-        constexpr int kTiles = BM / 64;     // 16-row tiles of the quarter
-        constexpr int kStride = UNITS / 4 * kGroup;   // items until this warp's next group
-        float *turn_mem = s_turn + (warp - 4) * kGroup * kItem * kPitch;
+        const int half = (warp - 4) >> 2;   // its half of the tile's columns
+        const int row = BM == 64 ? 16 * q + (lane & 15) : 32 * q + lane;
         const uint32_t open0 = PAIR ? peer_addr(open(0), 0) : open(0);
-        int buf = 0, turn = 0;
-        uint32_t bph = 0, iph = 0;
-        bool ok = true;
+        const float cap = args.softcap, inv_cap = 1.0f / cap, k2 = 2.0f * 1.4426950408889634f / cap;
+        const size_t ldo = (size_t)args.n_cb * args.vocab;
+        const int cols = args.nb / 2;       // a multiple of 8
+        int buf = 0;
+        uint32_t bph = 0;
+        bool ok = true, waited = false;
         for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
             int b0, c, v0;
             tile_at(tile, b0, c, v0);
-            // this lane's rows of each adapter's B: mma.sync's rows g and g + 8 of one or two
-            // 16-row tiles; past the codebook any row will do
-            int b_row[kTiles][2];
-#pragma unroll
-            for (int m = 0; m < kTiles; m++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int row = v0 + (BM / 4) * q + 16 * m + 8 * h + g;
-                    b_row[m][h] = (c * args.rows_per_cb + (row < args.vocab ? row : 0)) * args.rank + 4 * k4;
-                }
-            for (int part = 0; part < parts; part++, turn++) {
-                if (turn >= bufs) {   // its sums have been read
-                    ok = mbar_wait(cleared(buf), bph ^ 1u) && !aborted();
-                    ok = __all_sync(kFull, ok);
-                    if (!ok) break;
-                }
-                tc_fence_after();
-                const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * args.buf_cols);
-                if (part == parts - 1) {
-                    ok = mbar_wait(ifull, iph) && !aborted();
-                    ok = __all_sync(kFull, ok);
-                    if (!ok) break;
-                    iph ^= 1u;
-                    const int items = (int)*(volatile uint32_t *)s_items;
-                    // A step is 16 ranks of a group of items; two steps are in flight.  The ranks are
-                    // permuted alike for both operands, so that a lane loads four neighbours: ranks
-                    // 4 k4 .. 4 k4 + 3 of its rows of B, and of the t of each item's row g.
-                    struct Step {
-                        uint2 w[kGroup][kTiles][2];
-                        float4 t[kGroup];
-                    } step[2];
-                    const int item1 = ((warp - 4) >> 2) * kGroup;   // this warp's first group
-                    int fi = item1, fk = 0, left = 0;               // the next step to fetch; steps fetched, not used
-                    auto fetch = [&](Step &s) {
-                        if (fi >= items) return;
-                        left++;
-#pragma unroll
-                        for (int n = 0; n < kGroup; n++) {
-                            const uint4 item = lds_u4(item0 + 16u * (uint32_t)min(fi + n, items - 1));
-                            const bool in = item.x != kNone && fi + n < items && fk + 4 * k4 < args.rank;
-                            const int r = min(g, (int)item.y - 1);
-                            const uint32_t col = (r < 4 ? item.z : item.w) >> (8 * (r & 3)) & 255u;
-                            const __nv_bfloat16 *from = args.B + (size_t)item.x * args.wide * args.rank + fk;
-#pragma unroll
-                            for (int m = 0; m < kTiles; m++)
-#pragma unroll
-                                for (int h = 0; h < 2; h++)
-                                    s.w[n][m][h] = in ? __ldg(reinterpret_cast<const uint2 *>(from + b_row[m][h])) : make_uint2(0u, 0u);
-                            s.t[n] = in ? *reinterpret_cast<const float4 *>(args.t + (size_t)(b0 + (int)col) * args.rank + fk + 4 * k4)
-                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        }
-                        fk += 16;
-                        if (fk >= args.rank) {
-                            fk = 0;
-                            fi += kStride;
-                        }
-                    };
-                    int it = item1, k = 0;    // the step to use
-                    float d[kGroup][kTiles][4] = {};
-                    auto use = [&](const Step &s) {
-                        left--;
-#pragma unroll
-                        for (int n = 0; n < kGroup; n++) {
-                            uint32_t h0, h1, m0, m1, l0, l1;
-                            split3(s.t[n].x, s.t[n].y, h0, m0, l0);
-                            split3(s.t[n].z, s.t[n].w, h1, m1, l1);
-#pragma unroll
-                            for (int m = 0; m < kTiles; m++) {
-                                const uint2 a = s.w[n][m][0], b = s.w[n][m][1];
-                                float e[4] = {};   // steps are summed with rounding to nearest
-                                mma_16816(e, a.x, b.x, a.y, b.y, l0, l1);
-                                mma_16816(e, a.x, b.x, a.y, b.y, m0, m1);
-                                mma_16816(e, a.x, b.x, a.y, b.y, h0, h1);
-#pragma unroll
-                                for (int i = 0; i < 4; i++) d[n][m][i] += e[i];
-                            }
-                        }
-                        k += 16;
-                    };
-                    auto finish = [&]() {   // rows of the tile to lanes, through this warp's shared memory
-#pragma unroll
-                        for (int n = 0; n < kGroup; n++)
-#pragma unroll
-                            for (int m = 0; m < kTiles; m++)
-#pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    turn_mem[(n * kItem + 2 * k4 + (i & 1)) * kPitch + 16 * m + 8 * (i >> 1) + g] = d[n][m][i];
-                                    d[n][m][i] = 0.0f;
-                                }
-                        uint4 item[kGroup];
-#pragma unroll
-                        for (int n = 0; n < kGroup; n++) item[n] = lds_u4(item0 + 16u * (uint32_t)min(it + n, items - 1));
-                        __syncwarp();
-                        float v[kGroup][kItem];
-#pragma unroll
-                        for (int n = 0; n < kGroup; n++)
-#pragma unroll
-                            for (int j = 0; j < kItem; j++) v[n][j] = turn_mem[(n * kItem + j) * kPitch + (BM == 64 ? lane & 15 : lane)];
-#pragma unroll
-                        for (int n = 0; n < kGroup; n++)
-#pragma unroll
-                            for (int j = 0; j < kItem; j++)
-                                if (it + n < items && j < (int)item[n].y)
-                                    tmem_st1(tm + ((j < 4 ? item[n].z : item[n].w) >> (8 * (j & 3)) & 255u), v[n][j]);
-                        __syncwarp();
-                        k = 0;
-                        it += kStride;
-                    };
-                    fetch(step[0]);
-                    fetch(step[1]);
-                    while (left) {
-#pragma unroll
-                        for (int n = 0; n < 2; n++) {
-                            if (!left) break;
-                            use(step[n]);
-                            fetch(step[n]);
-                            if (k >= args.rank) finish();
-                        }
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(iempty);
-                }
-                if (!ok) break;
-                tmem_wait_st();
+            const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(half * cols);
+            auto clear = [&]() {   // the accumulator has been read: open it, go to the next
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
@@ -804,33 +680,6 @@ __global__ void __launch_bounds__(threads_of(UNITS), 1)
                     else
                         mbar_arrive(open(buf));
                 }
-                if (++buf == bufs) {
-                    buf = 0;
-                    bph ^= 1u;
-                }
-            }
-        }
-        if (!ok) s_abort = 1;
-    } else {
-        if constexpr (NB == kMaxN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
-        // ---- sums, softcap, stores
-        const int q = warp & 3;             // the TMEM lane quarter this warp may access
-        const int half = (warp - 4 - UNITS) >> 2;   // its half of the tile's columns
-        const int row = BM == 64 ? 16 * q + (lane & 15) : 32 * q + lane;
-        const float cap = args.softcap, inv_cap = 1.0f / cap, k2 = 2.0f * 1.4426950408889634f / cap;
-        const long long ldo = (long long)args.n_cb * args.vocab;
-        const int cols = args.nb / 2;       // a multiple of 8
-        int buf = 0;
-        uint32_t bph = 0;
-        bool ok = true;
-        for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
-            int b0, c, v0;
-            tile_at(tile, b0, c, v0);
-            const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(half * cols);
-            auto clear = [&]() {   // the accumulator has been read: hand it on, go to the next
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(cleared(buf));
                 if (++buf == bufs) {
                     buf = 0;
                     bph ^= 1u;
@@ -863,21 +712,38 @@ __global__ void __launch_bounds__(threads_of(UNITS), 1)
                 tmem_wait_st();
             }
             if (!ok) break;
+            if (!waited) {
+                asm volatile("griddepcontrol.wait;" ::: "memory");   // delta is complete
+                waited = true;
+            }
             const bool valid = v0 + row < args.vocab && (BM == 128 || lane < 16);
-            float *out = args.out + (size_t)c * args.vocab + v0 + row;
+            const size_t at_n = (size_t)c * args.vocab + v0 + row;
             const uint32_t at = lanes + (uint32_t)(buf * args.buf_cols);
             const int first = b0 + half * cols, end = min(args.batch, first + cols);
             // eight hidden rows at a time, the next eight on their way
-            uint32_t v[8], ahead[8];
-            if (first < end) tmem_ld8(at, ahead);
-            for (int b = first; b < end; b += 8) {
-                tmem_wait(ahead);
+            auto named = [&](int b) {   // which of the eight rows from b on name an adapter
+                bool has = false;
+                if (lane < 8 && b + lane < end) {
+                    const int a = __ldg(args.which + (b + lane) / args.rows_per_id);
+                    has = (unsigned)a < (unsigned)args.n_adapters;
+                }
+                return __ballot_sync(kFull, has);
+            };
+            auto fetch = [&](int b, uint32_t has, uint32_t (&v)[8], float (&d)[8]) {
+                tmem_ld8(at + (uint32_t)(b - first), v);
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = ahead[j];
-                if (b + 8 < end) tmem_ld8(at + (uint32_t)(b + 8 - first), ahead);
+                for (int j = 0; j < 8; j++)
+                    d[j] = (has >> j) & 1u && valid ? args.delta[(size_t)(b + j) * ldo + at_n] : 0.0f;
+            };
+            uint32_t v[8];
+            float d[8];
+            if (first < end) fetch(first, named(first), v, d);
+            for (int b = first; b < end; b += 8) {
+                tmem_wait(v);
                 float l[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) l[j] = __uint_as_float(v[j]);
+                for (int j = 0; j < 8; j++) l[j] = __uint_as_float(v[j]) + d[j];
+                if (b + 8 < end) fetch(b + 8, named(b + 8), v, d);
                 if (args.row_scale) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) l[j] *= __ldg(args.row_scale + min(b + j, args.batch - 1));
@@ -887,24 +753,23 @@ __global__ void __launch_bounds__(threads_of(UNITS), 1)
                     for (int j = 0; j < 8; j++) l[j] = softcap_exact(l[j], cap, inv_cap, k2);
                 }
                 if (!valid) continue;
-                if (!args.cfg && b + 8 <= end) {
-                    float *to = out + (long long)b * ldo;
+                float *to = args.out + (args.cfg ? (size_t)(b >> 1) : (size_t)b) * ldo + at_n;
+                if (args.cfg) {   // rows 2s, 2s + 1 (conditional, unconditional) are neighbours
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2, to += ldo)
+                        if (b + j < end) *to = __fadd_rn(l[j + 1], __fmul_rn(args.cfg_scale, __fsub_rn(l[j], l[j + 1])));
+                } else if (b + 8 <= end) {
 #pragma unroll
                     for (int j = 0; j < 8; j++, to += ldo) *to = l[j];
-                } else if (!args.cfg) {
+                } else {
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (b + j < end) out[(long long)(b + j) * ldo] = l[j];
-                } else {   // rows 2s, 2s + 1 (conditional, unconditional) are neighbours
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2)
-                        if (b + j < end)
-                            out[(long long)((b + j) >> 1) * ldo] =
-                                __fadd_rn(l[j + 1], __fmul_rn(args.cfg_scale, __fsub_rn(l[j], l[j + 1])));
+                    for (int j = 0; j < 8; j++, to += ldo)
+                        if (b + j < end) *to = l[j];
                 }
             }
             clear();
         }
+        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (!ok) s_abort = 1;
     }
 
@@ -922,13 +787,9 @@ __global__ void __launch_bounds__(threads_of(UNITS), 1)
 
 typedef void (*HeadKernel)(CUtensorMap, CUtensorMap, GemmArgs);
 
-enum : int { kSmall = 0, kMedium = 1, kLarge = 2, kShapes = 3 };
-
-HeadKernel head_kernel(int shape)
+HeadKernel head_kernel(bool pair)
 {
-    return shape == kSmall    ? adapter_head_kernel<1, 64, 64, 8>
-           : shape == kMedium ? adapter_head_kernel<2, 128, 128, 4>
-                              : adapter_head_kernel<2, 128, kMaxN, 4>;
+    return pair ? adapter_head_kernel<2, 128, kPairN> : adapter_head_kernel<1, 64, kSmallN>;
 }
 
 // 2-D bf16 tensor map over rows x cols (cols contiguous), box box_cols x box_rows.
@@ -963,12 +824,12 @@ cudaError_t device_info(DeviceInfo *out)
     DeviceInfo &d = info[dev];
     if (!d.ready) {
         e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
-        for (int i = 0; i < kShapes && e == cudaSuccess; i++)
+        for (int i = 0; i < 2 && e == cudaSuccess; i++)
             e = cudaFuncSetAttribute(head_kernel(i), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - 1024);
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(2 * (d.sms / 2)));
-        cfg.blockDim = dim3((unsigned)threads_of(4));
+        cfg.blockDim = dim3(kThreads);
         cfg.dynamicSmemBytes = kSmemMax - 1024;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -976,7 +837,7 @@ cudaError_t device_info(DeviceInfo *out)
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaOccupancyMaxActiveClusters(&d.pairs, head_kernel(kLarge), &cfg);
+        e = cudaOccupancyMaxActiveClusters(&d.pairs, head_kernel(true), &cfg);
         if (e != cudaSuccess) return e;
         if (d.pairs < 1) d.pairs = 1;
         d.ready = true;
@@ -992,7 +853,7 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     const long long wide = (long long)h.n_cb * h.rows_per_cb;
     if (h.dim % 8 != 0 || ad.rank % 8 != 0 || ad.n_adapters > kMaxAdapters ||
         (uintptr_t)h.W % 16 || (uintptr_t)h.hidden % 16 || (uintptr_t)ad.A % 16 ||
-        (uintptr_t)ad.B % 16 || wide * ad.n_adapters > INT_MAX - 1024)
+        (uintptr_t)ad.B % 16 || wide > INT_MAX / 2)
         return cudaErrorNotSupported;
     DeviceInfo dev;
     cudaError_t e = device_info(&dev);
@@ -1006,55 +867,58 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     cfg.attrs = attr;
     cfg.numAttrs = 1;
 
-    // 64 weight rows per CTA up to 64 hidden rows; then pairs of CTAs, with up to 512 rows
-    // in two tiles (every SM gets one) and 256 a tile beyond.
-    const int shape = h.batch <= 64 ? kSmall : h.batch <= 256 ? kMedium : kLarge;
-    const bool pair = shape != kSmall;
-    const int bm = pair ? 128 : 64;         // weight rows per CTA
-    const int m = pair ? 2 * bm : bm;
-    const int n_max = shape == kSmall ? 64 : shape == kMedium ? 128 : kMaxN;
-    int tiles_b = (h.batch + n_max - 1) / n_max;
-    if (pair && tiles_b < 2) tiles_b = 2;
-    const int even = (h.batch + tiles_b - 1) / tiles_b, step = pair ? 32 : 16;
-    const int nb = (even + step - 1) / step * step;
-    tiles_b = (h.batch + nb - 1) / nb;
-
-    const bool many = (long long)h.batch * ad.rank > kFewMost;
+    // ---- order, t, delta
     float *t = static_cast<float *>(ad.work);
-    uint32_t *list = reinterpret_cast<uint32_t *>(t + (size_t)h.batch * ad.rank);
-    int32_t *order = reinterpret_cast<int32_t *>(list + h.batch);
-    DownArgs d{static_cast<const __nv_bfloat16 *>(h.hidden), static_cast<const __nv_bfloat16 *>(ad.A),
-               ad.scale, ad.which, order, h.batch, h.dim, ad.n_adapters, ad.rank, ad.rows_per_id, t, list, nb, 0};
-    if (many) {
-        cfg.gridDim = dim3((unsigned)tiles_b);
-        cfg.blockDim = dim3(kOrderThreads);
-        cfg.dynamicSmemBytes = 2 * sizeof(int) * (size_t)(ad.n_adapters + 1);
-        e = cudaLaunchKernelEx(&cfg, order_rows_kernel, ad.which, h.batch, nb, ad.rows_per_id,
-                               ad.n_adapters, list, order);
-        if (e != cudaSuccess) return e;
+    Order order;
+    order.rows = reinterpret_cast<int32_t *>(t + (size_t)h.batch * ad.rank);
+    order.n_items = order.rows + h.batch;
+    order.items = reinterpret_cast<int2 *>(order.n_items + (h.batch % 2 ? 1 : 2));
+    cfg.gridDim = dim3((unsigned)((h.batch + kOrderThreads - 1) / kOrderThreads));
+    cfg.blockDim = dim3(kOrderThreads);
+    cfg.dynamicSmemBytes = 2 * sizeof(int) * (size_t)(ad.n_adapters + 1);
+    e = cudaLaunchKernelEx(&cfg, order_rows_kernel, ad.which, h.batch, ad.rows_per_id, ad.n_adapters, order);
+    if (e != cudaSuccess) return e;
+    const DownArgs d{static_cast<const __nv_bfloat16 *>(h.hidden), static_cast<const __nv_bfloat16 *>(ad.A),
+                     ad.scale, ad.which, h.batch, h.dim, ad.n_adapters, ad.rank, ad.rows_per_id, t, order};
+    cfg.dynamicSmemBytes = 0;
+    if ((long long)h.batch * ad.rank > kFewMost) {
         cfg.gridDim = dim3((unsigned)((h.batch + kDownRows - 1) / kDownRows), (unsigned)((ad.rank + kDownRank - 1) / kDownRank));
         cfg.blockDim = dim3(32 * kDownWarps);
-        cfg.dynamicSmemBytes = 0;
         e = cudaLaunchKernelEx(&cfg, adapter_down_mma_kernel, d);
     } else {
-        d.down_blocks = (h.batch * ((ad.rank + 3) / 4) + kFewWarps - 1) / kFewWarps;
-        cfg.gridDim = dim3((unsigned)(d.down_blocks + tiles_b));
+        cfg.gridDim = dim3((unsigned)((h.batch * (ad.rank / 4) + kFewWarps - 1) / kFewWarps));
         cfg.blockDim = dim3(32 * kFewWarps);
         e = cudaLaunchKernelEx(&cfg, adapter_down_few_kernel, d);
     }
     if (e != cudaSuccess) return e;
+    float *delta = ad.delta ? ad.delta : h.out;
+    const UpArgs u{static_cast<const __nv_bfloat16 *>(ad.B), t, order, h.batch, h.n_cb, h.vocab, h.rows_per_cb,
+                   ad.rank, ad.n_adapters, ad.which, ad.rows_per_id, delta};
+    const int up_per_cb = (h.vocab + kUpWarps * kUpRows - 1) / (kUpWarps * kUpRows);
+    cfg.gridDim = dim3((unsigned)max_items(h.batch, ad.n_adapters), (unsigned)(h.n_cb * up_per_cb));
+    cfg.blockDim = dim3(32 * kUpWarps);
+    e = cudaLaunchKernelEx(&cfg, adapter_up_kernel, u);
+    if (e != cudaSuccess) return e;
 
+    // ---- the GEMM: 64 weight rows per CTA up to 64 hidden rows; pairs of CTAs beyond, in
+    // two tiles or more (the model's 36 x 256 weight rows then give nearly every SM one)
+    const bool pair = h.batch > kSmallN;
+    const int bm = pair ? 128 : 64;         // weight rows per CTA
+    const int m = pair ? 2 * bm : bm;
+    const int n_max = pair ? kPairN : kSmallN;
     GemmArgs g{};
+    g.tiles_b = (h.batch + n_max - 1) / n_max;
+    if (pair && g.tiles_b < 2) g.tiles_b = 2;
+    const int even = (h.batch + g.tiles_b - 1) / g.tiles_b, step = pair ? 32 : 16;
+    g.nb = (even + step - 1) / step * step;
+    g.tiles_b = (h.batch + g.nb - 1) / g.nb;
     g.batch = h.batch;
-    g.wide = (int)wide;
     // codebooks whose rows follow each other without a gap are one run of rows
-    const bool joined = h.rows_per_cb == h.vocab && wide <= INT_MAX / 2;
+    const bool joined = h.rows_per_cb == h.vocab;
     g.n_cb = joined ? 1 : h.n_cb;
     g.vocab = joined ? (int)wide : h.vocab;
     g.rows_per_cb = joined ? (int)wide : h.rows_per_cb;
     g.dim = h.dim;
-    g.tiles_b = tiles_b;
-    g.nb = nb;
     g.per_cb = (g.vocab + m - 1) / m;
     g.n_tiles = g.tiles_b * g.n_cb * g.per_cb;
     g.softcap = h.softcap;
@@ -1062,14 +926,13 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     g.cfg = h.cfg;
     g.cfg_scale = h.cfg_scale;
     g.row_scale = h.row_scale;
-    g.rank = ad.rank;
-    g.B = static_cast<const __nv_bfloat16 *>(ad.B);
-    g.t = t;
-    g.list = list;
+    g.which = ad.which;
+    g.rows_per_id = ad.rows_per_id;
+    g.n_adapters = ad.n_adapters;
+    g.delta = delta;
     const int nb_own = pair ? g.nb / 2 : g.nb;
-    const int ksub = pair ? 1 : 2;
-    const int stage = ksub * (bm + nb_own) * kBK * 2;
-    const int kb = (h.dim + ksub * kBK - 1) / (ksub * kBK);
+    const int stage = kKsub * (bm + nb_own) * kBK * 2;
+    const int kb = (h.dim + kKsub * kBK - 1) / (kKsub * kBK);
     g.parts = (h.dim / 16 + kPartSteps - 1) / kPartSteps;
     if (g.parts < 1) g.parts = 1;
     g.parts = (kb + (kb + g.parts - 1) / g.parts - 1) / ((kb + g.parts - 1) / g.parts);   // none empty
@@ -1078,19 +941,16 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     if (g.bufs > g.parts + 1) g.bufs = g.parts + 1;
     g.tmem_cols = 32;
     while (g.tmem_cols < g.bufs * g.buf_cols) g.tmem_cols *= 2;
-    // the kernel's shared memory after the stages: items, transpositions, barriers
-    const int unit_warps = shape == kSmall ? 8 : 4;
-    const int fixed = 1024 + 16 * n_max + 16 + 4 * unit_warps * kGroup * kItem * kPitch + 8 * kBars + 64;
+    const int fixed = 1024 + 8 * kBars + 64;   // alignment, barriers, the TMEM slot
     g.stages = (kSmemMax - 1024 - fixed) / stage;
     if (g.stages > kMaxStages) g.stages = kMaxStages;
-    const size_t smem = (size_t)(g.stages * stage + fixed);
 
     CUtensorMap mw, mh;
     if (!map_2d(&mw, h.W, (uint64_t)wide, (uint64_t)h.dim, (uint32_t)bm, kBK, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !map_2d(&mh, h.hidden, (uint64_t)h.batch, (uint64_t)h.dim, (uint32_t)nb_own, kBK, CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
-    cfg.blockDim = dim3((unsigned)threads_of(unit_warps));
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)(g.stages * stage + fixed);
     if (!pair) {
         cfg.gridDim = dim3((unsigned)(g.n_tiles < dev.sms ? g.n_tiles : dev.sms));
     } else {
@@ -1100,7 +960,7 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
         cfg.numAttrs = 2;
         cfg.gridDim = dim3((unsigned)(2 * (g.n_tiles < dev.pairs ? g.n_tiles : dev.pairs)));
     }
-    return cudaLaunchKernelEx(&cfg, head_kernel(shape), mw, mh, g);
+    return cudaLaunchKernelEx(&cfg, head_kernel(pair), mw, mh, g);
 }
 
 }  // namespace z2
