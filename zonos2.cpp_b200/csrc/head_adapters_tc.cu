@@ -198,7 +198,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 // The depth is permuted alike for both operands, so that every thread loads 16
 // consecutive bytes: of a 32-deep slice, thread q of a quad holds elements 8q ..
 // 8q+7 of its rows, two of them per register of two 16-deep MMAs.
-__global__ void __launch_bounds__(32 * kDownWarps, 2) adapter_down_mma_kernel(const DownArgs g)
+__global__ void __launch_bounds__(32 * kDownWarps, 1) adapter_down_mma_kernel(const DownArgs g)
 {
     __shared__ int s_row[kDownRows], s_key[kDownRows];
     __shared__ float s_sum[kDownWarps][kDownRows][kDownRank + 1];
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(32 * kDownWarps, 2) adapter_down_mma_kernel(co
             for (int i = 0; i < 2; i++)
                 w[i] = g.A + ((size_t)a * g.rank + min(r0 + 8 * i + quad, g.rank - 1)) * g.dim + 8 * q;
             float d[2][2][4] = {};
-#pragma unroll 2
+#pragma unroll 4
             for (int k = 32 * warp; k < g.dim; k += 32 * kDownWarps) {
                 const bool in = k + 8 * q < g.dim;
                 uint4 xv[4], wv[2];
@@ -304,25 +304,28 @@ struct UpArgs {
 };
 
 constexpr int kUpWarps = 4;
-constexpr int kUpRows = 64;        // weight rows per warp: four 16-row tiles
+constexpr int kUpRows = 64;        // weight rows per step of a warp: four 16-row tiles
 constexpr int kUpTiles = kUpRows / 16;
+constexpr int kUpSteps = 4;        // steps per warp
+constexpr int kUpSpan = kUpWarps * kUpRows * kUpSteps;   // weight rows per CTA
 
-// CTA (i, j): item i and kUpWarps * kUpRows weight rows of one codebook; a warp takes
-// kUpRows of them.  mma.sync with the weight rows as M and the item's rows as N; ranks
-// are permuted alike for both operands, so that a lane loads four neighbours (4 k4 ..
-// 4 k4 + 3 of 16) of its rows of B and of the t of row g.
+// CTA (i, j): item i and kUpSpan weight rows of one codebook.  mma.sync with the weight
+// rows as M and the item's rows as N; ranks are permuted alike for both operands, so
+// that a lane loads four neighbours (4 k4 .. 4 k4 + 3 of 16) of its rows of B and of the
+// t of row g.  The result goes through shared memory, so that 128 neighbouring bytes of
+// a row are stored at once.
 // Bound: the store of delta (with 32 adapters, 151 MB for 4096 rows of 9 x 1024).
 __global__ void __launch_bounds__(32 * kUpWarps) adapter_up_kernel(const UpArgs a)
 {
+    __shared__ float s_turn[kUpWarps][kItem][kUpRows + 4];   // rows 4 banks apart: no conflicts
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, k4 = lane & 3;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int items = *a.order.n_items, me = (int)blockIdx.x;
     if (me >= items) return;
     const int2 item = a.order.items[me];
-    const int per_cb = (a.vocab + kUpWarps * kUpRows - 1) / (kUpWarps * kUpRows);
-    const int c = (int)blockIdx.y / per_cb, v0 = ((int)blockIdx.y % per_cb) * kUpWarps * kUpRows + warp * kUpRows;
-    if (v0 >= a.vocab) return;
+    const int per_cb = (a.vocab + kUpSpan - 1) / kUpSpan;
+    const int c = (int)blockIdx.y / per_cb, first = ((int)blockIdx.y % per_cb) * kUpSpan + warp * kUpRows;
     // the item's rows: those of the same adapter from its place on
     int row = -1;
     if (lane < kItem && item.y + lane < a.batch) {
@@ -330,46 +333,52 @@ __global__ void __launch_bounds__(32 * kUpWarps) adapter_up_kernel(const UpArgs 
         if (a.which[row / a.rows_per_id] != item.x) row = -1;
     }
     const int len = __popc(__ballot_sync(kFull, row >= 0));
-    const int row_g = __shfl_sync(kFull, row, min(g, len - 1));
-    float d[kUpTiles][4] = {};
-    const __nv_bfloat16 *base = a.B + ((size_t)item.x * a.n_cb * a.rows_per_cb + (size_t)c * a.rows_per_cb) * a.rank;
-    for (int k = 0; k < a.rank; k += 16) {
-        const bool in = k + 4 * k4 < a.rank;
-        const float4 t = in ? *reinterpret_cast<const float4 *>(a.t + (size_t)row_g * a.rank + k + 4 * k4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        uint2 w[kUpTiles][2];
-#pragma unroll
-        for (int m = 0; m < kUpTiles; m++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int v = min(v0 + 16 * m + 8 * h + g, a.vocab - 1);
-                w[m][h] = in ? __ldg(reinterpret_cast<const uint2 *>(base + (size_t)v * a.rank + k + 4 * k4)) : make_uint2(0u, 0u);
-            }
-        uint32_t h0, h1, m0, m1, l0, l1;
-        split3(t.x, t.y, h0, m0, l0);
-        split3(t.z, t.w, h1, m1, l1);
-#pragma unroll
-        for (int m = 0; m < kUpTiles; m++) {
-            float e[4] = {};   // the tensor cores add by truncation: 16 ranks at a time, then rounded
-            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, l0, l1);
-            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, m0, m1);
-            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, h0, h1);
-#pragma unroll
-            for (int i = 0; i < 4; i++) d[m][i] += e[i];
-        }
-    }
+    const float *t_row = a.t + (size_t)__shfl_sync(kFull, row, min(g, len - 1)) * a.rank + 4 * k4;
+    const __nv_bfloat16 *base = a.B + ((size_t)item.x * a.n_cb * a.rows_per_cb + (size_t)c * a.rows_per_cb) * a.rank + 4 * k4;
     const size_t ldo = (size_t)a.n_cb * a.vocab;
+    for (int step = 0; step < kUpSteps; step++) {
+        const int v0 = first + step * kUpWarps * kUpRows;
+        if (v0 >= a.vocab) break;
+        float d[kUpTiles][4] = {};
+        for (int k = 0; k < a.rank; k += 16) {
+            const bool in = k + 4 * k4 < a.rank;
+            const float4 t = in ? *reinterpret_cast<const float4 *>(t_row + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            uint2 w[kUpTiles][2];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {   // this lane's two rows: 2 k4 and 2 k4 + 1
-        const int r = __shfl_sync(kFull, row, 2 * k4 + i);
-        if (2 * k4 + i >= len) continue;
-        float *to = a.delta + (size_t)r * ldo + (size_t)c * a.vocab;
+            for (int m = 0; m < kUpTiles; m++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int v = min(v0 + 16 * m + 8 * h + g, a.vocab - 1);
+                    w[m][h] = in ? __ldg(reinterpret_cast<const uint2 *>(base + (size_t)v * a.rank + k)) : make_uint2(0u, 0u);
+                }
+            uint32_t h0, h1, m0, m1, l0, l1;
+            split3(t.x, t.y, h0, m0, l0);
+            split3(t.z, t.w, h1, m1, l1);
+#pragma unroll
+            for (int m = 0; m < kUpTiles; m++) {
+                float e[4] = {};   // the tensor cores add by truncation: 16 ranks at a time, then rounded
+                mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, l0, l1);
+                mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, m0, m1);
+                mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, h0, h1);
+#pragma unroll
+                for (int i = 0; i < 4; i++) d[m][i] += e[i];
+            }
+        }
 #pragma unroll
         for (int m = 0; m < kUpTiles; m++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int v = v0 + 16 * m + 8 * h + g;
-                if (v < a.vocab) to[v] = d[m][2 * h + i];
-            }
+            for (int i = 0; i < 4; i++) s_turn[warp][2 * k4 + (i & 1)][16 * m + 8 * (i >> 1) + g] = d[m][i];
+        __syncwarp();
+        float *to = a.delta + (size_t)c * a.vocab + v0 + lane;
+#pragma unroll
+        for (int j = 0; j < kItem; j++) {
+            const size_t r = (size_t)__shfl_sync(kFull, row, j) * ldo;
+            if (j >= len) continue;
+#pragma unroll
+            for (int i = 0; i < kUpRows; i += 32)
+                if (v0 + i + lane < a.vocab) to[r + i] = s_turn[warp][j][i + lane];
+        }
+        __syncwarp();
     }
 }
 
@@ -670,6 +679,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
             int b0, c, v0;
             tile_at(tile, b0, c, v0);
+            const bool valid = v0 + row < args.vocab && (BM == 128 || lane < 16);
+            const size_t at_n = (size_t)c * args.vocab + v0 + row;
+            const int first = b0 + half * cols, end = min(args.batch, first + cols);
+            auto names = [&](int b) {   // whether hidden row b names an adapter
+                if (b >= end) return false;
+                const int a = __ldg(args.which + b / args.rows_per_id);
+                return (unsigned)a < (unsigned)args.n_adapters;
+            };
             const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(half * cols);
             auto clear = [&]() {   // the accumulator has been read: open it, go to the next
                 tc_fence_before();
@@ -690,80 +707,84 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < NB / 2; i++) sum[i] = 0.0f;   // not live from tile to tile
                 for (int part = 0; part < parts; part++) {
+                    const bool last = part == parts - 1;
+                    if (last) {   // delta is complete; this warp's part of it goes towards L2
+                        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+                        waited = true;
+                        if (v0 + BM / 4 * q < args.vocab)
+                            for (int i = lane; i < cols; i += 32)
+                                if (names(first + i))
+                                    asm volatile("prefetch.global.L2 [%0];" ::"l"(args.delta + (size_t)(first + i) * ldo +
+                                                                                  (size_t)c * args.vocab + v0 + BM / 4 * q));
+                    }
                     ok = mbar_wait(done(buf), bph) && !aborted();
                     ok = __all_sync(kFull, ok);
                     if (!ok) break;
                     tc_fence_after();
                     if (parts == 1) break;
                     const uint32_t at = lanes + (uint32_t)(buf * args.buf_cols);
-                    const bool last = part == parts - 1;
 #pragma unroll
-                    for (int g = 0; g < NB / 2; g += 8) {
+                    for (int g = 0; g < NB / 2; g += 16) {
                         if (g >= cols) continue;
-                        uint32_t v[8];
+                        uint32_t v[16];
                         tmem_ld8(at + (uint32_t)g, v);
+                        if (g + 8 < cols) tmem_ld8(at + (uint32_t)(g + 8), v + 8);
                         tmem_wait(v);
 #pragma unroll
-                        for (int j = 0; j < 8; j++) sum[g + j] += __uint_as_float(v[j]);
-                        if (last) tmem_st8(at + (uint32_t)g, sum + g);
+                        for (int j = 0; j < 16; j++) sum[g + j] += __uint_as_float(v[j]);
+                        if (last) {
+                            tmem_st8(at + (uint32_t)g, sum + g);
+                            if (g + 8 < cols) tmem_st8(at + (uint32_t)(g + 8), sum + g + 8);
+                        }
                     }
                     if (!last) clear();
                 }
                 tmem_wait_st();
             }
             if (!ok) break;
-            if (!waited) {
-                asm volatile("griddepcontrol.wait;" ::: "memory");   // delta is complete
-                waited = true;
-            }
-            const bool valid = v0 + row < args.vocab && (BM == 128 || lane < 16);
-            const size_t at_n = (size_t)c * args.vocab + v0 + row;
             const uint32_t at = lanes + (uint32_t)(buf * args.buf_cols);
-            const int first = b0 + half * cols, end = min(args.batch, first + cols);
-            // eight hidden rows at a time, the next eight on their way
-            auto named = [&](int b) {   // which of the eight rows from b on name an adapter
-                bool has = false;
-                if (lane < 8 && b + lane < end) {
-                    const int a = __ldg(args.which + (b + lane) / args.rows_per_id);
-                    has = (unsigned)a < (unsigned)args.n_adapters;
-                }
-                return __ballot_sync(kFull, has);
-            };
-            auto fetch = [&](int b, uint32_t has, uint32_t (&v)[8], float (&d)[8]) {
-                tmem_ld8(at + (uint32_t)(b - first), v);
+            uint32_t named[4] = {};
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    d[j] = (has >> j) & 1u && valid ? args.delta[(size_t)(b + j) * ldo + at_n] : 0.0f;
+            for (int i = 0; i < NB / 2; i += 32) named[i / 32] = __ballot_sync(kFull, i + lane < cols && names(first + i + lane));
+            // sixteen hidden rows at a time, the next sixteen on their way
+            auto fetch = [&](int b, uint32_t (&v)[16], float (&d)[16]) {
+                const int i = b - first;
+                tmem_ld8(at + (uint32_t)i, v);
+                if (i + 8 < cols) tmem_ld8(at + (uint32_t)(i + 8), v + 8);
+                const uint32_t has = (i < 32 ? named[0] : i < 64 ? named[1] : i < 96 ? named[2] : named[3]) >> (i & 31);
+                const float *from = args.delta + (size_t)b * ldo + at_n;
+#pragma unroll
+                for (int j = 0; j < 16; j++, from += ldo) d[j] = (has >> j) & 1u && valid ? *from : 0.0f;
             };
-            uint32_t v[8];
-            float d[8];
-            if (first < end) fetch(first, named(first), v, d);
-            for (int b = first; b < end; b += 8) {
+            uint32_t v[16];
+            float d[16];
+            if (first < end) fetch(first, v, d);
+            for (int b = first; b < end; b += 16) {
                 tmem_wait(v);
-                float l[8];
+                float l[16];
 #pragma unroll
-                for (int j = 0; j < 8; j++) l[j] = __uint_as_float(v[j]) + d[j];
-                if (b + 8 < end) fetch(b + 8, named(b + 8), v, d);
+                for (int j = 0; j < 16; j++) l[j] = __uint_as_float(v[j]) + d[j];
+                if (b + 16 < end) fetch(b + 16, v, d);
                 if (args.row_scale) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) l[j] *= __ldg(args.row_scale + min(b + j, args.batch - 1));
+                    for (int j = 0; j < 16; j++) l[j] *= __ldg(args.row_scale + min(b + j, args.batch - 1));
                 }
-                if (cap > 0.0f) {   // (no branch per column: the eight chains overlap)
+                if (cap > 0.0f) {   // (no branch per column: the chains overlap)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) l[j] = softcap_exact(l[j], cap, inv_cap, k2);
+                    for (int j = 0; j < 16; j++) l[j] = softcap_exact(l[j], cap, inv_cap, k2);
                 }
                 if (!valid) continue;
                 float *to = args.out + (args.cfg ? (size_t)(b >> 1) : (size_t)b) * ldo + at_n;
                 if (args.cfg) {   // rows 2s, 2s + 1 (conditional, unconditional) are neighbours
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2, to += ldo)
+                    for (int j = 0; j < 16; j += 2, to += ldo)
                         if (b + j < end) *to = __fadd_rn(l[j + 1], __fmul_rn(args.cfg_scale, __fsub_rn(l[j], l[j + 1])));
-                } else if (b + 8 <= end) {
+                } else if (b + 16 <= end) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++, to += ldo) *to = l[j];
+                    for (int j = 0; j < 16; j++, to += ldo) *to = l[j];
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; j++, to += ldo)
+                    for (int j = 0; j < 16; j++, to += ldo)
                         if (b + j < end) *to = l[j];
                 }
             }
@@ -894,7 +915,7 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     float *delta = ad.delta ? ad.delta : h.out;
     const UpArgs u{static_cast<const __nv_bfloat16 *>(ad.B), t, order, h.batch, h.n_cb, h.vocab, h.rows_per_cb,
                    ad.rank, ad.n_adapters, ad.which, ad.rows_per_id, delta};
-    const int up_per_cb = (h.vocab + kUpWarps * kUpRows - 1) / (kUpWarps * kUpRows);
+    const int up_per_cb = (h.vocab + kUpSpan - 1) / kUpSpan;
     cfg.gridDim = dim3((unsigned)max_items(h.batch, ad.n_adapters), (unsigned)(h.n_cb * up_per_cb));
     cfg.blockDim = dim3(32 * kUpWarps);
     e = cudaLaunchKernelEx(&cfg, adapter_up_kernel, u);
