@@ -426,22 +426,41 @@ struct GemmArgs {
     const float *delta;         // rows that name an adapter; may be out
 };
 
-// cap * tanh(l / cap): an odd polynomial (Taylor to y^11) below |y| = 0.35, where its
-// remainder is under 2e-8 of the value, and cap - 2 cap / (exp(2 y) + 1) above, whose
-// rounding (a few 2^-24 of cap) is small against the value there.
-__device__ __forceinline__ float softcap_exact(float l, float cap, float inv_cap, float k2)
+// cap * tanh(l / cap) of N values: an odd polynomial (Taylor to y^11) below |y| = 0.35,
+// where its remainder is under 2e-8 of the value, and cap - 2 cap / (exp(2 y) + 1) above,
+// whose rounding (a few 2^-24 of cap) is small against the value there.  Where all of the
+// warp's values are small, as an output head's mostly are, only the polynomial is
+// computed, two values to an instruction.
+template <int N>
+__device__ __forceinline__ void softcap_exact(float (&l)[N], float cap)
 {
-    const float y = l * inv_cap, z = y * y;
-    float p = fmaf(z, -1382.0f / 155925.0f, 62.0f / 2835.0f);
-    p = fmaf(z, p, -17.0f / 315.0f);
-    p = fmaf(z, p, 2.0f / 15.0f);
-    p = fmaf(z, p, -1.0f / 3.0f);
-    const float small = fmaf(l * z, p, l);
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(l * k2));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
-    const float large = fmaf(-2.0f * cap, r, cap);
-    return fabsf(y) < 0.35f ? small : large;
+    const float inv_cap = 1.0f / cap;
+    float most = fabsf(l[0]);
+#pragma unroll
+    for (int i = 1; i < N; i++) most = fmaxf(most, fabsf(l[i]));
+    const bool tiny = __all_sync(kFull, most * inv_cap < 0.35f);
+    const float k2 = 2.0f * 1.4426950408889634f * inv_cap;
+    auto both = [](float x) { return make_float2(x, x); };
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float2 x = make_float2(l[i], l[i + 1]), y = __fmul2_rn(x, both(inv_cap)), z = __fmul2_rn(y, y);
+        float2 p = __ffma2_rn(z, both(-1382.0f / 155925.0f), both(62.0f / 2835.0f));
+        p = __ffma2_rn(z, p, both(-17.0f / 315.0f));
+        p = __ffma2_rn(z, p, both(2.0f / 15.0f));
+        p = __ffma2_rn(z, p, both(-1.0f / 3.0f));
+        p = __ffma2_rn(__fmul2_rn(x, z), p, x);
+        if (!tiny) {
+            float e0, e1, r0, r1;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(x.x * k2));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(x.y * k2));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(e0 + 1.0f));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(e1 + 1.0f));
+            if (!(fabsf(y.x) < 0.35f)) p.x = fmaf(-2.0f * cap, r0, cap);
+            if (!(fabsf(y.y) < 0.35f)) p.y = fmaf(-2.0f * cap, r1, cap);
+        }
+        l[i] = p.x;
+        l[i + 1] = p.y;
+    }
 }
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *r)
@@ -471,6 +490,16 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[N])
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// *p, or 0 without the load; a predicate, not a branch, so that a run of these is in
+// flight together.
+__device__ __forceinline__ float load_if(const float *p, bool yes)
+{
+    float v;
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@q ld.global.f32 %0, [%1];\n\t}"
+                 : "=f"(v) : "l"(p), "r"((uint32_t)yes) : "memory");
+    return v;
+}
 
 // CTAS: 2 for a two-SM pair; BM: weight rows per CTA (TMEM lanes; 64 of them lie in the
 // first 16 lanes of each quarter); NB: hidden rows per tile at most.
@@ -670,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int half = (warp - 4) >> 2;   // its half of the tile's columns
         const int row = BM == 64 ? 16 * q + (lane & 15) : 32 * q + lane;
         const uint32_t open0 = PAIR ? peer_addr(open(0), 0) : open(0);
-        const float cap = args.softcap, inv_cap = 1.0f / cap, k2 = 2.0f * 1.4426950408889634f / cap;
+        const float cap = args.softcap;
         const size_t ldo = (size_t)args.n_cb * args.vocab;
         const int cols = args.nb / 2;       // a multiple of 8
         int buf = 0;
@@ -693,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) {
                     if (PAIR)
-                        mbar_arrive_cluster(open0 + 8u * (uint32_t)buf);
+                        mbar_arrive_cluster_relaxed(open0 + 8u * (uint32_t)buf);
                     else
                         mbar_arrive(open(buf));
                 }
@@ -754,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t has = (i < 32 ? named[0] : i < 64 ? named[1] : i < 96 ? named[2] : named[3]) >> (i & 31);
                 const float *from = args.delta + (size_t)b * ldo + at_n;
 #pragma unroll
-                for (int j = 0; j < 16; j++, from += ldo) d[j] = (has >> j) & 1u && valid ? *from : 0.0f;
+                for (int j = 0; j < 16; j++, from += ldo) d[j] = load_if(from, (has >> j) & 1u && valid);
             };
             uint32_t v[16];
             float d[16];
@@ -769,10 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 16; j++) l[j] *= __ldg(args.row_scale + min(b + j, args.batch - 1));
                 }
-                if (cap > 0.0f) {   // (no branch per column: the chains overlap)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) l[j] = softcap_exact(l[j], cap, inv_cap, k2);
-                }
+                if (cap > 0.0f) softcap_exact(l, cap);
                 if (!valid) continue;
                 float *to = args.out + (args.cfg ? (size_t)(b >> 1) : (size_t)b) * ldo + at_n;
                 if (args.cfg) {   // rows 2s, 2s + 1 (conditional, unconditional) are neighbours
