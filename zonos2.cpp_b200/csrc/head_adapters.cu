@@ -116,8 +116,9 @@ size_t adapter_work_bytes(bool bf16, int batch, int rank)
 {
     const size_t t = (size_t)batch * (size_t)rank;
     // beside t (a multiple of 8 ranks), the tensor-core path keeps the rows' order and its
-    // items: at most batch + 2 + 2 (batch / 8 + batch) words, 3.25 batch + 2
-    return !bf16 ? 8 * t : rank % 8 == 0 ? 4 * (t + 4 * (size_t)batch) : 4 * t;
+    // items: batch + 3 words, and two for each of at most batch / 8 + batch items
+    const size_t b = (size_t)batch;
+    return !bf16 ? 8 * t : rank % 8 == 0 ? 4 * (t + b + 3 + 2 * (b / 8 + b)) : 4 * t;
 }
 
 cudaError_t launch_head_adapters(const HeadArgs &h, const AdapterArgs &ad, bool bf16,

@@ -2,24 +2,25 @@
 // cores (sm_100a):
 //
 //     t[b]         = s_a * (A_a h[b])                     adapter_down_*_kernel
-//     delta[b, n]  = B_a[n] . t[b]                        adapter_up_kernel
+//     delta[b, n]  = B_a[n] . t[b]
 //     logits[b, n] = softcap(W[n] . h[b] + delta[b, n])   adapter_head_kernel
 //
-// delta goes through the logits' own buffer: the GEMM reads an element, adds it and
-// stores the logit in its place.  The kernels are chained by programmatic dependent
-// launch, and only the GEMM's last step waits for delta, so its main loop covers the
-// small kernels of a batch that fills the SMs once.
+// Up to 64 hidden rows, delta is made inside the GEMM: eight warps of its own put it into
+// the accumulator that the last part of the tile's depth adds to, while W streams in.
+// Beyond, adapter_up_kernel writes it to the logits' own buffer, and the GEMM reads an
+// element, adds it and stores the logit in its place.  The kernels are chained by
+// programmatic dependent launch, and only the steps that need t or delta wait for it, so
+// the GEMM's main loop covers the small kernels of a batch that fills the SMs once.
 //
 // Everything is as good as f32: t enters its MMA as three bf16 parts, which hold all
 // of its 24 bits, and the GEMM's depth is summed in parts (kPartSteps).
 //
-// Measured against keeping delta in the GEMM, for 4096 rows of 32 adapters, rank 16:
-// added in the epilogue on the FMA pipe, t broadcast from shared memory, 0.37-0.54 ms;
-// by mma.sync in four or eight warps beside the main loop into the accumulators,
-// 0.28-0.37 ms (with several adapters in every 256 rows, the warps' latency per adapter
-// exceeds the tile's MMAs); hidden rows gathered by adapter with TMA gather4, 0.54 ms
-// (a quarter of the plain copies' rate).  The separate kernel moves the logits once
-// more through memory, which the compute-bound GEMM hides.
+// Measured (9 x 1024 x 2048, 32 adapters, rank 16, in a graph): delta in the GEMM against
+// the separate kernel 16 / 26 us at 1 row, 27 / 34 at 64, 284 / 224 at 4096: with more than
+// a few rows per SM, the warps' latency per adapter exceeds the tile's MMAs.  Slower still
+// at 4096 rows: added in the epilogue on the FMA pipe, t broadcast from shared memory (16 B
+// per 512 B of register writes), 370-540 us; hidden rows gathered by adapter with TMA
+// gather4 (a quarter of the plain copies' rate), 540 us.
 #include <cuda_bf16.h>
 #include <limits.h>
 #include <math.h>
@@ -34,62 +35,60 @@ int read_and_clear_adapter_error(int *value) { return take_device_error(value); 
 
 namespace {
 
-constexpr int kMaxAdapters = 4096;
+constexpr int kMaxAdapters = 4096;   // below kNone
 constexpr int kItem = 8;   // hidden rows per item at most: rows of one adapter
 
 // ---- the rows' order ---------------------------------------------------------
 
-// Scratch, after t: order[batch], the rows by (adapter, row), those without one last;
-// items[], (adapter, first place in the order) each; their number.
+// Scratch, after t: the rows by (adapter, row), those without an adapter last; and the
+// items, of the adapters and then of the rows without one.
 struct Order {
-    int32_t *rows;
-    int2 *items;
-    int32_t *n_items;
+    int32_t *rows;      // [batch]
+    int32_t *n_items;   // [2]: of the adapters, of all rows
+    int2 *items;        // x: adapter (kNone: none) | rows << 16, y: the first row's place
 };
+constexpr int kNone = 0xffff;
 
 // At most this many items.
-__host__ __device__ __forceinline__ int max_items(int batch, int n_adapters)
+__host__ __device__ constexpr int max_items(int batch, int n_adapters)
 {
-    return batch / kItem + min(batch, n_adapters);
+    return batch / kItem + (batch <= n_adapters ? batch : n_adapters + 1);
 }
 
-constexpr int kOrderThreads = 256;
+constexpr int kOrderRows = 256;   // rows per CTA
+constexpr size_t order_bytes(int n_adapters) { return 2 * sizeof(int) * (size_t)(n_adapters + 1); }
 
-// One CTA per kOrderThreads rows: every CTA counts all rows, ranks its own by counting,
-// and the first lists the items.
-__global__ void __launch_bounds__(kOrderThreads)
-    order_rows_kernel(const int32_t *__restrict__ which, int batch, int rows_per_id, int n_adapters, Order o)
+// CTA `block` of those that order the rows (of at most 256 threads): it counts all rows
+// and ranks its own kOrderRows by counting.  `s_count`: order_bytes() of shared memory.
+__device__ __forceinline__ void order_rows(const int32_t *which, int batch, int rows_per_id, int n, const Order &o,
+                                           int block, int *s_count)
 {
-    extern __shared__ int s_count[];   // [n + 1] rows of each key (n: none), then [n + 1] before this CTA's
-    __shared__ int s_part[2][kOrderThreads / 32];
-    __shared__ __align__(16) int s_key[kOrderThreads];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = n_adapters;
-    const int b0 = (int)blockIdx.x * kOrderThreads, rows = min(kOrderThreads, batch - b0);
-    int *before = s_count + n + 1;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ int s_part[2][8];
+    __shared__ int s_key[kOrderRows];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+    const int b0 = block * kOrderRows, rows = min(kOrderRows, batch - b0);
+    int *s_before = s_count + n + 1;   // rows of each key (n: none) before this CTA's
     auto key_of = [&](int b) {
         const int a = __ldg(which + b / rows_per_id);
         return (unsigned)a < (unsigned)n ? a : n;
     };
-    for (int i = tid; i < 2 * (n + 1); i += kOrderThreads) s_count[i] = 0;
-    const int mine = tid < rows ? key_of(b0 + tid) : INT_MAX;
-    s_key[tid] = mine;
+    for (int i = tid; i < 2 * (n + 1); i += threads) s_count[i] = 0;
+    for (int i = tid; i < kOrderRows; i += threads) s_key[i] = i < rows ? key_of(b0 + i) : -1;
     __syncthreads();
 #pragma unroll 4
-    for (int i = tid; i < batch; i += kOrderThreads) {
+    for (int i = tid; i < batch; i += threads) {
         const int k = key_of(i);
         atomicAdd(&s_count[k], 1);
-        if (i < b0) atomicAdd(&before[k], 1);
+        if (i < b0) atomicAdd(&s_before[k], 1);
     }
     __syncthreads();
     // the first place and the first item of each key
-    const int per = (n + kOrderThreads) / kOrderThreads;
+    const int per = (n + threads) / threads;
     const int a0 = min(tid * per, n + 1), a1 = min(a0 + per, n + 1);
     int own = 0, own_items = 0;
     for (int a = a0; a < a1; a++) {
         own += s_count[a];
-        own_items += a < n ? (s_count[a] + kItem - 1) / kItem : 0;
+        own_items += (s_count[a] + kItem - 1) / kItem;
     }
     int sum = own, sum_items = own_items;
 #pragma unroll
@@ -111,19 +110,35 @@ __global__ void __launch_bounds__(kOrderThreads)
         item += s_part[1][w];
     }
     for (int a = a0; a < a1; a++) {
-        const int c = s_count[a];
-        if (blockIdx.x == 0 && a < n)
-            for (int i = 0; i < c; i += kItem) o.items[item++] = make_int2(a, base + i);
+        const int c = s_count[a], k = (c + kItem - 1) / kItem;
+        if (block == 0) {
+            for (int i = 0; i < k; i++)
+                o.items[item + i] = make_int2((a < n ? a : kNone) | min(kItem, c - i * kItem) << 16, base + i * kItem);
+            if (a == n) {
+                o.n_items[0] = item;
+                o.n_items[1] = item + k;
+            }
+        }
         s_count[a] = base;
         base += c;
+        item += k;
     }
-    if (blockIdx.x == 0 && tid == kOrderThreads - 1) *o.n_items = item;
     __syncthreads();
-    if (tid < rows) {   // the rows with this key before this one
+    for (int i = tid; i < rows; i += threads) {   // after the rows with this key before this one
+        const int mine = s_key[i];
         int same = 0;
-        for (int i = 0; i < tid; i++) same += s_key[i] == mine;
-        o.rows[s_count[mine] + before[mine] + same] = b0 + tid;
+        for (int j = 0; j < i; j++) same += s_key[j] == mine;
+        o.rows[s_count[mine] + s_before[mine] + same] = b0 + i;
     }
+}
+
+__global__ void __launch_bounds__(256)
+    order_rows_kernel(const int32_t *__restrict__ which, int batch, int rows_per_id, int n_adapters, Order o)
+{
+    extern __shared__ int s_count[];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    order_rows(which, batch, rows_per_id, n_adapters, o, (int)blockIdx.x, s_count);
 }
 
 // ---- t = s_a A_a h ---------------------------------------------------------
@@ -135,9 +150,11 @@ struct DownArgs {
     int batch, dim, n_adapters, rank, rows_per_id;
     float *t;                       // [batch][rank]
     Order order;
+    int down_blocks;                // few rows: the blocks after these order the rows
 };
 
-// Few rows: one warp per row and four ranks, which share the row's loads.
+// Few rows: one warp per row and four ranks, which share the row's loads; the last blocks
+// order the rows.
 constexpr int kFewWarps = 4;
 constexpr long long kFewMost = 8192;   // rows x ranks
 
@@ -147,6 +164,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) adapter_down_few_kernel(const 
     const int i = (int)blockIdx.x * kFewWarps + (int)(threadIdx.x >> 5);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if ((int)blockIdx.x >= g.down_blocks) {
+        extern __shared__ int s_count[];
+        order_rows(g.which, g.batch, g.rows_per_id, g.n_adapters, g.order, (int)blockIdx.x - g.down_blocks, s_count);
+        return;
+    }
     if (i >= g.batch * quads) return;
     const int b = i / quads, r0 = 4 * (i % quads);
     const int a = __ldg(g.which + b / g.rows_per_id);
@@ -297,9 +319,7 @@ struct UpArgs {
     const __nv_bfloat16 *B;
     const float *t;                // [batch][rank]
     Order order;
-    int batch, n_cb, vocab, rows_per_cb, rank, n_adapters;
-    const int32_t *which;
-    int rows_per_id;
+    int n_cb, vocab, rows_per_cb, rank;
     float *delta;                  // [batch][n_cb * vocab]
 };
 
@@ -321,20 +341,15 @@ __global__ void __launch_bounds__(32 * kUpWarps) adapter_up_kernel(const UpArgs 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, k4 = lane & 3;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int items = *a.order.n_items, me = (int)blockIdx.x;
+    const int me = (int)blockIdx.x, items = *a.order.n_items;
+    const int2 item = a.order.items[me];   // (the buffer holds gridDim.x of them)
     if (me >= items) return;
-    const int2 item = a.order.items[me];
     const int per_cb = (a.vocab + kUpSpan - 1) / kUpSpan;
     const int c = (int)blockIdx.y / per_cb, first = ((int)blockIdx.y % per_cb) * kUpSpan + warp * kUpRows;
-    // the item's rows: those of the same adapter from its place on
-    int row = -1;
-    if (lane < kItem && item.y + lane < a.batch) {
-        row = a.order.rows[item.y + lane];
-        if (a.which[row / a.rows_per_id] != item.x) row = -1;
-    }
-    const int len = __popc(__ballot_sync(kFull, row >= 0));
-    const float *t_row = a.t + (size_t)__shfl_sync(kFull, row, min(g, len - 1)) * a.rank + 4 * k4;
-    const __nv_bfloat16 *base = a.B + ((size_t)item.x * a.n_cb * a.rows_per_cb + (size_t)c * a.rows_per_cb) * a.rank + 4 * k4;
+    const int adapter = item.x & 0xffff, len = item.x >> 16;
+    const int row = a.order.rows[item.y + min(lane, len - 1)];
+    const float *t_row = a.t + (size_t)__shfl_sync(kFull, row, g) * a.rank + 4 * k4;
+    const __nv_bfloat16 *base = a.B + ((size_t)adapter * a.n_cb * a.rows_per_cb + (size_t)c * a.rows_per_cb) * a.rank + 4 * k4;
     const size_t ldo = (size_t)a.n_cb * a.vocab;
     for (int step = 0; step < kUpSteps; step++) {
         const int v0 = first + step * kUpWarps * kUpRows;
@@ -390,20 +405,29 @@ __global__ void __launch_bounds__(32 * kUpWarps) adapter_up_kernel(const UpArgs 
 // logits of one hidden row are 128 consecutive bytes.
 //   warp 0       TMA producer of the weight and hidden tiles (128-byte swizzle);
 //   warp 1       TMEM allocation, tcgen05.mma (M = 64, or 256 over a two-SM pair);
-//   warps 4..11  the sums of the parts of the depth, delta, softcap, stores (two warps
-//                per TMEM lane quarter, each half of the columns).
+//   warp 2       (UNITS) brings the items to shared memory;
+//   UNITS warps  delta, two items at a time, into the accumulator that the last part adds
+//                to (two warps per TMEM lane quarter);
+//   SUMS warps   the sums of the parts of the depth, delta (no UNITS), softcap, stores (two
+//                or four warps per TMEM lane quarter, each its share of the columns).
 // Every wait is bounded, as in head_tc.cu: a warp whose wait expires sets the error
 // word, stops waiting and copying, and the CTA winds down (copies in flight waited
 // for, TMEM freed).  No TMA load here uses cluster multicast.
 
 constexpr int kBK = 64;             // bf16 elements per 128-byte swizzled row
 constexpr int kSmallN = 64, kPairN = 256;   // hidden rows per tile (TMEM columns) at most
-constexpr int kThreads = 384;       // three warps per scheduler: 168 registers
-constexpr int kSumWarps = 8;
+constexpr int kUnits = 8, kSmallSums = 8, kPairSums = 16;
+// The pair kernel's five warp groups (roles, four of sums) split the launch's 5 * 96
+// registers a thread as 32 + 4 * 112 = 480: nothing may spill, since shared memory leaves
+// the L1 so little that a spilled value costs a trip to L2.
+constexpr int kRoleRegs = 32, kSumRegs = 112;
+constexpr int kGroup = 2;           // items that a unit warp works on at once
+constexpr int kPitch = 36;          // floats per column of a warp's transposition (conflict-free)
+constexpr int threads_of(int units, int sums) { return 32 * (4 + units + sums); }
 constexpr int kKsub = 2;            // 64-deep slices per stage
 constexpr int kMaxStages = 12;
 constexpr int kMaxBufs = 4;
-constexpr int kBars = 2 * kMaxStages + 2 * kMaxBufs;
+constexpr int kBars = 2 * kMaxStages + 3 * kMaxBufs + 1;
 constexpr int kSmemMax = 232448;
 // The tensor cores add to an f32 accumulator by truncation, which costs about
 // depth * 2^-30 of the logits' size: 2e-6 over 2048.  The depth is therefore cut into
@@ -423,7 +447,12 @@ struct GemmArgs {
     const float *row_scale;
     const int32_t *which;
     int rows_per_id, n_adapters;
-    const float *delta;         // rows that name an adapter; may be out
+    const float *delta;         // (no UNITS) rows that name an adapter; may be out
+    int rank;                   // (UNITS)
+    uint32_t b_stride;          // elements of one adapter's B
+    const __nv_bfloat16 *B;
+    const float *t;             // [batch][rank]
+    Order order;
 };
 
 // cap * tanh(l / cap) of N values: an odd polynomial (Taylor to y^11) below |y| = 0.35,
@@ -470,15 +499,17 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *r)
                  : "r"(taddr));
 }
 
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float *v)
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v)
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
-                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
-                 "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
-                 "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
-                 : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
 }
 
+__device__ __forceinline__ uint4 lds_u4(uint32_t a)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
 // Waits for the loads issued so far; their values pass through, so that no use of
 // them moves ahead of the wait.
 template <int N>
@@ -502,11 +533,10 @@ __device__ __forceinline__ float load_if(const float *p, bool yes)
 }
 
 // CTAS: 2 for a two-SM pair; BM: weight rows per CTA (TMEM lanes; 64 of them lie in the
-// first 16 lanes of each quarter); NB: hidden rows per tile at most.
-// A sum warp holds NB / 2 sums per thread.  Nothing may spill: shared memory leaves the
-// L1 so little that a spilled value costs a trip to L2.
-template <int CTAS, int BM, int NB>
-__global__ void __launch_bounds__(kThreads, 1)
+// first 16 lanes of each quarter); NB: hidden rows per tile at most; UNITS: unit warps (a
+// kernel with one tile of hidden rows), or 0; SUMS: sum warps.
+template <int CTAS, int BM, int NB, int UNITS, int SUMS>
+__global__ void __launch_bounds__(threads_of(UNITS, SUMS), 1)
     adapter_head_kernel(const __grid_constant__ CUtensorMap map_w,
                         const __grid_constant__ CUtensorMap map_h, const __grid_constant__ GemmArgs args)
 {
@@ -520,7 +550,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t stage_bytes = kKsub * sub_bytes;
     const int stages = args.stages, bufs = args.bufs;
     const uint32_t smem0 = smem_u32(smem);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (size_t)stages * stage_bytes);
+    // after the stages: (UNITS) the items (16 bytes each) and their number, the unit warps'
+    // transpositions
+    unsigned char *tail = smem + (size_t)stages * stage_bytes;
+    const uint32_t item0 = smem_u32(tail);
+    int *s_items = reinterpret_cast<int *>(tail + 16 * max_items(NB, NB));
+    float *s_turn = reinterpret_cast<float *>(s_items + 4);   // [UNITS][kGroup * kItem][kPitch]
+    uint64_t *bars = UNITS ? reinterpret_cast<uint64_t *>(s_turn + UNITS * kGroup * kItem * kPitch)
+                           : reinterpret_cast<uint64_t *>(tail);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     __shared__ int s_abort;
 
@@ -532,7 +569,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
     auto empty = [&](int s) { return bar0 + 8u * (uint32_t)(kMaxStages + s); };
     auto done = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + b); };                  // MMA -> sums
-    auto open = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + kMaxBufs + b); };   // sums -> MMA
+    auto open = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + kMaxBufs + b); };   // -> MMA
+    auto cleared = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + 2 * kMaxBufs + b); };   // (UNITS) sums -> units
+    const uint32_t ifull = bar0 + 8u * (uint32_t)(2 * kMaxStages + 3 * kMaxBufs);
     auto aborted = [&]() { return *(volatile int *)&s_abort != 0; };
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -544,8 +583,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < bufs; b++) {
             mbar_init(done(b), 1);
-            mbar_init(open(b), CTAS * kSumWarps);
+            mbar_init(open(b), UNITS ? UNITS : CTAS * SUMS);
+            mbar_init(cleared(b), SUMS);
         }
+        mbar_init(ifull, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         prefetch_map(&map_w);
@@ -575,11 +616,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     // The hidden states and W were complete before the kernels that make delta started
-    // (they wait for all work before them), so they are loaded at once; only the sum warps
-    // wait for delta.
+    // (they wait for all work before them), so they are loaded at once; only the sum or the
+    // unit warps wait for delta or t.
     //
-    // A tile's depth is computed in `parts`, each in the next of `bufs` accumulators, which
-    // the sum warps open again once they have read it.
+    // A tile's depth is computed in `parts`, each in the next of `bufs` accumulators.  The sum
+    // warps open an accumulator again once they have read it; with UNITS they only clear it,
+    // and the unit warps open it, after storing delta there before a tile's last part.
+    if constexpr (PAIR) {
+        if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
+    }
     if (warp == 0) {
         if (lane == 0) {
             int s = 0, used = 0;
@@ -640,13 +685,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
                 for (int k0 = 0; k0 < KB && ok; k0 += per_part) {   // one part of the depth
                     const int k1 = min(k0 + per_part, KB);
-                    if (!(PAIR ? mbar_wait_cl(open(buf), bph ^ 1u) : mbar_wait(open(buf), bph ^ 1u))) {
+                    if (!(PAIR ? mbar_wait_cl(open(buf), bph ^ 1u) : mbar_wait(open(buf), UNITS ? bph : bph ^ 1u))) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + (uint32_t)(buf * args.buf_cols);
-                        for (int kb = k0; kb < k1; kb++) {
+                        const bool onto = UNITS && k1 == KB;   // the last part adds to delta
+                    for (int kb = k0; kb < k1; kb++) {
                         if (!(PAIR ? mbar_wait_cl(full(s), ph) : mbar_wait(full(s), ph)) || aborted()) {
                             ok = false;
                             break;
@@ -659,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint64_t hd = sw128_desc(sa + (uint32_t)j * sub_bytes + kWBytes);
 #pragma unroll
                             for (int k = 0; k < kBK / 16; k++) {
-                                const uint32_t more = kb != k0 || (j | k) != 0;
+                                const uint32_t more = onto || kb != k0 || (j | k) != 0;
                                 if (PAIR)
                                     mma_bf16_pair(d_tmem, wd + (uint64_t)(2 * k), hd + (uint64_t)(2 * k), idesc, more);
                                 else
@@ -693,15 +739,178 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!ok) s_abort = 1;
         }
-    } else if (warp >= 4) {
+    } else if (UNITS && warp == 2) {
+        // ---- items, 16 bytes each: the adapter, -, eight columns (the last one repeated)
+        asm volatile("griddepcontrol.wait;" ::: "memory");   // t and the order are complete
+        const int items = args.order.n_items[1];
+        for (int i = lane; i < items; i += 32) {
+            const int2 item = args.order.items[i];
+            const int len = item.x >> 16;
+            uint32_t col[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < kItem; j++)
+                col[j >> 2] |= (uint32_t)args.order.rows[item.y + min(j, len - 1)] << (8 * (j & 3));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(item0 + 16u * (uint32_t)i), "r"(item.x & 0xffff), "r"(0),
+                         "r"(col[0]), "r"(col[1])
+                         : "memory");
+        }
+        if (lane == 0) *s_items = items;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ifull);
+    } else if (UNITS && warp >= 4 && warp < 4 + UNITS) {
+        // ---- units: opens the turns' accumulators
+        const int q = warp & 3;             // the TMEM lane quarter this warp may access
+        const int g = lane >> 2, k4 = lane & 3;
+        constexpr int kTiles = BM / 64;     // 16-row tiles of the quarter
+        constexpr int kStride = UNITS / 4 * kGroup;   // items until this warp's next group
+        float *turn_mem = s_turn + (warp - 4) * kGroup * kItem * kPitch;
+        int buf = 0, turn = 0;
+        uint32_t bph = 0;
+        bool ok = true;
+        for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
+            int b0, c, v0;
+            tile_at(tile, b0, c, v0);
+            // this lane's rows of each adapter's B: mma.sync's rows g and g + 8 of one or two
+            // 16-row tiles; past the codebook any row will do
+            int b_row[kTiles][2];
+#pragma unroll
+            for (int m = 0; m < kTiles; m++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int row = v0 + (BM / 4) * q + 16 * m + 8 * h + g;
+                    b_row[m][h] = (c * args.rows_per_cb + (row < args.vocab ? row : 0)) * args.rank + 4 * k4;
+                }
+            for (int part = 0; part < parts; part++, turn++) {
+                if (turn >= bufs) {   // its sums have been read
+                    ok = mbar_wait(cleared(buf), bph ^ 1u) && !aborted();
+                    ok = __all_sync(kFull, ok);
+                    if (!ok) break;
+                }
+                tc_fence_after();
+                const uint32_t tm = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * args.buf_cols);
+                if (part == parts - 1) {
+                    ok = mbar_wait(ifull, 0) && !aborted();   // once: every tile has the same rows
+                    ok = __all_sync(kFull, ok);
+                    if (!ok) break;
+                    const int items = *(volatile int *)s_items;
+                    // A step is 16 ranks of a group of items; two steps are in flight.  The ranks are
+                    // permuted alike for both operands, so that a lane loads four neighbours: ranks
+                    // 4 k4 .. 4 k4 + 3 of its rows of B, and of the t of each item's row g.
+                    struct Step {
+                        uint2 w[kGroup][kTiles][2];
+                        float4 t[kGroup];
+                    } step[2];
+                    const int item1 = ((warp - 4) >> 2) * kGroup;   // this warp's first group
+                    int fi = item1, fk = 0, left = 0;               // the next step to fetch; steps fetched, not used
+                    auto fetch = [&](Step &s) {
+                        if (fi >= items) return;
+                        left++;
+#pragma unroll
+                        for (int n = 0; n < kGroup; n++) {
+                            // past the last item: the last one again, with the same result
+                            const uint4 item = lds_u4(item0 + 16u * (uint32_t)min(fi + n, items - 1));
+                            const bool in = item.x != (uint32_t)kNone && fk + 4 * k4 < args.rank;
+                            const uint32_t col = (g < 4 ? item.z : item.w) >> (8 * (g & 3)) & 255u;
+                            const __nv_bfloat16 *from = args.B + (size_t)item.x * args.b_stride + fk;
+#pragma unroll
+                            for (int m = 0; m < kTiles; m++)
+#pragma unroll
+                                for (int h = 0; h < 2; h++)
+                                    s.w[n][m][h] = in ? __ldg(reinterpret_cast<const uint2 *>(from + b_row[m][h])) : make_uint2(0u, 0u);
+                            s.t[n] = in ? *reinterpret_cast<const float4 *>(args.t + (size_t)(b0 + (int)col) * args.rank + fk + 4 * k4)
+                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        }
+                        fk += 16;
+                        if (fk >= args.rank) {
+                            fk = 0;
+                            fi += kStride;
+                        }
+                    };
+                    int it = item1, k = 0;    // the step to use
+                    float d[kGroup][kTiles][4] = {};
+                    auto use = [&](const Step &s) {
+                        left--;
+#pragma unroll
+                        for (int n = 0; n < kGroup; n++) {
+                            uint32_t h0, h1, m0, m1, l0, l1;
+                            split3(s.t[n].x, s.t[n].y, h0, m0, l0);
+                            split3(s.t[n].z, s.t[n].w, h1, m1, l1);
+#pragma unroll
+                            for (int m = 0; m < kTiles; m++) {
+                                const uint2 a = s.w[n][m][0], b = s.w[n][m][1];
+                                float e[4] = {};   // steps are summed with rounding to nearest
+                                mma_16816(e, a.x, b.x, a.y, b.y, l0, l1);
+                                mma_16816(e, a.x, b.x, a.y, b.y, m0, m1);
+                                mma_16816(e, a.x, b.x, a.y, b.y, h0, h1);
+#pragma unroll
+                                for (int i = 0; i < 4; i++) d[n][m][i] += e[i];
+                            }
+                        }
+                        k += 16;
+                    };
+                    auto finish = [&]() {   // rows of the tile to lanes, through this warp's shared memory
+#pragma unroll
+                        for (int n = 0; n < kGroup; n++)
+#pragma unroll
+                            for (int m = 0; m < kTiles; m++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    turn_mem[(n * kItem + 2 * k4 + (i & 1)) * kPitch + 16 * m + 8 * (i >> 1) + g] = d[n][m][i];
+                                    d[n][m][i] = 0.0f;
+                                }
+                        uint4 item[kGroup];
+#pragma unroll
+                        for (int n = 0; n < kGroup; n++) item[n] = lds_u4(item0 + 16u * (uint32_t)min(it + n, items - 1));
+                        __syncwarp();
+                        float v[kGroup][kItem];
+#pragma unroll
+                        for (int n = 0; n < kGroup; n++)
+#pragma unroll
+                            for (int j = 0; j < kItem; j++) v[n][j] = turn_mem[(n * kItem + j) * kPitch + (BM == 64 ? lane & 15 : lane)];
+#pragma unroll
+                        for (int n = 0; n < kGroup; n++)
+#pragma unroll
+                            for (int j = 0; j < kItem; j++)
+                                tmem_st1(tm + ((j < 4 ? item[n].z : item[n].w) >> (8 * (j & 3)) & 255u), v[n][j]);
+                        __syncwarp();
+                        k = 0;
+                        it += kStride;
+                    };
+                    fetch(step[0]);
+                    fetch(step[1]);
+                    while (left) {
+#pragma unroll
+                        for (int n = 0; n < 2; n++) {
+                            if (!left) break;
+                            use(step[n]);
+                            fetch(step[n]);
+                            if (k >= args.rank) finish();
+                        }
+                    }
+                }
+                if (!ok) break;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(open(buf));
+                if (++buf == bufs) {
+                    buf = 0;
+                    bph ^= 1u;
+                }
+            }
+        }
+        if (!ok) s_abort = 1;
+    } else if (warp >= 4 + UNITS) {
+        if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
         // ---- sums, softcap, stores
         const int q = warp & 3;             // the TMEM lane quarter this warp may access
-        const int half = (warp - 4) >> 2;   // its half of the tile's columns
+        const int share = (warp - 4 - UNITS) >> 2;   // its share of the tile's columns
+        constexpr int kShares = SUMS / 4, kCols = NB / kShares;
         const int row = BM == 64 ? 16 * q + (lane & 15) : 32 * q + lane;
         const uint32_t open0 = PAIR ? peer_addr(open(0), 0) : open(0);
         const float cap = args.softcap;
         const size_t ldo = (size_t)args.n_cb * args.vocab;
-        const int cols = args.nb / 2;       // a multiple of 8
+        const int cols = args.nb / kShares;          // a multiple of 8
         int buf = 0;
         uint32_t bph = 0;
         bool ok = true, waited = false;
@@ -710,18 +919,48 @@ __global__ void __launch_bounds__(kThreads, 1)
             tile_at(tile, b0, c, v0);
             const bool valid = v0 + row < args.vocab && (BM == 128 || lane < 16);
             const size_t at_n = (size_t)c * args.vocab + v0 + row;
-            const int first = b0 + half * cols, end = min(args.batch, first + cols);
+            const int first = b0 + share * cols, end = min(args.batch, first + cols);
             auto names = [&](int b) {   // whether hidden row b names an adapter
                 if (b >= end) return false;
                 const int a = __ldg(args.which + b / args.rows_per_id);
                 return (unsigned)a < (unsigned)args.n_adapters;
             };
-            const uint32_t lanes = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(half * cols);
-            auto clear = [&]() {   // the accumulator has been read: open it, go to the next
+            float sum[kCols];
+#pragma unroll
+            for (int i = 0; i < kCols; i++) sum[i] = 0.0f;   // not live from tile to tile
+            for (int part = 0; part < parts; part++) {
+                if (!UNITS && part == parts - 1) {   // delta is complete; this warp's part of it goes towards L2
+                    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+                    waited = true;
+                    if (v0 + BM / 4 * q < args.vocab)
+                        for (int i = lane; i < cols; i += 32)
+                            if (names(first + i))
+                                asm volatile("prefetch.global.L2 [%0];" ::"l"(args.delta + (size_t)(first + i) * ldo +
+                                                                              (size_t)c * args.vocab + v0 + BM / 4 * q));
+                }
+                ok = mbar_wait(done(buf), bph) && !aborted();
+                ok = __all_sync(kFull, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * args.buf_cols + share * cols);
+#pragma unroll
+                for (int g = 0; g < kCols; g += 16) {
+                    if (g >= cols) continue;
+                    uint32_t v[16];
+                    tmem_ld8(at + (uint32_t)g, v);
+                    if (g + 8 < cols) tmem_ld8(at + (uint32_t)(g + 8), v + 8);
+                    tmem_wait(v);
+#pragma unroll
+                    for (int j = 0; j < 16 && g + j < kCols; j++) sum[g + j] += __uint_as_float(v[j]);
+                }
+                // the accumulator has been read: it goes on before the stores below, which wait
+                // for memory
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if (PAIR)
+                    if (UNITS)
+                        mbar_arrive(cleared(buf));
+                    else if (PAIR)
                         mbar_arrive_cluster_relaxed(open0 + 8u * (uint32_t)buf);
                     else
                         mbar_arrive(open(buf));
@@ -730,93 +969,46 @@ __global__ void __launch_bounds__(kThreads, 1)
                     buf = 0;
                     bph ^= 1u;
                 }
-            };
-            {
-                float sum[NB / 2];
-#pragma unroll
-                for (int i = 0; i < NB / 2; i++) sum[i] = 0.0f;   // not live from tile to tile
-                for (int part = 0; part < parts; part++) {
-                    const bool last = part == parts - 1;
-                    if (last) {   // delta is complete; this warp's part of it goes towards L2
-                        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-                        waited = true;
-                        if (v0 + BM / 4 * q < args.vocab)
-                            for (int i = lane; i < cols; i += 32)
-                                if (names(first + i))
-                                    asm volatile("prefetch.global.L2 [%0];" ::"l"(args.delta + (size_t)(first + i) * ldo +
-                                                                                  (size_t)c * args.vocab + v0 + BM / 4 * q));
-                    }
-                    ok = mbar_wait(done(buf), bph) && !aborted();
-                    ok = __all_sync(kFull, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (parts == 1) break;
-                    const uint32_t at = lanes + (uint32_t)(buf * args.buf_cols);
-#pragma unroll
-                    for (int g = 0; g < NB / 2; g += 16) {
-                        if (g >= cols) continue;
-                        uint32_t v[16];
-                        tmem_ld8(at + (uint32_t)g, v);
-                        if (g + 8 < cols) tmem_ld8(at + (uint32_t)(g + 8), v + 8);
-                        tmem_wait(v);
-#pragma unroll
-                        for (int j = 0; j < 16; j++) sum[g + j] += __uint_as_float(v[j]);
-                        if (last) {
-                            tmem_st8(at + (uint32_t)g, sum + g);
-                            if (g + 8 < cols) tmem_st8(at + (uint32_t)(g + 8), sum + g + 8);
-                        }
-                    }
-                    if (!last) clear();
-                }
-                tmem_wait_st();
             }
             if (!ok) break;
-            const uint32_t at = lanes + (uint32_t)(buf * args.buf_cols);
-            uint32_t named[4] = {};
+            // kStep hidden rows at a time
+            constexpr int kStep = 16;
 #pragma unroll
-            for (int i = 0; i < NB / 2; i += 32) named[i / 32] = __ballot_sync(kFull, i + lane < cols && names(first + i + lane));
-            // sixteen hidden rows at a time, the next sixteen on their way
-            auto fetch = [&](int b, uint32_t (&v)[16], float (&d)[16]) {
-                const int i = b - first;
-                tmem_ld8(at + (uint32_t)i, v);
-                if (i + 8 < cols) tmem_ld8(at + (uint32_t)(i + 8), v + 8);
-                const uint32_t has = (i < 32 ? named[0] : i < 64 ? named[1] : i < 96 ? named[2] : named[3]) >> (i & 31);
-                const float *from = args.delta + (size_t)b * ldo + at_n;
+            for (int g = 0; g < kCols; g += kStep) {
+                const int b = first + g;
+                if (g >= cols || b >= end) continue;
+                float l[kStep];
+                if (!UNITS) {
+                    const uint32_t named = __ballot_sync(kFull, lane < kStep && g + lane < cols && names(b + lane));
+                    const float *from = args.delta + (size_t)b * ldo + at_n;
 #pragma unroll
-                for (int j = 0; j < 16; j++, from += ldo) d[j] = load_if(from, (has >> j) & 1u && valid);
-            };
-            uint32_t v[16];
-            float d[16];
-            if (first < end) fetch(first, v, d);
-            for (int b = first; b < end; b += 16) {
-                tmem_wait(v);
-                float l[16];
+                    for (int j = 0; j < kStep; j++, from += ldo) l[j] = load_if(from, (named >> j) & 1u && valid);
+                }
 #pragma unroll
-                for (int j = 0; j < 16; j++) l[j] = __uint_as_float(v[j]) + d[j];
-                if (b + 16 < end) fetch(b + 16, v, d);
+                for (int j = 0; j < kStep; j++) l[j] = UNITS ? sum[g + j] : sum[g + j] + l[j];
                 if (args.row_scale) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) l[j] *= __ldg(args.row_scale + min(b + j, args.batch - 1));
+                    for (int j = 0; j < kStep; j++) l[j] *= __ldg(args.row_scale + min(b + j, args.batch - 1));
                 }
                 if (cap > 0.0f) softcap_exact(l, cap);
                 if (!valid) continue;
+                const int n = min(min(kStep, cols - g), end - b);
                 float *to = args.out + (args.cfg ? (size_t)(b >> 1) : (size_t)b) * ldo + at_n;
                 if (args.cfg) {   // rows 2s, 2s + 1 (conditional, unconditional) are neighbours
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2, to += ldo)
-                        if (b + j < end) *to = __fadd_rn(l[j + 1], __fmul_rn(args.cfg_scale, __fsub_rn(l[j], l[j + 1])));
-                } else if (b + 16 <= end) {
+                    for (int j = 0; j < kStep; j += 2, to += ldo)
+                        if (j < n) *to = __fadd_rn(l[j + 1], __fmul_rn(args.cfg_scale, __fsub_rn(l[j], l[j + 1])));
+                } else if (n == kStep) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++, to += ldo) *to = l[j];
+                    for (int j = 0; j < kStep; j++, to += ldo) *to = l[j];
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; j++, to += ldo)
-                        if (b + j < end) *to = l[j];
+                    for (int j = 0; j < kStep; j++, to += ldo)
+                        if (j < n) *to = l[j];
                 }
             }
-            clear();
         }
-        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (!UNITS && !waited) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (!ok) s_abort = 1;
     }
 
@@ -836,7 +1028,7 @@ typedef void (*HeadKernel)(CUtensorMap, CUtensorMap, GemmArgs);
 
 HeadKernel head_kernel(bool pair)
 {
-    return pair ? adapter_head_kernel<2, 128, kPairN> : adapter_head_kernel<1, 64, kSmallN>;
+    return pair ? adapter_head_kernel<2, 128, kPairN, 0, kPairSums> : adapter_head_kernel<1, 64, kSmallN, kUnits, kSmallSums>;
 }
 
 // 2-D bf16 tensor map over rows x cols (cols contiguous), box box_cols x box_rows.
@@ -876,7 +1068,7 @@ cudaError_t device_info(DeviceInfo *out)
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(2 * (d.sms / 2)));
-        cfg.blockDim = dim3(kThreads);
+        cfg.blockDim = dim3(threads_of(0, kPairSums));
         cfg.dynamicSmemBytes = kSmemMax - 1024;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -900,7 +1092,7 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     const long long wide = (long long)h.n_cb * h.rows_per_cb;
     if (h.dim % 8 != 0 || ad.rank % 8 != 0 || ad.n_adapters > kMaxAdapters ||
         (uintptr_t)h.W % 16 || (uintptr_t)h.hidden % 16 || (uintptr_t)ad.A % 16 ||
-        (uintptr_t)ad.B % 16 || wide > INT_MAX / 2)
+        (uintptr_t)ad.B % 16 || wide * ad.rank > INT_MAX / 2)
         return cudaErrorNotSupported;
     DeviceInfo dev;
     cudaError_t e = device_info(&dev);
@@ -914,42 +1106,46 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     cfg.attrs = attr;
     cfg.numAttrs = 1;
 
-    // ---- order, t, delta
+    // ---- t and the rows' order; delta
+    const bool pair = h.batch > kSmallN;
     float *t = static_cast<float *>(ad.work);
     Order order;
     order.rows = reinterpret_cast<int32_t *>(t + (size_t)h.batch * ad.rank);
-    order.n_items = order.rows + h.batch;
-    order.items = reinterpret_cast<int2 *>(order.n_items + (h.batch % 2 ? 1 : 2));
-    cfg.gridDim = dim3((unsigned)((h.batch + kOrderThreads - 1) / kOrderThreads));
-    cfg.blockDim = dim3(kOrderThreads);
-    cfg.dynamicSmemBytes = 2 * sizeof(int) * (size_t)(ad.n_adapters + 1);
-    e = cudaLaunchKernelEx(&cfg, order_rows_kernel, ad.which, h.batch, ad.rows_per_id, ad.n_adapters, order);
-    if (e != cudaSuccess) return e;
-    const DownArgs d{static_cast<const __nv_bfloat16 *>(h.hidden), static_cast<const __nv_bfloat16 *>(ad.A),
-                     ad.scale, ad.which, h.batch, h.dim, ad.n_adapters, ad.rank, ad.rows_per_id, t, order};
-    cfg.dynamicSmemBytes = 0;
-    if ((long long)h.batch * ad.rank > kFewMost) {
-        cfg.gridDim = dim3((unsigned)((h.batch + kDownRows - 1) / kDownRows), (unsigned)((ad.rank + kDownRank - 1) / kDownRank));
-        cfg.blockDim = dim3(32 * kDownWarps);
-        e = cudaLaunchKernelEx(&cfg, adapter_down_mma_kernel, d);
-    } else {
-        cfg.gridDim = dim3((unsigned)((h.batch * (ad.rank / 4) + kFewWarps - 1) / kFewWarps));
+    order.n_items = order.rows + (h.batch + 1) / 2 * 2;
+    order.items = reinterpret_cast<int2 *>(order.n_items + 2);
+    DownArgs d{static_cast<const __nv_bfloat16 *>(h.hidden), static_cast<const __nv_bfloat16 *>(ad.A),
+               ad.scale, ad.which, h.batch, h.dim, ad.n_adapters, ad.rank, ad.rows_per_id, t, order, 0};
+    const unsigned order_blocks = (unsigned)((h.batch + kOrderRows - 1) / kOrderRows);
+    cfg.dynamicSmemBytes = order_bytes(ad.n_adapters);
+    if ((long long)h.batch * ad.rank <= kFewMost) {
+        d.down_blocks = (h.batch * (ad.rank / 4) + kFewWarps - 1) / kFewWarps;
+        cfg.gridDim = dim3((unsigned)d.down_blocks + order_blocks);
         cfg.blockDim = dim3(32 * kFewWarps);
         e = cudaLaunchKernelEx(&cfg, adapter_down_few_kernel, d);
+    } else {
+        cfg.gridDim = dim3(order_blocks);
+        cfg.blockDim = dim3(256);
+        e = cudaLaunchKernelEx(&cfg, order_rows_kernel, ad.which, h.batch, ad.rows_per_id, ad.n_adapters, order);
+        if (e != cudaSuccess) return e;
+        cfg.gridDim = dim3((unsigned)((h.batch + kDownRows - 1) / kDownRows), (unsigned)((ad.rank + kDownRank - 1) / kDownRank));
+        cfg.blockDim = dim3(32 * kDownWarps);
+        cfg.dynamicSmemBytes = 0;
+        e = cudaLaunchKernelEx(&cfg, adapter_down_mma_kernel, d);
     }
     if (e != cudaSuccess) return e;
     float *delta = ad.delta ? ad.delta : h.out;
-    const UpArgs u{static_cast<const __nv_bfloat16 *>(ad.B), t, order, h.batch, h.n_cb, h.vocab, h.rows_per_cb,
-                   ad.rank, ad.n_adapters, ad.which, ad.rows_per_id, delta};
-    const int up_per_cb = (h.vocab + kUpSpan - 1) / kUpSpan;
-    cfg.gridDim = dim3((unsigned)max_items(h.batch, ad.n_adapters), (unsigned)(h.n_cb * up_per_cb));
-    cfg.blockDim = dim3(32 * kUpWarps);
-    e = cudaLaunchKernelEx(&cfg, adapter_up_kernel, u);
-    if (e != cudaSuccess) return e;
+    if (pair) {
+        const UpArgs u{static_cast<const __nv_bfloat16 *>(ad.B), t, order, h.n_cb, h.vocab, h.rows_per_cb, ad.rank, delta};
+        const int up_per_cb = (h.vocab + kUpSpan - 1) / kUpSpan;
+        cfg.gridDim = dim3((unsigned)max_items(h.batch, ad.n_adapters), (unsigned)(h.n_cb * up_per_cb));
+        cfg.blockDim = dim3(32 * kUpWarps);
+        cfg.dynamicSmemBytes = 0;
+        e = cudaLaunchKernelEx(&cfg, adapter_up_kernel, u);
+        if (e != cudaSuccess) return e;
+    }
 
     // ---- the GEMM: 64 weight rows per CTA up to 64 hidden rows; pairs of CTAs beyond, in
     // two tiles or more (the model's 36 x 256 weight rows then give nearly every SM one)
-    const bool pair = h.batch > kSmallN;
     const int bm = pair ? 128 : 64;         // weight rows per CTA
     const int m = pair ? 2 * bm : bm;
     const int n_max = pair ? kPairN : kSmallN;
@@ -977,6 +1173,11 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     g.rows_per_id = ad.rows_per_id;
     g.n_adapters = ad.n_adapters;
     g.delta = delta;
+    g.rank = ad.rank;
+    g.b_stride = (uint32_t)(wide * ad.rank);
+    g.B = static_cast<const __nv_bfloat16 *>(ad.B);
+    g.t = t;
+    g.order = order;
     const int nb_own = pair ? g.nb / 2 : g.nb;
     const int stage = kKsub * (bm + nb_own) * kBK * 2;
     const int kb = (h.dim + kKsub * kBK - 1) / (kKsub * kBK);
@@ -988,7 +1189,9 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     if (g.bufs > g.parts + 1) g.bufs = g.parts + 1;
     g.tmem_cols = 32;
     while (g.tmem_cols < g.bufs * g.buf_cols) g.tmem_cols *= 2;
-    const int fixed = 1024 + 8 * kBars + 64;   // alignment, barriers, the TMEM slot
+    // beside the stages: alignment, barriers, the TMEM slot, what the unit warps keep
+    const int fixed = 1024 + 8 * kBars + 64 +
+                      (pair ? 0 : 16 * max_items(kSmallN, kSmallN) + 16 + 4 * kUnits * kGroup * kItem * kPitch);
     g.stages = (kSmemMax - 1024 - fixed) / stage;
     if (g.stages > kMaxStages) g.stages = kMaxStages;
 
@@ -996,7 +1199,7 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     if (!map_2d(&mw, h.W, (uint64_t)wide, (uint64_t)h.dim, (uint32_t)bm, kBK, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !map_2d(&mh, h.hidden, (uint64_t)h.batch, (uint64_t)h.dim, (uint32_t)nb_own, kBK, CU_TENSOR_MAP_SWIZZLE_128B))
         return cudaErrorInvalidValue;
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3((unsigned)(pair ? threads_of(0, kPairSums) : threads_of(kUnits, kSmallSums)));
     cfg.dynamicSmemBytes = (size_t)(g.stages * stage + fixed);
     if (!pair) {
         cfg.gridDim = dim3((unsigned)(g.n_tiles < dev.sms ? g.n_tiles : dev.sms));
