@@ -333,8 +333,10 @@ constexpr int kUpSpan = kUpWarps * kUpRows * kUpSteps;   // weight rows per CTA
 // rows as M and the item's rows as N; ranks are permuted alike for both operands, so
 // that a lane loads four neighbours (4 k4 .. 4 k4 + 3 of 16) of its rows of B and of the
 // t of row g.  The result goes through shared memory, so that 128 neighbouring bytes of
-// a row are stored at once.
+// a row are stored at once.  KT: with at most 16 KT ranks, t's parts stay in registers and
+// the next step's rows of B are on their way; 0: any number.
 // Bound: the store of delta (with 32 adapters, 151 MB for 4096 rows of 9 x 1024).
+template <int KT>
 __global__ void __launch_bounds__(32 * kUpWarps) adapter_up_kernel(const UpArgs a)
 {
     __shared__ float s_turn[kUpWarps][kItem][kUpRows + 4];   // rows 4 banks apart: no conflicts
@@ -350,33 +352,59 @@ __global__ void __launch_bounds__(32 * kUpWarps) adapter_up_kernel(const UpArgs 
     const int row = a.order.rows[item.y + min(lane, len - 1)];
     const float *t_row = a.t + (size_t)__shfl_sync(kFull, row, g) * a.rank + 4 * k4;
     const __nv_bfloat16 *base = a.B + ((size_t)adapter * a.n_cb * a.rows_per_cb + (size_t)c * a.rows_per_cb) * a.rank + 4 * k4;
-    const size_t ldo = (size_t)a.n_cb * a.vocab;
+    const uint32_t ldo = (uint32_t)(a.n_cb * a.vocab);
+    uint32_t to_row[kItem];
+#pragma unroll
+    for (int j = 0; j < kItem; j++) to_row[j] = (uint32_t)__shfl_sync(kFull, row, j);
+
+    struct Parts {   // t's parts of 16 ranks, as the MMA's B
+        uint32_t h[2], m[2], l[2];
+    };
+    auto parts = [&](int k, Parts &p) {
+        const float4 t = k + 4 * k4 < a.rank ? *reinterpret_cast<const float4 *>(t_row + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        split3(t.x, t.y, p.h[0], p.m[0], p.l[0]);
+        split3(t.z, t.w, p.h[1], p.m[1], p.l[1]);
+    };
+    auto rows_of_b = [&](int v0, int k, uint2 (&w)[kUpTiles][2]) {
+        const bool in = k + 4 * k4 < a.rank && v0 < a.vocab;
+        const __nv_bfloat16 *from = base + (uint32_t)((v0 + g) * a.rank + k);
+#pragma unroll
+        for (int i = 0; i < 2 * kUpTiles; i++, from += 8 * a.rank)
+            w[i >> 1][i & 1] = in && v0 + 8 * i + g < a.vocab ? __ldg(reinterpret_cast<const uint2 *>(from)) : make_uint2(0u, 0u);
+    };
+    auto multiply = [&](const uint2 (&w)[kUpTiles][2], const Parts &p, float (&d)[kUpTiles][4], bool add) {
+#pragma unroll
+        for (int m = 0; m < kUpTiles; m++) {
+            float e[4] = {};   // the tensor cores add by truncation: 16 ranks at a time, then rounded
+            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, p.l[0], p.l[1]);
+            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, p.m[0], p.m[1]);
+            mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, p.h[0], p.h[1]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[m][i] = add ? d[m][i] + e[i] : e[i];
+        }
+    };
+    Parts kept[KT ? KT : 1];
+    uint2 w[KT ? KT : 1][kUpTiles][2];
+#pragma unroll
+    for (int k = 0; k < KT; k++) {
+        rows_of_b(first, 16 * k, w[k]);
+        parts(16 * k, kept[k]);
+    }
     for (int step = 0; step < kUpSteps; step++) {
         const int v0 = first + step * kUpWarps * kUpRows;
         if (v0 >= a.vocab) break;
-        float d[kUpTiles][4] = {};
-        for (int k = 0; k < a.rank; k += 16) {
-            const bool in = k + 4 * k4 < a.rank;
-            const float4 t = in ? *reinterpret_cast<const float4 *>(t_row + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            uint2 w[kUpTiles][2];
+        float d[kUpTiles][4];
+        if (KT) {
 #pragma unroll
-            for (int m = 0; m < kUpTiles; m++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int v = min(v0 + 16 * m + 8 * h + g, a.vocab - 1);
-                    w[m][h] = in ? __ldg(reinterpret_cast<const uint2 *>(base + (size_t)v * a.rank + k)) : make_uint2(0u, 0u);
-                }
-            uint32_t h0, h1, m0, m1, l0, l1;
-            split3(t.x, t.y, h0, m0, l0);
-            split3(t.z, t.w, h1, m1, l1);
-#pragma unroll
-            for (int m = 0; m < kUpTiles; m++) {
-                float e[4] = {};   // the tensor cores add by truncation: 16 ranks at a time, then rounded
-                mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, l0, l1);
-                mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, m0, m1);
-                mma_16816(e, w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, h0, h1);
-#pragma unroll
-                for (int i = 0; i < 4; i++) d[m][i] += e[i];
+            for (int k = 0; k < KT; k++) {
+                multiply(w[k], kept[k], d, k > 0);
+                if (step + 1 < kUpSteps) rows_of_b(v0 + kUpWarps * kUpRows, 16 * k, w[k]);
+            }
+        } else {
+            for (int k = 0; k < a.rank; k += 16) {
+                rows_of_b(v0, k, w[0]);
+                parts(k, kept[0]);
+                multiply(w[0], kept[0], d, k > 0);
             }
         }
 #pragma unroll
@@ -385,13 +413,14 @@ __global__ void __launch_bounds__(32 * kUpWarps) adapter_up_kernel(const UpArgs 
             for (int i = 0; i < 4; i++) s_turn[warp][2 * k4 + (i & 1)][16 * m + 8 * (i >> 1) + g] = d[m][i];
         __syncwarp();
         float *to = a.delta + (size_t)c * a.vocab + v0 + lane;
+        const bool in0 = v0 + lane < a.vocab, in1 = v0 + 32 + lane < a.vocab;
 #pragma unroll
         for (int j = 0; j < kItem; j++) {
-            const size_t r = (size_t)__shfl_sync(kFull, row, j) * ldo;
             if (j >= len) continue;
-#pragma unroll
-            for (int i = 0; i < kUpRows; i += 32)
-                if (v0 + i + lane < a.vocab) to[r + i] = s_turn[warp][j][i + lane];
+            float *at = to + (size_t)to_row[j] * ldo;
+            const float x = s_turn[warp][j][lane], y = s_turn[warp][j][32 + lane];
+            if (in0) at[0] = x;
+            if (in1) at[32] = y;
         }
         __syncwarp();
     }
@@ -1140,7 +1169,9 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
         cfg.gridDim = dim3((unsigned)max_items(h.batch, ad.n_adapters), (unsigned)(h.n_cb * up_per_cb));
         cfg.blockDim = dim3(32 * kUpWarps);
         cfg.dynamicSmemBytes = 0;
-        e = cudaLaunchKernelEx(&cfg, adapter_up_kernel, u);
+        e = ad.rank <= 16   ? cudaLaunchKernelEx(&cfg, adapter_up_kernel<1>, u)
+            : ad.rank <= 32 ? cudaLaunchKernelEx(&cfg, adapter_up_kernel<2>, u)
+                            : cudaLaunchKernelEx(&cfg, adapter_up_kernel<0>, u);
         if (e != cudaSuccess) return e;
     }
 
