@@ -9,8 +9,8 @@
 //
 // r and n are computed in f32 and rounded once, each on its own store: n is
 // taken from the unrounded r, so a bf16 residual stream costs n no second
-// rounding.  The sums of squares are f32: every thread's partial sum has at most
-// 32 terms and the rest is a tree, so their error is a few ulp.
+// rounding.  The sums of squares are f32: 8 terms in a thread of block_norm_kernel,
+// the rest a tree, so their error is a few ulp.
 //
 // Bound: memory.  A row is read once (residual, block output, gate) and written
 // twice; it stays in registers between its two reductions.
@@ -37,7 +37,8 @@ __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ float sigmoid(float g) { return __frcp_rn(1.0f + expf(-g)); }
+// The approximate reciprocal is off by an ulp, as expf is.
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + expf(-g)); }
 
 // The sum over the block's threads, in every thread.  `part` holds one float per warp.
 __device__ __forceinline__ float block_sum(float v, float *part)
@@ -58,6 +59,143 @@ __device__ __forceinline__ float block_sum(float v, float *part)
 __device__ __forceinline__ float rcp_rms(float ss, int dim, float eps)
 {
     return __fdiv_rn(1.0f, sqrtf(__fdiv_rn(ss, (float)dim) + eps));
+}
+
+// 16 bytes of a row.  Not the read-only path: the sums may go back to where the row was.
+__device__ __forceinline__ uint4 load16(const void *p)
+{
+    uint4 u;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p) : "memory");
+    return u;
+}
+
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);   // elements of a 16-byte vector
+
+__device__ __forceinline__ void widen(const uint4 &u, float (&f)[4])
+{
+    f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void widen(const uint4 &u, float (&f)[8])
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ uint4 narrow(const float (&f)[4])
+{
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 narrow(const float (&f)[8])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A vector of 16 bytes per thread, blockDim.x / 32 warps per row (threadIdx.y: the row
+// within the block).  A block walks over rows a grid apart, so that its weights are loaded
+// once, into registers, and the next row's loads are under way while this one is reduced;
+// each reduction costs one barrier, its partial sums alternating between two buffers.
+template <typename T>
+__global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
+{
+    constexpr int V = kVec<T>;
+    __shared__ float part[2][32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    const int first = threadIdx.y * warps, warp = first + (threadIdx.x >> 5);
+    const int d = threadIdx.x * V;
+    const bool in_row = d < a.dim;
+    const bool by_row = a.gate && !a.gate_col_stride, by_elem = a.gate && a.gate_col_stride;
+    const long long step = (long long)gridDim.x * blockDim.y;
+    long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    uint4 x, y, g;
+    float g_row = 1.0f;
+    auto fetch = [&](long long r) {
+        x = y = g = make_uint4(0, 0, 0, 0);
+        if (r >= a.rows) return;
+        if (in_row) {
+            y = load16(static_cast<const T *>(a.block) + r * a.block_stride + d);
+            if (by_elem) g = load16(static_cast<const T *>(a.gate) + r * a.gate_row_stride + d);
+            x = load16(static_cast<const T *>(a.resid) + r * a.resid_stride + d);
+        }
+        if (by_row) g_row = to_f<T>(static_cast<const T *>(a.gate)[r * a.gate_row_stride]);
+    };
+    fetch(row);
+    float wp[V], wn[V];
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+        float4 p = make_float4(1.0f, 1.0f, 1.0f, 1.0f), n = p;
+        if (a.post_weight && in_row) p = __ldg(reinterpret_cast<const float4 *>(a.post_weight + d + j));
+        if (a.norm_weight && in_row) n = __ldg(reinterpret_cast<const float4 *>(a.norm_weight + d + j));
+        wp[j] = p.x, wp[j + 1] = p.y, wp[j + 2] = p.z, wp[j + 3] = p.w;
+        wn[j] = n.x, wn[j + 1] = n.y, wn[j + 2] = n.z, wn[j + 3] = n.w;
+    }
+    int buf = 0;
+    auto row_sum = [&](float v) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+        if (warps == 1) return v;
+        if (lane == 0) part[buf][warp] = v;
+        __syncthreads();
+        v = lane < warps ? part[buf][first + lane] : 0.0f;
+        buf ^= 1;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+        return v;
+    };
+    // By the block's first row: all its threads take the same number of turns and barriers.
+    for (long long r0 = (long long)blockIdx.x * blockDim.y; r0 < a.rows; r0 += step, row += step) {
+        float s[V];
+        widen(y, s);
+        const uint4 x0 = x, g0 = g;
+        const float gate_row = a.gate_sigmoid && by_row ? sigmoid(g_row) : g_row;
+        fetch(row + step);
+        if (a.post_norm) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; j++) ss = fmaf(s[j], s[j], ss);
+            const float rcp = rcp_rms(row_sum(ss), a.dim, a.post_eps);
+#pragma unroll
+            for (int j = 0; j < V; j++) s[j] = s[j] * rcp * wp[j];
+        }
+        if (by_elem) {
+            float t[V];
+            widen(g0, t);
+            if (a.gate_sigmoid) {
+#pragma unroll
+                for (int j = 0; j < V; j++) t[j] = sigmoid(t[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < V; j++) s[j] *= t[j];
+        } else if (by_row) {
+#pragma unroll
+            for (int j = 0; j < V; j++) s[j] *= gate_row;
+        }
+        float f[V];
+        widen(x0, f);
+#pragma unroll
+        for (int j = 0; j < V; j++) s[j] = fmaf(a.scale, s[j], f[j]);
+        const bool store = in_row && row < a.rows;
+        if (a.resid_out && store)
+            *reinterpret_cast<uint4 *>(static_cast<T *>(a.resid_out) + row * a.out_stride + d) = narrow(s);
+        if (a.normed_out) {
+            float ss = 0.0f;
+            if (in_row) {
+#pragma unroll
+                for (int j = 0; j < V; j++) ss = fmaf(s[j], s[j], ss);
+            }
+            const float rcp = rcp_rms(row_sum(ss), a.dim, a.norm_eps);
+#pragma unroll
+            for (int j = 0; j < V; j++) s[j] = s[j] * rcp * wn[j];
+            if (store) *reinterpret_cast<uint4 *>(static_cast<T *>(a.normed_out) + row * a.out_stride + d) = narrow(s);
+        }
+    }
 }
 
 // One block per row, elements one by one, the row re-read (from L1 or L2) by
@@ -109,11 +247,11 @@ __global__ void __launch_bounds__(1024) block_norm_any_kernel(const BlockNormArg
 }
 
 template <class Kernel>
-cudaError_t launch(Kernel kernel, int grid, int threads, const BlockNormArgs &a, cudaStream_t stream)
+cudaError_t launch(Kernel kernel, unsigned grid, dim3 block, const BlockNormArgs &a, cudaStream_t stream)
 {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3((unsigned)threads);
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = block;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -123,15 +261,43 @@ cudaError_t launch(Kernel kernel, int grid, int threads, const BlockNormArgs &a,
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+template <typename T>
+cudaError_t launch_vec(const BlockNormArgs &a, cudaStream_t stream)
+{
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    const int x = (a.dim / kVec<T> + 31) & ~31;
+    // Short rows share a block of up to 256 threads, unless there are too few for all SMs.
+    int y = x < 256 ? 256 / x : 1;
+    while (y > 1 && a.rows < (long long)sms * y) y--;
+    const int blocks = (a.rows + y - 1) / y;
+    const int most = sms * max(1, 1024 / (x * y));   // at a time: 1024 threads of 64 registers an SM
+    return launch(block_norm_kernel<T>, (unsigned)min(blocks, most), dim3(x, y), a, stream);
+}
+
+template <typename T>
+cudaError_t launch_type(const BlockNormArgs &a, cudaStream_t stream)
+{
+    auto fits = [&](const void *p, long long stride) {   // absent, or whole vectors
+        return !p || ((uintptr_t)p % 16 == 0 && stride % kVec<T> == 0);
+    };
+    const bool vec = a.dim % kVec<T> == 0 && fits(a.resid, a.resid_stride) && fits(a.block, a.block_stride) &&
+                     (!a.gate_col_stride || fits(a.gate, a.gate_row_stride)) && fits(a.resid_out, a.out_stride) &&
+                     fits(a.normed_out, a.out_stride) && fits(a.post_weight, 0) && fits(a.norm_weight, 0);
+    if (vec && a.dim <= 1024 * kVec<T>) return launch_vec<T>(a, stream);
+    int threads = 32;
+    while (threads < 1024 && threads * 4 < a.dim) threads *= 2;
+    return launch(block_norm_any_kernel<T>, (unsigned)a.rows, dim3(threads), a, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_block_norm(const BlockNormArgs &a, bool bf16, cudaStream_t stream)
 {
     if (a.rows == 0) return cudaSuccess;
-    int threads = 32;
-    while (threads < 1024 && threads * 4 < a.dim) threads *= 2;
-    return bf16 ? launch(block_norm_any_kernel<__nv_bfloat16>, a.rows, threads, a, stream)
-                : launch(block_norm_any_kernel<float>, a.rows, threads, a, stream);
+    return bf16 ? launch_type<__nv_bfloat16>(a, stream) : launch_type<float>(a, stream);
 }
 
 }  // namespace z2

@@ -35,6 +35,15 @@ struct Acc<float> {
     using type = double;
 };
 
+// Four neighbouring elements.
+__device__ __forceinline__ float4 load4(const float *p) { return __ldg(reinterpret_cast<const float4 *>(p)); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16 *p)
+{
+    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xffff0000u));
+}
+
 // t[b][r], one warp per element.
 template <typename T>
 __global__ void __launch_bounds__(32 * kWarps)
@@ -50,49 +59,100 @@ __global__ void __launch_bounds__(32 * kWarps)
     const T *x = static_cast<const T *>(h.hidden) + (size_t)b * h.dim;
     const T *w = static_cast<const T *>(ad.A) + ((size_t)a * ad.rank + r) * h.dim;
     S acc = 0;
+#pragma unroll 8
     for (int d = lane; d < h.dim; d += 32) acc += (S)load_f(x + d) * (S)load_f(w + d);
 #pragma unroll
     for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(kFull, acc, o);
     if (lane == 0) static_cast<S *>(ad.work)[i] = acc * (S)(ad.scale ? __ldg(ad.scale + a) : 1.0f);
 }
 
-// The logits, one warp per weight row.
-template <typename T>
+constexpr int kRows = 2;    // weight rows per warp
+constexpr int kBatch = 4;   // hidden rows at a time: a weight is read and widened once for four
+
+// The logits, one warp per kRows weight rows of one codebook.  An f32 head widens both
+// operands to f64 (exact products, one rounding at the end), and what bounds it beside
+// the reading of W are those conversions: kRows x kBatch products share them.  VEC: rows
+// 16-byte aligned (f32) or 8-byte aligned (bf16) and dim a multiple of 4.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kWarps)
     adapter_any_kernel(const HeadArgs h, const AdapterArgs ad)
 {
     using S = typename Acc<T>::type;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, per_cb = (h.vocab + kRows - 1) / kRows;
     const int o = blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (o >= h.n_cb * h.vocab) return;
-    const int c = o / h.vocab, v = o - c * h.vocab;
+    if (o >= h.n_cb * per_cb) return;
+    const int c = o / per_cb, v = (o - c * per_cb) * kRows, rows = min(kRows, h.vocab - v);
     const size_t n = (size_t)c * h.rows_per_cb + v;
     const T *w = static_cast<const T *>(h.W) + n * h.dim;
-    float cond = 0.0f;   // with guidance: the logit of the pair's conditional row
-    for (int b = 0; b < h.batch; b++) {
-        const T *x = static_cast<const T *>(h.hidden) + (size_t)b * h.dim;
-        S acc = 0;
-        for (int d = lane; d < h.dim; d += 32) acc += (S)load_f(w + d) * (S)load_f(x + d);
-        const int a = ad.which[b / ad.rows_per_id];
-        if ((unsigned)a < (unsigned)ad.n_adapters) {
-            const T *up = static_cast<const T *>(ad.B) +
-                          ((size_t)a * h.n_cb * h.rows_per_cb + n) * ad.rank;
-            const S *t = static_cast<const S *>(ad.work) + (size_t)b * ad.rank;
-            for (int r = lane; r < ad.rank; r += 32) acc += (S)load_f(up + r) * t[r];
-        }
+    const int second = rows > 1 ? h.dim : 0;   // offset of the second row
+    for (int b0 = 0; b0 < h.batch; b0 += kBatch) {
+        const T *x[kBatch];
 #pragma unroll
-        for (int s = 16; s; s >>= 1) acc += __shfl_xor_sync(kFull, acc, s);
-        if (lane == 0) {
-            float l = (float)acc;
-            if (h.row_scale) l *= __ldg(h.row_scale + b);
-            if (h.softcap > 0.0f) l = h.softcap * tanhf(l / h.softcap);
-            if (!h.cfg) {
-                h.out[((size_t)b * h.n_cb + c) * h.vocab + v] = l;
-            } else if ((b & 1) == 0) {
-                cond = l;
-            } else {
-                h.out[((size_t)(b >> 1) * h.n_cb + c) * h.vocab + v] =
-                    __fadd_rn(l, __fmul_rn(h.cfg_scale, __fsub_rn(cond, l)));
+        for (int i = 0; i < kBatch; i++)
+            x[i] = static_cast<const T *>(h.hidden) + (size_t)min(b0 + i, h.batch - 1) * h.dim;
+        S acc[kRows][kBatch] = {};
+        if (VEC) {
+#pragma unroll 2
+            for (int d = 4 * lane; d < h.dim; d += 128) {
+                const float4 w0 = load4(w + d), w1 = load4(w + second + d);
+                const S u0[4] = {(S)w0.x, (S)w0.y, (S)w0.z, (S)w0.w}, u1[4] = {(S)w1.x, (S)w1.y, (S)w1.z, (S)w1.w};
+#pragma unroll
+                for (int i = 0; i < kBatch; i++) {
+                    const float4 f = load4(x[i] + d);
+                    const S y[4] = {(S)f.x, (S)f.y, (S)f.z, (S)f.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        acc[0][i] += u0[j] * y[j];
+                        acc[1][i] += u1[j] * y[j];
+                    }
+                }
+            }
+        } else {
+            for (int d = lane; d < h.dim; d += 32) {
+                const S u0 = (S)load_f(w + d), u1 = (S)load_f(w + second + d);
+#pragma unroll
+                for (int i = 0; i < kBatch; i++) {
+                    const S y = (S)load_f(x[i] + d);
+                    acc[0][i] += u0 * y;
+                    acc[1][i] += u1 * y;
+                }
+            }
+        }
+        float l[kRows][kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            const int b = b0 + i;
+            if (b >= h.batch) break;
+            const int a = ad.which[b / ad.rows_per_id];
+            const bool has = (unsigned)a < (unsigned)ad.n_adapters;
+#pragma unroll
+            for (int m = 0; m < kRows; m++) {
+                S sum = acc[m][i];
+                if (has && m < rows) {
+                    const T *up = static_cast<const T *>(ad.B) + ((size_t)a * h.n_cb * h.rows_per_cb + n + m) * ad.rank;
+                    const S *t = static_cast<const S *>(ad.work) + (size_t)b * ad.rank;
+                    for (int r = lane; r < ad.rank; r += 32) sum += (S)load_f(up + r) * t[r];
+                }
+#pragma unroll
+                for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(kFull, sum, s);
+                float f = (float)sum;
+                if (h.row_scale) f *= __ldg(h.row_scale + b);
+                l[m][i] = h.softcap > 0.0f ? h.softcap * tanhf(f / h.softcap) : f;
+            }
+        }
+        if (lane < rows) {   // lane m stores row m (every lane has the sums)
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) {
+                const int b = b0 + i;
+                if (b >= h.batch) break;
+                const float f = lane ? l[1][i] : l[0][i];
+                if (!h.cfg) {
+                    h.out[((size_t)b * h.n_cb + c) * h.vocab + v + lane] = f;
+                } else if (i & 1) {   // the pair's blend; its conditional row came before
+                    const float cond = lane ? l[1][i - 1] : l[0][i - 1];
+                    h.out[((size_t)(b >> 1) * h.n_cb + c) * h.vocab + v + lane] =
+                        __fadd_rn(f, __fmul_rn(h.cfg_scale, __fsub_rn(cond, f)));
+                }
             }
         }
     }
@@ -105,8 +165,13 @@ cudaError_t launch_any(const HeadArgs &h, const AdapterArgs &ad, cudaStream_t st
     adapter_down_kernel<T><<<(unsigned)((down + kWarps - 1) / kWarps), 32 * kWarps, 0, stream>>>(h, ad);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const int rows = h.n_cb * h.vocab;
-    adapter_any_kernel<T><<<(unsigned)((rows + kWarps - 1) / kWarps), 32 * kWarps, 0, stream>>>(h, ad);
+    const int warps = h.n_cb * ((h.vocab + kRows - 1) / kRows);
+    const unsigned blocks = (unsigned)((warps + kWarps - 1) / kWarps);
+    const bool vec = h.dim % 4 == 0 && (uintptr_t)h.W % (4 * sizeof(T)) == 0 && (uintptr_t)h.hidden % (4 * sizeof(T)) == 0;
+    if (vec)
+        adapter_any_kernel<T, true><<<blocks, 32 * kWarps, 0, stream>>>(h, ad);
+    else
+        adapter_any_kernel<T, false><<<blocks, 32 * kWarps, 0, stream>>>(h, ad);
     return cudaGetLastError();
 }
 

@@ -240,36 +240,60 @@ def head_softcap(W, dtype: int, rows_per_cb: int, n_cb: int, vocab: int, hidden,
     _check(rc, "zonos2cu_head_softcap")
 
 
+_TYPES: dict = {}    # torch's types -> the library's, filled on first use
+_raw_stream = None   # torch's own lookup of a device's current stream handle
+
+
 def _dtype(t) -> int:
     """The library's type of a torch tensor's elements."""
-    import torch
-    if t.dtype == torch.bfloat16:
-        return BF16
-    if t.dtype == torch.float32:
-        return F32
-    raise TypeError(f"expected bfloat16 or float32, got {t.dtype}")
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.bfloat16: BF16, torch.float32: F32})
+    dt = _TYPES.get(t.dtype)
+    if dt is None:
+        raise TypeError(f"expected bfloat16 or float32, got {t.dtype}")
+    return dt
 
 
 def _launch(fn: str, on, stream, *args) -> None:
     """Call entry point ``fn`` on the device of tensor ``on``; the stream (default: that
     device's current one) is its last argument."""
-    import torch
+    global _raw_stream
     dev = on.get_device()
     if dev < 0:
         raise TypeError(f"{fn}: CUDA tensors expected")
+    import torch
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _launch(fn, on, stream, *args)
-    rc = getattr(lib(), fn)(*args, _stream(stream))
+    if stream is None:
+        # Half the cost of making a Stream object per call, which a small launch would feel.
+        if _raw_stream is None:
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                                  lambda d: torch.cuda.current_stream(d).cuda_stream)
+        stream = _raw_stream(dev)
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
+    rc = getattr(lib(), fn)(*args, stream)
     if rc < 0:
         raise Zonos2cuError(rc, fn)
 
 
 def _rows(t, what: str) -> int:
     """The row stride of a 2-D tensor whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.is_contiguous():
+        return t.shape[1]
+    if t.shape[1] > 1 and t.stride(1) != 1:
         raise ValueError(f"{what}: expected [rows, dim] with contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t.stride(0)
+
+
+def _whole(what: str, *tensors) -> None:
+    """Each tensor of the (tensor, elements) pairs, where given, is contiguous and of that size."""
+    for t, n in tensors:
+        if t is not None and (t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"{what}: a contiguous tensor of {n} elements expected, got "
+                             f"{tuple(t.shape)}")
 
 
 def head_adapters_work(dtype: int, batch: int, rank: int) -> int:
@@ -288,12 +312,8 @@ def head_adapters(W, dtype: int, rows_per_cb: int, n_cb: int, vocab: int, hidden
     batch, dim = hidden.shape
     n, rank, _ = A.shape
     wide = n_cb * rows_per_cb
-    for t, size in ((W, wide * dim), (hidden, batch * dim), (A, n * rank * dim),
-                    (B, n * wide * rank), (adapter, batch), (out, batch * n_cb * vocab),
-                    (scale, n)):
-        if t is not None and (t.numel() != size or not t.is_contiguous()):
-            raise ValueError(f"head_adapters: a contiguous tensor of {size} elements expected, got "
-                             f"{tuple(t.shape)}")
+    _whole("head_adapters", (W, wide * dim), (hidden, batch * dim), (A, n * rank * dim),
+           (B, n * wide * rank), (adapter, batch), (out, batch * n_cb * vocab), (scale, n))
     _launch("zonos2cu_head_adapters", hidden, stream, W.data_ptr(), dtype, rows_per_cb, n_cb, vocab,
             dim, hidden.data_ptr(), batch, softcap, A.data_ptr(), B.data_ptr(), _ptr(scale), n,
             rank, adapter.data_ptr(), work.data_ptr(), work.numel() * work.element_size(),
@@ -309,28 +329,32 @@ def block_norm(resid, block, resid_out, normed_out, *, post_weight=None, post_ep
     (n) likewise, one of them may be None, and may be resid or block itself; gate: None or a
     2-D tensor that broadcasts to [rows, dim]; weights [dim] f32 or None; post_eps < 0 leaves
     the block's output as it is."""
-    dt, (rows, dim) = _dtype(resid), resid.shape
-    outs = [t for t in (resid_out, normed_out) if t is not None]
-    for t in (block, *outs):
-        if t.shape != resid.shape or t.dtype != resid.dtype:
+    dt, shape = _dtype(resid), resid.shape
+    rows, dim = shape
+    for t in (block, resid_out, normed_out):
+        if t is not None and (t.shape != shape or t.dtype != resid.dtype):
             raise ValueError("block_norm: block and outputs must match resid")
-    strides = {_rows(t, "block_norm") for t in outs}
-    if len(strides) != 1:
+    if resid_out is None and normed_out is None:
+        raise ValueError("block_norm: no output given")
+    out_stride = _rows(normed_out if resid_out is None else resid_out, "block_norm")
+    if normed_out is not None and _rows(normed_out, "block_norm") != out_stride:
         raise ValueError("block_norm: the outputs need one row stride")
     gate_row = gate_col = 0
     if gate is not None:
-        if gate.dtype != resid.dtype or gate.dim() != 2 or any(
-                n not in (1, m) for n, m in zip(gate.shape, resid.shape)):
+        given = gate.shape
+        if (gate.dtype != resid.dtype or len(given) != 2 or given[0] not in (1, rows)
+                or given[1] not in (1, dim)):
             raise ValueError("block_norm: the gate must broadcast to [rows, dim]")
-        gate_row = 0 if gate.shape[0] == 1 else gate.stride(0)
-        gate_col = 0 if gate.shape[1] == 1 else gate.stride(1)
+        strides = gate.stride()
+        gate_row = 0 if given[0] == 1 else strides[0]
+        gate_col = 0 if given[1] == 1 else strides[1]
     for w in (post_weight, norm_weight):
-        if w is not None and (w.shape != (dim,) or _dtype(w) != F32 or not w.is_contiguous()):
+        if w is not None and (w.numel() != dim or _dtype(w) != F32 or not w.is_contiguous()):
             raise ValueError("block_norm: weights are [dim] f32")
     _launch("zonos2cu_block_norm", resid, stream, resid.data_ptr(), block.data_ptr(), dt, rows, dim,
             _rows(resid, "block_norm"), _rows(block, "block_norm"), _ptr(post_weight), post_eps,
             _ptr(gate), gate_row, gate_col, int(gate_sigmoid), scale, _ptr(norm_weight), norm_eps,
-            _ptr(resid_out), _ptr(normed_out), strides.pop())
+            _ptr(resid_out), _ptr(normed_out), out_stride)
 
 
 def verify_drafts(logits, params: SampleParams, drafts, uniforms, codes, n_accepted, *,
@@ -345,13 +369,12 @@ def verify_drafts(logits, params: SampleParams, drafts, uniforms, codes, n_accep
     S, D1, Cb, stride = logits.shape
     V = stride if vocab is None else vocab
     H = 0 if hist is None else hist.shape[-1]
-    for t, n in ((logits, S * D1 * Cb * stride), (drafts, S * (D1 - 1) * Cb),
-                 (uniforms, 2 * S * D1 * Cb), (draft_probs, S * (D1 - 1) * Cb * V), (n_drafts, S),
-                 (codes, S * D1 * Cb), (flags, S * D1 * Cb), (n_accepted, S), (hist, S * Cb * H),
-                 (hist_pos, S), (allow, S * ((V + 31) // 32))):
-        if t is not None and (t.numel() != n or not t.is_contiguous()):
-            raise ValueError(f"verify_drafts: a contiguous tensor of {n} elements expected, got "
-                             f"{tuple(t.shape)}")
+    _whole("verify_drafts", (logits, S * D1 * Cb * stride), (drafts, S * (D1 - 1) * Cb),
+           (uniforms, 2 * S * D1 * Cb), (draft_probs, S * (D1 - 1) * Cb * V), (n_drafts, S),
+           (codes, S * D1 * Cb), (flags, S * D1 * Cb), (n_accepted, S), (hist, S * Cb * H),
+           (hist_pos, S), (allow, S * ((V + 31) // 32)))
+    for t in (logits, drafts, uniforms, draft_probs, n_drafts, codes, flags, n_accepted, hist,
+              hist_pos, allow):
         if t is not None and t.element_size() != 4:
             raise TypeError("verify_drafts: f32 and int32 tensors expected")
     _launch("zonos2cu_verify_drafts", logits, stream, logits.data_ptr(), S, D1 - 1, Cb, V, stride,
