@@ -13,7 +13,11 @@
 // the rest a tree, so their error is a few ulp.
 //
 // Bound: memory.  A row is read once (residual, block output, gate) and written
-// twice; it stays in registers between its two reductions.
+// twice; it stays in registers between its two reductions.  16384 bf16 rows of 2048 with a
+// full sigmoid gate (336 MB): 60 us, 5.6 TB/s; 297 us by block_norm_any_kernel, which
+// re-reads the row and works element by element.  The issue slots come next: with
+// full-precision divisions and exponentials everywhere the same bytes took 83 us, so the
+// reciprocal root, the sigmoid and the join of a row's partial sums are kept short.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -37,8 +41,20 @@ __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// The approximate reciprocal is off by an ulp, as expf is.
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + expf(-g)); }
+// 1 / (1 + exp(-g)), 1 + exp(-g) being 1 at least and perhaps infinite.  A bf16 gate takes the
+// exponential as a power of two: rounding g log2(e) costs |g| 2^-24 of it, less than
+// a hundredth of a bf16 step for any g whose sigmoid is not lost in the sum.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float g)
+{
+    float e, r;
+    if (sizeof(T) == 2)
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
+    else
+        e = expf(-g);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
 
 // The sum over the block's threads, in every thread.  `part` holds one float per warp.
 __device__ __forceinline__ float block_sum(float v, float *part)
@@ -56,9 +72,10 @@ __device__ __forceinline__ float block_sum(float v, float *part)
     return v;
 }
 
-__device__ __forceinline__ float rcp_rms(float ss, int dim, float eps)
+// rsqrtf is off by 2 ulp at most.
+__device__ __forceinline__ float rcp_rms(float ss, const BlockNormArgs &a, float eps)
 {
-    return __fdiv_rn(1.0f, sqrtf(__fdiv_rn(ss, (float)dim) + eps));
+    return rsqrtf(fmaf(ss, a.rcp_dim, eps));
 }
 
 // 16 bytes of a row.  Not the read-only path: the sums may go back to where the row was.
@@ -104,27 +121,30 @@ template <typename T>
 __global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
 {
     constexpr int V = kVec<T>;
-    __shared__ float part[2][32];
+    __shared__ float4 part[2][8];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    const int first = threadIdx.y * warps, warp = first + (threadIdx.x >> 5);
+    const int first = threadIdx.y * ((warps + 3) >> 2), warp = 4 * first + (threadIdx.x >> 5);
+    if (threadIdx.y == 0 && threadIdx.x < 32) reinterpret_cast<float2 *>(part)[lane] = make_float2(0.0f, 0.0f);
+    __syncthreads();   // part's places past a row's warps stay zero
     const int d = threadIdx.x * V;
     const bool in_row = d < a.dim;
     const bool by_row = a.gate && !a.gate_col_stride, by_elem = a.gate && a.gate_col_stride;
-    const long long step = (long long)gridDim.x * blockDim.y;
-    long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    const uint32_t step = gridDim.x * blockDim.y, rows = a.rows;   // the sums below stay under 2^32
+    const uint32_t rs = a.resid_stride, bs = a.block_stride, gs = a.gate_row_stride, os = a.out_stride;
+    uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
     uint4 x, y, g;
     float g_row = 1.0f;
-    auto fetch = [&](long long r) {
+    auto fetch = [&](uint32_t r) {
         x = y = g = make_uint4(0, 0, 0, 0);
-        if (r >= a.rows) return;
+        if (r >= rows) return;
         if (in_row) {
-            y = load16(static_cast<const T *>(a.block) + r * a.block_stride + d);
-            if (by_elem) g = load16(static_cast<const T *>(a.gate) + r * a.gate_row_stride + d);
-            x = load16(static_cast<const T *>(a.resid) + r * a.resid_stride + d);
+            y = load16(static_cast<const T *>(a.block) + (size_t)r * bs + d);
+            if (by_elem) g = load16(static_cast<const T *>(a.gate) + (size_t)r * gs + d);
+            x = load16(static_cast<const T *>(a.resid) + (size_t)r * rs + d);
         }
-        if (by_row) g_row = to_f<T>(static_cast<const T *>(a.gate)[r * a.gate_row_stride]);
+        if (by_row) g_row = to_f<T>(static_cast<const T *>(a.gate)[(size_t)r * gs]);
     };
     fetch(row);
     float wp[V], wn[V];
@@ -141,26 +161,28 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
 #pragma unroll
         for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
         if (warps == 1) return v;
-        if (lane == 0) part[buf][warp] = v;
+        if (lane == 0) reinterpret_cast<float *>(part[buf])[warp] = v;
         __syncthreads();
-        v = lane < warps ? part[buf][first + lane] : 0.0f;
+        v = 0.0f;
+        for (int i = 0; i < warps; i += 4) {
+            const float4 p = part[buf][first + (i >> 2)];
+            v += (p.x + p.y) + (p.z + p.w);
+        }
         buf ^= 1;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
         return v;
     };
     // By the block's first row: all its threads take the same number of turns and barriers.
-    for (long long r0 = (long long)blockIdx.x * blockDim.y; r0 < a.rows; r0 += step, row += step) {
+    for (uint32_t r0 = blockIdx.x * blockDim.y; r0 < rows; r0 += step, row += step) {
         float s[V];
         widen(y, s);
         const uint4 x0 = x, g0 = g;
-        const float gate_row = a.gate_sigmoid && by_row ? sigmoid(g_row) : g_row;
+        const float gate_row = a.gate_sigmoid && by_row ? sigmoid<T>(g_row) : g_row;
         fetch(row + step);
         if (a.post_norm) {
             float ss = 0.0f;
 #pragma unroll
             for (int j = 0; j < V; j++) ss = fmaf(s[j], s[j], ss);
-            const float rcp = rcp_rms(row_sum(ss), a.dim, a.post_eps);
+            const float rcp = rcp_rms(row_sum(ss), a, a.post_eps);
 #pragma unroll
             for (int j = 0; j < V; j++) s[j] = s[j] * rcp * wp[j];
         }
@@ -169,7 +191,7 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
             widen(g0, t);
             if (a.gate_sigmoid) {
 #pragma unroll
-                for (int j = 0; j < V; j++) t[j] = sigmoid(t[j]);
+                for (int j = 0; j < V; j++) t[j] = sigmoid<T>(t[j]);
             }
 #pragma unroll
             for (int j = 0; j < V; j++) s[j] *= t[j];
@@ -181,19 +203,19 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
         widen(x0, f);
 #pragma unroll
         for (int j = 0; j < V; j++) s[j] = fmaf(a.scale, s[j], f[j]);
-        const bool store = in_row && row < a.rows;
+        const bool store = in_row && row < rows;
         if (a.resid_out && store)
-            *reinterpret_cast<uint4 *>(static_cast<T *>(a.resid_out) + row * a.out_stride + d) = narrow(s);
+            *reinterpret_cast<uint4 *>(static_cast<T *>(a.resid_out) + (size_t)row * os + d) = narrow(s);
         if (a.normed_out) {
             float ss = 0.0f;
             if (in_row) {
 #pragma unroll
                 for (int j = 0; j < V; j++) ss = fmaf(s[j], s[j], ss);
             }
-            const float rcp = rcp_rms(row_sum(ss), a.dim, a.norm_eps);
+            const float rcp = rcp_rms(row_sum(ss), a, a.norm_eps);
 #pragma unroll
             for (int j = 0; j < V; j++) s[j] = s[j] * rcp * wn[j];
-            if (store) *reinterpret_cast<uint4 *>(static_cast<T *>(a.normed_out) + row * a.out_stride + d) = narrow(s);
+            if (store) *reinterpret_cast<uint4 *>(static_cast<T *>(a.normed_out) + (size_t)row * os + d) = narrow(s);
         }
     }
 }
@@ -217,14 +239,14 @@ __global__ void __launch_bounds__(1024) block_norm_any_kernel(const BlockNormArg
             const float v = to_f<T>(y[d]);
             ss = fmaf(v, v, ss);
         }
-        rcp = rcp_rms(block_sum(ss, part[0]), a.dim, a.post_eps);
+        rcp = rcp_rms(block_sum(ss, part[0]), a, a.post_eps);
     }
     auto sum_at = [&](int d) {
         float v = to_f<T>(y[d]);
         if (a.post_norm) v = v * rcp * (a.post_weight ? a.post_weight[d] : 1.0f);
         if (g) {
             const float t = to_f<T>(g[(size_t)d * a.gate_col_stride]);
-            v *= a.gate_sigmoid ? sigmoid(t) : t;
+            v *= a.gate_sigmoid ? sigmoid<T>(t) : t;
         }
         return fmaf(a.scale, v, to_f<T>(x[d]));
     };
@@ -235,7 +257,7 @@ __global__ void __launch_bounds__(1024) block_norm_any_kernel(const BlockNormArg
             const float v = sum_at(d);
             ss = fmaf(v, v, ss);
         }
-        rcp2 = rcp_rms(block_sum(ss, part[1]), a.dim, a.norm_eps);
+        rcp2 = rcp_rms(block_sum(ss, part[1]), a, a.norm_eps);
     }
     T *ro = a.resid_out ? static_cast<T *>(a.resid_out) + row * a.out_stride : nullptr;
     T *no = a.normed_out ? static_cast<T *>(a.normed_out) + row * a.out_stride : nullptr;
@@ -281,10 +303,10 @@ template <typename T>
 cudaError_t launch_type(const BlockNormArgs &a, cudaStream_t stream)
 {
     auto fits = [&](const void *p, long long stride) {   // absent, or whole vectors
-        return !p || ((uintptr_t)p % 16 == 0 && stride % kVec<T> == 0);
+        return !p || ((uintptr_t)p % 16 == 0 && stride % kVec<T> == 0 && stride <= INT32_MAX);
     };
     const bool vec = a.dim % kVec<T> == 0 && fits(a.resid, a.resid_stride) && fits(a.block, a.block_stride) &&
-                     (!a.gate_col_stride || fits(a.gate, a.gate_row_stride)) && fits(a.resid_out, a.out_stride) &&
+                     (a.gate_col_stride ? fits(a.gate, a.gate_row_stride) : a.gate_row_stride <= INT32_MAX) && fits(a.resid_out, a.out_stride) &&
                      fits(a.normed_out, a.out_stride) && fits(a.post_weight, 0) && fits(a.norm_weight, 0);
     if (vec && a.dim <= 1024 * kVec<T>) return launch_vec<T>(a, stream);
     int threads = 32;

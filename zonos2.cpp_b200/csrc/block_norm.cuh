@@ -11,6 +11,7 @@ struct BlockNormArgs {
     const void *block;        // [rows] of block_stride elements
     long long resid_stride, block_stride;
     int rows, dim;
+    float rcp_dim;            // 1 / dim
     int post_norm;            // normalise the block's output first
     const float *post_weight; // [dim] or nullptr
     float post_eps;

@@ -434,6 +434,7 @@ int zonos2cu_block_norm(const void *resid_dev, const void *block_dev, zonos2cu_d
     a.block_stride = block_stride;
     a.rows = rows;
     a.dim = dim;
+    a.rcp_dim = 1.0f / (float)dim;
     a.post_norm = post_eps >= 0.0f;
     a.post_weight = post_weight_dev;
     a.post_eps = post_eps;
