@@ -486,6 +486,7 @@ int zonos2cu_verify_drafts(const float *logits_dev, int n_streams, int n_draft, 
     a.rho = params->repetition_penalty;
     a.inv_rho = 1.0f / params->repetition_penalty;
     a.inv_temp = 1.0 / (double)params->temperature;
+    a.log2_scale = (float)(1.4426950408889634 * a.inv_temp);
     a.top_k = params->top_k;
     a.pad_id = params->pad_id;
     a.drafts = drafts_dev;

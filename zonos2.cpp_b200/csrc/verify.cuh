@@ -12,6 +12,7 @@ struct VerifyArgs {
     int n_streams, n_draft, n_cb, vocab;
     float temperature, top_p, min_p, rho, inv_rho;
     double inv_temp;
+    float log2_scale;         // log2(e) / temperature
     int top_k, pad_id;
     const int32_t *drafts;    // [n_streams][n_draft][n_cb]
     const float *probs;       // [n_streams][n_draft][n_cb][vocab] or nullptr: drafts are certain
