@@ -44,12 +44,19 @@ __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p)
                        __uint_as_float(u.y & 0xffff0000u));
 }
 
-// t[b][r], one warp per element.
-template <typename T>
+__device__ __forceinline__ float dot4(const float4 &a, const float4 &b)
+{
+    return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, a.x * b.x)));
+}
+
+// t[b][r], one warp per element.  VEC: as below.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kWarps)
     adapter_down_kernel(const HeadArgs h, const AdapterArgs ad)
 {
     using S = typename Acc<T>::type;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (i >= (long long)h.batch * ad.rank) return;
@@ -59,8 +66,13 @@ __global__ void __launch_bounds__(32 * kWarps)
     const T *x = static_cast<const T *>(h.hidden) + (size_t)b * h.dim;
     const T *w = static_cast<const T *>(ad.A) + ((size_t)a * ad.rank + r) * h.dim;
     S acc = 0;
+    if (VEC) {
 #pragma unroll 8
-    for (int d = lane; d < h.dim; d += 32) acc += (S)load_f(x + d) * (S)load_f(w + d);
+        for (int d = 4 * lane; d < h.dim; d += 128) acc += (S)dot4(load4(x + d), load4(w + d));
+    } else {
+#pragma unroll 8
+        for (int d = lane; d < h.dim; d += 32) acc += (S)load_f(x + d) * (S)load_f(w + d);
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(kFull, acc, o);
     if (lane == 0) static_cast<S *>(ad.work)[i] = acc * (S)(ad.scale ? __ldg(ad.scale + a) : 1.0f);
@@ -69,12 +81,16 @@ __global__ void __launch_bounds__(32 * kWarps)
 constexpr int kRows = 2;    // weight rows per warp
 constexpr int kBatch = 4;   // hidden rows at a time: a weight is read and widened once for four
 
-// The logits, one warp per kRows weight rows of one codebook.  An f32 head widens both
-// operands to f64 (exact products, one rounding at the end), and what bounds it beside
-// the reading of W are those conversions: kRows x kBatch products share them.  VEC: rows
-// 16-byte aligned (f32) or 8-byte aligned (bf16) and dim a multiple of 4.
+// The logits, one warp per kRows weight rows of one codebook.  VEC: rows 16-byte aligned
+// (f32) or 8-byte aligned (bf16) and dim a multiple of 4.  An f32 head's sums are f64, of
+// single products or (VEC) of four in f32: their roundings, half a step of the products each,
+// average out over dim / 4 terms, and the conversions, of which an SM makes 16 a cycle,
+// are few: widening both operands takes six times as many.  Four blocks an SM (64 registers)
+// hold all of a head's 4608 warps at once, and W's part runs beside adapter_down_kernel.
+// 4 rows by 9216 x 2048 f32 with rank 12: 23.5 us, 3.3 TB/s; 52 us with widened operands,
+// two blocks an SM and the kernels one after the other, 104 us with a row and a warp each.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(32 * kWarps)
+__global__ void __launch_bounds__(32 * kWarps, 4)
     adapter_any_kernel(const HeadArgs h, const AdapterArgs ad)
 {
     using S = typename Acc<T>::type;
@@ -87,24 +103,23 @@ __global__ void __launch_bounds__(32 * kWarps)
     const int second = rows > 1 ? h.dim : 0;   // offset of the second row
     for (int b0 = 0; b0 < h.batch; b0 += kBatch) {
         const T *x[kBatch];
+        int id[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; i++)
-            x[i] = static_cast<const T *>(h.hidden) + (size_t)min(b0 + i, h.batch - 1) * h.dim;
+        for (int i = 0; i < kBatch; i++) {
+            const int b = min(b0 + i, h.batch - 1);
+            x[i] = static_cast<const T *>(h.hidden) + (size_t)b * h.dim;
+            id[i] = ad.which[b / ad.rows_per_id];
+        }
         S acc[kRows][kBatch] = {};
         if (VEC) {
-#pragma unroll 2
+#pragma unroll 4
             for (int d = 4 * lane; d < h.dim; d += 128) {
                 const float4 w0 = load4(w + d), w1 = load4(w + second + d);
-                const S u0[4] = {(S)w0.x, (S)w0.y, (S)w0.z, (S)w0.w}, u1[4] = {(S)w1.x, (S)w1.y, (S)w1.z, (S)w1.w};
 #pragma unroll
                 for (int i = 0; i < kBatch; i++) {
                     const float4 f = load4(x[i] + d);
-                    const S y[4] = {(S)f.x, (S)f.y, (S)f.z, (S)f.w};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        acc[0][i] += u0[j] * y[j];
-                        acc[1][i] += u1[j] * y[j];
-                    }
+                    acc[0][i] += (S)dot4(w0, f);
+                    acc[1][i] += (S)dot4(w1, f);
                 }
             }
         } else {
@@ -118,25 +133,28 @@ __global__ void __launch_bounds__(32 * kWarps)
                 }
             }
         }
+        // W's part needed nothing of adapter_down_kernel's, which ran beside it.
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (int r = lane; r < ad.rank; r += 32) {
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) {
+                if (b0 + i >= h.batch || (unsigned)id[i] >= (unsigned)ad.n_adapters) continue;
+                const T *up = static_cast<const T *>(ad.B) + ((size_t)id[i] * h.n_cb * h.rows_per_cb + n) * ad.rank + r;
+                const S t = static_cast<const S *>(ad.work)[(size_t)(b0 + i) * ad.rank + r];
+                acc[0][i] += (S)load_f(up) * t;
+                if (rows > 1) acc[1][i] += (S)load_f(up + ad.rank) * t;
+            }
+        }
         float l[kRows][kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            const int b = b0 + i;
-            if (b >= h.batch) break;
-            const int a = ad.which[b / ad.rows_per_id];
-            const bool has = (unsigned)a < (unsigned)ad.n_adapters;
 #pragma unroll
             for (int m = 0; m < kRows; m++) {
                 S sum = acc[m][i];
-                if (has && m < rows) {
-                    const T *up = static_cast<const T *>(ad.B) + ((size_t)a * h.n_cb * h.rows_per_cb + n + m) * ad.rank;
-                    const S *t = static_cast<const S *>(ad.work) + (size_t)b * ad.rank;
-                    for (int r = lane; r < ad.rank; r += 32) sum += (S)load_f(up + r) * t[r];
-                }
 #pragma unroll
                 for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(kFull, sum, s);
                 float f = (float)sum;
-                if (h.row_scale) f *= __ldg(h.row_scale + b);
+                if (h.row_scale) f *= __ldg(h.row_scale + min(b0 + i, h.batch - 1));
                 l[m][i] = h.softcap > 0.0f ? h.softcap * tanhf(f / h.softcap) : f;
             }
         }
@@ -158,21 +176,31 @@ __global__ void __launch_bounds__(32 * kWarps)
     }
 }
 
+template <class Kernel>
+cudaError_t launch(Kernel kernel, long long warps, const HeadArgs &h, const AdapterArgs &ad, cudaStream_t stream)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((warps + kWarps - 1) / kWarps));
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, h, ad);
+}
+
 template <typename T>
 cudaError_t launch_any(const HeadArgs &h, const AdapterArgs &ad, cudaStream_t stream)
 {
-    const long long down = (long long)h.batch * ad.rank;
-    adapter_down_kernel<T><<<(unsigned)((down + kWarps - 1) / kWarps), 32 * kWarps, 0, stream>>>(h, ad);
-    cudaError_t e = cudaGetLastError();
+    const auto fits = [&](const void *p) { return h.dim % 4 == 0 && (uintptr_t)p % (4 * sizeof(T)) == 0; };
+    const long long down = (long long)h.batch * ad.rank, warps = (long long)h.n_cb * ((h.vocab + kRows - 1) / kRows);
+    const cudaError_t e = fits(ad.A) && fits(h.hidden) ? launch(adapter_down_kernel<T, true>, down, h, ad, stream)
+                                                       : launch(adapter_down_kernel<T, false>, down, h, ad, stream);
     if (e != cudaSuccess) return e;
-    const int warps = h.n_cb * ((h.vocab + kRows - 1) / kRows);
-    const unsigned blocks = (unsigned)((warps + kWarps - 1) / kWarps);
-    const bool vec = h.dim % 4 == 0 && (uintptr_t)h.W % (4 * sizeof(T)) == 0 && (uintptr_t)h.hidden % (4 * sizeof(T)) == 0;
-    if (vec)
-        adapter_any_kernel<T, true><<<blocks, 32 * kWarps, 0, stream>>>(h, ad);
-    else
-        adapter_any_kernel<T, false><<<blocks, 32 * kWarps, 0, stream>>>(h, ad);
-    return cudaGetLastError();
+    return fits(h.W) && fits(h.hidden) ? launch(adapter_any_kernel<T, true>, warps, h, ad, stream)
+                                       : launch(adapter_any_kernel<T, false>, warps, h, ad, stream);
 }
 
 }  // namespace
