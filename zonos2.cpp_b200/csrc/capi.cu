@@ -471,8 +471,13 @@ int zonos2cu_verify_drafts(const float *logits_dev, int n_streams, int n_draft, 
     if (!logits_dev || !uniforms_dev || !codes_dev || !n_accepted_dev ||
         (n_draft > 0 && !drafts_dev))
         return ZONOS2CU_EINVAL;
-    if ((uintptr_t)logits_dev % 4 || (uintptr_t)draft_probs_dev % 4 || (uintptr_t)uniforms_dev % 4)
-        return ZONOS2CU_EINVAL;
+    for (const void *p : {(const void *)logits_dev, (const void *)draft_probs_dev,
+                          (const void *)uniforms_dev, (const void *)drafts_dev,
+                          (const void *)n_drafts_dev, (const void *)hist_dev,
+                          (const void *)hist_pos_dev, (const void *)allow_dev,
+                          (const void *)codes_dev, (const void *)n_accepted_dev,
+                          (const void *)flags_dev})
+        if ((uintptr_t)p % 4) return ZONOS2CU_EINVAL;
     z2::VerifyArgs a{};
     a.logits = logits_dev;
     a.row_stride = row_stride;
@@ -1025,8 +1030,10 @@ int zonos2cu_set_adapters(zonos2cu_ctx *c, const void *A_host, const void *B_hos
     c->n_adapters = n_adapters;
     c->adapter_rank = rank;
     c->adapter_dtype = dtype;
-    const int rc = ensure_adapter_delta(c);
-    return rc ? rc : refold_head(c);
+    int rc = ensure_adapter_delta(c);
+    if (!rc) rc = refold_head(c);
+    if (rc) free_adapters(c);
+    return rc;
 }
 
 int zonos2cu_set_stream_adapters(zonos2cu_ctx *c, const int32_t *ids_host)

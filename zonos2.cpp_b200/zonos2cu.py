@@ -289,11 +289,16 @@ def _rows(t, what: str) -> int:
 
 
 def _whole(what: str, *tensors) -> None:
-    """Each tensor of the (tensor, elements) pairs, where given, is contiguous and of that size."""
-    for t, n in tensors:
-        if t is not None and (t.numel() != n or not t.is_contiguous()):
+    """Each tensor of the (tensor, elements, types) triples, where given, is contiguous, of that
+    size and of one of those types."""
+    for t, n, types in tensors:
+        if t is None:
+            continue
+        if t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{what}: a contiguous tensor of {n} elements expected, got "
                              f"{tuple(t.shape)}")
+        if t.dtype not in types:
+            raise TypeError(f"{what}: {' or '.join(map(str, types))} expected, got {t.dtype}")
 
 
 def head_adapters_work(dtype: int, batch: int, rank: int) -> int:
@@ -312,8 +317,11 @@ def head_adapters(W, dtype: int, rows_per_cb: int, n_cb: int, vocab: int, hidden
     batch, dim = hidden.shape
     n, rank, _ = A.shape
     wide = n_cb * rows_per_cb
-    _whole("head_adapters", (W, wide * dim), (hidden, batch * dim), (A, n * rank * dim),
-           (B, n * wide * rank), (adapter, batch), (out, batch * n_cb * vocab), (scale, n))
+    import torch
+    own, f32 = (torch.bfloat16 if dtype == BF16 else torch.float32,), (torch.float32,)
+    _whole("head_adapters", (W, wide * dim, own), (hidden, batch * dim, own),
+           (A, n * rank * dim, own), (B, n * wide * rank, own), (adapter, batch, (torch.int32,)),
+           (out, batch * n_cb * vocab, f32), (scale, n, f32))
     _launch("zonos2cu_head_adapters", hidden, stream, W.data_ptr(), dtype, rows_per_cb, n_cb, vocab,
             dim, hidden.data_ptr(), batch, softcap, A.data_ptr(), B.data_ptr(), _ptr(scale), n,
             rank, adapter.data_ptr(), work.data_ptr(), work.numel() * work.element_size(),
@@ -369,14 +377,13 @@ def verify_drafts(logits, params: SampleParams, drafts, uniforms, codes, n_accep
     S, D1, Cb, stride = logits.shape
     V = stride if vocab is None else vocab
     H = 0 if hist is None else hist.shape[-1]
-    _whole("verify_drafts", (logits, S * D1 * Cb * stride), (drafts, S * (D1 - 1) * Cb),
-           (uniforms, 2 * S * D1 * Cb), (draft_probs, S * (D1 - 1) * Cb * V), (n_drafts, S),
-           (codes, S * D1 * Cb), (flags, S * D1 * Cb), (n_accepted, S), (hist, S * Cb * H),
-           (hist_pos, S), (allow, S * ((V + 31) // 32)))
-    for t in (logits, drafts, uniforms, draft_probs, n_drafts, codes, flags, n_accepted, hist,
-              hist_pos, allow):
-        if t is not None and t.element_size() != 4:
-            raise TypeError("verify_drafts: f32 and int32 tensors expected")
+    import torch
+    f32, i32, bits = (torch.float32,), (torch.int32,), (torch.int32, torch.uint32)
+    _whole("verify_drafts", (logits, S * D1 * Cb * stride, f32), (drafts, S * (D1 - 1) * Cb, i32),
+           (uniforms, 2 * S * D1 * Cb, f32), (draft_probs, S * (D1 - 1) * Cb * V, f32),
+           (n_drafts, S, i32), (codes, S * D1 * Cb, i32), (flags, S * D1 * Cb, i32),
+           (n_accepted, S, i32), (hist, S * Cb * H, i32), (hist_pos, S, i32),
+           (allow, S * ((V + 31) // 32), bits))
     _launch("zonos2cu_verify_drafts", logits, stream, logits.data_ptr(), S, D1 - 1, Cb, V, stride,
             C.byref(params), _ptr(drafts), _ptr(draft_probs), _ptr(n_drafts), _ptr(uniforms),
             _ptr(hist), H, _ptr(hist_pos), _ptr(allow), delay_step, _ptr(codes), _ptr(n_accepted),
