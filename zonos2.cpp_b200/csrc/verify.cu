@@ -373,16 +373,34 @@ __device__ __forceinline__ float4 row_vec(const float *row, int lane, int j)
     return *reinterpret_cast<const float4 *>(row + row_at(4 * (lane + 32 * j)));
 }
 
-// The code of a row by the candidates of buckets up to `last`, at most 32 K of them.
+// Whether a drafted code of weight et stands, for certain: the kept sum is at most `upper`, the
+// list's sum at least `lower`, and no more than `ge` of it lies in the order up to the code.
+__device__ __forceinline__ bool surely_stands(const VerifyArgs &a, const Row &r, float et, float ge, float lower,
+                                              float upper)
+{
+    const float q = r.q ? __ldg(r.q + r.t) : 1.0f;
+    return et > 0.0f && !(et < a.min_p * (1.0f + kMargin)) &&
+           (!(a.top_p < 1.0f) || (ge - et) + kMargin * upper <= a.top_p * lower) &&
+           (float)r.u0 * q * upper * (1.0f + 2.0f * kMargin) < et;
+}
+
+// The candidates are the logits from here on: one comparison with the buckets' edge.  Rounding
+// may put a logit at the edge on its other side, so they are counted again.
+__device__ __forceinline__ float bucket_edge(float top, int last, float scale)
+{
+    return __fsub_rn(top, __fdividef((float)last + 0.5f, scale));
+}
+
+// The code of a row by the candidates of buckets up to `last`, at most 32 K of them; `all` is
+// the row's sum where its list is the whole row and they do not cover it.
 template <int K>
 __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, List li, const float *row,
-                                             uint32_t *cand, float scale, int last, int full, bool *taken)
+                                             uint32_t *cand, float scale, int last, int full, float all,
+                                             bool *taken)
 {
     const int lane = threadIdx.x & 31;
     const float top = li.top;
-    // By one comparison with the buckets' edge: rounding may put a logit at the edge on its other
-    // side, so the candidates are counted again.
-    const float edge = __fsub_rn(top, __fdividef((float)last + 0.5f, scale));
+    const float edge = bucket_edge(top, last, scale);
     uint32_t pick = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -428,14 +446,11 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
             key[j] |= min((uint32_t)__fmul_rn(__fsub_rn(top, x[j]), fine), 4194302u) << 10;
         }
     }
-    // Without the order.  The kept sum lies below `upper`, the list's sum above `lower`
-    // (the buckets before the one where the list ends), and no more than `ge` stands in
-    // the order up to the drafted code.
-    float all = 0.0f;
     const bool f32 = a.log2_scale < 1e30f;
-    if (f32 && (li.covers ? r.drafted : li.whole && a.top_p < 1.0f)) {
-        const bool in = r.drafted && (unsigned)r.t < (unsigned)a.vocab;
-        const float xt = in ? row[row_at(r.t)] : INFINITY;
+    if (f32 && li.covers && r.drafted && (unsigned)r.t < (unsigned)a.vocab) {
+        // Without the order.  The kept sum lies below `upper`, the list's above `lower` (the
+        // buckets before the one where the list ends).
+        const float xt = row[row_at(r.t)];
         float upper = 0.0f, lower = 0.0f, ge = 0.0f;
 #pragma unroll
         for (int j = 0; j < K; j++) {
@@ -446,37 +461,11 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
                 if (x[j] >= xt) ge += e;
             }
         }
-        upper = warp_sum(upper);
-        bool sure = in, beyond = false;
-        if (li.covers) {
-            lower = warp_sum(lower);
-            sure = sure && (li.n == li.limit ? xt >= edge : gap_bucket(top, xt, scale) < full);
-        } else {   // the whole row is the list
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float4 v = row_vec(row, lane, j);
-                all += (power<float>(a, v.x, top) + power<float>(a, v.y, top)) +
-                       (power<float>(a, v.z, top) + power<float>(a, v.w, top));
-            }
-            all = warp_sum(all);
-            // whether the nucleus is certain to reach beyond the candidates: no use in sorting them
-            beyond = !(a.min_p > 0.0f) && upper < (a.top_p - 2.0f * kMargin) * all;
-            lower = upper = all;
-            sure = sure && xt >= edge;
+        if ((li.n == li.limit ? xt >= edge : gap_bucket(top, xt, scale) < full) &&
+            surely_stands(a, r, power<float>(a, xt, top), warp_sum(ge), warp_sum(lower), warp_sum(upper))) {
+            *taken = true;
+            return r.t;
         }
-        if (sure) {
-            const float et = power<float>(a, xt, top);
-            ge = warp_sum(ge);
-            const float q = r.q ? __ldg(r.q + r.t) : 1.0f;
-            sure = et > 0.0f && !(et < a.min_p * (1.0f + kMargin)) &&
-                   (!(a.top_p < 1.0f) || (ge - et) + kMargin * upper <= a.top_p * lower) &&
-                   (float)r.u0 * q * upper * (1.0f + 2.0f * kMargin) < et;
-            if (sure) {
-                *taken = true;
-                return r.t;
-            }
-        }
-        if (beyond) return kOutside;
     }
     sort_keys<K>(key, lane);
     int token[K];
@@ -530,9 +519,10 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
 
 // As above with 256 candidates: for few rows, and apart, so that its registers cost the others none.
 __device__ __noinline__ int by_more_candidates(const VerifyArgs &a, const Row &r, const List &li, const float *row,
-                                               uint32_t *cand, float scale, int last, int full, bool *taken)
+                                               uint32_t *cand, float scale, int last, int full, float all,
+                                               bool *taken)
 {
-    return by_candidates<8>(a, r, li, row, cand, scale, last, full, taken);
+    return by_candidates<8>(a, r, li, row, cand, scale, last, full, all, taken);
 }
 
 // The row (s, d, c): its code, its flag, and whether the drafted code stands.
@@ -697,19 +687,51 @@ __device__ __forceinline__ int verify_row(const VerifyArgs &a, long long s, int 
     // last whose cumulative count fits the candidates; the open bucket is never taken
     const int limit = li.limit;
     const int full = __reduce_add_sync(kFull, (c0 < limit) + (c1 < limit) + (c2 < limit) + (c3 < limit));
-    int tried = -1;
-#pragma unroll 1
-    for (int k = 4; k <= 8; k += 4) {
-        const int most = 32 * k;
+    int last[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int most = 128 << k;
         const int fits = __reduce_add_sync(kFull, (c0 <= most) + (c1 <= most) + (c2 <= most) +
                                                       (lane < 31 && c3 <= most)) - 1;
-        const int last = min(full, min(fits, kOpen - 1));
-        if (last <= tried) continue;
-        tried = last;
-        // not the list's end, and no cut that could lie before it: as in by_candidates
-        if (last < full && !(a.top_p < 1.0f ? li.whole : a.min_p > 0.0f)) continue;
-        const int code = k == 4 ? by_candidates<4>(a, r, li, row, cand, scale, last, full, taken)
-                                : by_more_candidates(a, r, li, row, cand, scale, last, full, taken);
+        last[k] = min(full, min(fits, kOpen - 1));
+    }
+    // With candidates that do not reach the list's end a cut has to lie inside, and top-p's
+    // needs the list's sum.
+    const bool cuts = a.top_p < 1.0f ? li.whole : a.min_p > 0.0f;
+    bool try_first = last[0] >= 0 && (last[0] == full || cuts);
+    bool try_second = last[1] > last[0] && (last[1] == full || cuts);
+    float all = 0.0f;
+    if (li.whole && a.top_p < 1.0f && last[0] < full && a.log2_scale < 1e30f) {
+        // A nucleus of the whole row: the masses of the row, of either set of candidates, and
+        // of the order up to the drafted code tell which of them it needs, or that the code stands.
+        const float edge0 = bucket_edge(top, last[0], scale), edge1 = bucket_edge(top, last[1], scale);
+        const bool in = r.drafted && (unsigned)r.t < (unsigned)V;
+        const float xt = in ? row[row_at(r.t)] : INFINITY;
+        float mass0 = 0.0f, mass1 = 0.0f, ge = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const float e = power<float>(a, x[i], top);
+            all += e;
+            if (x[i] >= edge0) mass0 += e;
+            if (x[i] >= edge1) mass1 += e;
+            if (x[i] >= xt) ge += e;
+        }
+        all = warp_sum(all);
+        if (in && surely_stands(a, r, power<float>(a, xt, top), warp_sum(ge), all, all)) {
+            *taken = true;
+            return r.t;
+        }
+        const float least = (a.top_p - 2.0f * kMargin) * all;
+        if (!(a.min_p > 0.0f)) {
+            try_first = try_first && warp_sum(mass0) >= least;
+            try_second = try_second && warp_sum(mass1) >= least;
+        }
+    }
+#pragma unroll 1
+    for (int k = 0; k < 2; k++) {
+        if (!(k ? try_second : try_first)) continue;
+        const int code = k ? by_more_candidates(a, r, li, row, cand, scale, last[1], full, all, taken)
+                           : by_candidates<4>(a, r, li, row, cand, scale, last[0], full, all, taken);
         if (code >= 0) return code;
         __syncwarp();
     }
