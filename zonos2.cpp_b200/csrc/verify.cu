@@ -851,8 +851,9 @@ cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream)
     // 64 streams that all refuse their first frame take 18.9 us, with this 15.7, 14.0 in order.
     const int parts = max(1, min(min(a.n_draft + 1, 8), sms / a.n_streams));
     if (a.n_cb > 9) return launch(verify_kernel<kSamplerCbMax, 1>, a, parts, stream);
-    // Three blocks an SM, at the price of some spills, where there are enough of them.
-    return a.n_streams > 2 * sms ? launch(verify_kernel<9, 3>, a, parts, stream)
+    // Three blocks an SM at the price of spills where two do not hold nearly all: 300 streams
+    // 60.9 us with three, 50.9 with two; 2048 streams 178 and 183.
+    return a.n_streams > 3 * sms ? launch(verify_kernel<9, 3>, a, parts, stream)
                                  : launch(verify_kernel<9, 2>, a, parts, stream);
 }
 
