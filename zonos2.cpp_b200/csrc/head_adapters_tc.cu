@@ -55,7 +55,7 @@ __host__ __device__ constexpr int max_items(int batch, int n_adapters)
     return batch / kItem + (batch <= n_adapters ? batch : n_adapters + 1);
 }
 
-constexpr int kOrderRows = 256;   // rows per CTA
+constexpr int kOrderRows = 128;   // rows per CTA
 constexpr size_t order_bytes(int n_adapters) { return 2 * sizeof(int) * (size_t)(n_adapters + 1); }
 
 // CTA `block` of those that order the rows (of at most 256 threads): it counts all rows
@@ -64,7 +64,7 @@ __device__ __forceinline__ void order_rows(const int32_t *which, int batch, int 
                                            int block, int *s_count)
 {
     __shared__ int s_part[2][8];
-    __shared__ int s_key[kOrderRows];
+    __shared__ __align__(16) int s_key[kOrderRows];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
     const int b0 = block * kOrderRows, rows = min(kOrderRows, batch - b0);
     int *s_before = s_count + n + 1;   // rows of each key (n: none) before this CTA's
@@ -77,7 +77,7 @@ __device__ __forceinline__ void order_rows(const int32_t *which, int batch, int 
     __syncthreads();
 #pragma unroll 4
     for (int i = tid; i < batch; i += threads) {
-        const int k = key_of(i);
+        const int k = batch <= kOrderRows ? s_key[i] : key_of(i);
         atomicAdd(&s_count[k], 1);
         if (i < b0) atomicAdd(&s_before[k], 1);
     }
@@ -127,7 +127,11 @@ __device__ __forceinline__ void order_rows(const int32_t *which, int batch, int 
     for (int i = tid; i < rows; i += threads) {   // after the rows with this key before this one
         const int mine = s_key[i];
         int same = 0;
-        for (int j = 0; j < i; j++) same += s_key[j] == mine;
+#pragma unroll 4
+        for (int j = 0; j < i; j += 4) {
+            const int4 k = *reinterpret_cast<const int4 *>(&s_key[j]);
+            same += (k.x == mine) + (k.y == mine && j + 1 < i) + (k.z == mine && j + 2 < i) + (k.w == mine && j + 3 < i);
+        }
         o.rows[s_count[mine] + s_before[mine] + same] = b0 + i;
     }
 }
@@ -150,55 +154,81 @@ struct DownArgs {
     int batch, dim, n_adapters, rank, rows_per_id;
     float *t;                       // [batch][rank]
     Order order;
-    int down_blocks;                // few rows: the blocks after these order the rows
+    int order_blocks;               // few rows: the first blocks order the rows
 };
 
-// Few rows: one warp per row and four ranks, which share the row's loads; the last blocks
-// order the rows.
+// Few rows: a CTA per row and four ranks, which share the row's loads, a quarter of the
+// depth per warp, so that all loads are in flight at once and done before the GEMM, which may
+// start after them, fills the memory's queues with W's: FIGURE.
+// The first blocks order the rows.
 constexpr int kFewWarps = 4;
 constexpr long long kFewMost = 8192;   // rows x ranks
 
 __global__ void __launch_bounds__(32 * kFewWarps) adapter_down_few_kernel(const DownArgs g)
 {
-    const int lane = threadIdx.x & 31, quads = g.rank / 4;   // rank is a multiple of 8
-    const int i = (int)blockIdx.x * kFewWarps + (int)(threadIdx.x >> 5);
+    __shared__ float s_sum[kFewWarps][4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quads = g.rank / 4;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if ((int)blockIdx.x >= g.down_blocks) {
+    if ((int)blockIdx.x < g.order_blocks) {
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         extern __shared__ int s_count[];
-        order_rows(g.which, g.batch, g.rows_per_id, g.n_adapters, g.order, (int)blockIdx.x - g.down_blocks, s_count);
+        order_rows(g.which, g.batch, g.rows_per_id, g.n_adapters, g.order, (int)blockIdx.x, s_count);
         return;
     }
-    if (i >= g.batch * quads) return;
-    const int b = i / quads, r0 = 4 * (i % quads);
+    const int block = (int)blockIdx.x - g.order_blocks, b = block / quads, r0 = 4 * (block % quads);
     const int a = __ldg(g.which + b / g.rows_per_id);
     if ((unsigned)a >= (unsigned)g.n_adapters) return;
+    const float s = g.scale ? __ldg(g.scale + a) : 1.0f;
     const uint4 *x = reinterpret_cast<const uint4 *>(g.hidden + (size_t)b * g.dim);
     const uint4 *w = reinterpret_cast<const uint4 *>(g.A + ((size_t)a * g.rank + r0) * g.dim);
     const int n = g.dim / 8;
     float acc[4] = {};
-#pragma unroll 2
-    for (int k = lane; k < n; k += 32) {
-        const uint4 xv = __ldg(x + k);
+    auto add = [&](const uint4 &xv, const uint4 (&wv)[4]) {
         const uint32_t xs[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const uint4 wv = __ldg(w + (size_t)r * n + k);
-            const uint32_t ws[4] = {wv.x, wv.y, wv.z, wv.w};
+            const uint32_t ws[4] = {wv[r].x, wv[r].y, wv[r].z, wv[r].w};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 acc[r] = fmaf(__uint_as_float(xs[j] << 16), __uint_as_float(ws[j] << 16), acc[r]);
                 acc[r] = fmaf(__uint_as_float(xs[j] & 0xffff0000u), __uint_as_float(ws[j] & 0xffff0000u), acc[r]);
             }
         }
+    };
+    constexpr int kAhead = 2, kStep = 32 * kFewWarps;   // 2048 deep: all of a lane's loads
+    uint4 xv[kAhead] = {}, wv[kAhead][4] = {};
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+        const int k = threadIdx.x + i * kStep;
+        if (k >= n) continue;
+        xv[i] = __ldg(x + k);
+#pragma unroll
+        for (int r = 0; r < 4; r++) wv[i][r] = __ldg(w + (size_t)r * n + k);
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) add(xv[i], wv[i]);
+    for (int k = threadIdx.x + kAhead * kStep; k < n; k += kStep) {
+        const uint4 xk = __ldg(x + k);
+        uint4 wk[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) wk[r] = __ldg(w + (size_t)r * n + k);
+        add(xk, wk);
     }
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
         for (int o = 16; o; o >>= 1) acc[r] += __shfl_xor_sync(kFull, acc[r], o);
-    const float s = g.scale ? __ldg(g.scale + a) : 1.0f;
     if (lane == 0)
-        *reinterpret_cast<float4 *>(g.t + (size_t)b * g.rank + r0) = make_float4(s * acc[0], s * acc[1], s * acc[2], s * acc[3]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) s_sum[warp][r] = acc[r];
+    __syncthreads();
+    if (threadIdx.x < 4) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kFewWarps; v++) sum += s_sum[v][threadIdx.x];
+        g.t[(size_t)b * g.rank + r0 + threadIdx.x] = s * sum;
+    }
 }
 
 constexpr int kDownRows = 32;    // rows per CTA
@@ -1147,8 +1177,8 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     const unsigned order_blocks = (unsigned)((h.batch + kOrderRows - 1) / kOrderRows);
     cfg.dynamicSmemBytes = order_bytes(ad.n_adapters);
     if ((long long)h.batch * ad.rank <= kFewMost) {
-        d.down_blocks = (h.batch * (ad.rank / 4) + kFewWarps - 1) / kFewWarps;
-        cfg.gridDim = dim3((unsigned)d.down_blocks + order_blocks);
+        d.order_blocks = (int)order_blocks;
+        cfg.gridDim = dim3(order_blocks + (unsigned)(h.batch * (ad.rank / 4)));
         cfg.blockDim = dim3(32 * kFewWarps);
         e = cudaLaunchKernelEx(&cfg, adapter_down_few_kernel, d);
     } else {
