@@ -15,12 +15,16 @@
 // Everything is as good as f32: t enters its MMA as three bf16 parts, which hold all
 // of its 24 bits, and the GEMM's depth is summed in parts (kPartSteps).
 //
-// Measured (9 x 1024 x 2048, 32 adapters, rank 16, in a graph): delta in the GEMM against
-// the separate kernel 16 / 26 us at 1 row, 27 / 34 at 64, 284 / 224 at 4096: with more than
-// a few rows per SM, the warps' latency per adapter exceeds the tile's MMAs.  Slower still
-// at 4096 rows: added in the epilogue on the FMA pipe, t broadcast from shared memory (16 B
-// per 512 B of register writes), 370-540 us; hidden rows gathered by adapter with TMA
-// gather4 (a quarter of the plain copies' rate), 540 us.
+// Measured (9 x 1024 x 2048, 32 adapters, rank 16, in a graph): 14.8 us at 1 row (38 MB of
+// weights, 2.6 TB/s), 19.7 at 64, 33 at 333, 57 at 1024, 188 at 4096 (155 GFLOP, 0.82
+// PFLOP/s; 145 where no row has an adapter).
+// Up to 64 rows the GEMM's stream of W bounds it, beyond a few hundred the MMAs, and
+// between them the chain of three kernels.  Delta in the GEMM against the separate kernel
+// measured 16 / 26 us at 1 row, 27 / 34 at 64, 284 / 224 at 4096, when both were first built:
+// with more than a few rows per SM, the warps' latency per adapter exceeds the tile's MMAs.
+// Slower still at 4096 rows: added in the epilogue on the FMA pipe, t broadcast from shared
+// memory (16 B per 512 B of register writes), 370-540 us; hidden rows gathered by adapter
+// with TMA gather4 (a quarter of the plain copies' rate), 540 us.
 #include <cuda_bf16.h>
 #include <limits.h>
 #include <math.h>
@@ -158,11 +162,16 @@ struct DownArgs {
 };
 
 // Few rows: a CTA per row and four ranks, which share the row's loads, a quarter of the
-// depth per warp, so that all loads are in flight at once and done before the GEMM, which may
-// start after them, fills the memory's queues with W's: FIGURE.
+// depth per warp, so that all loads are in flight at once and ahead of those of the GEMM,
+// which may start after them and whose copies of W fill the memory's queues.  64 rows of
+// 2048, rank 16: t is there after 2.2 us; with a warp per CTA's work, its loads behind W's,
+// after 11.5 us, and the whole call took 25.7 us instead of 19.7.
 // The first blocks order the rows.
+// Up to kFewMost rows x ranks the loads of A by every row (from L2) cost less than the
+// ordering as a step of its own: 1024 x 16 57 us against 70 by adapter_down_mma_kernel,
+// 2048 x 16 102 / 105, 4096 x 16 196 / 189.
 constexpr int kFewWarps = 4;
-constexpr long long kFewMost = 8192;   // rows x ranks
+constexpr long long kFewMost = 32768;   // rows x ranks
 
 __global__ void __launch_bounds__(32 * kFewWarps) adapter_down_few_kernel(const DownArgs g)
 {
