@@ -14,8 +14,8 @@
 //
 // Bound: memory.  A row is read once (residual, block output, gate) and written
 // twice; it stays in registers between its two reductions.  16384 bf16 rows of 2048 with a
-// full sigmoid gate (336 MB): 60 us, 5.6 TB/s; 297 us by block_norm_any_kernel, which
-// re-reads the row and works element by element.  The issue slots come next: with
+// full sigmoid gate (336 MB): 59 us, 5.7 TB/s; 297 us by block_norm_any_kernel, which
+// re-reads the row and works element by element (now rows past 8192).  The issue slots come next: with
 // full-precision divisions and exponentials everywhere the same bytes took 83 us, so the
 // reciprocal root, the sigmoid and the join of a row's partial sums are kept short.
 #include <cuda_bf16.h>
@@ -113,10 +113,42 @@ __device__ __forceinline__ uint4 narrow(const float (&f)[8])
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A vector of 16 bytes per thread, blockDim.x / 32 warps per row (threadIdx.y: the row
-// within the block).  A block walks over rows a grid apart, so that its weights are loaded
-// once, into registers, and the next row's loads are under way while this one is reduced;
-// each reduction costs one barrier, its partial sums alternating between two buffers.
+// The sum over a row's threads, in each of them; blockDim.x / 32 warps make a row, and
+// threadIdx.y is the row within the block.  One barrier, the block's: the partial sums
+// alternate between two buffers.
+struct RowSum {
+    float4 (*part)[8];
+    int warps, first, warp, lane, buf;
+
+    __device__ __forceinline__ RowSum(float4 (*p)[8]) : part(p), buf(0)
+    {
+        warps = blockDim.x >> 5;
+        lane = threadIdx.x & 31;
+        first = threadIdx.y * ((warps + 3) >> 2);
+        warp = 4 * first + (threadIdx.x >> 5);
+        if (threadIdx.y == 0 && threadIdx.x < 32) reinterpret_cast<float2 *>(part)[lane] = make_float2(0.0f, 0.0f);
+        __syncthreads();   // places past a row's warps stay zero
+    }
+    __device__ __forceinline__ float operator()(float v)
+    {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+        if (warps == 1) return v;
+        if (lane == 0) reinterpret_cast<float *>(part[buf])[warp] = v;
+        __syncthreads();
+        v = 0.0f;
+        for (int i = 0; i < warps; i += 4) {
+            const float4 p = part[buf][first + (i >> 2)];
+            v += (p.x + p.y) + (p.z + p.w);
+        }
+        buf ^= 1;
+        return v;
+    }
+};
+
+// A vector of 16 bytes per thread.  A block walks over rows a grid apart, so that its weights
+// are loaded once, into registers, and the next row's loads are under way while this one is
+// reduced.
 template <typename T>
 __global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
 {
@@ -124,10 +156,7 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
     __shared__ float4 part[2][8];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    const int first = threadIdx.y * ((warps + 3) >> 2), warp = 4 * first + (threadIdx.x >> 5);
-    if (threadIdx.y == 0 && threadIdx.x < 32) reinterpret_cast<float2 *>(part)[lane] = make_float2(0.0f, 0.0f);
-    __syncthreads();   // part's places past a row's warps stay zero
+    RowSum row_sum(part);
     const int d = threadIdx.x * V;
     const bool in_row = d < a.dim;
     const bool by_row = a.gate && !a.gate_col_stride, by_elem = a.gate && a.gate_col_stride;
@@ -156,21 +185,6 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
         wp[j] = p.x, wp[j + 1] = p.y, wp[j + 2] = p.z, wp[j + 3] = p.w;
         wn[j] = n.x, wn[j + 1] = n.y, wn[j + 2] = n.z, wn[j + 3] = n.w;
     }
-    int buf = 0;
-    auto row_sum = [&](float v) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-        if (warps == 1) return v;
-        if (lane == 0) reinterpret_cast<float *>(part[buf])[warp] = v;
-        __syncthreads();
-        v = 0.0f;
-        for (int i = 0; i < warps; i += 4) {
-            const float4 p = part[buf][first + (i >> 2)];
-            v += (p.x + p.y) + (p.z + p.w);
-        }
-        buf ^= 1;
-        return v;
-    };
     // By the block's first row: all its threads take the same number of turns and barriers.
     for (uint32_t r0 = blockIdx.x * blockDim.y; r0 < rows; r0 += step, row += step) {
         float s[V];
@@ -220,7 +234,75 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const BlockNormArgs a)
     }
 }
 
-// One block per row, elements one by one, the row re-read (from L1 or L2) by
+// E elements per thread, blockDim.x apart: any stride and alignment, rows up to 8192.  The loads
+// in flight are those of an SM's other rows.  16384 rows of 1023: bf16 61 us (issue slots: a
+// load and a store per element), f32 61 us, 5.5 TB/s; block_norm_any_kernel 110 and 122 us.
+template <typename T, int E>
+__global__ void __launch_bounds__(1024) block_norm_odd_kernel(const BlockNormArgs a)
+{
+    __shared__ float4 part[2][8];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    RowSum row_sum(part);
+    const uint32_t step = gridDim.x * blockDim.y, rows = a.rows;
+    uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
+    const int dim = a.dim, d0 = threadIdx.x, stride = blockDim.x;
+    float wp[E], wn[E];
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+        const int d = d0 + j * stride;
+        wp[j] = a.post_weight && d < dim ? __ldg(a.post_weight + d) : 1.0f;
+        wn[j] = a.norm_weight && d < dim ? __ldg(a.norm_weight + d) : 1.0f;
+    }
+    for (uint32_t r0 = blockIdx.x * blockDim.y; r0 < rows; r0 += step, row += step) {
+        const int end = row < rows ? dim : 0;
+        const T *yp = static_cast<const T *>(a.block) + (size_t)row * a.block_stride + d0;
+        const T *xp = static_cast<const T *>(a.resid) + (size_t)row * a.resid_stride + d0;
+        const T *gp = static_cast<const T *>(a.gate) + (size_t)row * a.gate_row_stride + (size_t)d0 * a.gate_col_stride;
+        T y[E], x[E], g[E];
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            const bool in = d0 + j * stride < end;
+            y[j] = x[j] = g[j] = from_f<T>(0.0f);
+            if (in) y[j] = yp[j * stride];
+            if (in && a.gate) g[j] = gp[j * stride * a.gate_col_stride];
+            if (in) x[j] = xp[j * stride];
+        }
+        float s[E], ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            s[j] = to_f<T>(y[j]);
+            ss = fmaf(s[j], s[j], ss);
+        }
+        if (a.post_norm) {
+            const float rcp = rcp_rms(row_sum(ss), a, a.post_eps);
+#pragma unroll
+            for (int j = 0; j < E; j++) s[j] = s[j] * rcp * wp[j];
+        }
+        if (a.gate) {
+#pragma unroll
+            for (int j = 0; j < E; j++) s[j] *= a.gate_sigmoid ? sigmoid<T>(to_f<T>(g[j])) : to_f<T>(g[j]);
+        }
+        T *ro = static_cast<T *>(a.resid_out) + (size_t)row * a.out_stride + d0;
+        T *no = static_cast<T *>(a.normed_out) + (size_t)row * a.out_stride + d0;
+        ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            const bool in = d0 + j * stride < end;
+            s[j] = fmaf(a.scale, s[j], to_f<T>(x[j]));
+            if (in) ss = fmaf(s[j], s[j], ss);
+            if (in && a.resid_out) ro[j * stride] = from_f<T>(s[j]);
+        }
+        if (a.normed_out) {
+            const float rcp = rcp_rms(row_sum(ss), a, a.norm_eps);
+#pragma unroll
+            for (int j = 0; j < E; j++)
+                if (d0 + j * stride < end) no[j * stride] = from_f<T>(s[j] * rcp * wn[j]);
+        }
+    }
+}
+
+// Longer rows still: one block per row, elements one by one, the row re-read (from L1 or L2) by
 // each of its reductions: any size, stride and alignment.
 template <typename T>
 __global__ void __launch_bounds__(1024) block_norm_any_kernel(const BlockNormArgs a)
@@ -283,20 +365,21 @@ cudaError_t launch(Kernel kernel, unsigned grid, dim3 block, const BlockNormArgs
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <typename T>
-cudaError_t launch_vec(const BlockNormArgs &a, cudaStream_t stream)
+// Rows of `x` threads each, on all SMs; short rows share a block of up to 256 threads, unless
+// there are too few of them for that.
+template <class Kernel>
+cudaError_t launch_rows(Kernel kernel, int x, const BlockNormArgs &a, cudaStream_t stream)
 {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
-    const int x = (a.dim / kVec<T> + 31) & ~31;
-    // Short rows share a block of up to 256 threads, unless there are too few for all SMs.
+    x = (x + 31) & ~31;
     int y = x < 256 ? 256 / x : 1;
     while (y > 1 && a.rows < (long long)sms * y) y--;
-    const int blocks = (a.rows + y - 1) / y;
+    const int blocks = (a.rows - 1) / y + 1;
     const int most = sms * max(1, 1024 / (x * y));   // at a time: 1024 threads of 64 registers an SM
-    return launch(block_norm_kernel<T>, (unsigned)min(blocks, most), dim3(x, y), a, stream);
+    return launch(kernel, (unsigned)min(blocks, most), dim3(x, y), a, stream);
 }
 
 template <typename T>
@@ -308,7 +391,11 @@ cudaError_t launch_type(const BlockNormArgs &a, cudaStream_t stream)
     const bool vec = a.dim % kVec<T> == 0 && fits(a.resid, a.resid_stride) && fits(a.block, a.block_stride) &&
                      (a.gate_col_stride ? fits(a.gate, a.gate_row_stride) : a.gate_row_stride <= INT32_MAX) && fits(a.resid_out, a.out_stride) &&
                      fits(a.normed_out, a.out_stride) && fits(a.post_weight, 0) && fits(a.norm_weight, 0);
-    if (vec && a.dim <= 1024 * kVec<T>) return launch_vec<T>(a, stream);
+    if (vec && a.dim <= 1024 * kVec<T>) return launch_rows(block_norm_kernel<T>, a.dim / kVec<T>, a, stream);
+    // One warp a row up to 256 elements.
+    if (a.dim <= 32) return launch_rows(block_norm_odd_kernel<T, 1>, a.dim, a, stream);
+    if (a.dim <= 64) return launch_rows(block_norm_odd_kernel<T, 2>, (a.dim + 1) / 2, a, stream);
+    if (a.dim <= 8192) return launch_rows(block_norm_odd_kernel<T, 8>, (a.dim + 7) / 8, a, stream);
     int threads = 32;
     while (threads < 1024 && threads * 4 < a.dim) threads *= 2;
     return launch(block_norm_any_kernel<T>, (unsigned)a.rows, dim3(threads), a, stream);
