@@ -169,9 +169,10 @@ int zonos2cu_head_softcap(const void *W_dev, zonos2cu_dtype dtype, int rows_per_
  *                zonos2cu_head_adapters_work(dtype, batch, rank) (8 bytes per row and
  *                rank always suffice).  Calls that may overlap need scratch of their own.
  * A h is kept in f32 beside a bf16 head and in f64 beside an f32 one, whose result
- * is rounded once.  Any dim, vocab and rank (<= ZONOS2CU_MAX_RANK); the bf16
- * tensor-core kernel runs where dim % 8 == 0, rank % 8 == 0 and W, hidden, A and B
- * are 16-byte aligned, a slower kernel elsewhere. */
+ * is rounded once (its products are summed by fours in f32 before).  Any dim, vocab
+ * and rank (<= ZONOS2CU_MAX_RANK); the bf16 tensor-core kernels run where dim % 8 ==
+ * 0, rank % 8 == 0, n_adapters <= 4096 and W, hidden, A and B are 16-byte aligned, a
+ * slower kernel elsewhere. */
 #define ZONOS2CU_MAX_RANK 256
 long long zonos2cu_head_adapters_work(zonos2cu_dtype dtype, int batch, int rank);
 int zonos2cu_head_adapters(const void *W_dev, zonos2cu_dtype dtype, int rows_per_cb, int n_cb,

@@ -255,6 +255,70 @@ def test_context_step_with_output_norm(z2, cuda, dtype, S, weight):
     ctx.close()
 
 
+@pytest.mark.parametrize("S", [4, 150])
+def test_context_calls_in_any_order(z2, cuda, S):
+    """Norm, head and adapters set in either order and set again give the same bits; without norm and
+    adapters they are those of a context that never had them; host and captured steps agree."""
+    import torch
+    n, rank, D, C, V = 3, 16, 512, 3, 256
+    c = _case(cuda, "bf16", S, C, V, V, D, n, rank, S, low=0.3)
+    W, A, B, sc = _bits(c["W"]), _bits(c["A"]), _bits(c["B"]), c["scale"].cpu().numpy()
+    rs = np.random.default_rng(S)
+    gamma, other = (rs.normal(1, 0.1, D).astype(np.float32) for _ in range(2))
+    ids = rs.integers(-1, n, S).astype(np.int32)
+    p = z2.SampleParams(0.7, 50, 0.9, 0.02, 1.0, V - 1)
+    codes = torch.zeros((S, C), dtype=torch.int32, device=cuda)
+
+    def logits(ctx):
+        out = torch.zeros((S, C, V), device=cuda)
+        ctx.step(c["h"], z2.BF16, p, codes, logits_out=out)
+        torch.cuda.synchronize()
+        return out
+
+    def adapt(ctx, a=A):
+        ctx.set_adapters(a, B, V, z2.BF16, sc)
+        ctx.set_stream_adapters(ids)
+
+    one, two, bare = (z2.Context(0, S, C, V, D, 0, seed=5) for _ in range(3))
+    for ctx in (one, two, bare):
+        ctx.set_head(W, z2.BF16, V)
+    one.set_out_norm(gamma, 1e-5)
+    adapt(one)
+    adapt(two, A[::-1].copy())
+    two.set_out_norm(other, 1e-5)
+    logits(two)
+    adapt(two)
+    two.set_out_norm(gamma, 1e-5)
+    two.set_head(W, z2.BF16, V)
+    first = logits(one)
+    assert torch.equal(first, logits(two))
+    host = np.zeros((S, C), np.int32)
+    one.set_rng(two.get_rng())
+    one.step_host(_bits(c["h"]), z2.BF16, p, host)
+    two.step(c["h"], z2.BF16, p, codes)
+    torch.cuda.synchronize()
+    assert np.array_equal(host, codes.cpu().numpy())
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros((S, C, V), device=cuda)
+    with torch.cuda.graph(graph):
+        one.step(c["h"], z2.BF16, p, codes, logits_out=out)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+    one.set_out_norm(enable=False)
+    one.set_stream_adapters(None)
+    two.set_out_norm(enable=False)
+    two.set_adapters(None, None, 0, z2.BF16)
+    plain = logits(bare)
+    assert torch.equal(plain, logits(two))
+    # no row has an adapter: the adapters' GEMM, within the sums' roundings of the head's own
+    c["ids"] = torch.full((S,), -1, dtype=torch.int32, device=cuda)
+    _check(c, logits(one))
+    assert z2.device_error() == 0
+    for ctx in (one, two, bare):
+        ctx.close()
+
+
 def test_another_head_type_is_refused(z2, cuda):
     import torch
     c = _case(cuda, "bf16", 2, 2, 64, 64, 64, 2, 8, 1)

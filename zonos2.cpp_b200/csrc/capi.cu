@@ -645,9 +645,8 @@ int grow(void **p, size_t *cap, size_t want)
 
 // The bf16 head with the output norm's weight folded into its columns, when both
 // are set (synchronises the context's stream).
-int refold_head(zonos2cu_ctx *c)
+int fold_norm(zonos2cu_ctx *c)
 {
-    if (!c->norm_on || !c->norm_has_w) return ZONOS2CU_OK;
     if (c->n_adapters && c->adapter_dtype == ZONOS2CU_BF16) {   // the adapters' projections too
         const size_t n = (size_t)c->n_adapters * c->adapter_rank, D = (size_t)c->dims.dim;
         if (!c->adapter_a_folded) Z2_CK(cudaMalloc(&c->adapter_a_folded, 2 * n * D));
@@ -662,6 +661,14 @@ int refold_head(zonos2cu_ctx *c)
                                   c->stream));
     Z2_CK(cudaStreamSynchronize(c->stream));
     return ZONOS2CU_OK;
+}
+
+int refold_head(zonos2cu_ctx *c)
+{
+    if (!c->norm_on || !c->norm_has_w) return ZONOS2CU_OK;
+    const int rc = fold_norm(c);
+    if (rc) c->norm_on = false;   // a step would read what is not there
+    return rc;
 }
 
 void free_adapters(zonos2cu_ctx *c)
@@ -981,7 +988,9 @@ int zonos2cu_set_cfg(zonos2cu_ctx *c, int enable, float scale)
     Z2_CK(cudaDeviceSynchronize());   // no step may still be using the state
     c->cfg_on = enable != 0;
     c->cfg_scale = scale;
-    return ensure_adapter_delta(c);
+    const int rc = ensure_adapter_delta(c);
+    if (rc) c->cfg_on = false;   // a step would lack the buffer
+    return rc;
 }
 
 int zonos2cu_set_adapters(zonos2cu_ctx *c, const void *A_host, const void *B_host,
