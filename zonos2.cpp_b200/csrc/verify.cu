@@ -50,6 +50,8 @@ constexpr float kMaskedAll = -1e9f;   // a row without a logit at or above this 
 // 2.5e-6 (the gaps' error weighs a term by its share, and -sum p log p < 7 for 1024
 // tokens; ten levels of additions), the drafts' products and the cuts by three more roundings.
 constexpr float kMargin = 1e-5f;
+// A row's answer: the code, its flags and whether the drafted code stands.
+constexpr int kAllMasked = 1 << 16, kNonfinite = 2 << 16, kTaken = 1 << 30;
 constexpr int kOutside = -1;          // a candidate path's answer: the cuts lie outside
 constexpr int kClose = -2;            // f32 cannot decide
 // Per warp: the row by token (4 pad floats after every 32), then the general
@@ -141,8 +143,8 @@ __device__ __forceinline__ bool stands(const Row &r, int vocab, double e, double
 
 // The general path: the whole row sorted in shared memory (x at row_at, tokens at
 // tok_at), each lane owning n / 32 consecutive positions of the order.
-__device__ __noinline__ int general_row(const VerifyArgs &a, const Row &r, float *x, uint16_t *tok,
-                                        float top, int limit, bool *taken)
+__device__ __noinline__ int general_row(const VerifyArgs &a, const Row r, float *x, uint16_t *tok,
+                                        float top, int limit)
 {
     const int lane = threadIdx.x & 31;
     int n = 64;
@@ -187,8 +189,7 @@ __device__ __noinline__ int general_row(const VerifyArgs &a, const Row &r, float
     for (int i = i0; i < i0 + per && i < m; i++)
         if (tok[tok_at(i)] == r.t) et = value(i);
     et = warp_sum(et);   // one lane's, or none
-    *taken = stands(r, a.vocab, et, sum);
-    if (*taken) return r.t;
+    if (stands(r, a.vocab, et, sum)) return r.t | kTaken;
     bool residual = r.drafted;
     double total = 0.0;
     for (;;) {   // the residual's weights, or p's where they are all zero
@@ -261,7 +262,7 @@ struct List {
 // that is its own list without the candidates covering it.
 template <typename S, int K>
 __device__ __forceinline__ int decide(const VerifyArgs &a, const Row &r, const List &li, const float (&l)[K],
-                                      const int (&token)[K], S all, bool *taken)
+                                      const int (&token)[K], S all)
 {
     constexpr bool kExact = sizeof(S) == 8;
     const S margin = kExact ? (S)0 : (S)kMargin;
@@ -316,8 +317,7 @@ __device__ __forceinline__ int decide(const VerifyArgs &a, const Row &r, const L
         const bool in = (unsigned)r.t < (unsigned)a.vocab;
         const S q = !in ? (S)0 : r.q ? (S)__ldg(r.q + r.t) : (S)1, need = (S)r.u0 * q * sum;
         if (!kExact && in && fabs(need - et) <= margin * fmax(need, et)) return kClose;
-        *taken = in && need < et;
-        if (*taken) return r.t;
+        if (in && need < et) return r.t | kTaken;
         residual = true;
     }
     S w[K], total = sum;
@@ -395,8 +395,7 @@ __device__ __forceinline__ float bucket_edge(float top, int last, float scale)
 // the row's sum where its list is the whole row and they do not cover it.
 template <int K>
 __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, List li, const float *row,
-                                             uint32_t *cand, float scale, int last, int full, float all,
-                                             bool *taken)
+                                             uint32_t *cand, float scale, int last, int full, float all)
 {
     const int lane = threadIdx.x & 31;
     const float top = li.top;
@@ -463,8 +462,7 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
         }
         if ((li.n == li.limit ? xt >= edge : gap_bucket(top, xt, scale) < full) &&
             surely_stands(a, r, power<float>(a, xt, top), warp_sum(ge), warp_sum(lower), warp_sum(upper))) {
-            *taken = true;
-            return r.t;
+            return r.t | kTaken;
         }
     }
     sort_keys<K>(key, lane);
@@ -501,7 +499,7 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
         if (!__any_sync(kFull, moved)) break;
     }
     if (f32) {
-        const int code = decide<float, K>(a, r, li, l, token, all, taken);
+        const int code = decide<float, K>(a, r, li, l, token, all);
         if (code != kClose) return code;
     }
     double sum = 0.0;
@@ -514,20 +512,19 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
         }
         sum = warp_sum(sum);
     }
-    return decide<double, K>(a, r, li, l, token, sum, taken);
+    return decide<double, K>(a, r, li, l, token, sum);
 }
 
 // As above with 256 candidates: for few rows, and apart, so that its registers cost the others none.
-__device__ __noinline__ int by_more_candidates(const VerifyArgs &a, const Row &r, const List &li, const float *row,
-                                               uint32_t *cand, float scale, int last, int full, float all,
-                                               bool *taken)
+__device__ __noinline__ int by_more_candidates(const VerifyArgs &a, const Row r, const List li, const float *row,
+                                               uint32_t *cand, float scale, int last, int full, float all)
 {
-    return by_candidates<8>(a, r, li, row, cand, scale, last, full, all, taken);
+    return by_candidates<8>(a, r, li, row, cand, scale, last, full, all);
 }
 
 // The row (s, d, c): its code, its flag, and whether the drafted code stands.
 __device__ __forceinline__ int verify_row(const VerifyArgs &a, long long s, int d, int c, int pos,
-                                          bool drafted, unsigned char *mem, int *flag, bool *taken)
+                                          bool drafted, unsigned char *mem)
 {
     const int lane = threadIdx.x & 31;
     float *row = reinterpret_cast<float *>(mem);
@@ -637,11 +634,9 @@ __device__ __forceinline__ int verify_row(const VerifyArgs &a, long long s, int 
 #pragma unroll
     for (int i = 1; i < 32; i++) top = fmaxf(top, x[i]);
     top = warp_max(top);
-    *flag = __any_sync(kFull, odd) ? 2 : 0;
+    const int flag = __any_sync(kFull, odd) ? kNonfinite : 0;
     if (!(top >= kMaskedAll)) {   // all masked: pad_id is certain
-        *flag |= 1;
-        *taken = r.t == a.pad_id && stands(r, V, 1.0, 1.0);
-        return a.pad_id;
+        return a.pad_id | flag | kAllMasked | (r.t == a.pad_id && stands(r, V, 1.0, 1.0) ? kTaken : 0);
     }
 
     // ---- the row in shared memory, and the histogram of its gaps
@@ -718,8 +713,7 @@ __device__ __forceinline__ int verify_row(const VerifyArgs &a, long long s, int 
         }
         all = warp_sum(all);
         if (in && surely_stands(a, r, power<float>(a, xt, top), warp_sum(ge), all, all)) {
-            *taken = true;
-            return r.t;
+            return r.t | kTaken | flag;
         }
         const float least = (a.top_p - 2.0f * kMargin) * all;
         if (!(a.min_p > 0.0f)) {
@@ -730,13 +724,13 @@ __device__ __forceinline__ int verify_row(const VerifyArgs &a, long long s, int 
 #pragma unroll 1
     for (int k = 0; k < 2; k++) {
         if (!(k ? try_second : try_first)) continue;
-        const int code = k ? by_more_candidates(a, r, li, row, cand, scale, last[1], full, all, taken)
-                           : by_candidates<4>(a, r, li, row, cand, scale, last[0], full, all, taken);
-        if (code >= 0) return code;
+        const int code = k ? by_more_candidates(a, r, li, row, cand, scale, last[1], full, all)
+                           : by_candidates<4>(a, r, li, row, cand, scale, last[0], full, all);
+        if (code >= 0) return code | flag;
         __syncwarp();
     }
     __syncwarp();
-    return general_row(a, r, row, tok, top, limit, taken);
+    return general_row(a, r, row, tok, top, limit) | flag;
 }
 
 __device__ __forceinline__ void cluster_barrier()
@@ -776,7 +770,12 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kMinCtas)
         const int d = own;
         int flag = 0, code = -1;
         bool taken = false;
-        if (d <= drafted) code = verify_row(a, s, d, c, pos, d < drafted, mem, &flag, &taken);
+        if (d <= drafted) {
+            code = verify_row(a, s, d, c, pos, d < drafted, mem);
+            taken = code & kTaken;
+            flag = code / kAllMasked & 3;
+            code &= kAllMasked - 1;
+        }
         const int no = __syncthreads_or(!taken);
         if (parts == 1) {
             if (no) last = d;
