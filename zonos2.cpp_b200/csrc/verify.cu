@@ -106,7 +106,7 @@ struct Row {
     const float *q;     // the draft's probabilities of the row (nullptr: certain of t)
     int t;              // the drafted code
     bool drafted;
-    double u0, u1;
+    float u0, u1;
 };
 
 template <typename S>
@@ -138,7 +138,7 @@ __device__ __forceinline__ bool stands(const Row &r, int vocab, double e, double
 {
     if (!r.drafted || (unsigned)r.t >= (unsigned)vocab) return false;
     const double q = r.q ? (double)__ldg(r.q + r.t) : 1.0;
-    return r.u0 * q * sum < e;
+    return (double)r.u0 * q * sum < e;
 }
 
 // The general path: the whole row sorted in shared memory (x at row_at, tokens at
@@ -203,7 +203,7 @@ __device__ __noinline__ int general_row(const VerifyArgs &a, const Row r, float 
         residual = false;
     }
     run = warp_before(own, lane);
-    const double goal = r.u1 * total;
+    const double goal = (double)r.u1 * total;
     int first = n, last = -1;
     for (int i = i0; i < i0 + per && i < m; i++) {
         const double e = value(i);
@@ -373,6 +373,30 @@ __device__ __forceinline__ float4 row_vec(const float *row, int lane, int j)
     return *reinterpret_cast<const float4 *>(row + row_at(4 * (lane + 32 * j)));
 }
 
+// The rare rows that f32 cannot decide: apart, so that their registers cost the others none.
+template <int K>
+struct Ordered {
+    float l[K];
+    int token[K];
+};
+
+template <int K>
+__device__ __noinline__ int decide_exact(const VerifyArgs &a, const Row r, const List li, const Ordered<K> o,
+                                         const float *row)
+{
+    double all = 0.0;
+    if (a.top_p < 1.0f && !li.covers && li.whole) {
+#pragma unroll 1
+        for (int j = 0; j < 8; j++) {
+            const float4 v = row_vec(row, threadIdx.x & 31, j);
+            all += (power<double>(a, v.x, li.top) + power<double>(a, v.y, li.top)) +
+                   (power<double>(a, v.z, li.top) + power<double>(a, v.w, li.top));
+        }
+        all = warp_sum(all);
+    }
+    return decide<double, K>(a, r, li, o.l, o.token, all);
+}
+
 // Whether a drafted code of weight et stands, for certain: the kept sum is at most `upper`, the
 // list's sum at least `lower`, and no more than `ge` of it lies in the order up to the code.
 __device__ __forceinline__ bool surely_stands(const VerifyArgs &a, const Row &r, float et, float ge, float lower,
@@ -381,7 +405,7 @@ __device__ __forceinline__ bool surely_stands(const VerifyArgs &a, const Row &r,
     const float q = r.q ? __ldg(r.q + r.t) : 1.0f;
     return et > 0.0f && !(et < a.min_p * (1.0f + kMargin)) &&
            (!(a.top_p < 1.0f) || (ge - et) + kMargin * upper <= a.top_p * lower) &&
-           (float)r.u0 * q * upper * (1.0f + 2.0f * kMargin) < et;
+           r.u0 * q * upper * (1.0f + 2.0f * kMargin) < et;
 }
 
 // The candidates are the logits from here on: one comparison with the buckets' edge.  Rounding
@@ -502,17 +526,10 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
         const int code = decide<float, K>(a, r, li, l, token, all);
         if (code != kClose) return code;
     }
-    double sum = 0.0;
-    if (a.top_p < 1.0f && !li.covers && li.whole) {
-#pragma unroll 1
-        for (int j = 0; j < 8; j++) {
-            const float4 v = row_vec(row, lane, j);
-            sum += (power<double>(a, v.x, top) + power<double>(a, v.y, top)) +
-                   (power<double>(a, v.z, top) + power<double>(a, v.w, top));
-        }
-        sum = warp_sum(sum);
-    }
-    return decide<double, K>(a, r, li, l, token, sum);
+    Ordered<K> o;
+#pragma unroll
+    for (int j = 0; j < K; j++) o.l[j] = l[j], o.token[j] = token[j];
+    return decide_exact<K>(a, r, li, o, row);
 }
 
 // As above with 256 candidates: for few rows, and apart, so that its registers cost the others none.
@@ -560,8 +577,8 @@ __device__ __forceinline__ int verify_row(const VerifyArgs &a, long long s, int 
     r.drafted = drafted;
     r.t = drafted ? __ldg(a.drafts + (s * D + d) * C + c) : -1;
     r.q = drafted && a.probs ? a.probs + ((s * D + d) * C + c) * (long long)V : nullptr;
-    r.u0 = (double)__ldg(a.uniforms + 2 * at);
-    r.u1 = (double)__ldg(a.uniforms + 2 * at + 1);
+    r.u0 = __ldg(a.uniforms + 2 * at);
+    r.u1 = __ldg(a.uniforms + 2 * at + 1);
 
     // the penalty's tokens: the ring without its d oldest entries, and the frames
     // drafted before (the newest of them where they fill the ring)
