@@ -448,9 +448,11 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
 #pragma unroll
     for (int j = 0; j < K; j += 4) reinterpret_cast<uint4 *>(cand)[lane + 8 * j] = make_uint4(~0u, ~0u, ~0u, ~0u);
     __syncwarp();
+    uint32_t to = (uint32_t)__cvta_generic_to_shared(cand) + 4u * (uint32_t)place;
 #pragma unroll
-    for (int i = 0; i < 32; i++)
-        if ((pick >> i) & 1u) cand[place++] = 4 * lane + 128 * (i >> 2) + (i & 3);
+    for (int i = 0; i < 32; i++)   // predicated, without a branch per token
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.shared.u32 [%0], %1;\n\t@p add.u32 %0, %0, 4;\n\t}"
+                     : "+r"(to) : "r"(4 * lane + 128 * (i >> 2) + (i & 3)), "r"(pick & (1u << i)) : "memory");
     __syncwarp();
     // sort keys: the gap in 22 bits, then the token
     const float fine = __fdividef(4194303.0f * scale, (float)(last + 1));
