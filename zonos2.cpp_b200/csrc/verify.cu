@@ -32,6 +32,13 @@
 // A CTA goes through its stream's positions in order and stops at the first
 // refusal: later logits are not read.  With too few streams for the SMs a stream has a
 // cluster of CTAs, each at a position of its own, which exchange their refusals.
+//
+// Bound: instruction issue and the rows' own latency, not memory.  2048 streams of 4 drafts
+// with q, top-k 100 and allowed tokens (52344 rows of 1024 logits read, 214 MB): 153 us, a row
+// about 1750 warp instructions (the row and its masks 520, the histogram 270, the
+// candidates 400, the bounds 210, sort and decisions 700 of those that need them).  One stream of 4
+// drafts: 9.4 us back to back.  All in f64 with every row sorted the first took 203 us; a
+// barrier per position costs less than codebooks that run ahead of a refusal (191 / 205 us).
 #include <math.h>
 
 #include "common.cuh"
