@@ -122,6 +122,32 @@ def test_row_without_an_adapter_is_the_heads(z2, cuda):
         assert not torch.isnan(got[rest]).any() and torch.equal(got[rest], same[rest])
 
 
+def test_tensors_elsewhere_are_refused(z2, cuda):
+    """A host tensor among device ones is found before anything is launched."""
+    import torch
+    c = _case(cuda, "bf16", 4, 2, 64, 64, 64, 2, 8, 1)
+    for k in ("W", "A", "B", "ids", "scale"):
+        with pytest.raises(ValueError):
+            _call(z2, dict(c, **{k: c[k].cpu()}))
+    with pytest.raises(ValueError):
+        _call(z2, c, work=torch.empty(4096, dtype=torch.uint8))
+    with pytest.raises(ValueError):
+        _call(z2, c, out=torch.empty(4, 2, 64))
+    x, w = c["h"], torch.ones(64, device=cuda)
+    for args, kw in (((x, x.cpu(), x.clone(), None), {}), ((x, x, x.cpu(), None), {}),
+                     ((x, x, x.clone(), None), dict(gate=x.cpu())),
+                     ((x, x, x.clone(), None), dict(norm_weight=w.cpu()))):
+        with pytest.raises(ValueError):
+            z2.block_norm(*args, **kw)
+    lg, i32 = torch.zeros(1, 2, 1, 8, device=cuda), torch.int32
+    a = [lg, z2.SampleParams(pad_id=7), torch.zeros(1, 1, 1, dtype=i32, device=cuda),
+         torch.zeros(1, 2, 1, 2, device=cuda), torch.zeros(1, 2, 1, dtype=i32, device=cuda),
+         torch.zeros(1, dtype=i32, device=cuda)]
+    for i in (2, 3, 4, 5):
+        with pytest.raises(ValueError):
+            z2.verify_drafts(*[t.cpu() if j == i else t for j, t in enumerate(a)])
+
+
 @pytest.mark.parametrize("dtype,batch", [("bf16", 7), ("bf16", 300), ("f32", 5)])
 def test_workspace_and_neighbours(z2, cuda, dtype, batch):
     """Exactly the stated scratch, neither side of it nor of the logits written; the same bits

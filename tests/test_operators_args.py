@@ -48,9 +48,9 @@ def test_head_adapters_work(z2):
 
 
 def _norm(z2, **kw):
-    a = dict(resid=P, block=P, dtype=z2.BF16, rows=4, dim=100, resid_stride=100, block_stride=100,
+    a = dict(resid=P, block=2 * P, dtype=z2.BF16, rows=4, dim=100, resid_stride=100, block_stride=100,
              post_weight=P, post_eps=1e-5, gate=P, gate_row=100, gate_col=1, sigmoid=1, scale=1.0,
-             norm_weight=P, norm_eps=1e-5, resid_out=P, normed_out=P, out_stride=100)
+             norm_weight=P, norm_eps=1e-5, resid_out=P, normed_out=2 * P, out_stride=100)
     a.update(kw)
     return z2.lib().zonos2cu_block_norm(*a.values(), None)
 
@@ -61,7 +61,8 @@ def _norm(z2, **kw):
     dict(post_eps=float("nan")), dict(scale=float("inf")), dict(norm_eps=-1.0),
     dict(norm_eps=float("nan")), dict(gate_col=2), dict(gate_row=-100), dict(gate_row=50),
     dict(resid=P + 1), dict(block=P + 1), dict(gate=P + 1), dict(resid_out=P + 1),
-    dict(normed_out=P + 1), dict(post_weight=P + 2), dict(norm_weight=P + 2)])
+    dict(normed_out=P + 1), dict(post_weight=P + 2), dict(norm_weight=P + 2), dict(normed_out=P),
+    dict(resid_stride=108), dict(block_stride=108), dict(out_stride=108)])
 def test_block_norm_refuses(z2, bad):
     assert _norm(z2, **bad) == z2.EINVAL
 

@@ -422,6 +422,11 @@ int zonos2cu_block_norm(const void *resid_dev, const void *block_dev, zonos2cu_d
     }
     if (rows == 0) return ZONOS2CU_OK;
     if (!resid_dev || !block_dev || (!resid_out_dev && !normed_out_dev)) return ZONOS2CU_EINVAL;
+    if (resid_out_dev == normed_out_dev) return ZONOS2CU_EINVAL;
+    for (const void *out : {(const void *)resid_out_dev, (const void *)normed_out_dev})   // in place
+        if (rows > 1 && ((out == resid_dev && out_stride != resid_stride) ||
+                         (out == block_dev && out_stride != block_stride)))
+            return ZONOS2CU_EINVAL;
     const uintptr_t es = dtype == ZONOS2CU_F32 ? 4 : 2;
     if ((uintptr_t)resid_dev % es || (uintptr_t)block_dev % es || (uintptr_t)gate_dev % es ||
         (uintptr_t)resid_out_dev % es || (uintptr_t)normed_out_dev % es ||

@@ -288,12 +288,15 @@ def _rows(t, what: str) -> int:
     return t.stride(0)
 
 
-def _whole(what: str, *tensors) -> None:
+def _whole(what: str, on, *tensors) -> None:
     """Each tensor of the (tensor, elements, types) triples, where given, is contiguous, of that
-    size and of one of those types."""
+    size and of one of those types, and on ``on``'s device."""
+    dev = on.get_device()
     for t, n, types in tensors:
         if t is None:
             continue
+        if t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on one device expected")
         if t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{what}: a contiguous tensor of {n} elements expected, got "
                              f"{tuple(t.shape)}")
@@ -319,9 +322,10 @@ def head_adapters(W, dtype: int, rows_per_cb: int, n_cb: int, vocab: int, hidden
     wide = n_cb * rows_per_cb
     import torch
     own, f32 = (torch.bfloat16 if dtype == BF16 else torch.float32,), (torch.float32,)
-    _whole("head_adapters", (W, wide * dim, own), (hidden, batch * dim, own),
+    _whole("head_adapters", hidden, (W, wide * dim, own), (hidden, batch * dim, own),
            (A, n * rank * dim, own), (B, n * wide * rank, own), (adapter, batch, (torch.int32,)),
-           (out, batch * n_cb * vocab, f32), (scale, n, f32))
+           (out, batch * n_cb * vocab, f32), (scale, n, f32),
+           (work, work.numel(), (work.dtype,)))
     _launch("zonos2cu_head_adapters", hidden, stream, W.data_ptr(), dtype, rows_per_cb, n_cb, vocab,
             dim, hidden.data_ptr(), batch, softcap, A.data_ptr(), B.data_ptr(), _ptr(scale), n,
             rank, adapter.data_ptr(), work.data_ptr(), work.numel() * work.element_size(),
@@ -339,6 +343,10 @@ def block_norm(resid, block, resid_out, normed_out, *, post_weight=None, post_ep
     the block's output as it is."""
     dt, shape = _dtype(resid), resid.shape
     rows, dim = shape
+    dev = resid.get_device()
+    for t in (block, resid_out, normed_out, gate, post_weight, norm_weight):
+        if t is not None and t.get_device() != dev:
+            raise ValueError("block_norm: tensors on one device expected")
     for t in (block, resid_out, normed_out):
         if t is not None and (t.shape != shape or t.dtype != resid.dtype):
             raise ValueError("block_norm: block and outputs must match resid")
@@ -379,7 +387,7 @@ def verify_drafts(logits, params: SampleParams, drafts, uniforms, codes, n_accep
     H = 0 if hist is None else hist.shape[-1]
     import torch
     f32, i32, bits = (torch.float32,), (torch.int32,), (torch.int32, torch.uint32)
-    _whole("verify_drafts", (logits, S * D1 * Cb * stride, f32), (drafts, S * (D1 - 1) * Cb, i32),
+    _whole("verify_drafts", logits, (logits, S * D1 * Cb * stride, f32), (drafts, S * (D1 - 1) * Cb, i32),
            (uniforms, 2 * S * D1 * Cb, f32), (draft_probs, S * (D1 - 1) * Cb * V, f32),
            (n_drafts, S, i32), (codes, S * D1 * Cb, i32), (flags, S * D1 * Cb, i32),
            (n_accepted, S, i32), (hist, S * Cb * H, i32), (hist_pos, S, i32),
