@@ -241,7 +241,7 @@ def head_softcap(W, dtype: int, rows_per_cb: int, n_cb: int, vocab: int, hidden,
 
 
 _TYPES: dict = {}    # torch's types -> the library's, filled on first use
-_raw_stream = None   # torch's own lookup of a device's current stream handle
+_now = None          # (current device, a device's current stream handle): _find_now
 
 
 def _dtype(t) -> int:
@@ -258,25 +258,33 @@ def _dtype(t) -> int:
 def _launch(fn: str, on, stream, *args) -> None:
     """Call entry point ``fn`` on the device of tensor ``on``; the stream (default: that
     device's current one) is its last argument."""
-    global _raw_stream
     dev = on.get_device()
     if dev < 0:
         raise TypeError(f"{fn}: CUDA tensors expected")
-    import torch
-    if dev != torch.cuda.current_device():
+    if _now is None:
+        _find_now()
+    current, raw_stream = _now
+    if dev != current():
+        import torch
         with torch.cuda.device(dev):
             return _launch(fn, on, stream, *args)
     if stream is None:
-        # Half the cost of making a Stream object per call, which a small launch would feel.
-        if _raw_stream is None:
-            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
-                                  lambda d: torch.cuda.current_stream(d).cuda_stream)
-        stream = _raw_stream(dev)
+        stream = raw_stream(dev)
     elif not isinstance(stream, int):
         stream = stream.cuda_stream
-    rc = getattr(lib(), fn)(*args, stream)
+    rc = getattr(_lib or lib(), fn)(*args, stream)
     if rc < 0:
         raise Zonos2cuError(rc, fn)
+
+
+def _find_now() -> None:
+    """torch's own lookups of the current device and of a device's current stream handle, without the
+    objects that its Python functions make: a small launch would feel those."""
+    global _now
+    import torch
+    _now = (getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+            getattr(torch._C, "_cuda_getCurrentRawStream",
+                    lambda d: torch.cuda.current_stream(d).cuda_stream))
 
 
 def _rows(t, what: str) -> int:
@@ -343,34 +351,40 @@ def block_norm(resid, block, resid_out, normed_out, *, post_weight=None, post_ep
     the block's output as it is."""
     dt, shape = _dtype(resid), resid.shape
     rows, dim = shape
-    dev = resid.get_device()
-    for t in (block, resid_out, normed_out, gate, post_weight, norm_weight):
-        if t is not None and t.get_device() != dev:
-            raise ValueError("block_norm: tensors on one device expected")
+    dtype, dev = resid.dtype, resid.get_device()
+    strides = [dim if resid.is_contiguous() else _rows(resid, "block_norm")]
     for t in (block, resid_out, normed_out):
-        if t is not None and (t.shape != shape or t.dtype != resid.dtype):
+        if t is None:
+            continue
+        if t.shape != shape or t.dtype != dtype:
             raise ValueError("block_norm: block and outputs must match resid")
-    if resid_out is None and normed_out is None:
-        raise ValueError("block_norm: no output given")
-    out_stride = _rows(normed_out if resid_out is None else resid_out, "block_norm")
-    if normed_out is not None and _rows(normed_out, "block_norm") != out_stride:
+        if t.get_device() != dev:
+            raise ValueError("block_norm: tensors on one device expected")
+        strides.append(dim if t.is_contiguous() else _rows(t, "block_norm"))
+    if len(strides) < 3:
+        raise ValueError("block_norm: an output expected")
+    if strides[2] != strides[-1]:
         raise ValueError("block_norm: the outputs need one row stride")
     gate_row = gate_col = 0
     if gate is not None:
-        given = gate.shape
-        if (gate.dtype != resid.dtype or len(given) != 2 or given[0] not in (1, rows)
-                or given[1] not in (1, dim)):
+        g_rows, g_cols = gate.shape if gate.dim() == 2 else (0, 0)
+        if gate.dtype != dtype or g_rows not in (1, rows) or g_cols not in (1, dim):
             raise ValueError("block_norm: the gate must broadcast to [rows, dim]")
-        strides = gate.stride()
-        gate_row = 0 if given[0] == 1 else strides[0]
-        gate_col = 0 if given[1] == 1 else strides[1]
+        gate_row, gate_col = gate.stride()
+        if g_rows == 1:
+            gate_row = 0
+        if g_cols == 1:
+            gate_col = 0
     for w in (post_weight, norm_weight):
         if w is not None and (w.numel() != dim or _dtype(w) != F32 or not w.is_contiguous()):
             raise ValueError("block_norm: weights are [dim] f32")
+    for t in (gate, post_weight, norm_weight):
+        if t is not None and t.get_device() != dev:
+            raise ValueError("block_norm: tensors on one device expected")
     _launch("zonos2cu_block_norm", resid, stream, resid.data_ptr(), block.data_ptr(), dt, rows, dim,
-            _rows(resid, "block_norm"), _rows(block, "block_norm"), _ptr(post_weight), post_eps,
-            _ptr(gate), gate_row, gate_col, int(gate_sigmoid), scale, _ptr(norm_weight), norm_eps,
-            _ptr(resid_out), _ptr(normed_out), out_stride)
+            strides[0], strides[1], _ptr(post_weight), post_eps, _ptr(gate), gate_row, gate_col,
+            int(gate_sigmoid), scale, _ptr(norm_weight), norm_eps, _ptr(resid_out),
+            _ptr(normed_out), strides[2])
 
 
 def verify_drafts(logits, params: SampleParams, drafts, uniforms, codes, n_accepted, *,
