@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(threads_of(UNITS, SUMS), 1)
                     }
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + (uint32_t)(buf * args.buf_cols);
-                        const bool onto = UNITS && k1 == KB;   // the last part adds to delta
+                    const bool onto = UNITS && k1 == KB;   // the last part adds to delta
                     for (int kb = k0; kb < k1; kb++) {
                         if (!(PAIR ? mbar_wait_cl(full(s), ph) : mbar_wait(full(s), ph)) || aborted()) {
                             ok = false;

@@ -600,9 +600,15 @@ __device__ __forceinline__ int verify_row(const VerifyArgs &a, long long s, int 
         auto mark = [&](int t) {
             if ((unsigned)t < (unsigned)V) atomicOr(&seen[(t >> 2) & 31], 1u << (4 * (t >> 7) + (t & 3)));
         };
-        for (int i = lane; i < H; i += 32) {
-            const int age = i >= pos ? i - pos : i - pos + H;
-            if (age >= d) mark(ring[i]);
+        for (int i0 = lane; i0 < H; i0 += 256) {   // eight loads at a time, then their marks
+            int t[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) t[j] = i0 + 32 * j < H ? ring[i0 + 32 * j] : -1;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int i = i0 + 32 * j, age = i >= pos ? i - pos : i - pos + H;
+                if (age >= d) mark(t[j]);
+            }
         }
         for (int j = (d > H ? d - H : 0) + lane; j < d; j += 32) mark(__ldg(a.drafts + (s * D + j) * C + c));
         __syncwarp();
