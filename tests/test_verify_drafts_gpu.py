@@ -212,3 +212,25 @@ def test_other_stream(z2, cuda):
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
     _compare(z2, cuda, s, _p(z2, 1024), 1024, stream=side)
+
+
+@pytest.mark.parametrize("temperature", [0.7, 0.83, 1.1])
+@pytest.mark.parametrize("top_k,top_p,min_p", [(0, 0.9, 0.0), (7, 0.97, 0.0), (0, 1.0, 0.05), (3, 0.9, 0.0)])
+def test_lists_that_end_on_a_bucket_edge(z2, cuda, temperature, top_k, top_p, min_p):
+    """The kernel sorts logits into buckets of an eighth of the temperature: lists whose last logit lies
+    on a bucket's rounded edge, a few steps of f32 to either side."""
+    V, S, m = 64, 6000, 6
+    r = np.random.default_rng(int(temperature * 100) + top_k)
+    s = _case(S, 0, 1, V, 3, certain=True)
+    scale = np.float32(8) * np.float32(1.0 / np.float64(np.float32(temperature)))
+    lg = np.full((S, V), -np.inf, np.float32)
+    for row in lg:
+        top = np.float32(r.uniform(-6, 6))
+        low = np.float32(np.float64(top) - (r.integers(0, 60) + 0.5) / np.float64(scale))
+        for _ in range(abs(k := int(r.integers(-2, 3)))):
+            low = np.nextafter(low, np.float32(np.copysign(np.inf, k)))
+        at = r.permutation(V)[:m]
+        row[at] = r.uniform(low, top, m)
+        row[at[:2]] = top, low
+    s["logits"][:, 0, 0] = lg
+    _compare(z2, cuda, s, _p(z2, V, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p), V)

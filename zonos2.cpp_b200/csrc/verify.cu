@@ -531,7 +531,8 @@ __device__ __forceinline__ int by_candidates(const VerifyArgs &a, const Row &r, 
         if (lane > 0 && wrong(pl, pt, l[0], token[0])) l[0] = pl, token[0] = pt, moved = true;
         if (!__any_sync(kFull, moved)) break;
     }
-    if (f32) {
+    // (Without its sum where a whole row's last logit lay on the edge: then in f64, which takes it.)
+    if (f32 && (li.covers || !(a.top_p < 1.0f) || all > 0.0f)) {
         const int code = decide<float, K>(a, r, li, l, token, all);
         if (code != kClose) return code;
     }
