@@ -878,10 +878,11 @@ cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream)
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
-    // A stream's positions at once where one block per SM allows (8: the portable cluster): one
-    // stream with 4 drafts 9.4 us, 16.1 us one after the other.  With two blocks per SM
-    // 64 streams that all refuse their first frame take 18.9 us, with this 15.7, 14.0 in order.
-    const int parts = max(1, min(min(a.n_draft + 1, 8), sms / a.n_streams));
+    // A stream's positions at once where half the SMs hold them (8: the portable cluster): one
+    // stream with 4 drafts 9.4 us, 16.1 us one after the other.  With more of them at work the
+    // positions past a refusal cost the next call more than this one gains: 64 streams with 3
+    // drafts 14.1 us in order, 18.1 us two and 18.5 us four at a time (37 and 33 us alone).
+    const int parts = max(1, min(min(a.n_draft + 1, 8), sms / 2 / a.n_streams));
     if (a.n_cb > 9) return launch(verify_kernel<kSamplerCbMax, 1>, a, parts, stream);
     // Three blocks an SM at the price of spills where two do not hold nearly all: 300 streams
     // 60.9 us with three, 50.9 with two; 2048 streams 178 and 183.
