@@ -41,6 +41,8 @@
 // barrier per position costs less than codebooks that run ahead of a refusal (191 / 205 us).
 #include <math.h>
 
+#include <mutex>
+
 #include "common.cuh"
 #include "sampler.cuh"
 #include "verify.cuh"
@@ -847,16 +849,38 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kMinCtas)
     }
 }
 
+// The SMs of the current device.  A kernel's shared-memory limit is one value for all host
+// threads: it is set to its most codebooks' on a device's first launch, and never lowered.
+cudaError_t device_sms(int *sms)
+{
+    static std::mutex mu;
+    static int known[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!known[dev]) {
+        constexpr auto kLimit = cudaFuncAttributeMaxDynamicSharedMemorySize;
+        int n = 0;
+        e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(verify_kernel<kSamplerCbMax, 1>, kLimit, kSamplerCbMax * kWarpBytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(verify_kernel<9, 3>, kLimit, 9 * kWarpBytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(verify_kernel<9, 2>, kLimit, 9 * kWarpBytes);
+        if (e != cudaSuccess) return e;
+        known[dev] = n;
+    }
+    *sms = known[dev];
+    return cudaSuccess;
+}
+
 template <class Kernel>
 cudaError_t launch(Kernel kernel, const VerifyArgs &a, int parts, cudaStream_t stream)
 {
-    const int smem = a.n_cb * kWarpBytes;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.n_streams * (unsigned)parts);
     cfg.blockDim = dim3(32u * (unsigned)a.n_cb);
-    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.dynamicSmemBytes = (size_t)(a.n_cb * kWarpBytes);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -874,9 +898,8 @@ cudaError_t launch(Kernel kernel, const VerifyArgs &a, int parts, cudaStream_t s
 cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream)
 {
     if (a.n_streams == 0) return cudaSuccess;
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int sms = 0;
+    const cudaError_t e = device_sms(&sms);
     if (e != cudaSuccess) return e;
     // A stream's positions at once where half the SMs hold them (8: the portable cluster): one
     // stream with 4 drafts 9.4 us, 16.1 us one after the other.  With more of them at work the
