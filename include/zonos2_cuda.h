@@ -303,7 +303,9 @@ int zonos2cu_set_allow(zonos2cu_ctx *ctx, const uint32_t *bits_host);
  * is [dim] f32, or NULL for no scale weight; enable = 0 turns it off.  With an
  * f32 head the norm is the reference's, exactly; with a bf16 head it is folded
  * into the head (the weight into W's columns, rounded to bf16 once; each row's
- * 1 / rms into the GEMM's epilogue), within the bf16 path's tolerance. */
+ * 1 / rms into the GEMM's epilogue), within the bf16 path's tolerance.  Where that
+ * folding fails, here or in zonos2cu_set_head, ctx_step returns ZONOS2CU_ESTATE
+ * until the norm is set again or turned off. */
 int zonos2cu_set_out_norm(zonos2cu_ctx *ctx, int enable, const float *weight_host, float eps);
 /* Classifier-free guidance in zonos2cu_ctx_step: the blend
  * uncond + scale * (cond - uncond) of softcapped logits that the reference
@@ -321,7 +323,8 @@ int zonos2cu_set_cfg(zonos2cu_ctx *ctx, int enable, float scale);
  * zonos2cu_set_stream_adapters gives each stream its adapter (-1: none; NULL: none
  * anywhere).  With guidance on, both rows of a stream use it; with the output norm's
  * weight folded into a bf16 head it is folded into A as well.  n_adapters = 0 removes
- * them. */
+ * them, and so does a call that fails past its argument checks (head, norm and
+ * guidance stay as they were). */
 int zonos2cu_set_adapters(zonos2cu_ctx *ctx, const void *A_host, const void *B_host,
                           const float *scale_host, int n_adapters, int rank,
                           zonos2cu_dtype dtype, int rows_per_cb);

@@ -6,6 +6,7 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -53,3 +54,113 @@ def test_a_call_leaves_other_threads_shared_memory_alone(host):
     before = L.fake_smem_limit(b"verify_kernel", 1)
     assert _verify(host, 10) == 0
     assert L.fake_smem_limit(b"verify_kernel", 1) == before
+
+
+S, CB, V, DIM, N, RANK = 2, 2, 1024, 2048, 3, 16
+
+
+def _context(z):
+    ctx = z.Context(0, S, CB, V, DIM, 0, seed=1)
+    ctx.set_head(np.zeros((CB * V, DIM), np.uint16), z.BF16, V)
+    return ctx
+
+
+def _adapters(ctx, z):
+    ctx.set_adapters(np.zeros((N, RANK, DIM), np.uint16), np.zeros((N, CB * V, RANK), np.uint16), V, z.BF16)
+
+
+def _step(ctx, z):
+    """A step's status and the kernels that it launches."""
+    import ctypes as C
+    L, p = z.lib(), z.SampleParams()
+    L.fake_forget()
+    codes = np.zeros((S, CB), np.int32)
+    rc = L.zonos2cu_ctx_step(ctx.h, P, z.BF16, C.byref(p), -1, codes.ctypes.data, None, None, None)
+    return rc, [L.fake_launched(i).decode() for i in range(L.fake_launches())]
+
+
+def test_failed_adapters_leave_head_and_norm(host):
+    """Whichever allocation of set_adapters fails: no adapters, and a step is the normed head's."""
+    z, failures = host, 0
+    gamma = np.ones(DIM, np.float32)
+    for earlier in (False, True):
+        for n in range(1, 20):
+            ctx = _context(z)
+            ctx.set_out_norm(gamma, 1e-5)
+            want = _step(ctx, z)
+            assert want[0] == 0 and any("rms" in k for k in want[1]), want
+            if earlier:
+                _adapters(ctx, z)
+                assert any("adapter" in k for k in _step(ctx, z)[1])
+            z.lib().fake_fail_alloc(n)
+            try:
+                _adapters(ctx, z)
+                done = True
+            except z.Zonos2cuError as e:
+                done = False
+                assert e.code == z.ENOMEM
+            z.lib().fake_fail_alloc(0)
+            if not done:
+                failures += 1
+                rc, kernels = _step(ctx, z)
+                assert rc == 0 and any("rms" in k for k in kernels) and not any("adapter" in k for k in kernels), (n, kernels)
+            ctx.close()
+            if done:
+                break
+    assert failures >= 8   # A, B, scale, work and the folded A, twice
+
+
+@pytest.mark.parametrize("adapters", [False, True])
+def test_failed_norm_is_not_stepped_over(host, adapters):
+    """Whichever allocation of set_out_norm fails: a step is the one before the call or refused, and
+    setting the norm again, or off, mends it."""
+    z, gamma, refused = host, np.ones(DIM, np.float32), 0
+    for n in range(1, 20):
+        ctx = _context(z)
+        if adapters:
+            _adapters(ctx, z)
+        want = _step(ctx, z)[1]
+        z.lib().fake_fail_alloc(n)
+        try:
+            ctx.set_out_norm(gamma, 1e-5)
+            done = True
+        except z.Zonos2cuError as e:
+            done = False
+            assert e.code == z.ENOMEM
+        z.lib().fake_fail_alloc(0)
+        rc, kernels = _step(ctx, z)
+        if done:
+            assert rc == 0 and any("rms" in k for k in kernels)
+            ctx.close()
+            break
+        # the first step of a context draws its generators' numbers first
+        assert rc == z.ESTATE and not kernels or rc == 0 and kernels == [k for k in want if "draw" not in k], (n, rc, kernels)
+        if rc:
+            refused += 1
+            ctx.set_out_norm(enable=False)
+            assert _step(ctx, z)[0] == 0
+        ctx.set_out_norm(gamma, 1e-5)
+        rc, kernels = _step(ctx, z)
+        assert rc == 0 and any("rms" in k for k in kernels)
+        ctx.close()
+    assert refused == (2 if adapters else 1)
+
+
+def test_contexts_free_what_they_allocate(host):
+    z = host
+    ctx = _context(z)
+    _adapters(ctx, z)
+    ctx.close()
+    before = z.lib().fake_live_allocs()
+    for n in range(1, 12):
+        ctx = _context(z)
+        z.lib().fake_fail_alloc(n)
+        try:
+            ctx.set_out_norm(np.ones(DIM, np.float32), 1e-5)
+            ctx.set_cfg(1.5)
+            _adapters(ctx, z)
+        except z.Zonos2cuError:
+            pass
+        z.lib().fake_fail_alloc(0)
+        ctx.close()
+        assert z.lib().fake_live_allocs() == before, n

@@ -586,6 +586,7 @@ struct zonos2cu_ctx {
     bool norm_has_w = false;
     void *normed = nullptr;      // [2S][D] f32: the normalised rows (f32 head)
     void *head_folded = nullptr; // bf16 head with the norm weight folded into its columns
+    bool folded = true;          // what is folded is there and of this head and norm
     float *row_rcp = nullptr;    // [2S]: 1 / rms of each hidden row (bf16 head)
     // classifier-free guidance (zonos2cu_set_cfg): steps take 2S hidden rows
     bool cfg_on = false;
@@ -648,18 +649,24 @@ int grow(void **p, size_t *cap, size_t want)
     return ZONOS2CU_OK;
 }
 
-// The bf16 head with the output norm's weight folded into its columns, when both
-// are set (synchronises the context's stream).
-int fold_norm(zonos2cu_ctx *c)
+// With the output norm's weight on, what a bf16 step reads has it folded into its columns: the
+// adapters' projections and the head (both synchronise the context's stream).
+int fold_adapters(zonos2cu_ctx *c)
 {
-    if (c->n_adapters && c->adapter_dtype == ZONOS2CU_BF16) {   // the adapters' projections too
-        const size_t n = (size_t)c->n_adapters * c->adapter_rank, D = (size_t)c->dims.dim;
-        if (!c->adapter_a_folded) Z2_CK(cudaMalloc(&c->adapter_a_folded, 2 * n * D));
-        Z2_CK(z2::launch_fold_columns(c->adapter_a, c->norm_w, (int)n, (int)D,
-                                      c->adapter_a_folded, c->stream));
-        Z2_CK(cudaStreamSynchronize(c->stream));
-    }
-    if (!c->head || c->head_dtype != ZONOS2CU_BF16) return ZONOS2CU_OK;
+    if (!c->norm_on || !c->norm_has_w || !c->n_adapters || c->adapter_dtype != ZONOS2CU_BF16)
+        return ZONOS2CU_OK;
+    const size_t n = (size_t)c->n_adapters * c->adapter_rank, D = (size_t)c->dims.dim;
+    if (!c->adapter_a_folded) Z2_CK(cudaMalloc(&c->adapter_a_folded, 2 * n * D));
+    Z2_CK(z2::launch_fold_columns(c->adapter_a, c->norm_w, (int)n, (int)D, c->adapter_a_folded,
+                                  c->stream));
+    Z2_CK(cudaStreamSynchronize(c->stream));
+    return ZONOS2CU_OK;
+}
+
+int fold_head(zonos2cu_ctx *c)
+{
+    if (!c->norm_on || !c->norm_has_w || !c->head || c->head_dtype != ZONOS2CU_BF16)
+        return ZONOS2CU_OK;
     const size_t rows = (size_t)c->dims.n_cb * c->dims.vocab, D = (size_t)c->dims.dim;
     if (!c->head_folded) Z2_CK(cudaMalloc(&c->head_folded, 2 * rows * D));
     Z2_CK(z2::launch_fold_columns(c->head, c->norm_w, (int)rows, (int)D, c->head_folded,
@@ -668,11 +675,12 @@ int fold_norm(zonos2cu_ctx *c)
     return ZONOS2CU_OK;
 }
 
-int refold_head(zonos2cu_ctx *c)
+// After a new head or norm.
+int refold(zonos2cu_ctx *c)
 {
-    if (!c->norm_on || !c->norm_has_w) return ZONOS2CU_OK;
-    const int rc = fold_norm(c);
-    if (rc) c->norm_on = false;   // a step would read what is not there
+    int rc = fold_adapters(c);
+    if (!rc) rc = fold_head(c);
+    c->folded = rc == ZONOS2CU_OK;
     return rc;
 }
 
@@ -869,7 +877,7 @@ int zonos2cu_set_head(zonos2cu_ctx *c, const void *W_host, zonos2cu_dtype dtype,
     if (!c->logits && n_rows(c)) Z2_CK(cudaMalloc(&c->logits, sizeof(float) * n_rows(c) * V));
     if (c->norm_on && dtype == ZONOS2CU_F32 && !c->normed && n_rows(c))
         Z2_CK(cudaMalloc(&c->normed, sizeof(float) * 2 * (size_t)c->dims.n_streams * c->dims.dim));
-    return refold_head(c);
+    return refold(c);
 }
 
 int zonos2cu_set_history(zonos2cu_ctx *c, const int32_t *hist_host, int hist_pos)
@@ -983,7 +991,7 @@ int zonos2cu_set_out_norm(zonos2cu_ctx *c, int enable, const float *weight_host,
     c->norm_has_w = weight_host != nullptr;
     c->norm_eps = eps;
     c->norm_on = true;
-    return refold_head(c);
+    return refold(c);
 }
 
 int zonos2cu_set_cfg(zonos2cu_ctx *c, int enable, float scale)
@@ -1045,8 +1053,8 @@ int zonos2cu_set_adapters(zonos2cu_ctx *c, const void *A_host, const void *B_hos
     c->adapter_rank = rank;
     c->adapter_dtype = dtype;
     int rc = ensure_adapter_delta(c);
-    if (!rc) rc = refold_head(c);
-    if (rc) free_adapters(c);
+    if (!rc) rc = fold_adapters(c);
+    if (rc) free_adapters(c);   // head and norm stay as they were
     return rc;
 }
 
@@ -1253,6 +1261,7 @@ int zonos2cu_ctx_step(zonos2cu_ctx *c, const void *hidden_dev, zonos2cu_dtype dt
     if (!c->head) return ZONOS2CU_ESTATE;
     if (dtype != c->head_dtype) return ZONOS2CU_EINVAL;
     if (c->n_adapters && c->adapter_dtype != c->head_dtype) return ZONOS2CU_ESTATE;
+    if (dtype == ZONOS2CU_BF16 && c->norm_on && !c->folded) return ZONOS2CU_ESTATE;
     DeviceGuard g(c->device);
     const zonos2cu_dims &d = c->dims;
     int rc = check_params(params, d.vocab);
