@@ -146,6 +146,44 @@ def test_failed_norm_is_not_stepped_over(host, adapters):
     assert refused == (2 if adapters else 1)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("earlier", [False, True])
+def test_failed_head_is_not_stepped_with(host, dtype, earlier):
+    """Whichever allocation of set_head fails, the logits' and the f32 norm's among them: no head."""
+    import ctypes as C
+    z, L = host, host.lib()
+    code, t = (z.F32, np.float32) if dtype == "f32" else (z.BF16, np.uint16)
+    p, codes = z.SampleParams(), np.zeros((S, CB), np.int32)
+    W = np.zeros((CB * V, DIM), t)
+
+    def step():
+        return L.zonos2cu_ctx_step(ctx.h, P, code, C.byref(p), -1, codes.ctypes.data, None, None, None)
+
+    failures = 0
+    for n in range(1, 20):
+        ctx = z.Context(0, S, CB, V, DIM, 0, seed=1)
+        if earlier:   # a head of the other type, and the norm
+            ctx.set_head(np.zeros((CB * V, DIM), np.uint16), z.BF16, V)
+        ctx.set_out_norm(None, 1e-5)
+        L.fake_fail_alloc(n)
+        try:
+            ctx.set_head(W, code, V)
+            done = True
+        except z.Zonos2cuError as e:
+            done = False
+            assert e.code == z.ENOMEM
+        L.fake_fail_alloc(0)
+        assert step() == (0 if done else z.ESTATE), n
+        failures += not done
+        ctx.set_head(W, code, V)
+        assert step() == 0
+        ctx.close()
+        if done:
+            break
+    # the head; without an earlier one the logits, with it the f32 norm's rows
+    assert failures == (2 if dtype == "f32" or not earlier else 1)
+
+
 def test_contexts_free_what_they_allocate(host):
     z = host
     ctx = _context(z)

@@ -684,6 +684,26 @@ int refold(zonos2cu_ctx *c)
     return rc;
 }
 
+// The sampled rows of the head (of c->head_dtype), and the buffers that a step with it needs.
+int upload_head(zonos2cu_ctx *c, const void *W_host, int rows_per_cb)
+{
+    const bool f32 = c->head_dtype == ZONOS2CU_F32;
+    const size_t row_bytes = (f32 ? 4 : 2) * (size_t)c->dims.dim;
+    const size_t V = (size_t)c->dims.vocab, C = (size_t)c->dims.n_cb;
+    Z2_CK(cudaMalloc(&c->head, row_bytes * V * C));
+    // keep the sampled rows of each codebook: one 2-D copy per codebook
+    for (size_t cb = 0; cb < C; cb++) {
+        const char *src = static_cast<const char *>(W_host) + cb * (size_t)rows_per_cb * row_bytes;
+        Z2_CK(cudaMemcpyAsync(static_cast<char *>(c->head) + cb * V * row_bytes, src, V * row_bytes,
+                              cudaMemcpyHostToDevice, c->stream));
+    }
+    Z2_CK(cudaStreamSynchronize(c->stream));
+    if (!c->logits && n_rows(c)) Z2_CK(cudaMalloc(&c->logits, sizeof(float) * n_rows(c) * V));
+    if (c->norm_on && f32 && !c->normed && n_rows(c))
+        Z2_CK(cudaMalloc(&c->normed, sizeof(float) * 2 * (size_t)c->dims.n_streams * c->dims.dim));
+    return ZONOS2CU_OK;
+}
+
 void free_adapters(zonos2cu_ctx *c)
 {
     cudaFree(c->adapter_a);
@@ -860,23 +880,15 @@ int zonos2cu_set_head(zonos2cu_ctx *c, const void *W_host, zonos2cu_dtype dtype,
     if (dtype != ZONOS2CU_F32 && dtype != ZONOS2CU_BF16) return ZONOS2CU_EINVAL;
     DeviceGuard g(c->device);
     Z2_CK(cudaDeviceSynchronize());   // no step may still be using the state
-    const size_t es = dtype == ZONOS2CU_F32 ? 4 : 2;
-    const size_t row_bytes = es * (size_t)c->dims.dim;
-    const size_t V = (size_t)c->dims.vocab, C = (size_t)c->dims.n_cb;
     cudaFree(c->head);
     c->head = nullptr;
-    Z2_CK(cudaMalloc(&c->head, row_bytes * V * C));
-    // keep the sampled rows of each codebook: one 2-D copy per codebook
-    for (size_t cb = 0; cb < C; cb++) {
-        const char *src = static_cast<const char *>(W_host) + cb * (size_t)rows_per_cb * row_bytes;
-        Z2_CK(cudaMemcpyAsync(static_cast<char *>(c->head) + cb * V * row_bytes, src, V * row_bytes,
-                              cudaMemcpyHostToDevice, c->stream));
-    }
-    Z2_CK(cudaStreamSynchronize(c->stream));
     c->head_dtype = dtype;
-    if (!c->logits && n_rows(c)) Z2_CK(cudaMalloc(&c->logits, sizeof(float) * n_rows(c) * V));
-    if (c->norm_on && dtype == ZONOS2CU_F32 && !c->normed && n_rows(c))
-        Z2_CK(cudaMalloc(&c->normed, sizeof(float) * 2 * (size_t)c->dims.n_streams * c->dims.dim));
+    int rc = upload_head(c, W_host, rows_per_cb);
+    if (rc) {   // a step would read what is not there
+        cudaFree(c->head);
+        c->head = nullptr;
+        return rc;
+    }
     return refold(c);
 }
 
