@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import operators_ref as R
+from test_head_adapters_gpu import F, _call, _case, _check
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,33 @@ def test_verification_from_two_threads(z2, cuda):
     for s, d, codes, acc, _ in jobs:
         want = R.verify_drafts(s["lg"], V, p, s["t"], s["u"])
         assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(acc.cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("batch,rank", [(3, 16), (3, 256), (70, 16), (300, 40), (600, 64), (5, 12)])
+@pytest.mark.parametrize("t", [2.0 ** 128 - 2.0 ** 104, 2.0 ** 128])
+def test_low_rank_products_at_the_end_of_f32(z2, cuda, batch, rank, t):
+    """One row whose A h is the largest f32 (it rounds to infinity in bf16) or past it: its logits are
+    the softcap, by B's sign; B times it; and nothing of it reaches the rows beside it."""
+    import torch
+    c = _case(cuda, "bf16", batch, 2, 130, 130, 128, 4, rank, batch)
+    c["scale"][1] = 2 - 2.0 ** -23 if t < 2.0 ** 128 else 1.0
+    row = batch // 2
+    c["ids"][row] = 1
+    c["A"][1, :, 5] = 0.0
+    c["A"][1, 3, 5] = 2.0 ** 7 if t < 2.0 ** 128 else 2.0 ** 8
+    c["W"][:, 5] = 0.0
+    b = c["B"][1, :, 3].double().view(2, 130)
+    assert (b != 0).all()
+    rest = torch.arange(batch, device=cuda) != row
+    clean, open_ = _call(z2, c), _call(z2, c, softcap=0.0)
+    c["h"][row] = 0.0
+    c["h"][row, 5] = 2.0 ** 120
+    got = _call(z2, c)
+    assert torch.equal(got[row].double(), 15.0 * b.sign()) and torch.equal(got[rest], clean[rest])
+    got = _call(z2, c, softcap=0.0)
+    if t < 2.0 ** 128:   # one product of three exact parts, then sums with zeros
+        assert ((got[row].double() - b * t).abs() <= 8 * F * (b * t).abs()).all()
+    else:
+        assert torch.equal(got[row].double(), b.sign() * float("inf"))
+    assert torch.equal(got[rest], open_[rest])
+    assert z2.device_error() == 0

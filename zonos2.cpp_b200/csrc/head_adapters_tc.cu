@@ -334,25 +334,22 @@ __global__ void __launch_bounds__(32 * kDownWarps, 1) adapter_down_mma_kernel(co
 
 // ---- delta = B_a t ----------------------------------------------------------
 
-// x = hi + mid + lo in bf16, exactly but for bits below 2^-25 of x; two values to a
-// register, the first in the low half.
-__device__ __forceinline__ uint32_t pack_bf16(float x, float y)
+// x = hi + mid + lo in bf16, two values to a register, the first in the low half.  Each part is the
+// leading 8 bits of what is left, cut off: exact for the 24 bits of x, and no x rounds up
+// to infinity.  An infinite x is its first part alone (what is left would be a NaN).
+__device__ __forceinline__ float cut_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_high(float x, float y)
 {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
-    return r;
+    return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
 }
 __device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
 {
-    hi = pack_bf16(x, y);
-    x -= __uint_as_float(hi << 16);
-    y -= __uint_as_float(hi & 0xffff0000u);
-    mid = pack_bf16(x, y);
-    x -= __uint_as_float(mid << 16);
-    y -= __uint_as_float(mid & 0xffff0000u);
-    lo = pack_bf16(x, y);
+    hi = pack_high(x, y);
+    x = x == cut_bf16(x) ? 0.0f : x - cut_bf16(x);
+    y = y == cut_bf16(y) ? 0.0f : y - cut_bf16(y);
+    mid = pack_high(x, y);
+    lo = pack_high(x - cut_bf16(x), y - cut_bf16(y));
 }
-
 
 struct UpArgs {
     const __nv_bfloat16 *B;
