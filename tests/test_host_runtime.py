@@ -56,6 +56,15 @@ def test_a_call_leaves_other_threads_shared_memory_alone(host):
     assert L.fake_smem_limit(b"verify_kernel", 1) == before
 
 
+@pytest.mark.parametrize("batch", [3, 100])
+@pytest.mark.parametrize("n_cb,vocab", [(65535, 1), (65536, 1), (1, 1024 * 65535), (1, 1024 * 65535 + 1)])
+def test_adapters_past_a_grids_limits(host, batch, n_cb, vocab):
+    """More codebooks, or parts of one, than a launch grid has rows for."""
+    z = host
+    assert z.lib().zonos2cu_head_adapters(P, z.BF16, vocab, n_cb, vocab, 8, P, batch, 15.0, P, P, None, 2, 8, P, P,
+                                          1 << 30, P, None) == 0
+
+
 S, CB, V, DIM, N, RANK = 2, 2, 1024, 2048, 3, 16
 
 

@@ -77,3 +77,11 @@ def test_low_rank_products_at_the_end_of_f32(z2, cuda, batch, rank, t):
         assert torch.equal(got[row].double(), b.sign() * float("inf"))
     assert torch.equal(got[rest], open_[rest])
     assert z2.device_error() == 0
+
+
+@pytest.mark.parametrize("n_cb", [65535, 65536])
+def test_many_codebooks(z2, cuda, n_cb):
+    """More codebooks than a launch grid has rows for."""
+    c = _case(cuda, "bf16", 66, n_cb, 2, 2, 8, 2, 8, 1)
+    _check(c, _call(z2, c))
+    assert z2.device_error() == 0

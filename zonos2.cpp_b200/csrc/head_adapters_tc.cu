@@ -1159,6 +1159,9 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
         (uintptr_t)h.W % 16 || (uintptr_t)h.hidden % 16 || (uintptr_t)ad.A % 16 ||
         (uintptr_t)ad.B % 16 || wide * ad.rank > INT_MAX / 2)
         return cudaErrorNotSupported;
+    const bool pair = h.batch > kSmallN;
+    const long long up_blocks = h.n_cb * (((long long)h.vocab + kUpSpan - 1) / kUpSpan);   // a grid's y
+    if (pair && up_blocks > 65535) return cudaErrorNotSupported;
     DeviceInfo dev;
     cudaError_t e = device_info(&dev);
     if (e != cudaSuccess) return e;
@@ -1172,7 +1175,6 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     cfg.numAttrs = 1;
 
     // ---- t and the rows' order; delta
-    const bool pair = h.batch > kSmallN;
     float *t = static_cast<float *>(ad.work);
     Order order;
     order.rows = reinterpret_cast<int32_t *>(t + (size_t)h.batch * ad.rank);
@@ -1201,8 +1203,7 @@ cudaError_t launch_head_adapters_tc(const HeadArgs &h, const AdapterArgs &ad, cu
     float *delta = ad.delta ? ad.delta : h.out;
     if (pair) {
         const UpArgs u{static_cast<const __nv_bfloat16 *>(ad.B), t, order, h.n_cb, h.vocab, h.rows_per_cb, ad.rank, delta};
-        const int up_per_cb = (h.vocab + kUpSpan - 1) / kUpSpan;
-        cfg.gridDim = dim3((unsigned)max_items(h.batch, ad.n_adapters), (unsigned)(h.n_cb * up_per_cb));
+        cfg.gridDim = dim3((unsigned)max_items(h.batch, ad.n_adapters), (unsigned)up_blocks);
         cfg.blockDim = dim3(32 * kUpWarps);
         cfg.dynamicSmemBytes = 0;
         e = ad.rank <= 16   ? cudaLaunchKernelEx(&cfg, adapter_up_kernel<1>, u)
