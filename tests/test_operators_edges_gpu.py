@@ -85,3 +85,197 @@ def test_many_codebooks(z2, cuda, n_cb):
     c = _case(cuda, "bf16", 66, n_cb, 2, 2, 8, 2, 8, 1)
     _check(c, _call(z2, c))
     assert z2.device_error() == 0
+
+
+def _exact(c, softcap=0.0):
+    """The logits in 64 bits, on the GPU."""
+    import torch
+    h, (n, rank, _) = c["h"].double(), c["A"].shape
+    keep = torch.cat([torch.arange(k * c["rows"], k * c["rows"] + c["vocab"], device=h.device) for k in range(c["n_cb"])])
+    y = h @ c["W"][keep].double().t()
+    for a in range(n):
+        at = (c["ids"] == a).nonzero()[:, 0]
+        if len(at):
+            y[at] += c["scale"][a].double() * (h[at] @ c["A"][a].double().t()) @ c["B"][a][keep].double().t()
+    return (softcap * torch.tanh(y / softcap) if softcap else y).view(len(h), c["n_cb"], c["vocab"])
+
+
+# Relative error of the logits in the 2-norm.  The tensor cores cut off what an f32 accumulator
+# does not hold: on average half a unit in the last place, which is ln 2 * 2^-24 of the
+# accumulator, itself 2/3 of its last value on average over a random walk's steps.  A part of the head's depth is
+# 48 steps: 1.32e-6.  A h: 16 steps of a warp at a depth of 2048 (32 at 4096), then additions of 8 warps
+# and a multiplication; its three parts and 16 ranks at a time of B t: four more; rounded
+# ones count 2^-24 / sqrt(3).
+STEP = np.log(2.0) * 2.0 ** -24 * 2 / 3
+
+
+def _low_rank(dim, rank):
+    return dim // 128 * STEP + (4 + 10 + rank / 16) * F
+
+
+# f32: four roundings in each sum of four products, of 1 to 4 of its terms' variance, then one of the
+# result: sqrt(10 / 4 + 1) * 2^-24 / sqrt(3), once for W h and, in A h's place, again.
+F32 = np.sqrt(3.5 / 3) * F
+
+
+@pytest.mark.parametrize("dtype,batch,n_cb,vocab,rows,dim,n,rank", [
+    ("bf16", 20, 12, 1024, 1024, 2048, 5, 16), ("bf16", 64, 13, 1000, 1002, 2048, 40, 24), ("bf16", 3, 40, 300, 301, 768, 2, 8),
+    ("bf16", 20, 9, 1024, 1026, 4096, 5, 16), ("bf16", 700, 9, 1024, 1024, 2048, 6, 16), ("bf16", 1000, 9, 1000, 1001, 4096, 32, 40),
+    ("bf16", 2500, 9, 1024, 1026, 1024, 100, 8), ("bf16", 130, 30, 700, 700, 2048, 3, 64), ("bf16", 21, 3, 500, 501, 2048, 4, 12),
+    ("f32", 5, 9, 1024, 1026, 2048, 3, 12), ("f32", 21, 4, 333, 334, 2047, 3, 16)])
+def test_precision_over_many_tiles(z2, cuda, dtype, batch, n_cb, vocab, rows, dim, n, rank):
+    """Sizes at which an SM takes more than one tile, and depths of several parts; the adapters' share
+    alone, so that W's does not hide it."""
+    c = _case(cuda, dtype, batch, n_cb, vocab, rows, dim, n, rank, batch + n_cb, low=0.3)
+    _check(c, _call(z2, c), rows=sorted({0, batch // 3, batch - 1}))
+    bf16 = dtype == "bf16"
+    low = _low_rank(dim, rank) if bf16 else 2 * F32
+    if bf16 and rank % 8:   # additions in f32 that are rounded: a lane's chain of dim / 128 fours, five levels
+        low = wide = (dim / 128 + 4 + 5) * F
+    else:
+        wide = min(dim // 16, 48) * STEP + 4 * F if bf16 else F32
+    for share, tol in (("all", wide + low), ("adapters", low)):
+        if share == "adapters":
+            c["W"].zero_()
+        got, want = _call(z2, c, softcap=0.0).double(), _exact(c)
+        err, size = (got - want).norm(dim=(1, 2)), want.norm(dim=(1, 2))
+        named = (c["ids"] >= 0) & (c["ids"] < n)
+        assert named.any() and not named.all()
+        assert (err <= tol * size).all(), (share, float((err / size.clamp(min=1e-30)).max()), tol)
+        assert (share == "all") or (got[~named] == 0).all()
+    assert z2.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,batch", [("bf16", 5), ("bf16", 100), ("bf16", 520), ("f32", 6)])
+def test_an_overflowing_row_reaches_no_other(z2, cuda, dtype, batch):
+    """Products past f32 in one row leave the bits of the rows beside it."""
+    import torch
+    c = _case(cuda, dtype, batch, 2, 130, 130, 128, 4, 16, batch)
+    for row in (0, batch // 2, batch - 1):
+        clean = _call(z2, c)
+        kept = c["h"][row].clone()
+        rest = torch.arange(batch, device=cuda) != row
+        for value in (3e38, float("inf"), float("nan")):
+            c["h"][row] = value
+            c["h"][row, ::2] *= -1
+            assert torch.equal(_call(z2, c)[rest], clean[rest])
+        c["h"][row] = kept
+
+
+@pytest.mark.parametrize("dtype,rows", [("bf16", 4), ("bf16", 60), ("bf16", 200), ("bf16", 1500), ("f32", 4)])
+def test_calls_behind_each_other(z2, cuda, dtype, rows):
+    """Tail, head and verification launched without a pause, each turn on what the last one left in
+    place: the bits of the same calls one at a time."""
+    import torch
+    C, V, dim, n, rank, D, turns = 2, 256, 512, 3, 16, 1, 12
+    c = _case(cuda, dtype, rows, C, V, V, dim, n, rank, rows)
+    code, S = (z2.BF16 if dtype == "bf16" else z2.F32), rows // (D + 1)
+    start = [torch.randn(rows, dim, device=cuda).to(c["h"].dtype) for _ in range(2)]
+    w = torch.rand(dim, device=cuda) + 0.5
+    g = torch.Generator(device=cuda)
+    g.manual_seed(rows)
+    u = torch.rand(turns, S, D + 1, C, 2, generator=g, device=cuda)
+    p = z2.SampleParams(0.9, 60, 0.95, 0.01, 1.2, V - 1)
+    work = torch.empty(z2.head_adapters_work(code, rows, rank), dtype=torch.uint8, device=cuda)
+
+    def go(wait):
+        resid, block = (t.clone() for t in start)
+        logits = torch.zeros(turns, rows, C, V, device=cuda)
+        codes = torch.zeros(turns, S, D + 1, C, dtype=torch.int32, device=cuda)
+        drafts = torch.zeros(S, D, C, dtype=torch.int32, device=cuda)
+        acc = torch.zeros(S, dtype=torch.int32, device=cuda)
+        hist = torch.full((S, C, 8), -1, dtype=torch.int32, device=cuda)
+        at = torch.zeros(S, dtype=torch.int32, device=cuda)
+        torch.cuda.synchronize()
+        for k in range(turns):
+            z2.block_norm(resid, block, resid, c["h"], scale=0.5, norm_weight=w)
+            if wait:
+                torch.cuda.synchronize()
+            _call(z2, c, logits[k], work)
+            if wait:
+                torch.cuda.synchronize()
+            z2.verify_drafts(logits[k].view(S, D + 1, C, V), p, drafts, u[k], codes[k], acc, hist=hist, hist_pos=at)
+            if wait:
+                torch.cuda.synchronize()
+            # the tail again, over the rows that the head has just read
+            z2.block_norm(c["h"], block, None, c["h"], post_eps=-1.0)
+            z2.block_norm(resid, c["h"], None, block, gate=c["h"], gate_sigmoid=True)
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return resid, block, logits, codes, acc, hist, at
+
+    for a, b in zip(go(False), go(True)):
+        assert torch.equal(a, b)
+    assert z2.device_error() == 0
+
+
+def _verified(z2, cuda, lg, t, u, p):
+    import torch
+    S, D1, C, V = lg.shape
+    dev = [torch.from_numpy(np.ascontiguousarray(a)).to(cuda) for a in (lg, t, u)]
+    codes = torch.zeros(S, D1, C, dtype=torch.int32, device=cuda)
+    acc = torch.zeros(S, dtype=torch.int32, device=cuda)
+    z2.verify_drafts(dev[0], p, dev[1], dev[2], codes, acc)
+    torch.cuda.synchronize()
+    want = R.verify_drafts(lg, V, p, t, u)
+    assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(acc.cpu().numpy(), want[1])
+    return acc.cpu().numpy()
+
+
+NEAR = (0.0, 1e-8, 1e-7, 1e-6, 3e-6, 6e-6, 9e-6, 1.1e-5, 2e-5, 3e-5)
+
+
+def _near_top_p(deep, temperature, spread, outside, V=1024, S=1500, top_p=0.9):
+    """Logits whose mass ahead of token t is within a few 1e-6 of top_p, by more weight on the tokens
+    behind the first one outside (they may overtake it) or less on those behind the last one inside."""
+    r = np.random.default_rng(deep + int(10 * spread))
+    lg = r.normal(0, spread, (S, V))
+    lg[:, r.permutation(V)[:deep]] -= r.uniform(15, 110, deep)
+    T, top_p = np.float64(np.float32(temperature)), np.float64(np.float32(top_p))
+    t = np.zeros(S, np.int32)
+    for i, row in enumerate(lg):
+        order = np.argsort(-row, kind="stable")
+        e = np.exp((row[order] - row[order[0]]) / T)
+        before = np.cumsum(e) - e
+        j = int(np.searchsorted(before, top_p * e.sum())) - (not outside)
+        near = NEAR[i % len(NEAR)] * (1 if i // len(NEAR) % 2 else -1)
+        more = before[j] / top_p / (1 + near) - e.sum()       # weight that the tail needs for it
+        tail = order[j + 1:]
+        row[tail] += T * np.log1p(more / e[j + 1:].sum())
+        t[i] = order[j]
+    return np.repeat(lg.astype(np.float32)[:, None, None], 2, 1), t[:, None, None], np.zeros((S, 2, 1, 2), np.float32)
+
+
+@pytest.mark.parametrize("outside", [True, False])
+@pytest.mark.parametrize("deep", [0, 400])
+@pytest.mark.parametrize("temperature,spread", [(1.0, 0.5), (0.7, 1.0), (1.3, 0.0)])
+def test_nuclei_that_end_at_the_drafted_code(z2, cuda, deep, temperature, spread, outside):
+    """Nuclei of hundreds of tokens, the mass ahead of the drafted code within a few 1e-6 of top_p: f32
+    may answer only what the definition in 64 bits does.  `deep` tokens lie far below the others."""
+    p = z2.SampleParams(temperature, 0, 0.9, 0.0, 1.0, 1023)
+    acc = _verified(z2, cuda, *_near_top_p(deep, temperature, spread, outside), p)
+    assert outside or 0.2 < acc.mean() < 0.8
+
+
+@pytest.mark.parametrize("top_k,top_p,min_p", [(0, 0.95, 0.0), (50, 0.9, 0.02), (100, 1.0, 0.0), (0, 1.0, 0.05)])
+def test_uniforms_next_to_the_drafted_codes_share(z2, cuda, top_k, top_p, min_p):
+    """u0 within a few 1e-6 of p(t), and u1 of the residual's cumulative weights."""
+    V, S = 1000, 1500
+    p = z2.SampleParams(0.8, top_k, top_p, min_p, 1.0, V - 1)
+    r = np.random.default_rng(top_k + int(100 * top_p))
+    lg = r.normal(0, 0.4, (S, V)).astype(np.float32)
+    t, u = np.zeros((S, 1, 1), np.int32), np.zeros((S, 2, 1, 2), np.float32)
+    for i, row in enumerate(lg):
+        tok, w, _ = R._distribution(row, np.zeros(V, bool), np.ones(V, bool), p)
+        j = int(r.integers(0, len(tok)))
+        t[i] = tok[j]
+        near = 1 + NEAR[i % len(NEAR)] * (1 if i // len(NEAR) % 2 else -1)
+        u[i, 0, 0, 0] = min(w[j] / w.sum() * near, 1 - 2.0 ** -24)
+        left = np.where(tok == t[i, 0, 0], 0.0, w)
+        for d, weights in ((0, left), (1, w)):
+            if weights.sum() > 0:
+                k = int(r.integers(0, len(tok)))
+                u[i, d, 0, 1] = min(np.cumsum(weights)[k] / weights.sum() * near, 1 - 2.0 ** -24)
+    acc = _verified(z2, cuda, np.repeat(lg[:, None, None], 2, 1), t, u, p)
+    assert 0.2 < acc.mean() < 0.8

@@ -54,10 +54,15 @@ namespace {
 constexpr int kOpen = 127;            // the histogram's open-ended last bucket: a gap of 16 temperatures
 constexpr int kMaxCand = 256;
 constexpr float kMaskedAll = -1e9f;   // a row without a logit at or above this is all masked
-// Within the candidates an f32 exponential is off by 3.2e-6 relative at most (2^-24 for
-// each of gap, factor and product, times a gap of 16, and 2^-22 for the power), a sum by
-// 2.5e-6 (the gaps' error weighs a term by its share, and -sum p log p < 7 for 1024
-// tokens; ten levels of additions), the drafts' products and the cuts by three more roundings.
+// An f32 exponential is off by 3 g 2^-24 + 2^-22 relative at most (gap, factor and product, each
+// 2^-24 of a gap of g temperatures; the power): 3.2e-6 for a candidate, whose gap is below 16.
+// In a sum, all the row's too, a term's error counts by its share, and sum p g <=
+// -sum p log p < 7 for 1024 tokens: 1.5e-6.  The additions, 8 of a lane and 5 levels for
+// candidates and 32 and 5 for a row, bring that to 2.3e-6 and 3.7e-6 of the sum's whole.
+// So a comparison of two sums is off by 7.4e-6 at most, beside three roundings of 2^-24 of the
+// drafts' products or the cuts.  A code that surely_stands accepts by whole-row sums leaves
+// kMargin less 7.6e-6 of the mass, 2e-6, to itself and the tokens behind it, none of them larger:
+// its gap is below log(1024 / 2e-6) = 20.1, its own error below 3.9e-6, and 2 kMargin holds both.
 constexpr float kMargin = 1e-5f;
 // A row's answer: the code, its flags and whether the drafted code stands.
 constexpr int kAllMasked = 1 << 16, kNonfinite = 2 << 16, kTaken = 1 << 30;
@@ -907,8 +912,9 @@ cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t stream)
     // drafts 14.1 us in order, 18.1 us two and 18.5 us four at a time (37 and 33 us alone).
     const int parts = max(1, min(min(a.n_draft + 1, 8), sms / 2 / a.n_streams));
     if (a.n_cb > 9) return launch(verify_kernel<kSamplerCbMax, 1>, a, parts, stream);
-    // Three blocks an SM at the price of spills where two do not hold nearly all: 300 streams
-    // 60.9 us with three, 50.9 with two; 2048 streams 178 and 183.
+    // Three blocks an SM (72 registers a thread, 96 with two; both spill, 120 and 180 bytes of
+    // stores, more in the functions kept apart) where two do not hold nearly all: 300 streams 60.9 us with
+    // three, 50.9 with two; 2048 streams 178 and 183.  Between those the crossover is not measured.
     return a.n_streams > 3 * sms ? launch(verify_kernel<9, 3>, a, parts, stream)
                                  : launch(verify_kernel<9, 2>, a, parts, stream);
 }
