@@ -171,8 +171,10 @@ int zonos2cu_head_softcap(const void *W_dev, zonos2cu_dtype dtype, int rows_per_
  * A h is kept in f32 beside a bf16 head and in f64 beside an f32 one, whose result
  * is rounded once (its products are summed by fours in f32 before).  Any dim, vocab
  * and rank (<= ZONOS2CU_MAX_RANK); the bf16 tensor-core kernels run where dim % 8 ==
- * 0, rank % 8 == 0, n_adapters <= 4096 and W, hidden, A and B are 16-byte aligned, a
- * slower kernel elsewhere. */
+ * 0, rank % 8 == 0, n_adapters <= 4096 and W, hidden, A and B are 16-byte aligned.
+ * Elsewhere, and for f32, a kernel runs that reads W again for every four hidden rows:
+ * meant for a few rows, its time grows with their number.  A product past the range of f32 is
+ * infinite, and its logit the end of the softcap. */
 #define ZONOS2CU_MAX_RANK 256
 long long zonos2cu_head_adapters_work(zonos2cu_dtype dtype, int batch, int rank);
 int zonos2cu_head_adapters(const void *W_dev, zonos2cu_dtype dtype, int rows_per_cb, int n_cb,
@@ -324,7 +326,11 @@ int zonos2cu_set_cfg(zonos2cu_ctx *ctx, int enable, float scale);
  * anywhere).  With guidance on, both rows of a stream use it; with the output norm's
  * weight folded into a bf16 head it is folded into A as well.  n_adapters = 0 removes
  * them, and so does a call that fails past its argument checks (head, norm and
- * guidance stay as they were). */
+ * guidance stay as they were).  While adapters are set, streams without one take the
+ * adapters' kernels as well: slower than the plain head's, and with its own roundings
+ * (an f32 head's products are summed by fours in f32), so that their logits may differ
+ * in the last bits.  A captured step holds the adapters' buffers: capture it again after
+ * this call (after zonos2cu_set_stream_adapters it reads the new ids). */
 int zonos2cu_set_adapters(zonos2cu_ctx *ctx, const void *A_host, const void *B_host,
                           const float *scale_host, int n_adapters, int rank,
                           zonos2cu_dtype dtype, int rows_per_cb);

@@ -85,10 +85,13 @@ constexpr int kBatch = 4;   // hidden rows at a time: a weight is read and widen
 // (f32) or 8-byte aligned (bf16) and dim a multiple of 4.  An f32 head's sums are f64, of
 // single products or (VEC) of four in f32: their roundings, half a step of the products each,
 // average out over dim / 4 terms, and the conversions, of which an SM makes 16 a cycle,
-// are few: widening both operands takes six times as many.  Four blocks an SM (64 registers)
-// hold all of a head's 4608 warps at once, and W's part runs beside adapter_down_kernel.
+// are few: widening both operands takes six times as many.  Four blocks an SM (64 registers, at
+// the price of 100 bytes of spills with VEC f32) hold all of a head's 4608 warps at once, and W's
+// part runs beside adapter_down_kernel.
 // 4 rows by 9216 x 2048 f32 with rank 12: 23.5 us, 3.3 TB/s; 52 us with widened operands,
-// two blocks an SM and the kernels one after the other, 104 us with a row and a warp each.
+// two blocks an SM and the kernels one after the other, 104 us with a row and a warp each.  W is
+// read again, mostly from L2, for every four hidden rows: 20 f32 rows of rank 16 take 97 us, 64
+// rows 259 us, 333 rows 1.30 ms, 64 bf16 rows of rank 12 212 us and 4096 of them 12.5 ms.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kWarps, 4)
     adapter_any_kernel(const HeadArgs h, const AdapterArgs ad)

@@ -17,10 +17,12 @@
 //
 // Measured (9 x 1024 x 2048, 32 adapters, rank 16, in a graph): 14.8 us at 1 row (38 MB of
 // weights, 2.6 TB/s), 19.7 at 64, 33 at 333, 57 at 1024, 188 at 4096 (155 GFLOP, 0.82
-// PFLOP/s; 145 where no row has an adapter).
+// PFLOP/s; 145 where no row has an adapter).  4096 rows at a time for seconds on end take 216 us:
+// at the power limit the SMs' clock falls from 1.97 to 1.55 GHz.
 // Up to 64 rows the GEMM's stream of W bounds it, beyond a few hundred the MMAs, and
 // between them the chain of three kernels.  Delta in the GEMM against the separate kernel
-// measured 16 / 26 us at 1 row, 27 / 34 at 64, 284 / 224 at 4096, when both were first built:
+// measured 16 / 26 us at 1 row, 27 / 34 at 64, 284 / 224 at 4096, when both were first built
+// (nothing between, and not since):
 // with more than a few rows per SM, the warps' latency per adapter exceeds the tile's MMAs.
 // Slower still at 4096 rows: added in the epilogue on the FMA pipe, t broadcast from shared
 // memory (16 B per 512 B of register writes), 370-540 us; hidden rows gathered by adapter
@@ -483,8 +485,8 @@ constexpr int kBK = 64;             // bf16 elements per 128-byte swizzled row
 constexpr int kSmallN = 64, kPairN = 256;   // hidden rows per tile (TMEM columns) at most
 constexpr int kUnits = 8, kSmallSums = 8, kPairSums = 16;
 // The pair kernel's five warp groups (roles, four of sums) split the launch's 5 * 96
-// registers a thread as 32 + 4 * 112 = 480: nothing may spill, since shared memory leaves
-// the L1 so little that a spilled value costs a trip to L2.
+// registers a thread as 32 + 4 * 112 = 480.  Spills are dear here, since shared memory leaves
+// the L1 so little that a spilled value costs a trip to L2; 24 bytes of stores are left.
 constexpr int kRoleRegs = 32, kSumRegs = 112;
 constexpr int kGroup = 2;           // items that a unit warp works on at once
 constexpr int kPitch = 36;          // floats per column of a warp's transposition (conflict-free)
