@@ -279,3 +279,88 @@ def test_uniforms_next_to_the_drafted_codes_share(z2, cuda, top_k, top_p, min_p)
                 u[i, d, 0, 1] = min(np.cumsum(weights)[k] / weights.sum() * near, 1 - 2.0 ** -24)
     acc = _verified(z2, cuda, np.repeat(lg[:, None, None], 2, 1), t, u, p)
     assert 0.2 < acc.mean() < 0.8
+
+
+@pytest.mark.parametrize("batch,n,rank", [(5, 4096, 8), (300, 4096, 16), (2500, 4096, 16), (300, 4097, 16), (300, 3, 256),
+                                          (2000, 7, 256)])
+def test_many_adapters_and_ranks(z2, cuda, batch, n, rank):
+    """The most adapters that the tensor-core kernels take and one more, and the most ranks."""
+    c = _case(cuda, "bf16", batch, 1, 70, 70, 128, n, rank, batch + n)
+    c["ids"][batch // 2], c["ids"][-1] = n - 1, n
+    _check(c, _call(z2, c))
+    assert z2.device_error() == 0
+
+
+def test_the_most_drafts(z2, cuda):
+    """4095 drafted frames that all stand but the last few, with the penalty's ring."""
+    import torch
+    V, D, C, H = 33, 4095, 1, 7
+    r = np.random.default_rng(2)
+    lg = r.normal(0, 1, (2, D + 1, C, V)).astype(np.float32)
+    t = r.integers(0, V, (2, D, C)).astype(np.int32)
+    np.put_along_axis(lg[:, :D], t[..., None].astype(np.int64), 40.0, -1)
+    lg[1, D - 3] = 0.0
+    u = r.random((2, D + 1, C, 2), np.float32)
+    hist, at = r.integers(-1, V, (2, C, H)).astype(np.int32), np.array([3, 9], np.int32)
+    p = z2.SampleParams(0.9, 10, 0.9, 0.0, 1.2, V - 1)
+    d = [torch.from_numpy(a.copy()).to(cuda) for a in (lg, t, u, hist, at)]
+    codes = torch.zeros(2, D + 1, C, dtype=torch.int32, device=cuda)
+    acc = torch.zeros(2, dtype=torch.int32, device=cuda)
+    z2.verify_drafts(d[0], p, d[1], d[2], codes, acc, hist=d[3], hist_pos=d[4])
+    torch.cuda.synchronize()
+    got = [x.cpu().numpy() for x in (codes, acc, d[3], d[4])]
+    assert got[1][0] == D and got[1][1] in range(D - 3, D)
+    # what was emitted are the drafts up to there, and the ring holds the last of the emitted frames
+    for s in range(2):
+        n = got[1][s]
+        assert np.array_equal(got[0][s, :n], t[s, :n]) and (got[0][s, n + 1:] == -1).all()
+        assert got[3][s] == (at[s] + n + 1) % H
+        for k in range(n - H + 1, n + 1):
+            assert got[2][s, 0, (at[s] + k) % H] == got[0][s, k, 0]
+
+
+def test_past_32_bits_of_elements(z2, cuda):
+    """Logits, hidden rows and tails of more than 2^31 elements: the last rows as in a call of their own."""
+    import torch
+    C, V, dim, n, rank = 9, 1024, 64, 5, 8
+    rows = (1 << 31) // (C * V) + 2000
+    c = _case(cuda, "bf16", 4000, C, V, V, dim, n, rank, 1)
+    last = dict(c)
+    c["h"] = c["h"].repeat((rows + 3999) // 4000, 1)[:rows].contiguous()
+    c["ids"] = c["ids"].repeat((rows + 3999) // 4000)[:rows].contiguous()
+    out = _call(z2, c)
+    last["h"], last["ids"] = c["h"][-100:].clone(), c["ids"][-100:].clone()
+    _check(last, out[-100:])
+    _check(last, _call(z2, last))
+    # the check of those logits, the last streams against a call of their own
+    S, D = rows // 5, 4
+    lg = out[:5 * S].view(S, D + 1, C, V)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(3)
+    t = torch.randint(0, V, (S, D, C), generator=g, device=cuda, dtype=torch.int32)
+    t[::2] = lg[::2, :D].argmax(-1).int()
+    u = torch.rand(S, D + 1, C, 2, generator=g, device=cuda)
+    u[::2, ..., 0] *= 1e-3   # these drafts stand
+    p = z2.SampleParams(pad_id=V - 1)
+
+    def check(lg, t, u):
+        codes = torch.zeros(len(lg), D + 1, C, dtype=torch.int32, device=cuda)
+        acc = torch.zeros(len(lg), dtype=torch.int32, device=cuda)
+        z2.verify_drafts(lg, p, t, u, codes, acc)
+        return codes, acc
+
+    whole, some = check(lg, t, u), check(lg[-50:].clone(), t[-50:], u[-50:])
+    assert torch.equal(whole[0][-50:], some[0]) and torch.equal(whole[1][-50:], some[1])
+    assert (some[1] == D).any() and (some[1] == 0).any()
+    del out, lg
+    for dim in (2048, 2047):
+        m = (1 << 31) // dim + 100
+        x = torch.zeros(m, dim, dtype=torch.bfloat16, device=cuda)
+        x[-64:] = torch.randn(64, dim, generator=g, device=cuda).bfloat16()
+        few = x[-64:].clone()
+        z2.block_norm(x, x, x, None, scale=0.5)
+        want = torch.empty_like(few)
+        z2.block_norm(few, few, want, None, scale=0.5)
+        assert torch.equal(x[-64:], want)
+        del x
+    torch.cuda.empty_cache()
