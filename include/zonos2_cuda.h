@@ -282,7 +282,8 @@ int zonos2cu_ctx_destroy(zonos2cu_ctx *ctx);
 
 /* Head weights from host memory, [n_cb*rows_per_cb][dim] of dtype
  * (rows_per_cb = 1026 for the reference's output.bin; only the first vocab
- * rows of each codebook are kept on the device). */
+ * rows of each codebook are kept on the device).  After a call that fails past
+ * its argument checks steps return ZONOS2CU_ESTATE. */
 int zonos2cu_set_head(zonos2cu_ctx *ctx, const void *W_host, zonos2cu_dtype dtype,
                       int rows_per_cb);
 /* History ring [n_streams][n_cb][hist_len] and its write position.  The

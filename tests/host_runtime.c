@@ -15,10 +15,7 @@ typedef struct {
 } Kernel;
 static Kernel g_kernels[kKernels];
 static int g_n_kernels;
-static struct {
-    int kernel;
-    long long smem;
-} g_launches[kLaunches];
+static int g_launches[kLaunches];   /* places in g_kernels */
 static int g_n_launches, g_fail_at, g_live, g_device;
 
 /* ---- what the tests use */
@@ -26,7 +23,7 @@ void fake_fail_alloc(int n) { g_fail_at = n; }   /* 1: the next one; 0: none */
 int fake_live_allocs(void) { return g_live; }
 int fake_launches(void) { return g_n_launches; }
 void fake_forget(void) { g_n_launches = 0; }
-const char *fake_launched(int i) { return g_kernels[g_launches[i].kernel].name; }
+const char *fake_launched(int i) { return g_kernels[g_launches[i]].name; }
 /* the smallest or largest limit among the kernels whose names hold `part`, -1 without one */
 int fake_smem_limit(const char *part, int largest)
 {
@@ -78,11 +75,7 @@ static int launch(const void *host, size_t smem)
 {
     Kernel *k = find(host);
     if ((long long)smem > k->smem) return kInvalidValue;
-    if (g_n_launches < kLaunches) {
-        g_launches[g_n_launches].kernel = (int)(k - g_kernels);
-        g_launches[g_n_launches].smem = (long long)smem;
-        g_n_launches++;
-    }
+    if (g_n_launches < kLaunches) g_launches[g_n_launches++] = (int)(k - g_kernels);
     return kOk;
 }
 unsigned __cudaPushCallConfiguration(Dim3 grid, Dim3 block, size_t smem, void *stream)
