@@ -212,6 +212,121 @@ int zonos2cu_block_norm(const void *resid_dev, const void *block_dev, zonos2cu_d
                         void *resid_out_dev, void *normed_out_dev, long long out_stride,
                         void *stream);
 
+/* ---- the output head in 8-bit integers (device pointers) ------------------- */
+
+/* Rows of x (bf16 or f32, their starts x_stride elements apart) rounded to 8 bits with a
+ * scale each (no counterpart in the reference):
+ *     scale[r] = max_k |x[r][k]| / 127,   q[r][k] = x[r][k] * 127 / max_k |x[r][k]|,
+ * q rounded once to the nearest integer, ties to even, so that |q| <= 127.  A row of
+ * zeros has scale 0; a row that holds a NaN or an infinity has q = 0 and scale NaN.
+ *   q_dev        [rows][dim] i8; scale_dev [rows] f32.
+ * For the weights of zonos2cu_head_i8 once, at set-up. */
+int zonos2cu_quantize_rows(const void *x_dev, zonos2cu_dtype dtype, int rows, int dim,
+                           long long x_stride, int8_t *q_dev, float *scale_dev, void *stream);
+
+/* zonos2cu_head_softcap with 8-bit weights and hidden rows rounded to 8 bits on the way, as
+ * zonos2cu_quantize_rows rounds them:
+ *   logits[b][c][v] = softcap * tanh(scale_b * w_scale[n] * (q_b . W[n]) / softcap)
+ * with n = c*rows_per_cb + v (softcap <= 0: no cap).  The products are summed exactly, in
+ * 32-bit integers; the rest is f32.  A hidden row that holds a NaN or an infinity has NaN
+ * logits.  With n_cb = 1 and no cap this is a plain product of 8-bit integers with a scale
+ * per row of either side.
+ *   W_dev        [n_cb*rows_per_cb][dim] i8, 16-byte aligned; w_scale_dev
+ *                [n_cb*rows_per_cb] f32.
+ *   hidden_dev   [batch][dim] of `dtype`, logits_dev [batch][n_cb][vocab].
+ *   work_dev     work_bytes of scratch, 16-byte aligned, at least
+ *                zonos2cu_head_i8_work(batch, dim).  Calls that may overlap need scratch of
+ *                their own.
+ * dim must be a multiple of 16 (ZONOS2CU_EUNSUPPORTED elsewhere), at most
+ * ZONOS2CU_MAX_I8_DIM (no sum of products then passes 32 bits). */
+#define ZONOS2CU_MAX_I8_DIM 131072
+long long zonos2cu_head_i8_work(int batch, int dim);
+int zonos2cu_head_i8(const int8_t *W_dev, const float *w_scale_dev, int rows_per_cb, int n_cb,
+                     int vocab, int dim, const void *hidden_dev, zonos2cu_dtype dtype, int batch,
+                     float softcap, void *work_dev, long long work_bytes, float *logits_dev,
+                     void *stream);
+
+/* ---- a paged cache of keys and values (device pointers) -------------------- */
+
+/* The attention state of n_streams decode streams, for the decoder blocks ahead of the
+ * head: pages of page_size tokens, and per stream a table of the pages its tokens lie on
+ * (replaces, for a batch, the flat cache of src/zonos2_generate.cpp:115-126).  Token j of
+ * stream s lies on page table[s][j / page_size] at slot j % page_size.
+ *   k_dev, v_dev  pages of `dtype`, page p at element p * page_stride, and in it
+ *                [n_kv_heads][page_size][head_dim] (page_stride >= their product: keys
+ *                and values may share one buffer, page by page).
+ *   table_dev     [n_streams][max_pages] i32.  An entry outside [0, n_pages) is no page:
+ *                nothing is written there, and its tokens are not attended (entries
+ *                behind a stream's last token are not read; pages that a window has left
+ *                behind may be given back and marked -1).
+ *   kv_len_dev    [n_streams] i32, the stream's tokens, the new ones of the call among
+ *                them (tokens past max_pages * page_size are nowhere).
+ *   q_start_dev   [n_streams + 1] i32, rising: rows [q_start[s], q_start[s+1]) of the
+ *                call's token rows are the last tokens of stream s, row i of its n at
+ *                position kv_len[s] - n + i.  A stream may have none.  Rows outside
+ *                [q_start[0], q_start[n_streams]) are not read and stay as they are.
+ * k_dev and v_dev are 16-byte aligned, head_dim is a multiple of 8 up to
+ * ZONOS2CU_MAX_HEAD_DIM, page_size a power of two from 8 to ZONOS2CU_MAX_PAGE, page_stride a
+ * multiple of 8 (ZONOS2CU_EUNSUPPORTED elsewhere). */
+#define ZONOS2CU_MAX_HEAD_DIM 256
+#define ZONOS2CU_MAX_PAGE 4096
+typedef struct {
+    void *k_dev, *v_dev;
+    zonos2cu_dtype dtype;
+    int n_pages, page_size, n_kv_heads, head_dim;
+    long long page_stride;
+    const int32_t *table_dev;
+    int n_streams, max_pages;
+    const int32_t *kv_len_dev;
+    const int32_t *q_start_dev;
+} zonos2cu_cache;
+
+/* The new tokens' queries and keys normalised and rotated, their keys and values written to
+ * the pages (attention_forward's QK-norm, rotation and cache write of src/zonos2_model.cpp, for a batch).
+ * Per token at position p and per head:
+ *     x' = x * weight / sqrt(mean(x^2) + eps)      (eps >= 0; x' = x below 0)
+ *     (a, b) -> (a cos(p f) - b sin(p f), b cos(p f) + a sin(p f))
+ * for the rot_dim / 2 pairs of the head's first rot_dim elements: neighbours
+ * (2i, 2i + 1), or with rot_halves (i, i + rot_dim / 2); f = freq[i].  In f32 (the angle
+ * in f64), rounded once to the cache's type.  Values are copied.
+ *   q_dev, k_dev, v_dev  [rows] token rows of n_heads, n_kv_heads and n_kv_heads heads
+ *                of head_dim elements, of the cache's type, their starts q_stride,
+ *                k_stride and v_stride elements apart.  q_dev may be NULL (keys and
+ *                values alone).
+ *   q_weight_dev, k_weight_dev  [head_dim] f32 or NULL (1).
+ *   freq_dev     [rot_dim / 2] f32, radians per position.  rot_dim = 0: no rotation.
+ *   q_out_dev    as q_dev, at q_out_stride; may be q_dev itself at the same stride.
+ * Rows are 16-byte aligned (ZONOS2CU_EUNSUPPORTED elsewhere).  No two streams' new tokens
+ * may lie on one page's slot.  No other overlap of buffers is allowed. */
+int zonos2cu_cache_append(const zonos2cu_cache *cache, int rows, int n_heads, const void *q_dev,
+                          long long q_stride, const void *k_dev, long long k_stride,
+                          const void *v_dev, long long v_stride, const float *q_weight_dev,
+                          const float *k_weight_dev, float eps, const float *freq_dev, int rot_dim,
+                          int rot_halves, void *q_out_dev, long long q_out_stride, void *stream);
+
+/* Attention of the new tokens over the pages, after zonos2cu_cache_append on the same stream
+ * (attention_forward's scores, softmax, values and head gate of src/zonos2_model.cpp, for a batch).
+ * Query head h of a token at position p, with key head h / (n_heads / n_kv_heads):
+ *     o = g * sum_j softmax_j(scale * q . k_j) v_j
+ * over the stream's tokens j <= p (j > p - window with window > 0) that lie on a page;
+ * zero where there is none.  What lies elsewhere, a NaN among it, has no part in it.
+ * g = 1 / (1 + exp(-gate)) (1 without gates).  Scores, sums and softmax are f32; with a
+ * bf16 cache the softmax's weights are rounded to bf16 before they meet the values (each
+ * is at most 1 beside the row's largest; their sum is taken unrounded).
+ *   q_dev, out_dev  [rows] token rows of n_heads heads of head_dim elements of the cache's
+ *                type, q_stride and out_stride elements apart, 16-byte aligned
+ *                (ZONOS2CU_EUNSUPPORTED elsewhere).  out_dev must not overlap the others.
+ *   gate_dev     NULL, or the gate of row r, head h at r * gate_stride + h.
+ *   max_new      the most new tokens that a stream has, as far as the caller knows (0:
+ *                not at all).  It chooses between kernels; chunks longer than it says are
+ *                still attended.
+ * n_heads is a multiple of n_kv_heads; scale is positive and finite.  Sums are taken in an
+ * order that the sizes alone give. */
+int zonos2cu_cache_attend(const zonos2cu_cache *cache, int rows, int n_heads, const void *q_dev,
+                          long long q_stride, float scale, int window, const void *gate_dev,
+                          long long gate_stride, int max_new, void *out_dev, long long out_stride,
+                          void *stream);
+
 /* ---- drafted frames against the target (device pointers) -------------------- */
 
 /* No counterpart in the reference.  A stream has up to n_draft drafted frames of

@@ -11,9 +11,11 @@
 #include <new>
 
 #include "block_norm.cuh"
+#include "cache.cuh"
 #include "common.cuh"
 #include "head.cuh"
 #include "head_adapters.cuh"
+#include "head_i8.cuh"
 #include "generate.cuh"
 #include "sampler.cuh"
 #include "verify.cuh"
@@ -457,6 +459,148 @@ int zonos2cu_block_norm(const void *resid_dev, const void *block_dev, zonos2cu_d
     return ZONOS2CU_OK;
 }
 
+int zonos2cu_quantize_rows(const void *x_dev, zonos2cu_dtype dtype, int rows, int dim,
+                           long long x_stride, int8_t *q_dev, float *scale_dev, void *stream)
+{
+    if (dtype != ZONOS2CU_F32 && dtype != ZONOS2CU_BF16) return ZONOS2CU_EINVAL;
+    if (rows < 0 || dim < 1 || x_stride < dim) return ZONOS2CU_EINVAL;
+    if (rows == 0) return ZONOS2CU_OK;
+    if (!x_dev || !q_dev || !scale_dev) return ZONOS2CU_EINVAL;
+    if ((uintptr_t)x_dev % (dtype == ZONOS2CU_F32 ? 4 : 2) || (uintptr_t)scale_dev % 4)
+        return ZONOS2CU_EINVAL;
+    Z2_CK(z2::launch_quantize_rows(x_dev, dtype == ZONOS2CU_BF16, rows, dim, x_stride, q_dev, scale_dev,
+                                   (cudaStream_t)stream));
+    return ZONOS2CU_OK;
+}
+
+long long zonos2cu_head_i8_work(int batch, int dim)
+{
+    if (batch < 0 || dim < 1 || dim > ZONOS2CU_MAX_I8_DIM) return ZONOS2CU_EINVAL;
+    return z2::head_i8_work_bytes(batch, dim);
+}
+
+int zonos2cu_head_i8(const int8_t *W_dev, const float *w_scale_dev, int rows_per_cb, int n_cb,
+                     int vocab, int dim, const void *hidden_dev, zonos2cu_dtype dtype, int batch,
+                     float softcap, void *work_dev, long long work_bytes, float *logits_dev,
+                     void *stream)
+{
+    const int rc = check_head(W_dev, dtype, rows_per_cb, n_cb, vocab, dim, hidden_dev, batch,
+                              softcap, logits_dev);
+    if (rc) return rc;
+    if (dim > ZONOS2CU_MAX_I8_DIM) return ZONOS2CU_EINVAL;
+    if (dim % 16) return ZONOS2CU_EUNSUPPORTED;
+    // rows, logits of a row and blocks of either are counted in 32 bits
+    if ((long long)n_cb * rows_per_cb > 0x3fffffff) return ZONOS2CU_EUNSUPPORTED;
+    if (batch == 0) return ZONOS2CU_OK;
+    if (!w_scale_dev || !work_dev) return ZONOS2CU_EINVAL;
+    if ((uintptr_t)W_dev % 16 || (uintptr_t)w_scale_dev % 4 || (uintptr_t)work_dev % 16 ||
+        (uintptr_t)hidden_dev % (dtype == ZONOS2CU_F32 ? 4 : 2) || (uintptr_t)logits_dev % 4)
+        return ZONOS2CU_EINVAL;
+    if (work_bytes < z2::head_i8_work_bytes(batch, dim)) return ZONOS2CU_EINVAL;
+    const z2::HeadI8Args a{W_dev, w_scale_dev, rows_per_cb, n_cb, vocab, dim, hidden_dev, batch,
+                           softcap, work_dev, logits_dev};
+    Z2_CK(z2::launch_head_i8(a, dtype == ZONOS2CU_BF16, (cudaStream_t)stream));
+    return ZONOS2CU_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// The checks that both calls on a cache make of it and of their token rows; *out is its form
+// for the kernels.
+int check_cache(const zonos2cu_cache *c, int rows, int n_heads, z2::CacheArgs *out)
+{
+    if (!c || rows < 0 || n_heads < 1) return ZONOS2CU_EINVAL;
+    if (c->dtype != ZONOS2CU_F32 && c->dtype != ZONOS2CU_BF16) return ZONOS2CU_EINVAL;
+    if (c->n_pages < 1 || c->n_kv_heads < 1 || c->head_dim < 1 || c->page_size < 1 ||
+        c->n_streams < 0 || c->max_pages < 1)
+        return ZONOS2CU_EINVAL;
+    if (c->head_dim % 8 || c->head_dim > ZONOS2CU_MAX_HEAD_DIM || c->page_size < 8 ||
+        c->page_size > ZONOS2CU_MAX_PAGE || (c->page_size & (c->page_size - 1)) || c->page_stride % 8)
+        return ZONOS2CU_EUNSUPPORTED;
+    // heads lie on a launch grid's third axis, or are counted beside a token's
+    if (c->n_kv_heads > 4096 || n_heads > 65535) return ZONOS2CU_EUNSUPPORTED;
+    if (c->page_stride < (long long)c->n_kv_heads * c->page_size * c->head_dim) return ZONOS2CU_EINVAL;
+    if (n_heads % c->n_kv_heads) return ZONOS2CU_EINVAL;
+    if (rows > 0 && c->n_streams > 0) {
+        if (!c->k_dev || !c->v_dev || !c->table_dev || !c->kv_len_dev || !c->q_start_dev)
+            return ZONOS2CU_EINVAL;
+        if ((uintptr_t)c->table_dev % 4 || (uintptr_t)c->kv_len_dev % 4 || (uintptr_t)c->q_start_dev % 4)
+            return ZONOS2CU_EINVAL;
+        if ((uintptr_t)c->k_dev % 16 || (uintptr_t)c->v_dev % 16) return ZONOS2CU_EUNSUPPORTED;
+    }
+    int shift = 0;
+    while ((1 << shift) < c->page_size) shift++;
+    *out = z2::CacheArgs{c->k_dev, c->v_dev, c->n_pages, shift, c->n_kv_heads, c->head_dim, c->page_stride,
+                         c->table_dev, c->n_streams, c->max_pages, c->kv_len_dev, c->q_start_dev, rows};
+    return ZONOS2CU_OK;
+}
+
+// Rows of `width` elements of `bytes` each whose starts lie `stride` apart: 16-byte aligned?
+int check_token_rows(const void *p, long long stride, long long width, int bytes)
+{
+    if (!p || stride < width) return ZONOS2CU_EINVAL;
+    return (uintptr_t)p % 16 || stride * bytes % 16 ? ZONOS2CU_EUNSUPPORTED : ZONOS2CU_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int zonos2cu_cache_append(const zonos2cu_cache *cache, int rows, int n_heads, const void *q_dev,
+                          long long q_stride, const void *k_dev, long long k_stride,
+                          const void *v_dev, long long v_stride, const float *q_weight_dev,
+                          const float *k_weight_dev, float eps, const float *freq_dev, int rot_dim,
+                          int rot_halves, void *q_out_dev, long long q_out_stride, void *stream)
+{
+    z2::CacheArgs c{};
+    int rc = check_cache(cache, rows, n_heads, &c);
+    if (rc) return rc;
+    if (!isfinite(eps) || rot_dim < 0 || rot_dim > c.dim || rot_dim % 2) return ZONOS2CU_EINVAL;
+    if (rows == 0 || c.n_streams == 0) return ZONOS2CU_OK;
+    const int bytes = cache->dtype == ZONOS2CU_F32 ? 4 : 2;
+    const long long q_width = (long long)n_heads * c.dim, kv_width = (long long)c.n_kv * c.dim;
+    if (q_dev && ((rc = check_token_rows(q_dev, q_stride, q_width, bytes)) ||
+                  (rc = check_token_rows(q_out_dev, q_out_stride, q_width, bytes))))
+        return rc;
+    if (q_dev && q_out_dev == q_dev && q_out_stride != q_stride && rows > 1) return ZONOS2CU_EINVAL;
+    if ((rc = check_token_rows(k_dev, k_stride, kv_width, bytes)) ||
+        (rc = check_token_rows(v_dev, v_stride, kv_width, bytes)))
+        return rc;
+    if (rot_dim > 0 && !freq_dev) return ZONOS2CU_EINVAL;
+    if ((uintptr_t)q_weight_dev % 4 || (uintptr_t)k_weight_dev % 4 || (uintptr_t)freq_dev % 4)
+        return ZONOS2CU_EINVAL;
+    const z2::AppendArgs a{q_dev, k_dev, v_dev, q_stride, k_stride, v_stride, n_heads, q_weight_dev,
+                           k_weight_dev, eps >= 0.0f, eps, freq_dev, rot_dim, rot_halves ? 1 : 0,
+                           q_out_dev, q_out_stride};
+    Z2_CK(z2::launch_cache_append(c, a, cache->dtype == ZONOS2CU_BF16, (cudaStream_t)stream));
+    return ZONOS2CU_OK;
+}
+
+int zonos2cu_cache_attend(const zonos2cu_cache *cache, int rows, int n_heads, const void *q_dev,
+                          long long q_stride, float scale, int window, const void *gate_dev,
+                          long long gate_stride, int max_new, void *out_dev, long long out_stride,
+                          void *stream)
+{
+    z2::CacheArgs c{};
+    int rc = check_cache(cache, rows, n_heads, &c);
+    if (rc) return rc;
+    if (!(scale > 0.0f) || !isfinite(scale)) return ZONOS2CU_EINVAL;
+    if (gate_dev && gate_stride < n_heads) return ZONOS2CU_EINVAL;
+    if (rows == 0 || c.n_streams == 0) return ZONOS2CU_OK;
+    const int bytes = cache->dtype == ZONOS2CU_F32 ? 4 : 2;
+    const long long width = (long long)n_heads * c.dim;
+    if ((rc = check_token_rows(q_dev, q_stride, width, bytes)) ||
+        (rc = check_token_rows(out_dev, out_stride, width, bytes)))
+        return rc;
+    if (q_dev == out_dev || (uintptr_t)gate_dev % bytes) return ZONOS2CU_EINVAL;
+    const z2::AttendArgs a{q_dev, q_stride, n_heads, n_heads / c.n_kv, scale, window, gate_dev,
+                           gate_stride, max_new, out_dev, out_stride};
+    Z2_CK(z2::launch_cache_attend(c, a, cache->dtype == ZONOS2CU_BF16, (cudaStream_t)stream));
+    return ZONOS2CU_OK;
+}
+
 int zonos2cu_verify_drafts(const float *logits_dev, int n_streams, int n_draft, int n_cb,
                            int vocab, long long row_stride, const zonos2cu_sample_params *params,
                            const int32_t *drafts_dev, const float *draft_probs_dev,
@@ -547,12 +691,13 @@ int zonos2cu_write_codes_bin(const char *path, const int32_t *frames_host, int n
 int zonos2cu_device_error(void)
 {
     Z2_CK(cudaDeviceSynchronize());
-    int v = 0, vs = 0, va = 0;
+    int v = 0, vs = 0, va = 0, vi = 0;
     int e = z2::read_and_clear_device_error(&v);
     if (!e) e = z2::read_and_clear_sampler_error(&vs);
     if (!e) e = z2::read_and_clear_adapter_error(&va);
+    if (!e) e = z2::read_and_clear_head_i8_error(&vi);
     if (e) return cuda_fail((cudaError_t)e, "device error word");
-    return v ? v : vs ? vs : va;
+    return v ? v : vs ? vs : va ? va : vi;
 }
 
 }  // extern "C"

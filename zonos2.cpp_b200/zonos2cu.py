@@ -47,7 +47,8 @@ EXPORTS = (
     "zonos2cu_ipc_alloc", "zonos2cu_ipc_free", "zonos2cu_ipc_open", "zonos2cu_ipc_close",
     "zonos2cu_push_codes", "zonos2cu_block_norm", "zonos2cu_verify_drafts",
     "zonos2cu_head_adapters", "zonos2cu_head_adapters_work", "zonos2cu_set_adapters",
-    "zonos2cu_set_stream_adapters",
+    "zonos2cu_set_stream_adapters", "zonos2cu_quantize_rows", "zonos2cu_head_i8_work",
+    "zonos2cu_head_i8", "zonos2cu_cache_append", "zonos2cu_cache_attend",
 )
 
 
@@ -77,6 +78,14 @@ class SampleParams(C.Structure):
 class Dims(C.Structure):
     _fields_ = [("n_streams", C.c_int), ("n_cb", C.c_int), ("vocab", C.c_int), ("dim", C.c_int),
                 ("hist_len", C.c_int), ("seed", C.c_uint64), ("first_stream", C.c_uint64)]
+
+
+class _Cache(C.Structure):
+    """zonos2cu_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("n_pages", C.c_int),
+                ("page_size", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_stride", C.c_longlong), ("table", C.c_void_p), ("n_streams", C.c_int),
+                ("max_pages", C.c_int), ("kv_len", C.c_void_p), ("q_start", C.c_void_p)]
 
 
 _lib = None
@@ -149,6 +158,12 @@ def lib() -> C.CDLL:
                                     ll, vp]),
         "zonos2cu_verify_drafts": (i, [vp, i, i, i, i, ll, C.POINTER(SampleParams), vp, vp, vp, vp,
                                        vp, i, vp, vp, i, vp, vp, vp, vp]),
+        "zonos2cu_quantize_rows": (i, [vp, i, i, i, ll, vp, vp, vp]),
+        "zonos2cu_head_i8_work": (ll, [i, i]),
+        "zonos2cu_head_i8": (i, [vp, vp, i, i, i, i, vp, i, i, f, vp, ll, vp, vp]),
+        "zonos2cu_cache_append": (i, [vp, i, i, vp, ll, vp, ll, vp, ll, vp, vp, f, vp, i, i, vp, ll,
+                                      vp]),
+        "zonos2cu_cache_attend": (i, [vp, i, i, vp, ll, f, i, vp, ll, i, vp, ll, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -385,6 +400,127 @@ def block_norm(resid, block, resid_out, normed_out, *, post_weight=None, post_ep
             strides[0], strides[1], _ptr(post_weight), post_eps, _ptr(gate), gate_row, gate_col,
             int(gate_sigmoid), scale, _ptr(norm_weight), norm_eps, _ptr(resid_out),
             _ptr(normed_out), strides[2])
+
+
+def quantize_rows(x, q, scale, *, stream=None) -> None:
+    """x [rows, dim] bf16 or f32 (row stride allowed) -> q int8 [rows, dim], scale f32 [rows]:
+    scale = max |x| / 127 and q = x * 127 / max |x|, rounded, row by row."""
+    rows, dim = x.shape
+    import torch
+    _whole("quantize_rows", x, (q, rows * dim, (torch.int8,)), (scale, rows, (torch.float32,)))
+    _launch("zonos2cu_quantize_rows", x, stream, x.data_ptr(), _dtype(x), rows, dim,
+            _rows(x, "quantize_rows"), q.data_ptr(), scale.data_ptr())
+
+
+def head_i8_work(batch: int, dim: int) -> int:
+    """Bytes of scratch that head_i8 needs."""
+    return _check(lib().zonos2cu_head_i8_work(batch, dim), "zonos2cu_head_i8_work")
+
+
+def head_i8(W, w_scale, rows_per_cb: int, n_cb: int, vocab: int, hidden, out, work, *,
+            softcap: float = 15.0, stream=None) -> None:
+    """head_softcap in 8-bit integers: W int8 [n_cb * rows_per_cb, dim] with w_scale f32 (as
+    quantize_rows gives them), hidden bf16 or f32 [batch, dim] rounded on the way; out f32
+    [batch, n_cb, vocab]; work: a scratch tensor of head_i8_work() bytes."""
+    batch, dim = hidden.shape
+    wide = n_cb * rows_per_cb
+    import torch
+    f32 = (torch.float32,)
+    _whole("head_i8", hidden, (W, wide * dim, (torch.int8,)), (w_scale, wide, f32),
+           (hidden, batch * dim, (hidden.dtype,)), (out, batch * n_cb * vocab, f32),
+           (work, work.numel(), (work.dtype,)))
+    _launch("zonos2cu_head_i8", hidden, stream, W.data_ptr(), w_scale.data_ptr(), rows_per_cb, n_cb,
+            vocab, dim, hidden.data_ptr(), _dtype(hidden), batch, softcap, work.data_ptr(),
+            work.numel() * work.element_size(), out.data_ptr())
+
+
+class PagedCache:
+    """A decoder block's paged cache of keys and values (zonos2cu_cache).
+
+    k_pages, v_pages [n_pages, n_kv_heads, page_size, head_dim] bf16 or f32 (a stride from page
+    to page allowed, the same for both); table int32 [n_streams, max_pages]; kv_len int32
+    [n_streams], the new tokens among them; q_start int32 [n_streams + 1], the token rows of each
+    stream.  The tensors are kept, and read by each call as they are then."""
+
+    def __init__(self, k_pages, v_pages, table, kv_len, q_start):
+        import torch
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError("PagedCache: keys and values [n_pages, n_kv_heads, page_size, head_dim]")
+        n_pages, kv, page, dim = k_pages.shape
+        for t in (k_pages, v_pages):
+            if t.stride()[1:] != (page * dim, dim, 1) or t.stride(0) != k_pages.stride(0):
+                raise ValueError("PagedCache: whole pages at one stride expected")
+        if table.dim() != 2:
+            raise ValueError("PagedCache: table [n_streams, max_pages]")
+        S, wide = table.shape
+        i32 = (torch.int32,)
+        _whole("PagedCache", k_pages, (table, S * wide, i32), (kv_len, S, i32), (q_start, S + 1, i32))
+        if v_pages.get_device() != k_pages.get_device():
+            raise ValueError("PagedCache: tensors on one device expected")
+        self.k_pages, self.v_pages, self.table = k_pages, v_pages, table
+        self.kv_len, self.q_start = kv_len, q_start
+        self.kv_heads, self.head_dim = kv, dim
+        self._dtype, self._dev = k_pages.dtype, k_pages.get_device()
+        self._c = _Cache(k_pages.data_ptr(), v_pages.data_ptr(), _dtype(k_pages), n_pages, page, kv, dim,
+                         k_pages.stride(0) if n_pages > 1 else kv * page * dim, table.data_ptr(), S, wide,
+                         kv_len.data_ptr(), q_start.data_ptr())
+        self._at = C.addressof(self._c)
+
+    def _tokens(self, what: str, t, rows: int, width: int) -> int:
+        """The row stride of token rows [rows, width] of the cache's type and device."""
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+            raise ValueError(f"{what}: [{rows}, {width}] expected, got {tuple(t.shape)}")
+        if t.dtype != self._dtype:
+            raise TypeError(f"{what}: {self._dtype} expected, got {t.dtype}")
+        if t.get_device() != self._dev:
+            raise ValueError(f"{what}: tensors on the cache's device expected")
+        return _rows(t, what)
+
+
+def cache_append(cache: PagedCache, q, k, v, q_out, *, freq=None, halves: bool = False, q_weight=None,
+                 k_weight=None, eps: float = 1e-5, stream=None) -> None:
+    """New tokens into the cache: queries and keys normalised per head (eps < 0: not) and rotated
+    by their positions, keys and values written to the pages.
+
+    q, q_out [rows, n_heads * head_dim] (q_out may be q; both None: keys and values alone); k, v
+    [rows, n_kv_heads * head_dim]; row strides allowed.  freq f32 [pairs], radians per position of
+    each rotated pair: neighbours, or with ``halves`` (i, i + pairs); None: no rotation.  Weights
+    f32 [head_dim] or None."""
+    rows, dim = k.shape[0], cache.head_dim
+    wide = cache.kv_heads * dim
+    ks, vs = cache._tokens("cache_append", k, rows, wide), cache._tokens("cache_append", v, rows, wide)
+    qs = os_ = 0
+    heads = cache.kv_heads
+    if q is not None:
+        heads = q.shape[1] // dim
+        qs = cache._tokens("cache_append", q, rows, heads * dim)
+        os_ = cache._tokens("cache_append", q_out, rows, heads * dim)
+    elif q_out is not None:
+        raise ValueError("cache_append: q_out without q")
+    pairs = 0 if freq is None else freq.numel()
+    import torch
+    f32 = (torch.float32,)
+    _whole("cache_append", k, (freq, pairs, f32), (q_weight, dim, f32), (k_weight, dim, f32))
+    _launch("zonos2cu_cache_append", k, stream, cache._at, rows, heads, _ptr(q), qs, k.data_ptr(), ks,
+            v.data_ptr(), vs, _ptr(q_weight), _ptr(k_weight), eps, _ptr(freq), 2 * pairs, int(halves),
+            _ptr(q_out), os_)
+
+
+def cache_attend(cache: PagedCache, q, out, *, scale: float | None = None, window: int = 0, gate=None,
+                 max_new: int = 0, stream=None) -> None:
+    """Attention of the new tokens over the cache's pages, causal, after cache_append.
+
+    q, out [rows, n_heads * head_dim] of the cache's type (row strides allowed); scale: 1 /
+    sqrt(head_dim) where None; window > 0: the last tokens that a token sees, itself among them;
+    gate [rows, n_heads] of the cache's type or None: sigmoid(gate) times each head's result;
+    max_new: the most new tokens a stream has, where known (it chooses between kernels)."""
+    rows, dim = q.shape[0], cache.head_dim
+    heads = q.shape[1] // dim
+    qs = cache._tokens("cache_attend", q, rows, heads * dim)
+    os_ = cache._tokens("cache_attend", out, rows, heads * dim)
+    gs = 0 if gate is None else cache._tokens("cache_attend", gate, rows, heads)
+    _launch("zonos2cu_cache_attend", q, stream, cache._at, rows, heads, q.data_ptr(), qs,
+            dim ** -0.5 if scale is None else scale, window, _ptr(gate), gs, max_new, out.data_ptr(), os_)
 
 
 def verify_drafts(logits, params: SampleParams, drafts, uniforms, codes, n_accepted, *,
