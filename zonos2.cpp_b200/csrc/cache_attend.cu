@@ -26,8 +26,11 @@ namespace z2 {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreadsRows = 32 * kWarps;
+#ifndef Z2_S2
+#define Z2_S2 3
+#define Z2_S1 3
+#define Z2_FILL 148*4
+#endif
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -37,7 +40,12 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool take)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// The same, or zeros without a read.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool take)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                  "r"(take ? 16 : 0)
@@ -94,23 +102,27 @@ struct Tile {
     int row0, rows;    // rows == 0: none
 };
 
-__device__ Tile find_tile(const CacheArgs &c, int group, int tile_rows, long long t, int *s_found)
+__device__ Tile find_tile(const CacheArgs &c, int group, int tile_rows, long long t, int4 *s_found)
 {
-    if (threadIdx.x == 0) *s_found = -1;
+    if (threadIdx.x == 0) *s_found = make_int4(-1, 0, 0, 0);
     __syncthreads();
-    auto number = [&](int s) {
-        const int a = min(max(__ldg(c.q_start + s), 0), c.rows);
-        return (long long)a * group / tile_rows + s;
-    };
-    for (int s = threadIdx.x; s < c.n_streams; s += blockDim.x)
-        if (number(s) <= t && t < number(s + 1)) *s_found = s;   // one stream's, as the starts rise
+    auto number = [&](int s, int first) { return (long long)first * group / tile_rows + s; };
+    for (int s = threadIdx.x; s < c.n_streams; s += blockDim.x) {
+        const Chunk ch = chunk_of(c, s);
+        const int end = min(max(__ldg(c.q_start + s + 1), 0), c.rows);
+        if (number(s, ch.first) <= t && t < number(s + 1, end))   // one stream's, as the starts rise
+            *s_found = make_int4(s, ch.first, ch.n, ch.len);
+    }
     __syncthreads();
+    const int4 f = *s_found;
     Tile tile;
     tile.rows = 0;
-    const int s = *s_found;
-    if (s < 0) return tile;
-    tile.ch = chunk_of(c, s);
-    const long long first = (t - number(s)) * tile_rows, all = (long long)tile.ch.n * group;
+    if (f.x < 0) return tile;
+    tile.ch.stream = f.x;
+    tile.ch.first = f.y;
+    tile.ch.n = f.z;
+    tile.ch.len = f.w;
+    const long long first = (t - number(f.x, f.y)) * tile_rows, all = (long long)f.z * group;
     if (first < all) {
         tile.row0 = (int)first;
         tile.rows = (int)(all - first < tile_rows ? all - first : tile_rows);
@@ -134,32 +146,63 @@ struct Ring {
     static constexpr int kStage = 2 * kHalf;
     static constexpr int kPieces = kRow / 16;
 
-    // Loads the keys [j0, j0 + KEYS) that lie in [low, high) and on a page; zeros elsewhere.
-    // Returns the bits of KEYS / 8 runs of eight that lie on a page.
-    __device__ static uint32_t load(const CacheArgs &c, int s, int kvh, int j0, int low, int high, int room,
+    // The pages of a group's runs of eight keys.
+    struct Pages {
+        int p[KEYS / 8];
+    };
+    __device__ static Pages look(const CacheArgs &c, int s, int j0, int room)
+    {
+        Pages pages;
+#pragma unroll
+        for (int e = 0; e < KEYS / 8; e++) pages.p[e] = j0 + 8 * e < room ? page_of(c, s, j0 + 8 * e) : -1;
+        return pages;
+    }
+
+    // Loads the keys (KV & 1) and values (KV & 2) [j0, j0 + KEYS) that lie in [low, high) and
+    // on a page; zeros elsewhere.  Returns the bits of KEYS / 8 runs of eight that lie on a page.
+    template <int KV>
+    __device__ static uint32_t load(const CacheArgs &c, const Pages &pages, int kvh, int j0, int low, int high,
                                     uint32_t stage)
     {
         const int lane = threadIdx.x & 31;
+        const int row0 = lane / kPieces, piece = lane % kPieces;
+        constexpr int kStep = 32 / kPieces > 0 ? 32 / kPieces : 1;          // rows of a warp's copy
+        constexpr int kAcross = kPieces > 32 ? kPieces / 32 : 1;            // copies of a row
+        // a run of eight lies on one page, and so do two unless pages hold eight
         long long base[KEYS / 8];
         uint32_t held = 0;
 #pragma unroll
         for (int e = 0; e < KEYS / 8; e++) {
-            const int j = j0 + 8 * e;
-            const int p = j < room ? page_of(c, s, j) : -1;
-            base[e] = p >= 0 ? row_on_page(c, p, kvh, j) : 0;
-            held |= p >= 0 ? 1u << e : 0u;
+            base[e] = pages.p[e] >= 0 ? row_on_page(c, pages.p[e], kvh, j0 + 8 * e) : 0;
+            held |= pages.p[e] >= 0 ? 1u << e : 0u;
+        }
+        const uint32_t to = stage + row0 * kRow;
+        if (held == (1u << KEYS / 8) - 1 && j0 >= low && j0 + KEYS <= high && c.dim == D &&
+            (KEYS == 8 || c.page_shift > 3)) {   // a whole group: its rows lie behind each other
+            const char *k = (const char *)((const T *)c.k + base[0]) + lane * 16;
+            const char *v = (const char *)((const T *)c.v + base[0]) + lane * 16;
+#pragma unroll
+            for (int i = 0; i < KEYS / kStep; i++)
+#pragma unroll
+                for (int x = 0; x < kAcross; x++) {
+                    const int r = i * kStep;   // row0 + r; row0 < kStep
+                    const uint32_t dst = to + r * kRow + (((piece + 32 * x) ^ ((row0 + r) & 7)) << 4);
+                    if (KV & 1) cp_async16(dst, k + (i * kAcross + x) * 512);
+                    if (KV & 2) cp_async16(dst + kHalf, v + (i * kAcross + x) * 512);
+                }
+            return held;
         }
         const int live = c.dim * (int)sizeof(T) / 16;   // pieces of a row that there are
-#pragma unroll
-        for (int i = 0; i < KEYS * kPieces / 32; i++) {
-            const int id = i * 32 + lane, r = id / kPieces, p = id % kPieces;
-            const int j = j0 + r;
-            const long long at = (KEYS == 8 || r < 8 ? base[0] : base[KEYS / 8 - 1]) + (r & 7) * c.dim;
+#pragma unroll 1
+        for (int i = 0; i < KEYS / kStep; i++) {
+            const int r = row0 + i * kStep, j = j0 + r;
             const bool take = (held >> (r >> 3) & 1u) && j >= low && j < high;
-            const uint32_t dst = stage + r * kRow + ((p ^ (r & 7)) << 4);
-            if (p < live) {
-                cp_async16(dst, (const T *)c.k + (take ? at : 0) + p * (16 / (int)sizeof(T)), take);
-                cp_async16(dst + kHalf, (const T *)c.v + (take ? at : 0) + p * (16 / (int)sizeof(T)), take);
+            const long long at = take ? (KEYS == 8 || r < 8 ? base[0] : base[KEYS / 8 - 1]) + (r & 7) * c.dim : 0;
+            for (int x = piece; x < live; x += 32) {
+                const uint32_t dst = stage + r * kRow + ((x ^ (r & 7)) << 4);
+                if (KV & 1) cp_async16_or_zero(dst, (const T *)c.k + at + x * (16 / (int)sizeof(T)), take);
+                if (KV & 2) cp_async16_or_zero(dst + kHalf, (const T *)c.v + at + x * (16 / (int)sizeof(T)), take);
+                if (kPieces <= 32) break;
             }
         }
         return held;
@@ -167,96 +210,116 @@ struct Ring {
 };
 
 // Joins the parts of the block's warps (and of the cluster's blocks) and stores the rows.
-// part: [kWarps][ROWS][D] f32 outputs, ml: [kWarps][ROWS] maxima and sums behind each other.
-template <typename T, int D, int ROWS>
+// part: [W][ROWS][D] f32 outputs, 16-byte piece p of row r at piece p ^ (2 r & 14) (rows of the
+// mma.sync kernel then fall on different banks); ml: [W][ROWS] maxima and sums; weight: room
+// for kMostRanks * ROWS factors, total for ROWS; gate: the rows' factors.
+constexpr int kMostRanks = 16;
+
+__device__ __forceinline__ int part_piece(int r, int p) { return p ^ ((2 * r) & 14); }
+
+// The rows' gates, to shared memory, ahead of their use.
+template <typename T>
+__device__ __forceinline__ void load_gates(const AttendArgs &a, const Tile &tile, int kvh, float *gate)
+{
+    for (int r = threadIdx.x; r < tile.rows; r += blockDim.x) {
+        const int row = tile.row0 + r;
+        const T *at = (const T *)a.gate + (long long)(tile.ch.first + row / a.group) * a.gate_stride;
+        gate[r] = a.gate ? 1.0f / (1.0f + expf(-as_f(at[kvh * a.group + row % a.group]))) : 1.0f;
+    }
+}
+
+template <typename T, int D, int ROWS, int W, int THREADS>
 __device__ void join_and_store(const CacheArgs &c, const AttendArgs &a, const Tile &tile, int kvh,
-                               float *part, float2 *ml, int ranks, int rank)
+                               float *part, float2 *ml, float *weight, float *total, const float *gate,
+                               int ranks, int rank)
 {
     constexpr int kQuads = ROWS * D / 4;
+    // A part without a visible token (m = -inf) weighs nothing; a NaN sum stays one.
     auto weigh = [](float m, float most) { return m == -INFINITY ? 0.0f : exp2_fast(m - most); };
+    auto add = [](float4 &sum, float f, const float4 &v) {
+        sum.x = fmaf(f, v.x, sum.x);
+        sum.y = fmaf(f, v.y, sum.y);
+        sum.z = fmaf(f, v.z, sum.z);
+        sum.w = fmaf(f, v.w, sum.w);
+    };
     __syncthreads();
     // the block's own warps, into warp 0's part
-    for (int i = threadIdx.x; i < kQuads; i += kThreadsRows) {
-        const int r = i / (D / 4);
-        float most = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) most = fmaxf(most, ml[w * ROWS + r].x);
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            const float f = weigh(ml[w * ROWS + r].x, most);
-            const float4 v = reinterpret_cast<const float4 *>(part)[w * kQuads + i];
-            if (f != 0.0f) {
-                sum.x += f * v.x;
-                sum.y += f * v.y;
-                sum.z += f * v.z;
-                sum.w += f * v.w;
-            }
-        }
-        reinterpret_cast<float4 *>(part)[i] = sum;
-    }
-    __syncthreads();
-    if (threadIdx.x < ROWS) {
-        const int r = threadIdx.x;
+    for (int r = threadIdx.x; r < ROWS; r += THREADS) {
         float most = -INFINITY, l = 0.0f;
-        for (int w = 0; w < kWarps; w++) most = fmaxf(most, ml[w * ROWS + r].x);
-        for (int w = 0; w < kWarps; w++) {
+#pragma unroll
+        for (int w = 0; w < W; w++) most = fmaxf(most, ml[w * ROWS + r].x);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
             const float f = weigh(ml[w * ROWS + r].x, most);
-            l += f != 0.0f ? f * ml[w * ROWS + r].y : 0.0f;
+            weight[w * ROWS + r] = f;   // W <= kMostRanks
+            l += f * ml[w * ROWS + r].y;
         }
-        // a NaN among the sums stays one whatever its weight
-        for (int w = 0; w < kWarps; w++)
-            if (isnan(ml[w * ROWS + r].y)) l = ml[w * ROWS + r].y;
         ml[r] = make_float2(most, l);
     }
-    if (ranks > 1)
+    __syncthreads();
+    for (int i = threadIdx.x; i < kQuads; i += THREADS) {
+        const int r = i / (D / 4);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < W; w++)
+            add(sum, weight[w * ROWS + r], reinterpret_cast<const float4 *>(part)[w * kQuads + i]);
+        reinterpret_cast<float4 *>(part)[i] = sum;
+    }
+    if (ranks > 1) {
         cluster_sync();
-    else
+        // every rank's maximum and sum, all asked for at once
+        for (int i = threadIdx.x; i < ranks * ROWS; i += THREADS) {
+            const int k = i / ROWS, r = i % ROWS;
+            float m, l;
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                         : "=f"(m), "=f"(l)
+                         : "r"(peer_addr(smem_u32(ml + r), k)));
+            reinterpret_cast<float2 *>(part + ROWS * D)[i] = make_float2(m, l);   // behind warp 0's part
+        }
         __syncthreads();
-    const uint32_t part0 = smem_u32(part), ml0 = smem_u32(ml);
+        for (int r = threadIdx.x; r < ROWS; r += THREADS) {
+            const float2 *all = reinterpret_cast<const float2 *>(part + ROWS * D) + r;
+            float most = -INFINITY, l = 0.0f;
+            for (int k = 0; k < ranks; k++) most = fmaxf(most, all[k * ROWS].x);
+            for (int k = 0; k < ranks; k++) {
+                const float f = weigh(all[k * ROWS].x, most);
+                weight[k * ROWS + r] = f;
+                l += f * all[k * ROWS].y;
+            }
+            total[r] = l;
+        }
+    } else {
+        for (int r = threadIdx.x; r < ROWS; r += THREADS) total[r] = ml[r].y;
+    }
+    __syncthreads();
     // this rank's share of the rows' quads
     const int per = (kQuads + ranks - 1) / ranks;
     const int end = min(kQuads, (rank + 1) * per);
-    for (int i = rank * per + threadIdx.x; i < end; i += kThreadsRows) {
-        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+    for (int i = rank * per + threadIdx.x; i < end; i += THREADS) {
+        const int r = i / (D / 4), d = part_piece(r, i % (D / 4)) * 4;
         if (r >= tile.rows || d >= c.dim) continue;
-        float4 sum = reinterpret_cast<const float4 *>(part)[i];
-        float l = ml[r].y;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (ranks > 1) {
-            float most = -INFINITY;
-            for (int k = 0; k < ranks; k++) {
-                float m;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m) : "r"(peer_addr(ml0 + r * 8, k)));
-                most = fmaxf(most, m);
+            const uint32_t at = smem_u32(part) + i * 16;
+            for (int k0 = 0; k0 < ranks; k0 += 4) {   // ranks: 2, or a multiple of 4
+                float4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (k0 + k < ranks)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w)
+                                     : "r"(peer_addr(at, k0 + k)));
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (k0 + k < ranks) add(sum, weight[(k0 + k) * ROWS + r], v[k]);
             }
-            sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            l = 0.0f;
-            for (int k = 0; k < ranks; k++) {
-                float m, lk;
-                float4 v;
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-                             : "=f"(m), "=f"(lk)
-                             : "r"(peer_addr(ml0 + r * 8, k)));
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                             : "r"(peer_addr(part0 + i * 16, k)));
-                const float f = weigh(m, most);
-                if (f != 0.0f || isnan(lk)) {
-                    l += f * lk;
-                    sum.x += f * v.x;
-                    sum.y += f * v.y;
-                    sum.z += f * v.z;
-                    sum.w += f * v.w;
-                }
-            }
+        } else {
+            sum = reinterpret_cast<const float4 *>(part)[i];
         }
+        const float l = total[r];
         const int row = tile.row0 + r, token = tile.ch.first + row / a.group;
         const int h = kvh * a.group + row % a.group;
-        float f = l == 0.0f ? 0.0f : 1.0f / l;
-        if (a.gate) {
-            const float g = as_f(((const T *)a.gate)[token * a.gate_stride + h]);
-            f *= 1.0f / (1.0f + expf(-g));
-        }
+        const float f = l == 0.0f ? 0.0f : gate[r] / l;
         T *to = (T *)a.out + token * a.out_stride + (long long)h * c.dim + d;
         if (sizeof(T) == 2) {
             *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(sum.x * f, sum.y * f), pack_bf16(sum.z * f, sum.w * f));
@@ -268,49 +331,27 @@ __device__ void join_and_store(const CacheArgs &c, const AttendArgs &a, const Ti
 }
 
 // ---- bf16, by mma.sync ------------------------------------------------------
-// 16 * MB rows to a tile, groups of 16 keys: S = Q K^T by m16n8k16 (rows x 8 keys x 16
-// elements), whose accumulators, rounded to bf16, are the left operand of O += P V.
-template <int D, int MB, int STAGES>
-__global__ void __launch_bounds__(kThreadsRows)
+// 16 * RB rows to a tile, groups of 16 keys: S = Q K^T by m16n8k16 (rows x 8 keys x 16
+// elements), whose accumulators, rounded to bf16, are the left operand of O += P V.  A ring's
+// groups are worked by RB warps, 16 rows each, which load them together (one the keys, the
+// other the values).
+template <int D, int RB, int STAGES, int W>
+__global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 3 : 2)
     attend_rows_bf16_kernel(const CacheArgs c, const AttendArgs a, int ranks)
 {
     typedef Ring<__nv_bfloat16, D, 16> R;
-    constexpr int ROWS = 16 * MB;
+    constexpr int ROWS = 16 * RB, kThreads = 32 * W * RB;
     extern __shared__ __align__(1024) unsigned char smem[];
-    // the warps' rings, then the queries; at the end the parts take the rings' place
-    __shared__ float2 s_ml[kWarps * ROWS];
-    __shared__ int s_found;
+    // the rings, then the queries; at the end the parts take the rings' place
+    __shared__ float2 s_ml[W * ROWS];
+    __shared__ float s_weight[kMostRanks * ROWS], s_total[ROWS], s_gate[ROWS];
+    __shared__ int4 s_found;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) / RB, rb = (threadIdx.x >> 5) % RB;
     const int rank = blockIdx.x % ranks, kvh = blockIdx.y;
     const Tile tile = find_tile(c, a.group, ROWS, blockIdx.x / ranks, &s_found);
     if (tile.rows == 0) return;   // the whole cluster's tile
-
-    const uint32_t ring = smem_u32(smem) + warp * STAGES * R::kStage;
-    const uint32_t s_q = smem_u32(smem) + kWarps * STAGES * R::kStage;
-    const int live = c.dim / 8;
-    // queries (zeros past the rows and the head's elements), swizzled like the keys
-    for (int i = threadIdx.x; i < ROWS * R::kPieces; i += kThreadsRows) {
-        const int r = i / R::kPieces, p = i % R::kPieces, row = tile.row0 + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < tile.rows && p < live)
-            v = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q +
-                                                 (tile.ch.first + row / a.group) * a.q_stride +
-                                                 (long long)(kvh * a.group + row % a.group) * c.dim + p * 8);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_q + r * R::kRow + ((p ^ (r & 7)) << 4)),
-                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                     : "memory");
-    }
-    if (live < R::kPieces)   // pieces that no copy fills
-        for (int i = lane; i < STAGES * 32 * R::kPieces; i += 32) {
-            const int r = i / R::kPieces, p = i % R::kPieces;
-            if (p >= live)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + r * R::kRow + ((p ^ (r & 7)) << 4)),
-                             "r"(0)
-                             : "memory");
-        }
-    __syncthreads();
 
     // the tokens that some row of the tile sees, in groups of 16
     const int room = room_of(c);
@@ -320,132 +361,170 @@ __global__ void __launch_bounds__(kThreadsRows)
     const int high = min(pos_last + 1, room);
     const int sees_all_from = a.window > 0 ? max(0, pos_last - a.window + 1) : 0;   // .. to pos_first
     const int first_group = low >> 4, groups = high > low ? ((high + 15) >> 4) - first_group : 0;
-    const int workers = ranks * kWarps, worker = rank * kWarps + warp;
+    const int workers = ranks * W, worker = rank * W + warp;
+    auto group_at = [&](int it) { return (first_group + worker + it * workers) * 16; };
+    auto look = [&](int it) { return R::look(c, tile.ch.stream, group_at(it), worker + it * workers < groups ? room : 0); };
+    typename R::Pages pages[STAGES];   // of the first turns, then [0]: of the next one to be fetched
+#pragma unroll
+    for (int i = 0; i < STAGES; i++) pages[i] = look(i);
 
-    int pos[2 * MB];   // of this lane's rows (those past the tile's take the last row's)
-#pragma unroll
-    for (int i = 0; i < 2 * MB; i++)
-        pos[i] = position_of(tile.ch, a.group, tile.row0 + min((i >> 1) * 16 + (i & 1) * 8 + (lane >> 2), tile.rows - 1));
-    float m[2 * MB], l[2 * MB], o[MB][D / 8][4];
-#pragma unroll
-    for (int i = 0; i < 2 * MB; i++) {
-        m[i] = -INFINITY;
-        l[i] = 0.0f;
+    const uint32_t ring = smem_u32(smem) + warp * STAGES * R::kStage;
+    const uint32_t s_q = smem_u32(smem) + W * STAGES * R::kStage;
+    const int live = c.dim / 8;
+    // queries (zeros past the rows and the head's elements), swizzled like the keys
+    for (int i = threadIdx.x; i < ROWS * R::kPieces; i += kThreads) {
+        const int r = i / R::kPieces, p = i % R::kPieces, row = tile.row0 + r;
+        const bool in = r < tile.rows && p < live;
+        const long long at = in ? (tile.ch.first + row / a.group) * a.q_stride +
+                                      (long long)(kvh * a.group + row % a.group) * c.dim + p * 8
+                                : 0;
+        cp_async16_or_zero(s_q + r * R::kRow + ((p ^ (r & 7)) << 4), (const __nv_bfloat16 *)a.q + at, in);
     }
-#pragma unroll
-    for (int b = 0; b < MB; b++)
-#pragma unroll
-        for (int n = 0; n < D / 8; n++) o[b][n][0] = o[b][n][1] = o[b][n][2] = o[b][n][3] = 0.0f;
-    const float factor = a.scale * kLog2e;
-
-    // ldmatrix: lane's row and piece of a 16 x 16 block
-    const int lm_key = (lane & 7) + ((lane >> 4) << 3), lm_kp = (lane >> 3) & 1;     // keys: n blocks of 8
-    const int lm_val = (lane & 7) + (((lane >> 3) & 1) << 3), lm_vp = lane >> 4;     // values, transposed
-    constexpr bool kQRegs = MB * D <= 128;
-    uint32_t qf[kQRegs ? MB : 1][kQRegs ? D / 16 : 1][4];
-    auto load_q = [&](int b, int kk, uint32_t (&f)[4]) {
-        const int r = b * 16 + (lane & 15), p = 2 * kk + (lane >> 4);
-        ldmatrix4(s_q + r * R::kRow + ((p ^ (r & 7)) << 4), f);
-    };
-    if (kQRegs) {
-#pragma unroll
-        for (int b = 0; b < MB; b++)
-#pragma unroll
-            for (int kk = 0; kk < D / 16; kk++) load_q(b, kk, qf[b][kk]);
-    }
-
+    cp_async_commit();
+    load_gates<__nv_bfloat16>(a, tile, kvh, s_gate);
+    if (live < R::kPieces)   // pieces that no copy fills
+        for (int i = lane; i < STAGES * 32 * R::kPieces; i += 32) {
+            const int r = i / R::kPieces, p = i % R::kPieces;
+            if (p >= live)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + r * R::kRow + ((p ^ (r & 7)) << 4)),
+                             "r"(0)
+                             : "memory");
+        }
     uint32_t held_bits = 0;   // two bits to a stage
-    auto fetch = [&](int it) {
-        const int g = worker + it * workers;
-        if (g < groups) {
+    auto fetch = [&](int it, const typename R::Pages &at) {
+        if (worker + it * workers < groups) {
             const int st = it % STAGES;
-            const uint32_t held = R::load(c, tile.ch.stream, kvh, (first_group + g) * 16, low, high, room,
-                                          ring + st * R::kStage);
+            const uint32_t to = ring + st * R::kStage;
+            uint32_t held;
+            if (RB == 1)
+                held = R::template load<3>(c, at, kvh, group_at(it), low, high, to);
+            else if (rb == 0)
+                held = R::template load<1>(c, at, kvh, group_at(it), low, high, to);
+            else
+                held = R::template load<2>(c, at, kvh, group_at(it), low, high, to);
             held_bits = (held_bits & ~(3u << (2 * st))) | held << (2 * st);
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) fetch(i);
+    for (int i = 0; i < STAGES - 1; i++) fetch(i, pages[i]);
+    pages[0] = pages[STAGES - 1];
+    cp_async_wait<STAGES - 1>();   // the queries
+    __syncthreads();
+
+    int pos[2];   // of this lane's rows (those past the tile's take the last row's)
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        pos[i] = position_of(tile.ch, a.group, tile.row0 + min(rb * 16 + i * 8 + (lane >> 2), tile.rows - 1));
+    float m[2], l[2], o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+    }
+#pragma unroll
+    for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    const float factor = a.scale * kLog2e;
+
+    // ldmatrix: lane's row and piece of a 16 x 16 block
+    const int lm_key = (lane & 7) + ((lane >> 4) << 3), lm_kp = (lane >> 3) & 1;     // keys: n blocks of 8
+    const int lm_val = (lane & 7) + (((lane >> 3) & 1) << 3), lm_vp = lane >> 4;     // values, transposed
+    constexpr bool kQRegs = RB == 1 && D <= 128;
+    uint32_t qf[kQRegs ? D / 16 : 1][4];
+    auto load_q = [&](int kk, uint32_t (&f)[4]) {
+        const int r = rb * 16 + (lane & 15), p = 2 * kk + (lane >> 4);
+        ldmatrix4(s_q + r * R::kRow + ((p ^ (r & 7)) << 4), f);
+    };
+    if (kQRegs) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk++) load_q(kk, qf[kk]);
+    }
+    auto meet = [&]() {   // the warps of the ring
+        if (RB == 1)
+            __syncwarp();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + warp), "n"(32 * RB) : "memory");
+    };
+
     for (int it = 0; worker + it * workers < groups; it++) {
-        fetch(it + STAGES - 1);
-        cp_async_wait<STAGES - 1>();
-        __syncwarp();
+        cp_async_wait<STAGES - 2>();
+        meet();   // the group has landed, and the one before it is done with
+        const typename R::Pages next = look(it + STAGES);
+        fetch(it + STAGES - 1, pages[0]);
+        pages[0] = next;
         const int st = it % STAGES;
         const uint32_t keys = ring + st * R::kStage, values = keys + R::kHalf;
-        const int j0 = (first_group + worker + it * workers) * 16;
+        const int j0 = group_at(it);
         const uint32_t held = held_bits >> (2 * st) & 3u;
-        float x[MB][2][4];
+        float x[2][4];
 #pragma unroll
-        for (int b = 0; b < MB; b++)
-#pragma unroll
-            for (int n = 0; n < 2; n++) x[b][n][0] = x[b][n][1] = x[b][n][2] = x[b][n][3] = 0.0f;
+        for (int n = 0; n < 2; n++) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < D / 16; kk++) {
-            uint32_t kf[4];
+            uint32_t kf[4], f[4];
             ldmatrix4(keys + lm_key * R::kRow + (((2 * kk + lm_kp) ^ (lm_key & 7)) << 4), kf);
-#pragma unroll
-            for (int b = 0; b < MB; b++) {
-                uint32_t f[4];
-                if (!kQRegs) load_q(b, kk, f);
-                mma_16816(x[b][0], kQRegs ? qf[b][kk] : f, kf[0], kf[1]);
-                mma_16816(x[b][1], kQRegs ? qf[b][kk] : f, kf[2], kf[3]);
-            }
+            if (!kQRegs) load_q(kk, f);
+            mma_16816(x[0], kQRegs ? qf[kQRegs ? kk : 0] : f, kf[0], kf[1]);
+            mma_16816(x[1], kQRegs ? qf[kQRegs ? kk : 0] : f, kf[2], kf[3]);
         }
-        // rows that do not see all of the group
+        // scores that a row does not see: out of the maximum, and of weight zero
         const bool partial = j0 < sees_all_from || j0 + 15 > pos_first || j0 + 15 >= high || held != 3u;
         auto sees = [&](int i, int j) {   // row slot i of this lane, token j
             return j <= pos[i] && j < high && (a.window <= 0 || j > pos[i] - a.window) && (held >> ((j - j0) >> 3) & 1u);
         };
-        float keep[2 * MB];
+        uint32_t seen = 0xffu;   // bit 4 i + 2 n + e
+        if (partial) {
+            seen = 0;
+#pragma unroll
+            for (int b = 0; b < 8; b++) {
+                const int i = b >> 2, n = (b >> 1) & 1, e = b & 1;
+                if (sees(i, j0 + 8 * n + 2 * (lane & 3) + e))
+                    seen |= 1u << b;
+                else
+                    x[n][i * 2 + e] = -INFINITY;
+            }
+        }
+        float top[2];
         bool same = true;
 #pragma unroll
-        for (int i = 0; i < 2 * MB; i++) {
-            float most = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float &v = x[i >> 1][n][(i & 1) * 2 + e];
-                    v *= factor;
-                    if (!partial || sees(i, j0 + 8 * n + 2 * (lane & 3) + e)) most = fmaxf(most, v);
-                }
+        for (int i = 0; i < 2; i++) {
+            float most = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
             most = fmaxf(most, __shfl_xor_sync(kFull, most, 1));
             most = fmaxf(most, __shfl_xor_sync(kFull, most, 2));
-            most = fmaxf(most, m[i]);
-            keep[i] = m[i] == -INFINITY ? 0.0f : exp2_fast(m[i] - most);
-            same = same && most == m[i];
-            m[i] = most;
+            top[i] = fmaxf(most * factor, m[i]);   // factor > 0
+            same = same && top[i] == m[i];
         }
         if (!__all_sync(kFull, same)) {
 #pragma unroll
-            for (int i = 0; i < 2 * MB; i++) {
-                l[i] *= keep[i];
+            for (int i = 0; i < 2; i++) {
+                const float keep = m[i] == -INFINITY ? 0.0f : exp2_fast(m[i] - top[i]);
+                m[i] = top[i];
+                l[i] *= keep;
 #pragma unroll
                 for (int n = 0; n < D / 8; n++) {
-                    o[i >> 1][n][(i & 1) * 2] *= keep[i];
-                    o[i >> 1][n][(i & 1) * 2 + 1] *= keep[i];
+                    o[n][i * 2] *= keep;
+                    o[n][i * 2 + 1] *= keep;
                 }
             }
         }
-        uint32_t pf[MB][4];
 #pragma unroll
-        for (int b = 0; b < MB; b++) {
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[n][e] = exp2_fast(fmaf(x[n][e], factor, -m[e >> 1]));
+        if (partial) {
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = 2 * b + (e >> 1);
-                    float w = exp2_fast(x[b][n][e] - m[i]);
-                    if (partial && !sees(i, j0 + 8 * n + 2 * (lane & 3) + (e & 1))) w = 0.0f;
-                    l[i] += w;
-                    x[b][n][e] = w;
-                }
-            pf[b][0] = pack_bf16(x[b][0][0], x[b][0][1]);
-            pf[b][1] = pack_bf16(x[b][0][2], x[b][0][3]);
-            pf[b][2] = pack_bf16(x[b][1][0], x[b][1][1]);
-            pf[b][3] = pack_bf16(x[b][1][2], x[b][1][3]);
+                for (int e = 0; e < 4; e++)
+                    if (!(seen >> (4 * (e >> 1) + 2 * n + (e & 1)) & 1u)) x[n][e] = 0.0f;
         }
+#pragma unroll
+        for (int i = 0; i < 2; i++) l[i] += (x[0][2 * i] + x[0][2 * i + 1]) + (x[1][2 * i] + x[1][2 * i + 1]);
+        uint32_t pf[4];
+        pf[0] = pack_bf16(x[0][0], x[0][1]);
+        pf[1] = pack_bf16(x[0][2], x[0][3]);
+        pf[2] = pack_bf16(x[1][0], x[1][1]);
+        pf[3] = pack_bf16(x[1][2], x[1][3]);
         if (partial) {
             // A value that is not finite would reach rows that do not see its token, as 0 times
             // it: it goes to the rows that do by itself, and is a zero to the product.
@@ -457,7 +536,8 @@ __global__ void __launch_bounds__(kThreadsRows)
                              : "r"(values + i * 16));
                 any |= odd2(v.x) || odd2(v.y) || odd2(v.z) || odd2(v.w);
             }
-            if (__any_sync(kFull, any)) {
+            if (__any_sync(kFull, any)) {   // the same for every warp of the ring
+#pragma unroll 1
                 for (int k = 0; k < 16; k++)
 #pragma unroll
                     for (int n = 0; n < D / 8; n++) {
@@ -468,13 +548,13 @@ __global__ void __launch_bounds__(kThreadsRows)
                         if (!odd2(w)) continue;
                         const float v0 = __uint_as_float(w << 16), v1 = __uint_as_float(w & 0xffff0000u);
 #pragma unroll
-                        for (int i = 0; i < 2 * MB; i++)
+                        for (int i = 0; i < 2; i++)
                             if (sees(i, j0 + k)) {
-                                if (odd(v0)) o[i >> 1][n][(i & 1) * 2] += v0;
-                                if (odd(v1)) o[i >> 1][n][(i & 1) * 2 + 1] += v1;
+                                if (odd(v0)) o[n][i * 2] += v0;
+                                if (odd(v1)) o[n][i * 2 + 1] += v1;
                             }
                     }
-                __syncwarp();
+                meet();
                 for (int i = lane; i < 64 * R::kPieces; i += 32) {
                     uint32_t w;
                     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(values + i * 4));
@@ -482,50 +562,47 @@ __global__ void __launch_bounds__(kThreadsRows)
                     if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(values + i * 4), "r"(w) : "memory");
                 }
-                __syncwarp();
+                meet();
             }
         }
 #pragma unroll
         for (int n = 0; n < D / 16; n++) {
             uint32_t vf[4];
             ldmatrix4_trans(values + lm_val * R::kRow + (((2 * n + lm_vp) ^ (lm_val & 7)) << 4), vf);
-#pragma unroll
-            for (int b = 0; b < MB; b++) {
-                mma_16816(o[b][2 * n], pf[b], vf[0], vf[1]);
-                mma_16816(o[b][2 * n + 1], pf[b], vf[2], vf[3]);
-            }
+            mma_16816(o[2 * n], pf, vf[0], vf[1]);
+            mma_16816(o[2 * n + 1], pf, vf[2], vf[3]);
         }
-        __syncwarp();   // the stage is free for the copies of the next turn
     }
     cp_async_wait<0>();
     __syncthreads();   // every warp is done with its ring: the parts take their place
     float *part = reinterpret_cast<float *>(smem);
 #pragma unroll
-    for (int i = 0; i < 2 * MB; i++) {
+    for (int i = 0; i < 2; i++) {
         l[i] += __shfl_xor_sync(kFull, l[i], 1);
         l[i] += __shfl_xor_sync(kFull, l[i], 2);
-        const int r = (i >> 1) * 16 + (i & 1) * 8 + (lane >> 2);
+        const int r = rb * 16 + i * 8 + (lane >> 2);
         if ((lane & 3) == 0) s_ml[warp * ROWS + r] = make_float2(m[i], l[i]);
 #pragma unroll
         for (int n = 0; n < D / 8; n++)
-            *reinterpret_cast<float2 *>(part + (warp * ROWS + r) * D + n * 8 + 2 * (lane & 3)) =
-                make_float2(o[i >> 1][n][(i & 1) * 2], o[i >> 1][n][(i & 1) * 2 + 1]);
+            *reinterpret_cast<float2 *>(part + (warp * ROWS + r) * D + part_piece(r, 2 * n + ((lane & 3) >> 1)) * 4 + 2 * (lane & 1)) =
+                make_float2(o[n][i * 2], o[n][i * 2 + 1]);
     }
-    join_and_store<__nv_bfloat16, D, ROWS>(c, a, tile, kvh, part, s_ml, ranks, rank);
+    join_and_store<__nv_bfloat16, D, ROWS, W, kThreads>(c, a, tile, kvh, part, s_ml, s_weight, s_total, s_gate, ranks, rank);
 }
 
 // ---- f32, on the FMA pipe ----------------------------------------------------
 // ROWS rows to a tile, groups of 8 keys.  A lane takes a quarter of a key's elements for
 // the scores of all rows (key lane / 4), then D / 32 of the output's columns.
-template <int D, int ROWS, int STAGES>
-__global__ void __launch_bounds__(kThreadsRows)
+template <int D, int ROWS, int STAGES, int W>
+__global__ void __launch_bounds__(32 * W)
     attend_rows_f32_kernel(const CacheArgs c, const AttendArgs a, int ranks)
 {
     typedef Ring<float, D, 8> R;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ float2 s_ml[kWarps * ROWS];
-    __shared__ __align__(16) float s_w[kWarps][8][ROWS];   // a group's weights
-    __shared__ int s_found;
+    __shared__ float2 s_ml[W * ROWS];
+    __shared__ float s_weight[kMostRanks * ROWS], s_total[ROWS], s_gate[ROWS];
+    __shared__ __align__(16) float s_w[W][8][ROWS];   // a group's weights
+    __shared__ int4 s_found;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -534,9 +611,9 @@ __global__ void __launch_bounds__(kThreadsRows)
     if (tile.rows == 0) return;
 
     const uint32_t ring = smem_u32(smem) + warp * STAGES * R::kStage;
-    float *s_q = reinterpret_cast<float *>(smem + kWarps * STAGES * R::kStage);   // [ROWS][D]
+    float *s_q = reinterpret_cast<float *>(smem + W * STAGES * R::kStage);   // [ROWS][D]
     const int live = c.dim / 4;
-    for (int i = threadIdx.x; i < ROWS * R::kPieces; i += kThreadsRows) {
+    for (int i = threadIdx.x; i < ROWS * R::kPieces; i += (32 * W)) {
         const int r = i / R::kPieces, p = i % R::kPieces, row = tile.row0 + r;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (r < tile.rows && p < live)
@@ -544,6 +621,7 @@ __global__ void __launch_bounds__(kThreadsRows)
                                                   (long long)(kvh * a.group + row % a.group) * c.dim + p * 4);
         reinterpret_cast<float4 *>(s_q)[i] = v;
     }
+    load_gates<float>(a, tile, kvh, s_gate);
     if (live < R::kPieces)
         for (int i = lane; i < STAGES * 16 * R::kPieces; i += 32) {
             const int r = i / R::kPieces, p = i % R::kPieces;
@@ -561,7 +639,7 @@ __global__ void __launch_bounds__(kThreadsRows)
     const int high = min(pos_last + 1, room);
     const int sees_all_from = a.window > 0 ? max(0, pos_last - a.window + 1) : 0;
     const int first_group = low >> 3, groups = high > low ? ((high + 7) >> 3) - first_group : 0;
-    const int workers = ranks * kWarps, worker = rank * kWarps + warp;
+    const int workers = ranks * W, worker = rank * W + warp;
 
     constexpr int kCols = D / 32;   // this lane's columns: 32 apart (piece lane / 4 + 8 i for more)
     float m[ROWS], l[ROWS], o[ROWS][kCols];
@@ -580,8 +658,9 @@ __global__ void __launch_bounds__(kThreadsRows)
         const int g = worker + it * workers;
         if (g < groups) {
             const int st = it % STAGES;
-            const uint32_t held = R::load(c, tile.ch.stream, kvh, (first_group + g) * 8, low, high, room,
-                                          ring + st * R::kStage);
+            const int j0 = (first_group + g) * 8;
+            const uint32_t held = R::template load<3>(c, R::look(c, tile.ch.stream, j0, room), kvh, j0, low, high,
+                                                      ring + st * R::kStage);
             held_bits = (held_bits & ~(1u << st)) | held << st;
         }
         cp_async_commit();
@@ -670,14 +749,24 @@ __global__ void __launch_bounds__(kThreadsRows)
         l[r] += __shfl_xor_sync(kFull, l[r], 16);
         if (lane == 0) s_ml[warp * ROWS + r] = make_float2(m[r], l[r]);
 #pragma unroll
-        for (int i = 0; i < kCols; i++) part[(warp * ROWS + r) * D + lane + 32 * i] = o[r][i];
+        for (int i = 0; i < kCols; i++)
+            part[(warp * ROWS + r) * D + part_piece(r, (lane + 32 * i) >> 2) * 4 + (lane & 3)] = o[r][i];
     }
-    join_and_store<float, D, ROWS>(c, a, tile, kvh, part, s_ml, ranks, rank);
+    join_and_store<float, D, ROWS, W, 32 * W>(c, a, tile, kvh, part, s_ml, s_weight, s_total, s_gate, ranks, rank);
+}
+
+// Tiles that hold rows, as far as the caller says.
+long long tiles_with_rows(const CacheArgs &c, const AttendArgs &a, int tile_rows)
+{
+    const long long tiles = (long long)c.rows * a.group / tile_rows + c.n_streams;
+    const int most_new = a.max_new > 0 && a.max_new < c.rows ? a.max_new : c.rows;
+    const long long filled = (long long)c.n_streams * (((long long)most_new * a.group + tile_rows - 1) / tile_rows);
+    return filled < tiles ? filled : tiles;
 }
 
 template <typename Kernel>
-cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, const CacheArgs &c, const AttendArgs &a,
-                        int keys, std::mutex &mu, bool (&ready)[64], cudaStream_t stream)
+cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, int warps, int threads, const CacheArgs &c,
+                        const AttendArgs &a, int keys, std::mutex &mu, bool (&ready)[64], cudaStream_t stream)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -693,20 +782,17 @@ cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, const CacheAr
         }
     }
     const long long tiles = (long long)c.rows * a.group / tile_rows + c.n_streams;
-    // tiles that hold rows, as far as the caller says
-    const int most_new = a.max_new > 0 && a.max_new < c.rows ? a.max_new : c.rows;
-    const long long filled = (long long)c.n_streams * (((long long)most_new * a.group + tile_rows - 1) / tile_rows);
-    const long long work = (filled < tiles ? filled : tiles) * c.n_kv;
-    const long long room = ((long long)c.max_pages << c.page_shift) / (keys * kWarps);
+    const long long work = tiles_with_rows(c, a, tile_rows) * c.n_kv;
+    const long long room = ((long long)c.max_pages << c.page_shift) / (keys * warps);
     int ranks = 1;
-    while (ranks < 16 && work * ranks < 148 * 4 && ranks < room) ranks *= 2;
+    while (ranks < kMostRanks && work * ranks < Z2_FILL && ranks < room) ranks *= 2;
 #ifdef Z2_RANKS
     ranks = Z2_RANKS;
 #endif
     if (tiles * ranks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * ranks), (unsigned)c.n_kv);
-    cfg.blockDim = dim3(kThreadsRows);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -720,15 +806,25 @@ cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, const CacheAr
     return cudaLaunchKernelEx(&cfg, kernel, c, a, ranks);
 }
 
-template <int D, int MB, int STAGES>
+template <int D, int RB, int STAGES, int W>
 cudaError_t launch_bf16(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
 {
     static std::mutex mu;
     static bool ready[64] = {false};
     typedef Ring<__nv_bfloat16, D, 16> R;
-    const size_t rings = kWarps * STAGES * R::kStage, parts = (size_t)kWarps * 16 * MB * D * 4;
-    const size_t smem = (rings > parts ? rings : parts) + 16 * MB * R::kRow;
-    return launch_rows(attend_rows_bf16_kernel<D, MB, STAGES>, smem, 16 * MB, c, a, 16, mu, ready, stream);
+    const size_t rings = W * STAGES * R::kStage, parts = (size_t)W * 16 * RB * D * 4;
+    const size_t smem = (rings > parts ? rings : parts) + 16 * RB * R::kRow;
+    return launch_rows(attend_rows_bf16_kernel<D, RB, STAGES, W>, smem, 16 * RB, W, 32 * W * RB, c, a, 16, mu, ready,
+                       stream);
+}
+
+// Blocks of eight rings where a cluster of the most blocks for each tile does not fill the SMs.
+template <int D, int RB, int STAGES>
+cudaError_t launch_bf16(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
+{
+    if (tiles_with_rows(c, a, 16 * RB) * c.n_kv * kMostRanks <= 148)
+        return launch_bf16<D, RB, 3, 8>(c, a, stream);
+    return launch_bf16<D, RB, STAGES, 4>(c, a, stream);
 }
 
 template <int D, int ROWS, int STAGES>
@@ -737,9 +833,10 @@ cudaError_t launch_f32(const CacheArgs &c, const AttendArgs &a, cudaStream_t str
     static std::mutex mu;
     static bool ready[64] = {false};
     typedef Ring<float, D, 8> R;
-    const size_t rings = kWarps * STAGES * R::kStage, parts = (size_t)kWarps * ROWS * D * 4;
+    constexpr int W = 4;
+    const size_t rings = W * STAGES * R::kStage, parts = (size_t)W * ROWS * D * 4;
     const size_t smem = (rings > parts ? rings : parts) + ROWS * R::kRow;
-    return launch_rows(attend_rows_f32_kernel<D, ROWS, STAGES>, smem, ROWS, c, a, 8, mu, ready, stream);
+    return launch_rows(attend_rows_f32_kernel<D, ROWS, STAGES, W>, smem, ROWS, W, 32 * W, c, a, 8, mu, ready, stream);
 }
 
 }  // namespace
@@ -750,8 +847,8 @@ cudaError_t launch_cache_attend(const CacheArgs &c, const AttendArgs &a, bool bf
     const int most_new = a.max_new > 0 && a.max_new < c.rows ? a.max_new : c.rows;
     const long long rows = (long long)most_new * a.group;
     if (bf16) {
-        if (c.dim > 128) return launch_bf16<256, 1, 3>(c, a, stream);
-        if (c.dim > 64) return rows > 16 ? launch_bf16<128, 2, 3>(c, a, stream) : launch_bf16<128, 1, 3>(c, a, stream);
+        if (c.dim > 128) return launch_bf16<256, 1, 3, 4>(c, a, stream);
+        if (c.dim > 64) return rows > 16 ? launch_bf16<128, 2, Z2_S2>(c, a, stream) : launch_bf16<128, 1, Z2_S1>(c, a, stream);
         return rows > 16 ? launch_bf16<64, 2, 4>(c, a, stream) : launch_bf16<64, 1, 4>(c, a, stream);
     }
     if (c.dim > 128) return rows > 4 ? launch_f32<256, 8, 3>(c, a, stream) : launch_f32<256, 4, 3>(c, a, stream);
