@@ -1,0 +1,540 @@
+// cache_attend_tc.cu -- attention of chunks of new tokens over a paged cache on the tcgen05
+// tensor cores (sm_100a): bf16, heads of 64 or 128 elements.
+//
+// A block takes 256 rows -- (token, query head) pairs that share a key head -- as two tiles of
+// 128, and the tokens they see in steps of 128 keys:
+//   warp 0        TMA producer: a step's keys and values, page by page (a box is a page or 128 of
+//                 its tokens), 128-byte swizzled, into a ring of 128 x D tiles;
+//   warp 1        allocates TMEM and issues tcgen05.mma: S = Q K^T (128 x 128, f32) and
+//                 O += P V (P in TMEM as bf16 in place of S, V read as it lies, rows of D);
+//   warps 4..7, 8..11  softmax of one tile each, a row to a thread: S from TMEM, its
+//                 maximum, 2^(x - m), P back to TMEM, and at the end O / l to global memory.
+// While one tile's softmax runs, the tensor core works for the other.  A step of both tiles
+// is 4 x 512 cycles of MMAs and 2 x 128 x 128 exponentials, 2048 cycles of the SM's 16 a
+// cycle: neither may wait for the other.  The running maximum is raised only when a row's scores
+// pass it by more than 2^8 (P is then at most 256 instead of 1, and the sum of the same scale:
+// no rounding changes), so that O is seldom rescaled.  Stages hand over through mbarriers, every
+// wait is bounded.
+// A value that is not finite in a step that some row does not wholly see would reach that row as
+// 0 times it: such values are set to zero in shared memory before the product and added, at the
+// end, to the rows that see them.
+#include <math.h>
+
+#include <mutex>
+
+#include "cache_attend.cuh"
+
+namespace z2 {
+
+int read_and_clear_attend_error(int *value) { return take_device_error(value); }
+
+namespace {
+
+constexpr int kTcThreads = 384;
+constexpr int kStep = 128;       // keys of a step
+constexpr int kSlots = 5;        // tiles of keys or values in shared memory
+constexpr float kSlack = 8.0f;   // how far scores may pass the running maximum, in powers of two
+
+template <int D>
+struct TcShape {
+    static constexpr uint32_t kHalves = D / 64;              // 128-byte columns of a tile
+    static constexpr uint32_t kTile = 128 * D * 2;           // bytes of 128 rows
+    static constexpr uint32_t kQ = 2 * kTile;
+    static constexpr size_t kSmem = kQ + kSlots * kTile + 1024 + 256;
+};
+
+// Shared-memory matrix descriptor, MN-major (rows of K, the product's columns behind each
+// other), 128-byte swizzle: 64 columns of 8 rows are 1024 bytes; 8 rows further on 1024 (SBO),
+// 64 columns further on one 128-row half (LBO).
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t addr)
+{
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)((128 * 128) >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// D += A B with A in TMEM.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+// After tcgen05.wait::ld: nothing reads these registers ahead of it.
+__device__ __forceinline__ void tmem_landed(uint32_t *r)
+{
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                   "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]));
+    asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+
+// What the rows of one 128-row tile see.
+struct Span {
+    int low, high;        // tokens that some row sees lie in [low, high)
+    int all_from, all_to; // .. and every row sees [all_from, all_to)
+};
+
+__device__ __forceinline__ Span span_of(const CacheArgs &c, const AttendArgs &a, const Chunk &ch, int row0, int rows)
+{
+    Span s;
+    const int first = position_of(ch, a.group, row0), last = position_of(ch, a.group, row0 + rows - 1);
+    s.low = a.window > 0 ? max(0, first - a.window + 1) : 0;
+    s.high = min(last + 1, room_of(c));
+    s.all_from = a.window > 0 ? max(0, last - a.window + 1) : 0;
+    s.all_to = min(first + 1, s.high);
+    return s;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attend_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const CacheArgs c, const AttendArgs a, int box_rows)
+{
+    typedef TcShape<D> Sh;
+    // kind::f16: D f32, A and B bf16; M = 128; S: N = 128, both K-major; O: N = D, B MN-major
+    constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (128u >> 3 << 17) | (128u >> 4 << 24);
+    constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)D >> 3 << 17) | (128u >> 4 << 24);
+    constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns: S (then P) of both tiles, O of both
+
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+    const uint32_t s_q = smem, s_kv = smem + Sh::kQ, s_bar = s_kv + kSlots * Sh::kTile;
+    auto full = [&](int s) { return s_bar + 8 * s; };
+    auto empty = [&](int s) { return s_bar + 8 * (kSlots + s); };
+    auto s_full = [&](int q) { return s_bar + 8 * (2 * kSlots + q); };    // S, and O before it, are done
+    auto p_ready = [&](int q) { return s_bar + 8 * (2 * kSlots + 2 + q); };
+    __shared__ uint32_t s_tmem;
+    __shared__ int4 s_found;
+    __shared__ int s_abort, s_odd;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        s_abort = s_odd = 0;
+        for (int s = 0; s < kSlots; s++) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int q = 0; q < 2; q++) {
+            mbar_init(s_full(q), 1);
+            mbar_init(p_ready(q), 128);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&map_k);
+        prefetch_map(&map_v);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int kvh = blockIdx.y;
+    // the last tiles of a stream see the most tokens: they come first
+    const Tile tile = find_tile(c, a.group, 256, (long long)gridDim.x - 1 - blockIdx.x, &s_found);   // (block-wide barriers)
+    const int rows0 = min(tile.rows, 128), rows1 = tile.rows - rows0;
+    Span span0 = {0, 0, 0, 0}, span1 = {0, 0, 0, 0};
+    if (rows0 > 0) span0 = span1 = span_of(c, a, tile.ch, tile.row0, rows0);
+    if (rows1 > 0) span1 = span_of(c, a, tile.ch, tile.row0 + 128, rows1);
+    const int low = min(span0.low, span1.low), high = max(span0.high, span1.high);
+    // tokens that every row of both tiles sees: the tiles share the values, and what is done to them
+    const int all_from = max(span0.all_from, span1.all_from), all_to = min(span0.all_to, span1.all_to);
+    const int step0 = low / kStep, steps = high > low ? (high + kStep - 1) / kStep - step0 : 0;
+
+    if (tile.rows > 0) {
+        // queries, swizzled as TMA does; zeros past the rows
+        for (int i = threadIdx.x; i < 256 * (D / 8); i += kTcThreads) {
+            const int r = i / (D / 8), p = i % (D / 8), row = tile.row0 + r;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < tile.rows)
+                v = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q +
+                                                     (long long)(tile.ch.first + row / a.group) * a.q_stride +
+                                                     (long long)(kvh * a.group + row % a.group) * D + p * 8);
+            const int q = r >> 7, rr = r & 127;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             s_q + q * Sh::kTile + (p >> 3) * (128 * 128) + rr * 128 + (((p & 7) ^ (rr & 7)) << 4)),
+                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                         : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    if (steps > 0) {
+        if (warp == 0) {
+            // ---- TMA producer: tile 2 i is step i's keys, 2 i + 1 its values
+            const int boxes = kStep / box_rows;          // of a step, for each half
+            const int room = room_of(c);
+            bool ok = true;
+            int it = 0;
+            for (int i = 0; i < steps && ok; i++) {
+                const int j0 = (step0 + i) * kStep;
+                // lane's box of the step's boxes x halves (16 x 2 at most)
+                const int b = lane % boxes, h = lane / boxes, j = j0 + b * box_rows;
+                const bool mine = h < (int)Sh::kHalves;
+                int page = -1;
+                if (mine && j < room) page = page_of(c, tile.ch.stream, j);
+                if (page < 0) page = c.n_pages;          // out of the map: zeros
+                const int slot_in_page = j & ((1 << c.page_shift) - 1);
+                for (int kv = 0; kv < 2; kv++, it++) {
+                    const int s = it % kSlots;
+                    ok = mbar_wait(empty(s), (((uint32_t)(it / kSlots)) & 1u) ^ 1u) && !*(volatile int *)&s_abort;
+                    ok = __all_sync(kFull, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(full(s), Sh::kTile);
+                    __syncwarp();
+                    if (mine)
+                        tma_load_4d(s_kv + s * Sh::kTile + h * (128 * 128) + b * box_rows * 128, kv ? &map_v : &map_k,
+                                    h * 64, slot_in_page, kvh, page, full(s));
+                }
+            }
+            if (!ok) {
+                s_abort = 1;
+                for (int k = 0; k < kSlots && k < it; k++) {   // copies still in flight land first
+                    const int t = it - 1 - k;
+                    mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u);
+                }
+            }
+        } else if (warp == 1) {
+            // ---- MMA issuer
+            if (lane == 0) {
+                bool ok = true;
+                auto wait = [&](uint32_t bar, uint32_t parity) {
+                    if (ok && (!mbar_wait(bar, parity) || *(volatile int *)&s_abort)) ok = false;
+                    tc_fence_after();
+                    return ok;
+                };
+                auto slot = [&](int t) { return s_kv + (uint32_t)(t % kSlots) * Sh::kTile; };
+                auto landed = [&](int t) { return wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u); };
+                auto scores = [&](int q, int t) {   // S of tile q by the keys in tile t
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; kk++) {
+                        const uint32_t off = (kk >> 2) * (128 * 128);
+                        mma_bf16(tmem + kColS + q * 128, sw128_desc(s_q + q * Sh::kTile + off) + 2 * (kk & 3),
+                                 sw128_desc(slot(t) + off) + 2 * (kk & 3), kIdescS, kk != 0);
+                    }
+                    mma_commit(s_full(q));
+                };
+                const int tiles = rows1 > 0 ? 2 : 1;
+                if (landed(0)) {
+                    for (int q = 0; q < tiles; q++) scores(q, 0);
+                    mma_commit(empty(0));
+                }
+                for (int i = 0; i < steps && ok; i++) {
+                    const bool more = i + 1 < steps;
+                    if (!landed(2 * i + 1)) break;
+                    for (int q = 0; q < tiles; q++) {
+                        if (!wait(p_ready(q), (uint32_t)i & 1u)) break;
+#pragma unroll
+                        for (int kk = 0; kk < kStep / 16; kk++)
+                            mma_bf16_ts(tmem + kColO + q * 128, tmem + kColS + q * 128 + 8 * kk,
+                                        sw128_desc_mn(slot(2 * i + 1) + kk * 16 * 128), kIdescO, (i | kk) != 0);
+                        if (q == tiles - 1) mma_commit(empty((2 * i + 1) % kSlots));
+                        if (more) {
+                            if (!landed(2 * i + 2)) break;
+                            scores(q, 2 * i + 2);
+                            if (q == tiles - 1) mma_commit(empty((2 * i + 2) % kSlots));
+                        } else {
+                            mma_commit(s_full(q));   // O is whole
+                        }
+                    }
+                }
+                if (!ok) s_abort = 1;
+            }
+        } else if (warp >= 4) {
+            // ---- softmax of tile q, this thread's row r of it
+            const int q = (warp - 4) >> 2, r = threadIdx.x & 127;
+            const int rows = q ? rows1 : rows0;
+            if (rows > 0) {
+                const uint32_t at = ((uint32_t)(warp & 3) * 32) << 16;   // this warp's TMEM lanes
+                const uint32_t t_s = tmem + at + kColS + q * 128, t_o = tmem + at + kColO + q * 128;
+                const int pos = position_of(tile.ch, a.group, tile.row0 + q * 128 + min(r, rows - 1));
+                const int from = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+                const int to = min(pos + 1, (q ? span1 : span0).high);   // this row sees [from, to)
+                const float factor = a.scale * kLog2e;
+                const int room = room_of(c);
+                // the pages of a step's runs of eight tokens, one step ahead; bit 8 e: run e is held
+                auto look = [&](int i) {
+                    const int j = (step0 + i) * kStep + 8 * lane;
+                    return lane < 16 && (i >= steps || (j < room && page_of(c, tile.ch.stream, j) >= 0));
+                };
+                float m = -INFINITY, l = 0.0f;
+                bool saw = false;   // a token that the row sees
+                bool ok = true;
+                bool held_next = look(0);
+                for (int i = 0; i < steps; i++) {
+                    const uint32_t held = __ballot_sync(kFull, held_next) & 0xffffu;
+                    held_next = look(i + 1);
+                    const int j0 = (step0 + i) * kStep;
+                    const bool partial = j0 < all_from || j0 + kStep > all_to || held != 0xffffu;
+                    ok = mbar_wait(s_full(q), (uint32_t)i & 1u) && !*(volatile int *)&s_abort;
+                    ok = __all_sync(kFull, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint32_t x[128];
+#pragma unroll
+                    for (int b = 0; b < 4; b++) tmem_ld32_start(t_s + 32 * b, x + 32 * b);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int b = 0; b < 4; b++) tmem_landed(x + 32 * b);
+                    if (partial) {
+                        const int begin = from - j0, end = to - j0;
+#pragma unroll
+                        for (int k = 0; k < 128; k++) {
+                            const bool in = k >= begin && k < end && (held >> (k >> 3) & 1u);
+                            if (!in) x[k] = 0xff800000u;
+                            saw |= in;
+                        }
+                    } else {
+                        saw = true;
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int b = 0; b < 4; b++) top[b] = __uint_as_float(x[b]);
+#pragma unroll
+                    for (int k = 4; k < 128; k++) top[k & 3] = fmaxf(top[k & 3], __uint_as_float(x[k]));
+                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
+                    const bool raise = most > m + kSlack;   // (m = -inf: a first token)
+                    if (__any_sync(kFull, raise)) {
+                        float keep = 1.0f;
+                        if (raise) {
+                            keep = m == -INFINITY ? 0.0f : exp2_fast(m - most);
+                            m = most;
+                            l *= keep;
+                        }
+                        if (i > 0) {   // O is idle: S came after its last product
+#pragma unroll 1
+                            for (int b = 0; b < D / 32; b++) {
+                                uint32_t o[32];
+                                tmem_ld32_start(t_o + 32 * b, o);
+                                tmem_wait_ld();
+                                tmem_landed(o);
+#pragma unroll
+                                for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                                tmem_st32(t_o + 32 * b, o);
+                            }
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.0f : -m;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        uint32_t p[32];
+#pragma unroll
+                        for (int k = 0; k < 32; k++) {
+                            const float w0 = exp2_fast(fmaf(__uint_as_float(x[64 * b + 2 * k]), factor, base));
+                            const float w1 = exp2_fast(fmaf(__uint_as_float(x[64 * b + 2 * k + 1]), factor, base));
+                            sum[(2 * k) & 3] += w0;
+                            sum[(2 * k + 1) & 3] += w1;
+                            p[k] = pack_bf16(w0, w1);
+                        }
+                        tmem_st32(t_s + 32 * b, p);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_wait_st();
+                    if (partial) {
+                        // values that are not finite: out of the product
+                        const int t = 2 * i + 1;
+                        ok = __all_sync(kFull, mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u));
+                        if (!ok) break;
+                        const uint32_t values = s_kv + (uint32_t)(t % kSlots) * Sh::kTile;
+                        for (int k = r; k < (int)Sh::kTile / 16; k += 128) {
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                         : "r"(values + k * 16));
+                            if (odd2(w[0]) || odd2(w[1]) || odd2(w[2]) || odd2(w[3])) {
+                                s_odd = 1;   // ahead of the zeros that the other tile's threads may find
+                                __threadfence_block();
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
+                                    if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0x0000ffffu;
+                                }
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + k * 16), "r"(w[0]),
+                                             "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                             : "memory");
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    tc_fence_before();
+                    mbar_arrive(p_ready(q));
+                }
+                // ---- O / l
+                ok = ok && mbar_wait(s_full(q), (uint32_t)steps & 1u) && !*(volatile int *)&s_abort;
+                if (__all_sync(kFull, ok)) {
+                    tc_fence_after();
+                    const bool odd_values = *(volatile int *)&s_odd;
+                    const int row = tile.row0 + q * 128 + r, token = tile.ch.first + row / a.group;
+                    const int h = kvh * a.group + row % a.group;
+                    const bool live = r < rows;
+                    float f = l == 0.0f ? (saw ? NAN : 0.0f) : 1.0f / l;
+                    if (a.gate && live) {
+                        const float g = as_f(((const __nv_bfloat16 *)a.gate)[(long long)token * a.gate_stride + h]);
+                        f *= 1.0f / (1.0f + expf(-g));
+                    }
+                    __nv_bfloat16 *out = (__nv_bfloat16 *)a.out + (long long)token * a.out_stride + (long long)h * D;
+#pragma unroll 1
+                    for (int b = 0; b < D / 32; b++) {
+                        uint32_t o[32];
+                        tmem_ld32_start(t_o + 32 * b, o);
+                        tmem_wait_ld();
+                        tmem_landed(o);
+                        if (odd_values && live) {
+                            for (int j = max(from, step0 * kStep); j < to; j++) {
+                                const int s0 = j & ~(kStep - 1);
+                                // steps that every row sees wholly went through the product as they are
+                                const int p = page_of(c, tile.ch.stream, j);
+                                bool whole = s0 >= all_from && s0 + kStep <= all_to;
+                                for (int e = 0; whole && e < kStep / 8; e++)
+                                    whole = s0 + 8 * e < room && page_of(c, tile.ch.stream, s0 + 8 * e) >= 0;
+                                if (p < 0 || whole) continue;
+                                const __nv_bfloat16 *v = (const __nv_bfloat16 *)c.v + row_on_page(c, p, kvh, j) + 32 * b;
+#pragma unroll
+                                for (int k = 0; k < 32; k++) {
+                                    const float y = as_f(v[k]);
+                                    if (odd(y)) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
+                                }
+                            }
+                        }
+                        if (live) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    w[e] = pack_bf16(f == 0.0f ? 0.0f : __uint_as_float(o[8 * k + 2 * e]) * f,
+                                                     f == 0.0f ? 0.0f : __uint_as_float(o[8 * k + 2 * e + 1]) * f);
+                                *reinterpret_cast<uint4 *>(out + 32 * b + 8 * k) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                } else {
+                    s_abort = 1;
+                }
+            }
+        }
+    } else {
+        // rows that see nothing
+        for (int i = threadIdx.x; i < tile.rows * (D / 8); i += kTcThreads) {
+            const int row = tile.row0 + i / (D / 8);
+            *reinterpret_cast<uint4 *>((__nv_bfloat16 *)a.out + (long long)(tile.ch.first + row / a.group) * a.out_stride +
+                                       (long long)(kvh * a.group + row % a.group) * D + i % (D / 8) * 8) =
+                make_uint4(0, 0, 0, 0);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Pages as a 4-D tensor (elements, tokens of a page, key heads, pages); a box is 64 elements of
+// `box_rows` tokens.
+bool make_page_map(CUtensorMap *m, const void *base, const CacheArgs &c, int box_rows)
+{
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t page = 1ull << c.page_shift;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.dim, page, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.dim * 2, page * c.dim * 2, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+cudaError_t launch_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
+{
+    static std::mutex mu;
+    static bool ready[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!ready[dev]) {
+            e = cudaFuncSetAttribute(attend_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TcShape<D>::kSmem);
+            if (e != cudaSuccess) return e;
+            ready[dev] = true;
+        }
+    }
+    const int page = 1 << c.page_shift, box_rows = page < kStep ? page : kStep;
+    CUtensorMap mk, mv;
+    if (!make_page_map(&mk, c.k, c, box_rows) || !make_page_map(&mv, c.v, c, box_rows)) return cudaErrorInvalidValue;
+    const long long tiles = (long long)c.rows * a.group / 256 + c.n_streams;
+    if (tiles > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles, (unsigned)c.n_kv);
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = TcShape<D>::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attend_tc_kernel<D>, mk, mv, c, a, box_rows);
+}
+
+}  // namespace
+
+cudaError_t launch_cache_attend_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
+{
+    return c.dim == 64 ? launch_tc<64>(c, a, stream) : launch_tc<128>(c, a, stream);
+}
+
+}  // namespace z2

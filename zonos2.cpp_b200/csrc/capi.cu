@@ -11,7 +11,7 @@
 #include <new>
 
 #include "block_norm.cuh"
-#include "cache.cuh"
+#include "cache_attend.cuh"
 #include "common.cuh"
 #include "head.cuh"
 #include "head_adapters.cuh"
@@ -691,13 +691,14 @@ int zonos2cu_write_codes_bin(const char *path, const int32_t *frames_host, int n
 int zonos2cu_device_error(void)
 {
     Z2_CK(cudaDeviceSynchronize());
-    int v = 0, vs = 0, va = 0, vi = 0;
+    int v = 0, vs = 0, va = 0, vi = 0, vc = 0;
     int e = z2::read_and_clear_device_error(&v);
     if (!e) e = z2::read_and_clear_sampler_error(&vs);
     if (!e) e = z2::read_and_clear_adapter_error(&va);
     if (!e) e = z2::read_and_clear_head_i8_error(&vi);
+    if (!e) e = z2::read_and_clear_attend_error(&vc);
     if (e) return cuda_fail((cudaError_t)e, "device error word");
-    return v ? v : vs ? vs : va ? va : vi;
+    return v ? v : vs ? vs : va ? va : vi ? vi : vc;
 }
 
 }  // extern "C"
