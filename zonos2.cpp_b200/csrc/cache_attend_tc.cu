@@ -64,6 +64,32 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Two f32 values at a time on the FMA pipe.
+__device__ __forceinline__ uint64_t two(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void both(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t *r)
 {
     asm volatile(
@@ -132,7 +158,7 @@ __device__ __forceinline__ Span span_of(const CacheArgs &c, const AttendArgs &a,
 template <int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attend_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                     const CacheArgs c, const AttendArgs a, int box_rows)
+                     const CacheArgs c, const AttendArgs a, int box_rows, int turns)
 {
     typedef TcShape<D> Sh;
     // kind::f16: D f32, A and B bf16; M = 128; S: N = 128, both K-major; O: N = D, B MN-major
@@ -146,13 +172,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     auto full = [&](int s) { return s_bar + 8 * s; };
     auto empty = [&](int s) { return s_bar + 8 * (kSlots + s); };
     auto s_full = [&](int q) { return s_bar + 8 * (2 * kSlots + q); };    // S, and O before it, are done
-    auto p_ready = [&](int q) { return s_bar + 8 * (2 * kSlots + 2 + q); };
+    auto p_ready = [&](int q, int h) { return s_bar + 8 * (2 * kSlots + 2 + 2 * q + h); };   // P of 64 keys
     __shared__ uint32_t s_tmem;
-    __shared__ int4 s_found;
     __shared__ int s_abort, s_odd;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // A stream's last tiles see the most tokens: every stream's come first.  (Where a stream has
+    // more tiles than it was launched for, a block takes every `turns`-th.)
+    const int kvh = blockIdx.x % c.n_kv, first_turn = blockIdx.x / c.n_kv / c.n_streams;
+    const Chunk ch = chunk_of(c, blockIdx.x / c.n_kv % c.n_streams);
+    const long long all_rows = (long long)ch.n * a.group;
+    const int n_tiles = (int)((all_rows + 255) / 256);
+    if (first_turn >= n_tiles) return;
     if (threadIdx.x == 0) {
         s_abort = s_odd = 0;
         for (int s = 0; s < kSlots; s++) {
@@ -161,7 +194,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         for (int q = 0; q < 2; q++) {
             mbar_init(s_full(q), 1);
-            mbar_init(p_ready(q), 128);
+            mbar_init(p_ready(q, 0), 4);   // the tile's warps
+            mbar_init(p_ready(q, 1), 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_map(&map_k);
@@ -173,40 +207,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int kvh = blockIdx.y;
-    // the last tiles of a stream see the most tokens: they come first
-    const Tile tile = find_tile(c, a.group, 256, (long long)gridDim.x - 1 - blockIdx.x, &s_found);   // (block-wide barriers)
-    const int rows0 = min(tile.rows, 128), rows1 = tile.rows - rows0;
-    Span span0 = {0, 0, 0, 0}, span1 = {0, 0, 0, 0};
-    if (rows0 > 0) span0 = span1 = span_of(c, a, tile.ch, tile.row0, rows0);
-    if (rows1 > 0) span1 = span_of(c, a, tile.ch, tile.row0 + 128, rows1);
+    uint32_t tmem = 0;
+    // phases of the barriers before this tile: tiles of keys and values, scores of either tile
+    int kv0 = 0, scored0 = 0, scored1 = 0, weighed0 = 0, weighed1 = 0;
+#ifdef Z2_REGS
+    if (warp < 4)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+#endif
+    for (int turn = first_turn; turn < n_tiles; turn += turns) {
+    const long long row_ll = (long long)(n_tiles - 1 - turn) * 256;
+    const int row0 = (int)row_ll;
+    const int tile_rows = (int)(all_rows - row_ll < 256 ? all_rows - row_ll : 256);
+    const int rows0 = min(tile_rows, 128), rows1 = tile_rows - rows0;
+    const Span span0 = span_of(c, a, ch, row0, rows0);
+    const Span span1 = rows1 > 0 ? span_of(c, a, ch, row0 + 128, rows1) : span0;
     const int low = min(span0.low, span1.low), high = max(span0.high, span1.high);
     // tokens that every row of both tiles sees: the tiles share the values, and what is done to them
     const int all_from = max(span0.all_from, span1.all_from), all_to = min(span0.all_to, span1.all_to);
     const int step0 = low / kStep, steps = high > low ? (high + kStep - 1) / kStep - step0 : 0;
 
-    if (tile.rows > 0) {
-        // queries, swizzled as TMA does; zeros past the rows
-        for (int i = threadIdx.x; i < 256 * (D / 8); i += kTcThreads) {
-            const int r = i / (D / 8), p = i % (D / 8), row = tile.row0 + r;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < tile.rows)
-                v = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q +
-                                                     (long long)(tile.ch.first + row / a.group) * a.q_stride +
-                                                     (long long)(kvh * a.group + row % a.group) * D + p * 8);
-            const int q = r >> 7, rr = r & 127;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                             s_q + q * Sh::kTile + (p >> 3) * (128 * 128) + rr * 128 + (((p & 7) ^ (rr & 7)) << 4)),
-                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                         : "memory");
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    // queries, swizzled as TMA does; zeros past the rows
+    for (int i = threadIdx.x; i < 256 * (D / 8); i += kTcThreads) {
+        const int r = i / (D / 8), p = i % (D / 8), row = row0 + r;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < tile_rows)
+            v = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q +
+                                                 (long long)(ch.first + row / a.group) * a.q_stride +
+                                                 (long long)(kvh * a.group + row % a.group) * D + p * 8);
+        const int q = r >> 7, rr = r & 127;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                         s_q + q * Sh::kTile + (p >> 3) * (128 * 128) + rr * 128 + (((p & 7) ^ (rr & 7)) << 4)),
+                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                     : "memory");
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    tmem = s_tmem;
 
     if (steps > 0) {
         if (warp == 0) {
@@ -214,14 +254,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int boxes = kStep / box_rows;          // of a step, for each half
             const int room = room_of(c);
             bool ok = true;
-            int it = 0;
+            int it = kv0;
             for (int i = 0; i < steps && ok; i++) {
                 const int j0 = (step0 + i) * kStep;
                 // lane's box of the step's boxes x halves (16 x 2 at most)
                 const int b = lane % boxes, h = lane / boxes, j = j0 + b * box_rows;
                 const bool mine = h < (int)Sh::kHalves;
                 int page = -1;
-                if (mine && j < room) page = page_of(c, tile.ch.stream, j);
+                if (mine && j < room) page = page_of(c, ch.stream, j);
                 if (page < 0) page = c.n_pages;          // out of the map: zeros
                 const int slot_in_page = j & ((1 << c.page_shift) - 1);
                 for (int kv = 0; kv < 2; kv++, it++) {
@@ -238,7 +278,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (!ok) {
                 s_abort = 1;
-                for (int k = 0; k < kSlots && k < it; k++) {   // copies still in flight land first
+                for (int k = 0; k < kSlots && k < it - kv0; k++) {   // copies still in flight land first
                     const int t = it - 1 - k;
                     mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u);
                 }
@@ -248,12 +288,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 0) {
                 bool ok = true;
                 auto wait = [&](uint32_t bar, uint32_t parity) {
-                    if (ok && (!mbar_wait(bar, parity) || *(volatile int *)&s_abort)) ok = false;
+                    ok = ok && mbar_wait(bar, parity);
                     tc_fence_after();
                     return ok;
                 };
-                auto slot = [&](int t) { return s_kv + (uint32_t)(t % kSlots) * Sh::kTile; };
-                auto landed = [&](int t) { return wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u); };
+                auto slot = [&](int t) { return s_kv + (uint32_t)((kv0 + t) % kSlots) * Sh::kTile; };
+                auto landed = [&](int t) { return wait(full((kv0 + t) % kSlots), (uint32_t)((kv0 + t) / kSlots) & 1u); };
+                auto done = [&](int t) { mma_commit(empty((kv0 + t) % kSlots)); };
                 auto scores = [&](int q, int t) {   // S of tile q by the keys in tile t
 #pragma unroll
                     for (int kk = 0; kk < D / 16; kk++) {
@@ -266,22 +307,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int tiles = rows1 > 0 ? 2 : 1;
                 if (landed(0)) {
                     for (int q = 0; q < tiles; q++) scores(q, 0);
-                    mma_commit(empty(0));
+                    done(0);
                 }
-                for (int i = 0; i < steps && ok; i++) {
+                for (int i = 0; i < steps && ok && !*(volatile int *)&s_abort; i++) {
                     const bool more = i + 1 < steps;
-                    if (!landed(2 * i + 1)) break;
+                    if (!landed(2 * i + 1) || (more && !landed(2 * i + 2))) break;
                     for (int q = 0; q < tiles; q++) {
-                        if (!wait(p_ready(q), (uint32_t)i & 1u)) break;
 #pragma unroll
-                        for (int kk = 0; kk < kStep / 16; kk++)
+                        for (int kk = 0; kk < kStep / 16; kk++) {
+                            if (kk % 4 == 0 && !wait(p_ready(q, kk / 4), (uint32_t)((q ? weighed1 : weighed0) + i) & 1u)) break;
                             mma_bf16_ts(tmem + kColO + q * 128, tmem + kColS + q * 128 + 8 * kk,
                                         sw128_desc_mn(slot(2 * i + 1) + kk * 16 * 128), kIdescO, (i | kk) != 0);
-                        if (q == tiles - 1) mma_commit(empty((2 * i + 1) % kSlots));
+                        }
+                        if (!ok) break;
+                        if (q == tiles - 1) done(2 * i + 1);
                         if (more) {
-                            if (!landed(2 * i + 2)) break;
                             scores(q, 2 * i + 2);
-                            if (q == tiles - 1) mma_commit(empty((2 * i + 2) % kSlots));
+                            if (q == tiles - 1) done(2 * i + 2);
                         } else {
                             mma_commit(s_full(q));   // O is whole
                         }
@@ -292,11 +334,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         } else if (warp >= 4) {
             // ---- softmax of tile q, this thread's row r of it
             const int q = (warp - 4) >> 2, r = threadIdx.x & 127;
-            const int rows = q ? rows1 : rows0;
+            const int rows = q ? rows1 : rows0, s_before = q ? scored1 : scored0;
             if (rows > 0) {
                 const uint32_t at = ((uint32_t)(warp & 3) * 32) << 16;   // this warp's TMEM lanes
                 const uint32_t t_s = tmem + at + kColS + q * 128, t_o = tmem + at + kColO + q * 128;
-                const int pos = position_of(tile.ch, a.group, tile.row0 + q * 128 + min(r, rows - 1));
+                const int pos = position_of(ch, a.group, row0 + q * 128 + min(r, rows - 1));
                 const int from = a.window > 0 ? max(0, pos - a.window + 1) : 0;
                 const int to = min(pos + 1, (q ? span1 : span0).high);   // this row sees [from, to)
                 const float factor = a.scale * kLog2e;
@@ -304,7 +346,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // the pages of a step's runs of eight tokens, one step ahead; bit 8 e: run e is held
                 auto look = [&](int i) {
                     const int j = (step0 + i) * kStep + 8 * lane;
-                    return lane < 16 && (i >= steps || (j < room && page_of(c, tile.ch.stream, j) >= 0));
+                    return lane < 16 && (i >= steps || (j < room && page_of(c, ch.stream, j) >= 0));
                 };
                 float m = -INFINITY, l = 0.0f;
                 bool saw = false;   // a token that the row sees
@@ -315,7 +357,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     held_next = look(i + 1);
                     const int j0 = (step0 + i) * kStep;
                     const bool partial = j0 < all_from || j0 + kStep > all_to || held != 0xffffu;
-                    ok = mbar_wait(s_full(q), (uint32_t)i & 1u) && !*(volatile int *)&s_abort;
+                    ok = mbar_wait(s_full(q), (uint32_t)(s_before + i) & 1u) && !*(volatile int *)&s_abort;
                     ok = __all_sync(kFull, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -333,14 +375,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             if (!in) x[k] = 0xff800000u;
                             saw |= in;
                         }
+                        // values that are not finite: out of the product
+                        const int t = kv0 + 2 * i + 1;
+                        ok = __all_sync(kFull, mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u));
+                        if (!ok) break;
+                        const uint32_t values = s_kv + (uint32_t)(t % kSlots) * Sh::kTile;
+                        for (int k = r; k < (int)Sh::kTile / 16; k += 128) {
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                         : "r"(values + k * 16));
+                            if (odd2(w[0]) || odd2(w[1]) || odd2(w[2]) || odd2(w[3])) {
+                                s_odd = 1;   // ahead of the zeros that the other tile's threads may find
+                                __threadfence_block();
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
+                                    if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0x0000ffffu;
+                                }
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + k * 16), "r"(w[0]),
+                                             "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                             : "memory");
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     } else {
                         saw = true;
                     }
                     float top[4];
 #pragma unroll
-                    for (int b = 0; b < 4; b++) top[b] = __uint_as_float(x[b]);
+                    for (int b = 0; b < 4; b++) top[b] = -INFINITY;
 #pragma unroll
-                    for (int k = 4; k < 128; k++) top[k & 3] = fmaxf(top[k & 3], __uint_as_float(x[k]));
+                    for (int k = 0; k < 128; k += 8)
+#pragma unroll
+                        for (int b = 0; b < 4; b++)
+                            top[b] = max3(top[b], __uint_as_float(x[k + 2 * b]), __uint_as_float(x[k + 2 * b + 1]));
                     const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
                     const bool raise = most > m + kSlack;   // (m = -inf: a first token)
                     if (__any_sync(kFull, raise)) {
@@ -364,57 +433,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : -m;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const uint64_t factor2 = two(factor, factor), base2 = two(base, base);
+                    uint64_t sum[2] = {0, 0};
 #pragma unroll
                     for (int b = 0; b < 2; b++) {
-                        uint32_t p[32];
 #pragma unroll
                         for (int k = 0; k < 32; k++) {
-                            const float w0 = exp2_fast(fmaf(__uint_as_float(x[64 * b + 2 * k]), factor, base));
-                            const float w1 = exp2_fast(fmaf(__uint_as_float(x[64 * b + 2 * k + 1]), factor, base));
-                            sum[(2 * k) & 3] += w0;
-                            sum[(2 * k + 1) & 3] += w1;
-                            p[k] = pack_bf16(w0, w1);
+                            const uint64_t y = fma2(two(__uint_as_float(x[64 * b + 2 * k]), __uint_as_float(x[64 * b + 2 * k + 1])),
+                                                    factor2, base2);
+                            float w0, w1;
+                            both(y, w0, w1);
+                            w0 = exp2_fast(w0);
+                            w1 = exp2_fast(w1);
+                            sum[k & 1] = add2(sum[k & 1], two(w0, w1));
+                            x[64 * b + k] = pack_bf16(w0, w1);   // (scores k and below have been used)
                         }
-                        tmem_st32(t_s + 32 * b, p);
+                        tmem_st32(t_s + 32 * b, x + 64 * b);
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_ready(q, b));
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_wait_st();
-                    if (partial) {
-                        // values that are not finite: out of the product
-                        const int t = 2 * i + 1;
-                        ok = __all_sync(kFull, mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u));
-                        if (!ok) break;
-                        const uint32_t values = s_kv + (uint32_t)(t % kSlots) * Sh::kTile;
-                        for (int k = r; k < (int)Sh::kTile / 16; k += 128) {
-                            uint32_t w[4];
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                         : "r"(values + k * 16));
-                            if (odd2(w[0]) || odd2(w[1]) || odd2(w[2]) || odd2(w[3])) {
-                                s_odd = 1;   // ahead of the zeros that the other tile's threads may find
-                                __threadfence_block();
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
-                                    if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0x0000ffffu;
-                                }
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + k * 16), "r"(w[0]),
-                                             "r"(w[1]), "r"(w[2]), "r"(w[3])
-                                             : "memory");
-                            }
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    }
-                    tc_fence_before();
-                    mbar_arrive(p_ready(q));
+                    float s0, s1;
+                    both(add2(sum[0], sum[1]), s0, s1);
+                    l += s0 + s1;
                 }
                 // ---- O / l
-                ok = ok && mbar_wait(s_full(q), (uint32_t)steps & 1u) && !*(volatile int *)&s_abort;
+                ok = ok && mbar_wait(s_full(q), (uint32_t)(s_before + steps) & 1u) && !*(volatile int *)&s_abort;
                 if (__all_sync(kFull, ok)) {
                     tc_fence_after();
                     const bool odd_values = *(volatile int *)&s_odd;
-                    const int row = tile.row0 + q * 128 + r, token = tile.ch.first + row / a.group;
+                    const int row = row0 + q * 128 + r, token = ch.first + row / a.group;
                     const int h = kvh * a.group + row % a.group;
                     const bool live = r < rows;
                     float f = l == 0.0f ? (saw ? NAN : 0.0f) : 1.0f / l;
@@ -433,10 +482,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int j = max(from, step0 * kStep); j < to; j++) {
                                 const int s0 = j & ~(kStep - 1);
                                 // steps that every row sees wholly went through the product as they are
-                                const int p = page_of(c, tile.ch.stream, j);
+                                const int p = page_of(c, ch.stream, j);
                                 bool whole = s0 >= all_from && s0 + kStep <= all_to;
                                 for (int e = 0; whole && e < kStep / 8; e++)
-                                    whole = s0 + 8 * e < room && page_of(c, tile.ch.stream, s0 + 8 * e) >= 0;
+                                    whole = s0 + 8 * e < room && page_of(c, ch.stream, s0 + 8 * e) >= 0;
                                 if (p < 0 || whole) continue;
                                 const __nv_bfloat16 *v = (const __nv_bfloat16 *)c.v + row_on_page(c, p, kvh, j) + 32 * b;
 #pragma unroll
@@ -465,16 +514,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     } else {
         // rows that see nothing
-        for (int i = threadIdx.x; i < tile.rows * (D / 8); i += kTcThreads) {
-            const int row = tile.row0 + i / (D / 8);
-            *reinterpret_cast<uint4 *>((__nv_bfloat16 *)a.out + (long long)(tile.ch.first + row / a.group) * a.out_stride +
+        for (int i = threadIdx.x; i < tile_rows * (D / 8); i += kTcThreads) {
+            const int row = row0 + i / (D / 8);
+            *reinterpret_cast<uint4 *>((__nv_bfloat16 *)a.out + (long long)(ch.first + row / a.group) * a.out_stride +
                                        (long long)(kvh * a.group + row % a.group) * D + i % (D / 8) * 8) =
                 make_uint4(0, 0, 0, 0);
         }
     }
     tc_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(*(volatile int *)&s_abort)) break;
     tc_fence_after();
+    if (threadIdx.x == 0) s_odd = 0;   // (the next tile's barrier follows)
+    if (steps > 0) {
+        kv0 += 2 * steps;
+        scored0 += steps + 1;
+        weighed0 += steps;
+        if (rows1 > 0) {
+            scored1 += steps + 1;
+            weighed1 += steps;
+        }
+    }
+    }
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
@@ -515,10 +575,13 @@ cudaError_t launch_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stre
     const int page = 1 << c.page_shift, box_rows = page < kStep ? page : kStep;
     CUtensorMap mk, mv;
     if (!make_page_map(&mk, c.k, c, box_rows) || !make_page_map(&mv, c.v, c, box_rows)) return cudaErrorInvalidValue;
-    const long long tiles = (long long)c.rows * a.group / 256 + c.n_streams;
-    if (tiles > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    // tiles of a stream, as far as the caller says (the mean where it says nothing)
+    const long long most_new = a.max_new > 0 && a.max_new < c.rows ? a.max_new : c.rows / c.n_streams + 1;
+    const long long turns = (most_new * a.group + 255) / 256;
+    const long long blocks = turns * c.n_streams * c.n_kv;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)tiles, (unsigned)c.n_kv);
+    cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(kTcThreads);
     cfg.dynamicSmemBytes = TcShape<D>::kSmem;
     cfg.stream = stream;
@@ -527,7 +590,7 @@ cudaError_t launch_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stre
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attend_tc_kernel<D>, mk, mv, c, a, box_rows);
+    return cudaLaunchKernelEx(&cfg, attend_tc_kernel<D>, mk, mv, c, a, box_rows, (int)turns);
 }
 
 }  // namespace
