@@ -129,6 +129,16 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r)
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar)
 {
     asm volatile(
@@ -210,12 +220,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint32_t tmem = 0;
     // phases of the barriers before this tile: tiles of keys and values, scores of either tile
     int kv0 = 0, scored0 = 0, scored1 = 0, weighed0 = 0, weighed1 = 0;
-#ifdef Z2_REGS
-    if (warp < 4)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    else
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-#endif
     for (int turn = first_turn; turn < n_tiles; turn += turns) {
     const long long row_ll = (long long)(n_tiles - 1 - turn) * 256;
     const int row0 = (int)row_ll;
@@ -229,19 +233,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int step0 = low / kStep, steps = high > low ? (high + kStep - 1) / kStep - step0 : 0;
 
     // queries, swizzled as TMA does; zeros past the rows
+#pragma unroll 4
     for (int i = threadIdx.x; i < 256 * (D / 8); i += kTcThreads) {
         const int r = i / (D / 8), p = i % (D / 8), row = row0 + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < tile_rows)
-            v = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)a.q +
-                                                 (long long)(ch.first + row / a.group) * a.q_stride +
-                                                 (long long)(kvh * a.group + row % a.group) * D + p * 8);
-        const int q = r >> 7, rr = r & 127;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                         s_q + q * Sh::kTile + (p >> 3) * (128 * 128) + rr * 128 + (((p & 7) ^ (rr & 7)) << 4)),
-                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                     : "memory");
+        const bool in = r < tile_rows;
+        const long long at = in ? (long long)(ch.first + row / a.group) * a.q_stride +
+                                      (long long)(kvh * a.group + row % a.group) * D + p * 8
+                                : 0;
+        cp_async16_or_zero(s_q + (r >> 7) * Sh::kTile + (p >> 3) * (128 * 128) + (r & 127) * 128 + (((p & 7) ^ (r & 7)) << 4),
+                           (const __nv_bfloat16 *)a.q + at, in);
     }
+    cp_async_commit();
+    cp_async_wait<0>();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
@@ -314,10 +317,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (!landed(2 * i + 1) || (more && !landed(2 * i + 2))) break;
                     for (int q = 0; q < tiles; q++) {
 #pragma unroll
-                        for (int kk = 0; kk < kStep / 16; kk++) {
-                            if (kk % 4 == 0 && !wait(p_ready(q, kk / 4), (uint32_t)((q ? weighed1 : weighed0) + i) & 1u)) break;
-                            mma_bf16_ts(tmem + kColO + q * 128, tmem + kColS + q * 128 + 8 * kk,
-                                        sw128_desc_mn(slot(2 * i + 1) + kk * 16 * 128), kIdescO, (i | kk) != 0);
+                        for (int k = 0; k < kStep / 16; k++) {
+                            const int kk = k ^ 4;   // the upper 64 keys' weights come first
+                            if (k % 4 == 0 && !wait(p_ready(q, kk / 4), (uint32_t)((q ? weighed1 : weighed0) + i) & 1u)) break;
+                            // 32 keys' weights lie in the first 16 of their scores' columns
+                            mma_bf16_ts(tmem + kColO + q * 128, tmem + kColS + q * 128 + 32 * (kk >> 1) + 8 * (kk & 1),
+                                        sw128_desc_mn(slot(2 * i + 1) + kk * 16 * 128), kIdescO, (i | k) != 0);
                         }
                         if (!ok) break;
                         if (q == tiles - 1) done(2 * i + 1);
@@ -361,20 +366,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     ok = __all_sync(kFull, ok);
                     if (!ok) break;
                     tc_fence_after();
-                    uint32_t x[128];
+                    // S passes through registers 32 columns at a time, once for the maximum and, but for the
+                    // last two pieces, which are still there, again for the weights: 128 columns at once
+                    // would leave the rest of the loop's values no registers.
+                    uint32_t x[2][32];
+                    auto start = [&](int piece) { tmem_ld32_start(t_s + 32 * piece, x[piece & 1]); };
+                    auto landed = [&](int piece) {
+                        tmem_wait_ld();
+                        tmem_landed(x[piece & 1]);
+                    };
+                    auto mask = [&](int piece) {
+                        const int begin = from - j0 - 32 * piece, end = to - j0 - 32 * piece;
 #pragma unroll
-                    for (int b = 0; b < 4; b++) tmem_ld32_start(t_s + 32 * b, x + 32 * b);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int b = 0; b < 4; b++) tmem_landed(x + 32 * b);
-                    if (partial) {
-                        const int begin = from - j0, end = to - j0;
-#pragma unroll
-                        for (int k = 0; k < 128; k++) {
-                            const bool in = k >= begin && k < end && (held >> (k >> 3) & 1u);
-                            if (!in) x[k] = 0xff800000u;
+                        for (int k = 0; k < 32; k++) {
+                            const bool in = k >= begin && k < end && (held >> (4 * piece + (k >> 3)) & 1u);
+                            if (!in) x[piece & 1][k] = 0xff800000u;
                             saw |= in;
                         }
+                    };
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    start(0);
+#pragma unroll
+                    for (int piece = 0; piece < 4; piece++) {
+                        landed(piece);
+                        if (piece < 3) start(piece + 1);
+                        if (partial) mask(piece);
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8)
+#pragma unroll
+                            for (int b = 0; b < 4; b++)
+                                top[b] = max3(top[b], __uint_as_float(x[piece & 1][k + 2 * b]),
+                                              __uint_as_float(x[piece & 1][k + 2 * b + 1]));
+                    }
+                    if (partial) {
                         // values that are not finite: out of the product
                         const int t = kv0 + 2 * i + 1;
                         ok = __all_sync(kFull, mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u));
@@ -402,14 +426,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     } else {
                         saw = true;
                     }
-                    float top[4];
-#pragma unroll
-                    for (int b = 0; b < 4; b++) top[b] = -INFINITY;
-#pragma unroll
-                    for (int k = 0; k < 128; k += 8)
-#pragma unroll
-                        for (int b = 0; b < 4; b++)
-                            top[b] = max3(top[b], __uint_as_float(x[k + 2 * b]), __uint_as_float(x[k + 2 * b + 1]));
                     const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
                     const bool raise = most > m + kSlack;   // (m = -inf: a first token)
                     if (__any_sync(kFull, raise)) {
@@ -436,23 +452,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const uint64_t factor2 = two(factor, factor), base2 = two(base, base);
                     uint64_t sum[2] = {0, 0};
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
+                    for (int piece = 3; piece >= 0; piece--) {
+                        uint32_t *y = x[piece & 1];
+                        if (piece < 2) {
+                            landed(piece);
+                            if (partial) mask(piece);
+                        }
 #pragma unroll
-                        for (int k = 0; k < 32; k++) {
-                            const uint64_t y = fma2(two(__uint_as_float(x[64 * b + 2 * k]), __uint_as_float(x[64 * b + 2 * k + 1])),
-                                                    factor2, base2);
+                        for (int k = 0; k < 16; k++) {
                             float w0, w1;
-                            both(y, w0, w1);
+                            both(fma2(two(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1])), factor2, base2), w0, w1);
                             w0 = exp2_fast(w0);
                             w1 = exp2_fast(w1);
                             sum[k & 1] = add2(sum[k & 1], two(w0, w1));
-                            x[64 * b + k] = pack_bf16(w0, w1);   // (scores k and below have been used)
+                            y[k] = pack_bf16(w0, w1);   // (scores k and below have been used)
                         }
-                        tmem_st32(t_s + 32 * b, x + 64 * b);
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(p_ready(q, b));
+                        tmem_st16(t_s + 32 * piece, y);   // in place of its scores
+                        if (piece >= 2) start(piece - 2);
+                        if (piece == 2 || piece == 0) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(p_ready(q, piece >> 1));
+                        }
                     }
                     float s0, s1;
                     both(add2(sum[0], sum[1]), s0, s1);
