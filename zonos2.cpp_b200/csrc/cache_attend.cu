@@ -528,6 +528,313 @@ __global__ void __launch_bounds__(32 * W)
     join_and_store<float, D, ROWS, W, 32 * W>(c, a, tile, kvh, part, s_ml, s_weight, s_total, s_gate, ranks, rank);
 }
 
+// ---- f32, many rows ----------------------------------------------------------
+// 64 rows to a tile, 16 to a warp, steps of 32 keys that the block's four warps share.  The
+// products run on the tensor cores in tf32 (11 bits of a significand), each operand as the sum
+// of two such parts, hi = its upper bits and lo = the rest:
+//     a b = hi_a hi_b + hi_a lo_b + lo_a hi_b + (2^-22 of it)
+// which leaves errors of the size of f32's own in a sum of 128 products.  The tensor cores add
+// to an accumulator by truncation, a bias that grows with the number of additions: the upper
+// parts' products, the mixed ones (2^-11 of them, and so their bias) and each 64 elements of the
+// depth or 32 keys have accumulators of their own, which are added with rounding to nearest (with
+// one accumulator for all of them 2500 keys were 5.5e-6 off, now 4e-7).  On the FMA pipe
+// (ROWS = 16 above) a step's operands come from shared memory four times as often for the same
+// products, and that bounds it.  Where an MMA's k runs over elements or keys, any order will
+// do that both operands share: a lane takes four neighbouring elements of a row in one load,
+// two for each of two MMAs; and the weights of a group of 8 keys, as the scores' accumulators
+// hold them, are the left operand of its values if those take their keys in the order 0, 2, 4,
+// 6, 1, 3, 5, 7.  The pitches keep those loads free of bank conflicts.
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo)
+{
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+// The product of the upper parts into d, the mixed ones into e.
+__device__ __forceinline__ void mma_3tf32(float (&d)[4], float (&e)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4],
+                                          uint32_t bh0, uint32_t bh1, uint32_t bl0, uint32_t bl1)
+{
+    mma_tf32(e, al, bh0, bh1);
+    mma_tf32(e, ah, bl0, bl1);
+    mma_tf32(d, ah, bh0, bh1);
+}
+
+constexpr int kTileKeys = 32, kTileRows = 64;
+
+template <int D>
+struct TileF32 {
+    static constexpr int kPitch = D + 16, kPitchV = D + 4;   // floats of a row of Q and K, of V
+    static constexpr int kStage = kTileKeys * (kPitch + kPitchV);
+    static constexpr size_t kSmem = (size_t)(kTileRows * kPitch + 2 * kStage) * 4;
+};
+
+template <int D>
+__global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
+    attend_tile_f32_kernel(const CacheArgs c, const AttendArgs a, int ranks)
+{
+    typedef TileF32<D> Sh;
+    constexpr int ROWS = kTileRows;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    float *s_q = reinterpret_cast<float *>(smem), *s_kv = s_q + ROWS * Sh::kPitch;   // at the end the part
+    __shared__ float2 s_ml[ROWS];
+    __shared__ float s_weight[kMostRanks * ROWS], s_total[ROWS], s_gate[ROWS];
+    __shared__ int s_held[2][4];
+    __shared__ int4 s_found;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int rank = blockIdx.x % ranks, kvh = blockIdx.y;
+    const Tile tile = find_tile(c, a.group, ROWS, (long long)(gridDim.x / ranks) - 1 - blockIdx.x / ranks, &s_found);
+    if (tile.rows == 0) return;   // the whole cluster's tile
+
+    const int room = room_of(c);
+    const int pos_first = position_of(tile.ch, a.group, tile.row0);
+    const int pos_last = position_of(tile.ch, a.group, tile.row0 + tile.rows - 1);
+    const int low = a.window > 0 ? max(0, pos_first - a.window + 1) : 0;
+    const int high = min(pos_last + 1, room);
+    const int sees_all_from = a.window > 0 ? max(0, pos_last - a.window + 1) : 0;   // .. to pos_first
+    const int first_step = low / kTileKeys, steps = high > low ? (high + kTileKeys - 1) / kTileKeys - first_step : 0;
+    const int mine = steps > rank ? (steps - rank + ranks - 1) / ranks : 0;   // this rank's steps
+    auto step_at = [&](int it) { return (first_step + rank + it * ranks) * kTileKeys; };
+    // a warp loads the step's run of eight keys that has its number
+    auto look = [&](int it) {
+        const int j = step_at(it) + 8 * warp;
+        return it < mine && j < room ? page_of(c, tile.ch.stream, j) : -1;
+    };
+    int page = look(0);
+    const int live = c.dim / 4;
+    for (int i = threadIdx.x; i < ROWS * (D / 4); i += 128) {
+        const int r = i / (D / 4), p = i % (D / 4), row = tile.row0 + r;
+        const bool in = r < tile.rows && p < live;
+        const long long at = in ? (long long)(tile.ch.first + row / a.group) * a.q_stride +
+                                      (long long)(kvh * a.group + row % a.group) * c.dim + p * 4
+                                : 0;
+        cp_async16_or_zero(smem_u32(s_q + r * Sh::kPitch + p * 4), (const float *)a.q + at, in);
+    }
+    load_gates<float>(a, tile, kvh, s_gate);
+    if (live < D / 4)   // pieces that no copy fills
+        for (int i = threadIdx.x; i < 2 * kTileKeys * (D / 4); i += 128) {
+            const int r = i / (D / 4), p = i % (D / 4);
+            if (p >= live) {
+                float *stage = s_kv + (r / kTileKeys) * Sh::kStage;
+                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                *reinterpret_cast<float4 *>(stage + (r % kTileKeys) * Sh::kPitch + p * 4) = zero;
+                *reinterpret_cast<float4 *>(stage + kTileKeys * Sh::kPitch + (r % kTileKeys) * Sh::kPitchV + p * 4) = zero;
+            }
+        }
+    auto fetch = [&](int it) {
+        if (it < mine) {
+            float *keys = s_kv + (it & 1) * Sh::kStage + 8 * warp * Sh::kPitch;
+            float *values = s_kv + (it & 1) * Sh::kStage + kTileKeys * Sh::kPitch + 8 * warp * Sh::kPitchV;
+            const int j0 = step_at(it) + 8 * warp;
+            if (lane == 0) s_held[it & 1][warp] = page >= 0;
+            const long long base = page >= 0 ? row_on_page(c, page, kvh, j0) : 0;
+            constexpr int kLanes = D / 4 < 32 ? D / 4 : 32;   // of a row's pieces
+#pragma unroll 4
+            for (int r = lane / kLanes; r < 8; r += 32 / kLanes) {
+                const bool take = page >= 0 && j0 + r >= low && j0 + r < high;
+                const long long at = take ? base + r * c.dim : 0;
+                for (int p = lane % kLanes; p < live; p += kLanes) {
+                    cp_async16_or_zero(smem_u32(keys + r * Sh::kPitch + p * 4), (const float *)c.k + at + p * 4, take);
+                    cp_async16_or_zero(smem_u32(values + r * Sh::kPitchV + p * 4), (const float *)c.v + at + p * 4, take);
+                }
+            }
+        }
+        cp_async_commit();
+        page = look(it + 1);
+    };
+    fetch(0);
+
+    int pos[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        pos[i] = position_of(tile.ch, a.group, tile.row0 + min(warp * 16 + i * 8 + g, tile.rows - 1));
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    const float factor = a.scale * kLog2e;
+    const float *q0 = s_q + (warp * 16 + g) * Sh::kPitch + 4 * t, *q1 = q0 + 8 * Sh::kPitch;
+    const bool idle = warp * 16 >= tile.rows;   // none of this warp's rows is one
+
+    for (int it = 0; it < mine; it++) {
+        cp_async_wait<0>();
+        __syncthreads();   // the step has landed, and the one before it is done with
+        fetch(it + 1);
+        const float *keys = s_kv + (it & 1) * Sh::kStage;
+        float *values = s_kv + (it & 1) * Sh::kStage + kTileKeys * Sh::kPitch;
+        const int j0 = step_at(it);
+        uint32_t held = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) held |= s_held[it & 1][e] ? 1u << e : 0u;
+        const bool partial = j0 < sees_all_from || j0 + kTileKeys - 1 > pos_first || j0 + kTileKeys > high || held != 15u;
+        auto sees = [&](int i, int j) {   // row slot i of this lane, token j
+            return j <= pos[i] && j < high && (a.window <= 0 || j > pos[i] - a.window) && (held >> ((j - j0) >> 3) & 1u);
+        };
+        if (partial) {
+            // values that are not finite: to the rows that see them by themselves, and zeros to the
+            // product, which would bring them to the others as 0 times them
+            bool any = false;
+            for (int i = threadIdx.x; i < kTileKeys * (D / 4); i += 128) {
+                const float4 v = *reinterpret_cast<const float4 *>(values + i / (D / 4) * Sh::kPitchV + i % (D / 4) * 4);
+                any |= odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w);
+            }
+            if (__syncthreads_or(any)) {
+#pragma unroll 1
+                for (int k = 0; k < kTileKeys; k++)
+#pragma unroll
+                    for (int n = 0; n < D / 8; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float v = values[k * Sh::kPitchV + 32 * (n >> 2) + 8 * t + 4 * e + (n & 3)];
+                            if (!odd(v)) continue;
+                            if (sees(0, j0 + k)) o[n][e] += v;
+                            if (sees(1, j0 + k)) o[n][2 + e] += v;
+                        }
+                __syncthreads();
+                for (int i = threadIdx.x; i < kTileKeys * D; i += 128) {
+                    float &v = values[i / D * Sh::kPitchV + i % D];
+                    if (odd(v)) v = 0.0f;
+                }
+                __syncthreads();
+            }
+        }
+        if (idle) continue;
+        float x[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+#pragma unroll 1
+        for (int part = 0; part < D / 64; part++) {
+        float hi[4][4], lo[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) hi[n][e] = lo[n][e] = 0.0f;
+#pragma unroll
+        for (int kd = 4 * part; kd < 4 * part + 4; kd++) {
+            const float4 qa = *reinterpret_cast<const float4 *>(q0 + 16 * kd), qb = *reinterpret_cast<const float4 *>(q1 + 16 * kd);
+            uint32_t h0[4], l0[4], h1[4], l1[4];
+            split_tf32(qa.x, h0[0], l0[0]);
+            split_tf32(qb.x, h0[1], l0[1]);
+            split_tf32(qa.y, h0[2], l0[2]);
+            split_tf32(qb.y, h0[3], l0[3]);
+            split_tf32(qa.z, h1[0], l1[0]);
+            split_tf32(qb.z, h1[1], l1[1]);
+            split_tf32(qa.w, h1[2], l1[2]);
+            split_tf32(qb.w, h1[3], l1[3]);
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const float4 k = *reinterpret_cast<const float4 *>(keys + (8 * n + g) * Sh::kPitch + 16 * kd + 4 * t);
+                uint32_t kh[4], kl[4];
+                split_tf32(k.x, kh[0], kl[0]);
+                split_tf32(k.y, kh[1], kl[1]);
+                split_tf32(k.z, kh[2], kl[2]);
+                split_tf32(k.w, kh[3], kl[3]);
+                mma_3tf32(hi[n], lo[n], h0, l0, kh[0], kh[1], kl[0], kl[1]);
+                mma_3tf32(hi[n], lo[n], h1, l1, kh[2], kh[3], kl[2], kl[3]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[n][e] += hi[n][e] + lo[n][e];
+        }
+        uint32_t seen = 0xffffu;   // bit 4 n + element
+        if (partial) {
+            seen = 0;
+#pragma unroll
+            for (int b = 0; b < 16; b++) {
+                if (sees((b >> 1) & 1, j0 + 8 * (b >> 2) + 2 * t + (b & 1)))
+                    seen |= 1u << b;
+                else
+                    x[b >> 2][b & 3] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; n++) most = fmaxf(most, fmaxf(x[n][2 * i], x[n][2 * i + 1]));
+            most = fmaxf(most, __shfl_xor_sync(kFull, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(kFull, most, 2)) * factor;
+            if (most > m[i]) {
+                const float keep = m[i] == -INFINITY ? 0.0f : exp2_fast(m[i] - most);
+                m[i] = most;
+                l[i] *= keep;
+#pragma unroll
+                for (int n = 0; n < D / 8; n++) {
+                    o[n][2 * i] *= keep;
+                    o[n][2 * i + 1] *= keep;
+                }
+            }
+        }
+        uint32_t ph[4][4], pl[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float w = exp2_fast(fmaf(x[n][e], factor, -m[e >> 1]));
+                if (partial && !(seen >> (4 * n + e) & 1u)) w = 0.0f;
+                l[e >> 1] += w;
+                x[n][e] = w;
+            }
+            split_tf32(x[n][0], ph[n][0], pl[n][0]);
+            split_tf32(x[n][2], ph[n][1], pl[n][1]);
+            split_tf32(x[n][1], ph[n][2], pl[n][2]);
+            split_tf32(x[n][3], ph[n][3], pl[n][3]);
+        }
+        const float *v0 = values + 2 * t * Sh::kPitchV + 4 * g;
+#pragma unroll
+        for (int b = 0; b < D / 32; b++) {
+            float hi[4][4], lo[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) hi[j][e] = lo[j][e] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const float4 va = *reinterpret_cast<const float4 *>(v0 + 8 * n * Sh::kPitchV + 32 * b);
+                const float4 vb = *reinterpret_cast<const float4 *>(v0 + (8 * n + 1) * Sh::kPitchV + 32 * b);
+                const float ea[4] = {va.x, va.y, va.z, va.w}, eb[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t ah, al, bh, bl;
+                    split_tf32(ea[j], ah, al);
+                    split_tf32(eb[j], bh, bl);
+                    mma_3tf32(hi[j], lo[j], ph[n], pl[n], ah, bh, al, bl);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[4 * b + j][e] += hi[j][e] + lo[j][e];
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();   // every warp is done with the stages: the part takes their place
+    float *part = s_q;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        l[i] += __shfl_xor_sync(kFull, l[i], 1);
+        l[i] += __shfl_xor_sync(kFull, l[i], 2);
+        const int r = warp * 16 + i * 8 + g;
+        if (t == 0) s_ml[r] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int b = 0; b < D / 32; b++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                *reinterpret_cast<float4 *>(part + r * D + part_piece(r, 8 * b + 2 * t + e) * 4) =
+                    make_float4(o[4 * b][2 * i + e], o[4 * b + 1][2 * i + e], o[4 * b + 2][2 * i + e], o[4 * b + 3][2 * i + e]);
+    }
+    join_and_store<float, D, ROWS, 1, 128>(c, a, tile, kvh, part, s_ml, s_weight, s_total, s_gate, ranks, rank);
+}
+
 template <typename Kernel>
 cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, int warps, int threads, const CacheArgs &c,
                         const AttendArgs &a, int keys, std::mutex &mu, bool (&ready)[64], cudaStream_t stream)
@@ -603,6 +910,14 @@ cudaError_t launch_f32(const CacheArgs &c, const AttendArgs &a, cudaStream_t str
     return launch_rows(attend_rows_f32_kernel<D, ROWS, STAGES, W>, smem, ROWS, W, 32 * W, c, a, 8, mu, ready, stream);
 }
 
+template <int D>
+cudaError_t launch_tile_f32(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
+{
+    static std::mutex mu;
+    static bool ready[64] = {false};
+    return launch_rows(attend_tile_f32_kernel<D>, TileF32<D>::kSmem, kTileRows, 1, 128, c, a, kTileKeys, mu, ready, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_cache_attend(const CacheArgs &c, const AttendArgs &a, bool bf16, cudaStream_t stream)
@@ -616,6 +931,9 @@ cudaError_t launch_cache_attend(const CacheArgs &c, const AttendArgs &a, bool bf
         if (c.dim > 64) return rows > 16 ? launch_bf16<128, 2, Z2_S2>(c, a, stream) : launch_bf16<128, 1, Z2_S1>(c, a, stream);
         return rows > 16 ? launch_bf16<64, 2, 4>(c, a, stream) : launch_bf16<64, 1, 4>(c, a, stream);
     }
+    if (rows > 16)
+        return c.dim > 128 ? launch_tile_f32<256>(c, a, stream)
+                           : c.dim > 64 ? launch_tile_f32<128>(c, a, stream) : launch_tile_f32<64>(c, a, stream);
     if (c.dim > 128) return rows > 4 ? launch_f32<256, 8, 3>(c, a, stream) : launch_f32<256, 4, 3>(c, a, stream);
     if (c.dim > 64) return rows > 4 ? launch_f32<128, 16, 3>(c, a, stream) : launch_f32<128, 4, 3>(c, a, stream);
     return rows > 4 ? launch_f32<64, 16, 4>(c, a, stream) : launch_f32<64, 4, 4>(c, a, stream);

@@ -181,7 +181,7 @@ __device__ void join_and_store(const CacheArgs &c, const AttendArgs &a, const Ti
             asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
                          : "=f"(m), "=f"(l)
                          : "r"(peer_addr(smem_u32(ml + r), k)));
-            reinterpret_cast<float2 *>(part + ROWS * D)[i] = make_float2(m, l);   // behind warp 0's part
+            reinterpret_cast<float2 *>(part + ROWS * D)[i] = make_float2(m, l);   // behind the block's part
         }
         __syncthreads();
         for (int r = threadIdx.x; r < ROWS; r += THREADS) {

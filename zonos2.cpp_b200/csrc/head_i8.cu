@@ -208,9 +208,10 @@ cudaError_t launch_quantize(const void *x, int rows, int dim, long long stride, 
 //                swizzled, into a ring of stages; the first stages' weights are asked for
 //                before the rounding kernel ahead has ended (it started after all else had);
 //   warp 1       TMEM allocation, tcgen05.mma kind::i8 (K = 32), two accumulators in turn;
-//   warps 2..9   epilogue, two to a TMEM lane quarter, each half of the hidden rows.
+//   warps 2..17  epilogue, four to a TMEM lane quarter, each a quarter of the hidden rows.
 // Every wait is bounded, as in head_tc.cu.  No load uses cluster multicast.
-constexpr int kI8Threads = 320;
+constexpr int kEpi = 16;             // epilogue warps
+constexpr int kI8Threads = 64 + 32 * kEpi;
 constexpr int kI8MaxStages = 16;
 constexpr int kI8SmemMax = 232448 - 1024;   // dynamic; the static part takes 1 KB
 
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(done(b), 1);
-            mbar_init(open(b), 8 * CTAS);   // the epilogue warps
+            mbar_init(open(b), kEpi * CTAS);   // the epilogue warps
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -340,7 +341,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             if (unit0 < args.n_tiles) {
                 int b0, c, v0;
                 tile_at(unit0, b0, c, v0);
-                for (; ahead < KB && ahead < stages; ahead++) load_w(ahead, ahead, c * args.rows_per_cb + v0);
+                for (; ahead < KB && ahead < stages; ahead++)
+                    load_w(ahead, ahead, c * args.rows_per_cb + v0);
             }
             asm volatile("griddepcontrol.wait;" ::: "memory");
             int it = 0;
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             if (!ok) s_abort = 1;
         }
     } else {
-        const int q = warp & 3, half = (warp - 2) >> 2;
+        const int q = warp & 3, part = (warp - 2) >> 2;
         const int row = BM == 64 ? 16 * q + (lane & 15) : 32 * q + lane;   // of the block's weight rows
         const uint32_t open0 = PAIR ? peer_addr(open(0), 0) : open(0);
         const long long wide = (long long)args.n_cb * args.vocab;
@@ -437,8 +439,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             const float ws = live ? __ldg(args.w_scale + (long long)c * args.rows_per_cb + v) : 0.0f;
             const int cols = min(args.nb, args.batch - b0);   // hidden rows of the tile
             // columns [from, to) in steps of 16
-            const int mid = ((args.nb / 16 + 1) / 2) * 16;
-            const int from = half ? mid : 0, to = min(half ? args.nb : mid, cols);
+            const int each = (args.nb / 16 + kEpi / 4 - 1) / (kEpi / 4) * 16;
+            const int from = part * each, to = min(from + each, cols);
             const bool got = mbar_wait(done(buf), (uint32_t)(local >> 1) & 1u) && !aborted();
             if (!__all_sync(kFull, got)) {
                 s_abort = 1;
