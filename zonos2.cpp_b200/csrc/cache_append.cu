@@ -143,13 +143,15 @@ __global__ void __launch_bounds__(kAppendThreads)
                 if (e < a.rot) other[i] = as_f(from[e < half ? e + half : e - half]);
             }
         }
+        float sum = 0.0f;
+        if (a.norm) {   // (every lane: a warp's heads may be keys and values)
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum += x[i] * x[i];
+#pragma unroll
+            for (int d = TEAM / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+        }
         if (!is_v) {
             if (a.norm) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) sum += x[i] * x[i];
-#pragma unroll
-                for (int d = TEAM / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
                 const float r = 1.0f / sqrtf(sum / (float)dim + a.eps);
                 const float *w = is_q ? a.q_weight : a.k_weight;
 #pragma unroll

@@ -774,6 +774,7 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
                 }
             }
         }
+        __syncwarp();
         uint32_t ph[4][4], pl[4][4];
 #pragma unroll
         for (int n = 0; n < 4; n++) {

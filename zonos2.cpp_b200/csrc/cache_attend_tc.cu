@@ -517,6 +517,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 }
                             }
                         }
+                        __syncwarp();
                         if (live) {
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
@@ -528,6 +529,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 *reinterpret_cast<uint4 *>(out + 32 * b + 8 * k) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
                         }
+                        __syncwarp();
                     }
                 } else {
                     s_abort = 1;

@@ -450,6 +450,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             float *out = args.out + (long long)b0 * wide + (long long)c * args.vocab + v;
             for (int j0 = from; j0 < to; j0 += 16) {
                 uint32_t r[16];
+                __syncwarp();
                 tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * args.nb + j0), r);
                 const float mine = lane < 16 && j0 + lane < cols ? __ldg(args.scale + b0 + j0 + lane) : 0.0f;
                 float l[16];
