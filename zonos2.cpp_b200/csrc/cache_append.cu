@@ -13,13 +13,15 @@
 // Bound: memory for prompts (every element is read once and written once), launch latency for
 // a few tokens.  A warp takes a token's heads one after another with the angles' sines kept, or
 // for few tokens one round of them, the token's heads shared out over warps.
+#include <type_traits>
+
 #include "cache.cuh"
 
 namespace z2 {
 
 namespace {
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 128, kAhead = 4;
 
 template <typename T>
 struct Eight;   // eight elements as they are loaded and stored
@@ -61,23 +63,32 @@ struct Eight<__nv_bfloat16> {
     }
 };
 
-// The stream of token row `row`: the last one that starts at or before it, 32 ways at a
-// time.  Every lane takes part; -1: before the first.
-__device__ __forceinline__ int stream_of(const CacheArgs &c, int row)
+// The stream of token row `row` (the last one that starts at or before it), found 32 ways at a
+// time, and its chunk: the last 32 streams' lengths come with their starts.  Every lane takes
+// part; n = 0: none.
+__device__ __forceinline__ Chunk chunk_with(const CacheArgs &c, int row)
 {
     const int lane = threadIdx.x & 31;
-    int low = 0, many = c.n_streams;   // the answer lies in [low, low + many)
-    if (__ldg(c.q_start) > row) return -1;
-    while (many > 1) {
+    int low = 0, many = c.n_streams;   // the answer lies in [low, low + many), if it lies anywhere
+    while (many > 32) {
         const int step = (many + 31) / 32;
-        const int at = low + lane * step;
-        const bool before = lane * step < many && __ldg(c.q_start + at) <= row;
-        const unsigned votes = __ballot_sync(kFull, before);
-        const int last = 31 - __clz(votes | 1u);   // the first always is, unless the starts fall
+        const bool before = lane * step < many && __ldg(c.q_start + low + lane * step) <= row;
+        const int last = 31 - __clz(__ballot_sync(kFull, before) | 1u);
         low += last * step;
         many = min(step, c.n_streams - low);
     }
-    return low;
+    const bool in = lane < many;
+    const int start = in ? __ldg(c.q_start + low + lane) : 0, next = in ? __ldg(c.q_start + low + lane + 1) : 0;
+    const int len = in ? __ldg(c.kv_len + low + lane) : 0;
+    const unsigned votes = __ballot_sync(kFull, in && start <= row);
+    const int last = 31 - __clz(votes | 1u);
+    Chunk k;
+    k.stream = low + last;
+    k.first = min(max(__shfl_sync(kFull, start, last), 0), c.rows);
+    k.n = min(max(__shfl_sync(kFull, next, last), k.first), c.rows) - k.first;
+    if (votes == 0) k.n = 0;
+    k.len = max(__shfl_sync(kFull, len, last), 0);
+    return k;
 }
 
 // TEAM lanes to a head (eight elements each).  LANE_PAIRS: rotation by neighbours, both of a
@@ -95,12 +106,10 @@ __global__ void __launch_bounds__(kAppendThreads)
     const int part = (int)(item % parts);   // which rounds of the token's heads
     if (row_ll >= c.rows) return;
     const int row = (int)row_ll;
-    const int s = stream_of(c, row);
-    if (s < 0) return;
-    const Chunk ch = chunk_of(c, s);
+    const Chunk ch = chunk_with(c, row);
     if (row < ch.first || row >= ch.first + ch.n) return;
     const int pos = ch.len - ch.n + (row - ch.first);
-    const int page = pos >= 0 && pos < room_of(c) ? page_of(c, s, pos) : -1;
+    const int page = pos >= 0 && pos < room_of(c) ? page_of(c, ch.stream, pos) : -1;
 
     const int e0 = sub * 8, dim = c.dim;
     const bool active = e0 < dim;
@@ -120,79 +129,95 @@ __global__ void __launch_bounds__(kAppendThreads)
             if (!LANE_PAIRS && e < half) sn[i] = -sn[i];   // a cos - b sin; b cos + a sin
         }
     }
-    const int first_head = a.q ? 0 : a.n_heads;
-    const int total = a.n_heads + 2 * c.n_kv;
-    for (int h0 = first_head + part * kHeads; h0 < total; h0 += parts * kHeads) {
-        const int h = h0 + team;
-        const bool on = active && h < total;
-        const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + c.n_kv;
-        const int kh = is_q ? 0 : is_v ? h - a.n_heads - c.n_kv : h - a.n_heads;
-        const T *from = is_q ? (const T *)a.q + row * a.q_stride + (long long)h * dim
-                             : is_v ? (const T *)a.v + row * a.v_stride + (long long)kh * dim
-                                    : (const T *)a.k + row * a.k_stride + (long long)kh * dim;
-        Eight<T> raw;
-        if (on) raw = *reinterpret_cast<const Eight<T> *>(from + e0);
-        float x[8], other[8];
+    const float rcp_dim = 1.0f / (float)dim;
+    // Rounds [first, end) of this part, kHeads heads each (from + h * dim to to + h * to_step, h the
+    // head's number among `heads`), the loads of kAhead of them in flight together.  Values (COPY) go
+    // as they are.
+    auto work = [&](auto copy, int first, int end, int heads, const T *from, T *to, long long to_step, const float *weight) {
+        constexpr bool COPY = decltype(copy)::value;
+        int round = first + ((part - first) % parts + parts) % parts;
+        if (round >= end) return;
+        float w[8];
+        if (!COPY) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = other[i] = 0.0f;
-        if (on) raw.get(x);
-        if (!LANE_PAIRS && on && !is_v && e0 < a.rot) {
+            for (int i = 0; i < 8; i++) w[i] = a.norm && weight && active ? __ldg(weight + e0 + i) : 1.0f;
+        }
+        for (; round < end; round += parts * kAhead) {
+            Eight<T> raws[kAhead];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int e = e0 + i;
-                if (e < a.rot) other[i] = as_f(from[e < half ? e + half : e - half]);
+            for (int u = 0; u < kAhead; u++) {
+                const int h = (round + u * parts - first) * kHeads + team;
+                if (active && h < heads) raws[u] = *reinterpret_cast<const Eight<T> *>(from + h * dim + e0);
             }
-        }
-        float sum = 0.0f;
-        if (a.norm) {   // (every lane: a warp's heads may be keys and values)
 #pragma unroll
-            for (int i = 0; i < 8; i++) sum += x[i] * x[i];
+            for (int u = 0; u < kAhead; u++) {
+                if (round + u * parts >= end) break;   // the same for the whole warp
+                const int h = (round + u * parts - first) * kHeads + team;
+                const bool on = active && h < heads;
+                if (!COPY) {
+                    float x[8], other[8];
 #pragma unroll
-            for (int d = TEAM / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-        }
-        if (!is_v) {
-            if (a.norm) {
-                const float r = 1.0f / sqrtf(sum / (float)dim + a.eps);
-                const float *w = is_q ? a.q_weight : a.k_weight;
+                    for (int i = 0; i < 8; i++) x[i] = other[i] = 0.0f;
+                    if (on) raws[u].get(x);
+                    if (!LANE_PAIRS && on && e0 < a.rot) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    x[i] *= r * (w && on ? __ldg(w + e0 + i) : 1.0f);
-                    if (!LANE_PAIRS) {
-                        const int e = e0 + i;
-                        if (on && e < a.rot)
-                            other[i] *= r * (w ? __ldg(w + (e < half ? e + half : e - half)) : 1.0f);
+                        for (int i = 0; i < 8; i++) {
+                            const int e = e0 + i;
+                            if (e < a.rot) other[i] = as_f(from[h * dim + (e < half ? e + half : e - half)]);
+                        }
                     }
-                }
-            }
-            float y[8];
-            if (LANE_PAIRS) {
+                    if (a.norm) {
+                        float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
-                    y[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
-                }
-            } else {
+                        for (int i = 0; i < 8; i++) sum += x[i] * x[i];
 #pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = x[i] * cs[i] + other[i] * sn[i];
+                        for (int d = TEAM / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+                        const float r = rsqrtf(fmaf(sum, rcp_dim, a.eps));   // 2 ulp
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            x[i] *= r * w[i];
+                            if (!LANE_PAIRS) {
+                                const int e = e0 + i;
+                                if (on && e < a.rot)
+                                    other[i] *= r * (weight ? __ldg(weight + (e < half ? e + half : e - half)) : 1.0f);
+                            }
+                        }
+                    }
+                    float y[8];
+                    if (LANE_PAIRS) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
+                            y[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) y[i] = x[i] * cs[i] + other[i] * sn[i];
+                    }
+                    raws[u].set(y);
+                    if (!LANE_PAIRS) __syncwarp();   // q_out may be q: the other half has been read
+                }
+                if (on) *reinterpret_cast<Eight<T> *>(to + h * to_step + e0) = raws[u];
             }
-            raw.set(y);
         }
-        if (!LANE_PAIRS) __syncwarp();   // q_out may be q: the other half has been read
-        if (on) {
-            T *to = nullptr;
-            if (is_q)
-                to = (T *)a.q_out + row * a.q_out_stride + (long long)h * dim;
-            else if (page >= 0)
-                to = (T *)(is_v ? c.v : c.k) + row_on_page(c, page, kh, pos);
-            if (to) *reinterpret_cast<Eight<T> *>(to + e0) = raw;
-        }
-    }
+    };
+    const int rounds_q = a.q ? (a.n_heads + kHeads - 1) / kHeads : 0, rounds_kv = (c.n_kv + kHeads - 1) / kHeads;
+    const long long page_step = (long long)dim << c.page_shift;   // from key head to key head
+    const long long at = page >= 0 ? row_on_page(c, page, 0, pos) : 0;
+    if (a.q)
+        work(std::false_type(), 0, rounds_q, a.n_heads, (const T *)a.q + row * a.q_stride, (T *)a.q_out + row * a.q_out_stride,
+             (long long)dim, a.q_weight);
+    if (page < 0) return;   // (the whole warp: a token's)
+    work(std::false_type(), rounds_q, rounds_q + rounds_kv, c.n_kv, (const T *)a.k + row * a.k_stride, (T *)c.k + at, page_step,
+         a.k_weight);
+    work(std::true_type(), rounds_q + rounds_kv, rounds_q + 2 * rounds_kv, c.n_kv, (const T *)a.v + row * a.v_stride, (T *)c.v + at,
+         page_step, nullptr);
 }
 
 template <typename T, int TEAM, bool LANE_PAIRS>
 cudaError_t launch(const CacheArgs &c, const AppendArgs &a, cudaStream_t stream)
 {
-    const int rounds = ((a.q ? a.n_heads : 0) + 2 * c.n_kv + 32 / TEAM - 1) / (32 / TEAM);
+    const int each = 32 / TEAM, rounds = (a.q ? (a.n_heads + each - 1) / each : 0) + 2 * ((c.n_kv + each - 1) / each);
     // few tokens: their heads shared out, until every SM has a warp of each scheduler
     int parts = 1;
     while (parts < rounds && (long long)c.rows * parts < 148 * 16) parts++;

@@ -14,7 +14,6 @@
 
 #include "common.cuh"
 #include "head_i8.cuh"
-#include "softcap.cuh"
 #include "tc.cuh"
 
 namespace z2 {
@@ -255,6 +254,41 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
     for (int i = 0; i < 16; i++) asm volatile("" : "+r"(r[i]));   // no use moves ahead of the wait
 }
 
+// cap * tanh(l / cap) of 16 values, two to an instruction: y (1 + z q(z)), z = y^2, below |y| =
+// 0.9, q of degree 5 with the least relative error (1.4e-8); past it, where a warp has such a value at
+// all, cap - 2 cap / (exp(2 y) + 1), whose rounding (a few 2^-24 of cap) is small against it.
+__device__ __forceinline__ void softcap16(float (&l)[16], float cap, float inv_cap)
+{
+    auto two = [](float x) { return make_float2(x, x); };
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) most = fmaxf(most, fmaxf(fabsf(l[i]), fabsf(l[i + 1])));
+    const bool small = __all_sync(kFull, most * inv_cap < 0.9f);
+    const float2 inv = two(inv_cap);
+    const float k2 = 2.0f * 1.4426950408889634f * inv_cap;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        const float2 x = make_float2(l[i], l[i + 1]), y = __fmul2_rn(x, inv), z = __fmul2_rn(y, y);
+        float2 p = __ffma2_rn(z, two(0.00128645188f), two(-0.00681405789f));
+        p = __ffma2_rn(z, p, two(0.0208577033f));
+        p = __ffma2_rn(z, p, two(-0.0536990522f));
+        p = __ffma2_rn(z, p, two(0.133298353f));
+        p = __ffma2_rn(z, p, two(-0.333331602f));
+        p = __ffma2_rn(__fmul2_rn(x, z), p, x);
+        l[i] = p.x;
+        l[i + 1] = p.y;
+        if (!small) {
+            float e0, e1, r0, r1;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(x.x * k2));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(x.y * k2));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(e0 + 1.0f));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(e1 + 1.0f));
+            if (!(fabsf(y.x) < 0.9f)) l[i] = fmaf(-2.0f * cap, r0, cap);
+            if (!(fabsf(y.y) < 0.9f)) l[i + 1] = fmaf(-2.0f * cap, r1, cap);
+        }
+    }
+}
+
 // BM: weight rows per block (64 of them lie in the first 16 lanes of each quarter).
 template <int CTAS, int BM>
 __global__ void __launch_bounds__(kI8Threads, 1)
@@ -428,6 +462,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         const int row = BM == 64 ? 16 * q + (lane & 15) : 32 * q + lane;   // of the block's weight rows
         const uint32_t open0 = PAIR ? peer_addr(open(0), 0) : open(0);
         const long long wide = (long long)args.n_cb * args.vocab;
+        const float inv_cap = 1.0f / args.softcap;
         asm volatile("griddepcontrol.wait;" ::: "memory");   // the hidden rows' scales
         int local = 0;
         for (int tile = unit0; tile < args.n_tiles; tile += units, local++) {
@@ -452,16 +487,27 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 uint32_t r[16];
                 __syncwarp();
                 tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * args.nb + j0), r);
-                const float mine = lane < 16 && j0 + lane < cols ? __ldg(args.scale + b0 + j0 + lane) : 0.0f;
+                const float4 *scale = reinterpret_cast<const float4 *>(args.scale + b0 + j0);   // (16 of them lie there)
                 float l[16];
 #pragma unroll
-                for (int j = 0; j < 16; j++)
-                    l[j] = (float)(int)r[j] * __shfl_sync(kFull, mine, j) * ws;
-                if (args.softcap > 0.0f) softcap_exact(l, args.softcap);
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 s = __ldg(scale + j / 4);
+                    l[j] = (float)(int)r[j] * s.x * ws;
+                    l[j + 1] = (float)(int)r[j + 1] * s.y * ws;
+                    l[j + 2] = (float)(int)r[j + 2] * s.z * ws;
+                    l[j + 3] = (float)(int)r[j + 3] * s.w * ws;
+                }
+                if (args.softcap > 0.0f) softcap16(l, args.softcap, inv_cap);
                 if (live) {
+                    float *to = out + j0 * wide;
+                    if (j0 + 16 <= cols) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        if (j0 + j < cols) out[(j0 + j) * wide] = l[j];
+                        for (int j = 0; j < 16; j++, to += wide) *to = l[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; j++, to += wide)
+                            if (j0 + j < cols) *to = l[j];
+                    }
                 }
             }
             tc_fence_before();

@@ -17,10 +17,10 @@ struct HeadI8Args {
     float *out;             // [batch][n_cb][vocab]
 };
 
-// The rounded hidden rows, and their scales behind them.
+// The rounded hidden rows, and their scales behind them, in whole steps of the epilogue's 16.
 inline long long head_i8_work_bytes(int batch, int dim)
 {
-    return (((long long)batch * dim + 15) & ~15ll) + 4ll * batch;
+    return (((long long)batch * dim + 15) & ~15ll) + 4ll * ((batch + 15ll) & ~15ll);
 }
 
 cudaError_t launch_quantize_rows(const void *x, bool bf16, int rows, int dim, long long stride,

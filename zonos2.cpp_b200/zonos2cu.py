@@ -468,13 +468,13 @@ class PagedCache:
 
     def _tokens(self, what: str, t, rows: int, width: int) -> int:
         """The row stride of token rows [rows, width] of the cache's type and device."""
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+        if t.shape != (rows, width):
             raise ValueError(f"{what}: [{rows}, {width}] expected, got {tuple(t.shape)}")
         if t.dtype != self._dtype:
             raise TypeError(f"{what}: {self._dtype} expected, got {t.dtype}")
         if t.get_device() != self._dev:
             raise ValueError(f"{what}: tensors on the cache's device expected")
-        return _rows(t, what)
+        return width if t.is_contiguous() else _rows(t, what)
 
 
 def cache_append(cache: PagedCache, q, k, v, q_out, *, freq=None, halves: bool = False, q_weight=None,
