@@ -203,7 +203,7 @@ cudaError_t launch_quantize(const void *x, int rows, int dim, long long stride, 
 // leave no part of a tile empty, and a warp's logits of one hidden row are 128 consecutive
 // bytes.  Persistent, one block per SM (or pair of blocks, CTAS = 2: M = 256, each half of
 // the weight rows and of the hidden rows):
-//   warp 0       TMA producer: BM x 128 bytes of weights and the hidden rows' 128 bytes, 128-byte
+//   warp 0       TMA producer: 128 x 128 bytes of weights and the hidden rows' 128 bytes, 128-byte
 //                swizzled, into a ring of stages; the first stages' weights are asked for
 //                before the rounding kernel ahead has ended (it started after all else had);
 //   warp 1       TMEM allocation, tcgen05.mma kind::i8 (K = 32), two accumulators in turn;
@@ -212,6 +212,7 @@ cudaError_t launch_quantize(const void *x, int rows, int dim, long long stride, 
 constexpr int kEpi = 16;             // epilogue warps
 constexpr int kI8Threads = 64 + 32 * kEpi;
 constexpr int kI8MaxStages = 16;
+constexpr int kI8Rows = 128;         // weight rows per block
 constexpr int kI8SmemMax = 232448 - 1024;   // dynamic; the static part takes 1 KB
 
 struct I8Args {
@@ -289,13 +290,13 @@ __device__ __forceinline__ void softcap16(float (&l)[16], float cap, float inv_c
     }
 }
 
-// BM: weight rows per block (64 of them lie in the first 16 lanes of each quarter).
-template <int CTAS, int BM>
+template <int CTAS>
 __global__ void __launch_bounds__(kI8Threads, 1)
     head_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h,
                    const __grid_constant__ I8Args args)
 {
     constexpr bool PAIR = CTAS == 2;
+    constexpr int BM = kI8Rows;
     constexpr uint32_t kWBytes = BM * 128;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -379,22 +380,28 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                     load_w(ahead, ahead, c * args.rows_per_cb + v0);
             }
             asm volatile("griddepcontrol.wait;" ::: "memory");
-            int it = 0;
+            // (a stage and its phase are counted up: a division by their number would cost a slice
+            // more than its MMAs)
+            int it = 0, s = 0;
+            uint32_t ph = 1;
             bool ok = true;
             for (int tile = unit0; tile < args.n_tiles && ok; tile += units) {
                 int b0, c, v0;
                 tile_at(tile, b0, c, v0);
                 const int w_row = c * args.rows_per_cb + v0, h_row = b0 + (int)rank * nb_own;
                 for (int kb = 0; kb < KB; kb++, it++) {
-                    const int s = it % stages;
                     if (it >= ahead) {
-                        if (!mbar_wait(empty(s), (((uint32_t)(it / stages)) & 1u) ^ 1u) || aborted()) {
+                        if (!mbar_wait(empty(s), ph) || aborted()) {
                             ok = false;
                             break;
                         }
                         load_w(s, kb, w_row);
                     }
                     load_h(s, kb, h_row);
+                    if (++s == stages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
                 }
             }
             if (!ok) {
@@ -411,9 +418,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             // kind::i8: D s32, A and B s8, both K-major
             const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(args.nb >> 3) << 17) |
                                    ((uint32_t)((CTAS * BM) >> 4) << 24);
-            int it = 0, local = 0;
+            int s = 0, local = 0;
+            uint32_t ph = 0;
             bool ok = true;
-            for (int tile = unit0; tile < args.n_tiles && ok; tile += units, local++) {
+            for (int tile = unit0; tile < args.n_tiles && ok && !aborted(); tile += units, local++) {
                 const int buf = local & 1;
                 const uint32_t bph = ((uint32_t)(local >> 1) & 1u) ^ 1u;
                 if (!(PAIR ? mbar_wait_cl(open(buf), bph) : mbar_wait(open(buf), bph))) {
@@ -422,14 +430,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)(buf * args.nb);
-                for (int kb = 0; kb < KB; kb++, it++) {
-                    const int s = it % stages;
-                    const uint32_t ph = (uint32_t)(it / stages) & 1u;
-                    if (!(PAIR ? mbar_wait_cl(full(s), ph) : mbar_wait(full(s), ph)) || aborted()) {
+                for (int kb = 0; kb < KB; kb++) {
+                    if (!(PAIR ? mbar_wait_cl(full(s), ph) : mbar_wait(full(s), ph))) {
                         ok = false;
                         break;
                     }
-                    tc_fence_after();
                     const uint32_t sa = smem0 + (uint32_t)s * stage_bytes;
                     const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + kWBytes);
 #pragma unroll
@@ -445,6 +450,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                     } else {
                         mma_commit(empty(s));
                     }
+                    if (++s == stages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
                 }
                 if (ok) {
                     if (PAIR) {
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         }
     } else {
         const int q = warp & 3, part = (warp - 2) >> 2;
-        const int row = BM == 64 ? 16 * q + (lane & 15) : 32 * q + lane;   // of the block's weight rows
+        const int row = 32 * q + lane;   // of the block's weight rows
         const uint32_t open0 = PAIR ? peer_addr(open(0), 0) : open(0);
         const long long wide = (long long)args.n_cb * args.vocab;
         const float inv_cap = 1.0f / args.softcap;
@@ -470,7 +479,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             int b0, c, v0;
             tile_at(tile, b0, c, v0);
             const int v = v0 + row;
-            const bool live = v < args.vocab && (BM == 128 || lane < 16);
+            const bool live = v < args.vocab;
             const float ws = live ? __ldg(args.w_scale + (long long)c * args.rows_per_cb + v) : 0.0f;
             const int cols = min(args.nb, args.batch - b0);   // hidden rows of the tile
             // columns [from, to) in steps of 16
@@ -547,10 +556,10 @@ bool make_map_i8(CUtensorMap *m, const void *base, long long rows, int dim, int 
 }
 
 struct Plan {
-    int ctas, bm, nb, tiles_b;
+    int ctas, nb, tiles_b;
 };
 
-template <int CTAS, int BM>
+template <int CTAS>
 cudaError_t launch_product(const HeadI8Args &a, const Plan &p, int dev, int sms, const int8_t *q, const float *scale,
                            cudaStream_t stream)
 {
@@ -560,7 +569,7 @@ cudaError_t launch_product(const HeadI8Args &a, const Plan &p, int dev, int sms,
     {
         std::lock_guard<std::mutex> lk(mu);
         if (units_at_once[dev] == 0) {
-            cudaError_t e = cudaFuncSetAttribute(head_i8_kernel<CTAS, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            cudaError_t e = cudaFuncSetAttribute(head_i8_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  kI8SmemMax);
             if (e != cudaSuccess) return e;
             int n = sms;
@@ -575,7 +584,7 @@ cudaError_t launch_product(const HeadI8Args &a, const Plan &p, int dev, int sms,
                 attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
                 cfg.attrs = attr;
                 cfg.numAttrs = 1;
-                e = cudaOccupancyMaxActiveClusters(&n, head_i8_kernel<CTAS, BM>, &cfg);
+                e = cudaOccupancyMaxActiveClusters(&n, head_i8_kernel<CTAS>, &cfg);
                 if (e != cudaSuccess) return e;
             }
             units_at_once[dev] = n > 0 ? n : 1;
@@ -583,7 +592,7 @@ cudaError_t launch_product(const HeadI8Args &a, const Plan &p, int dev, int sms,
         units = units_at_once[dev];
     }
     CUtensorMap mw, mh;
-    if (!make_map_i8(&mw, a.W, (long long)a.n_cb * a.rows_per_cb, a.dim, BM) ||
+    if (!make_map_i8(&mw, a.W, (long long)a.n_cb * a.rows_per_cb, a.dim, kI8Rows) ||
         !make_map_i8(&mh, q, a.batch, a.dim, p.nb / CTAS))
         return cudaErrorInvalidValue;
     I8Args t;
@@ -594,7 +603,7 @@ cudaError_t launch_product(const HeadI8Args &a, const Plan &p, int dev, int sms,
     t.dim = a.dim;
     t.nb = p.nb;
     t.tiles_b = p.tiles_b;
-    t.per_cb = (a.vocab + BM * CTAS - 1) / (BM * CTAS);
+    t.per_cb = (a.vocab + kI8Rows * CTAS - 1) / (kI8Rows * CTAS);
     const long long tiles = (long long)p.tiles_b * t.per_cb * a.n_cb;
     if (tiles > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     t.n_tiles = (int)tiles;
@@ -604,7 +613,7 @@ cudaError_t launch_product(const HeadI8Args &a, const Plan &p, int dev, int sms,
     t.out = a.out;
     t.tmem_cols = 32;
     while (t.tmem_cols < 2 * p.nb) t.tmem_cols *= 2;
-    const int stage = (BM + p.nb / CTAS) * 128, bars = 8 * (2 * kI8MaxStages + 4);
+    const int stage = (kI8Rows + p.nb / CTAS) * 128, bars = 8 * (2 * kI8MaxStages + 4);
     t.stages = (kI8SmemMax - 1024 - bars) / stage;
     if (t.stages > kI8MaxStages) t.stages = kI8MaxStages;
     const size_t smem = (size_t)t.stages * stage + bars + 1024;
@@ -621,28 +630,31 @@ cudaError_t launch_product(const HeadI8Args &a, const Plan &p, int dev, int sms,
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = CTAS == 2 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, head_i8_kernel<CTAS, BM>, mw, mh, t);
+    return cudaLaunchKernelEx(&cfg, head_i8_kernel<CTAS>, mw, mh, t);
 }
 
-// The tiles: for each kind of block, and each count of hidden tiles that its accumulators
-// allow, the waves times the rows of operands that an SM reads in one (they come from L2, which
-// bounds a wave; a fixed part stands for its start and end).
+// The tiles, by a model of the time fitted to a B200: for each kind of block (alone or in pairs) and
+// the counts of hidden tiles that its accumulators allow, the waves times a tile's hidden rows and a
+// fixed part.  Measured there, 9 x 1024 x 2048, us with the rounding (tiles of hidden rows):
+//   rows      64        128       256       333       512       700       1024      2048      4096
+//   alone   10.6 (1)  11.9 (2)  13.6 (2)  15.2 (2)  18.0 (2)  21.6 (4)  26.1 (4)  44.6 (8)  84.5 (16)
+//   pairs   11.4 (1)  13.1 (1)  14.8 (2)  15.9 (2)  17.3 (2)  23.4 (4)  25.6 (4)  41.6 (8)  77.8 (16)
+// Blocks of 64 weight rows were slower than of 128 from 16 hidden rows on, and no faster below.
 Plan plan_tiles(const HeadI8Args &a, int sms)
 {
-    Plan best{0, 0, 0, 0};
+    Plan best{0, 0, 0};
     long long best_cost = -1;
-    const int kinds[3][2] = {{1, 64}, {1, 128}, {2, 128}};
-    for (const auto &k : kinds) {
-        const int ctas = k[0], bm = k[1], unit = ctas == 2 ? 32 : 16;
-        const long long n = (long long)a.n_cb * ((a.vocab + bm * ctas - 1) / (bm * ctas));
+    for (int ctas = 1; ctas <= 2; ctas++) {
+        const int unit = 16 * ctas;
+        const long long n = (long long)a.n_cb * ((a.vocab + kI8Rows * ctas - 1) / (kI8Rows * ctas));
         const int least = (a.batch + 255) / 256;
         for (int tb = least; tb < least + 4; tb++) {
-            const int nb = ((a.batch + tb - 1) / tb + unit - 1) / unit * unit;
+            const int nb = ((a.batch + tb - 1) / tb + unit - 1) / unit * unit, wide = nb < 64 ? 64 : nb;
             const long long waves = (n * tb + sms / ctas - 1) / (sms / ctas);
-            const long long cost = waves * (bm + nb / ctas + 64);
+            const long long cost = ctas == 1 ? 300 + waves * (5 * wide + 200) : 500 + waves * (4 * wide + 250);
             if (best_cost < 0 || cost < best_cost) {
                 best_cost = cost;
-                best = Plan{ctas, bm, nb, (a.batch + nb - 1) / nb};
+                best = Plan{ctas, nb, (a.batch + nb - 1) / nb};
             }
         }
     }
@@ -669,20 +681,8 @@ cudaError_t launch_head_i8(const HeadI8Args &a, bool bf16, cudaStream_t stream)
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     e = launch_quantize_rows(a.hidden, bf16, a.batch, a.dim, a.dim, q, scale, stream);
     if (e != cudaSuccess) return e;
-    Plan p = plan_tiles(a, sms);
-#ifdef Z2_I8PLAN
-    static const char *env = getenv("I8PLAN");
-    if (env) {
-        int tb;
-        sscanf(env, "%d,%d,%d", &p.ctas, &p.bm, &tb);
-        const int unit = p.ctas == 2 ? 32 : 16;
-        p.nb = ((a.batch + tb - 1) / tb + unit - 1) / unit * unit;
-        p.tiles_b = (a.batch + p.nb - 1) / p.nb;
-    }
-#endif
-    if (p.ctas == 2) return launch_product<2, 128>(a, p, dev, sms, q, scale, stream);
-    if (p.bm == 128) return launch_product<1, 128>(a, p, dev, sms, q, scale, stream);
-    return launch_product<1, 64>(a, p, dev, sms, q, scale, stream);
+    const Plan p = plan_tiles(a, sms);
+    return p.ctas == 2 ? launch_product<2>(a, p, dev, sms, q, scale, stream) : launch_product<1>(a, p, dev, sms, q, scale, stream);
 }
 
 }  // namespace z2
