@@ -25,11 +25,6 @@ namespace z2 {
 
 namespace {
 
-#ifndef Z2_S2
-#define Z2_S2 3
-#define Z2_S1 3
-#define Z2_FILL 148*4
-#endif
 // KEYS keys and values of D elements (rows of `dim`) of one key head, as one stage of a warp's
 // ring: the keys' rows, then the values'.  16-byte piece p of row r lies at piece p ^ (r & 7), so
 // that eight rows' same piece falls on different banks.
@@ -52,9 +47,8 @@ struct Ring {
         return pages;
     }
 
-    // Loads the keys (KV & 1) and values (KV & 2) [j0, j0 + KEYS) that lie in [low, high) and
-    // on a page; zeros elsewhere.  Returns the bits of KEYS / 8 runs of eight that lie on a page.
-    template <int KV>
+    // Loads the keys and values [j0, j0 + KEYS) that lie in [low, high) and on a page; zeros
+    // elsewhere.  Returns the bits of KEYS / 8 runs of eight that lie on a page.
     __device__ static uint32_t load(const CacheArgs &c, const Pages &pages, int kvh, int j0, int low, int high,
                                     uint32_t stage)
     {
@@ -81,8 +75,8 @@ struct Ring {
                 for (int x = 0; x < kAcross; x++) {
                     const int r = i * kStep;   // row0 + r; row0 < kStep
                     const uint32_t dst = to + r * kRow + (((piece + 32 * x) ^ ((row0 + r) & 7)) << 4);
-                    if (KV & 1) cp_async16(dst, k + (i * kAcross + x) * 512);
-                    if (KV & 2) cp_async16(dst + kHalf, v + (i * kAcross + x) * 512);
+                    cp_async16(dst, k + (i * kAcross + x) * 512);
+                    cp_async16(dst + kHalf, v + (i * kAcross + x) * 512);
                 }
             return held;
         }
@@ -94,8 +88,8 @@ struct Ring {
             const long long at = take ? (KEYS == 8 || r < 8 ? base[0] : base[KEYS / 8 - 1]) + (r & 7) * c.dim : 0;
             for (int x = piece; x < live; x += 32) {
                 const uint32_t dst = stage + r * kRow + ((x ^ (r & 7)) << 4);
-                if (KV & 1) cp_async16_or_zero(dst, (const T *)c.k + at + x * (16 / (int)sizeof(T)), take);
-                if (KV & 2) cp_async16_or_zero(dst + kHalf, (const T *)c.v + at + x * (16 / (int)sizeof(T)), take);
+                cp_async16_or_zero(dst, (const T *)c.k + at + x * (16 / (int)sizeof(T)), take);
+                cp_async16_or_zero(dst + kHalf, (const T *)c.v + at + x * (16 / (int)sizeof(T)), take);
                 if (kPieces <= 32) break;
             }
         }
@@ -104,16 +98,17 @@ struct Ring {
 };
 
 // ---- bf16, by mma.sync ------------------------------------------------------
-// 16 * RB rows to a tile, groups of 16 keys: S = Q K^T by m16n8k16 (rows x 8 keys x 16
-// elements), whose accumulators, rounded to bf16, are the left operand of O += P V.  A ring's
-// groups are worked by RB warps, 16 rows each, which load them together (one the keys, the
-// other the values).
-template <int D, int RB, int STAGES, int W>
-__global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 3 : 2)
+// 16 rows to a tile, groups of 16 keys: S = Q K^T by m16n8k16 (rows x 8 keys x 16 elements),
+// whose accumulators, rounded to bf16, are the left operand of O += P V.
+// Two stages a ring, so that three blocks fit an SM: 64 streams of up to 6144 tokens and 20 rows
+// took 77 us with two stages, 92 with three; by pairs of warps that shared a ring's keys between
+// 32 rows 108 us, as most of the second 16 rows were none.
+template <int D, int STAGES, int W>
+__global__ void __launch_bounds__(32 * W, D > 128 || W > 4 ? 1 : 3)
     attend_rows_bf16_kernel(const CacheArgs c, const AttendArgs a, int ranks)
 {
     typedef Ring<__nv_bfloat16, D, 16> R;
-    constexpr int ROWS = 16 * RB, kThreads = 32 * W * RB;
+    constexpr int ROWS = 16, kThreads = 32 * W;
     extern __shared__ __align__(1024) unsigned char smem[];
     // the rings, then the queries; at the end the parts take the rings' place
     __shared__ float2 s_ml[W * ROWS];
@@ -121,7 +116,7 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
     __shared__ int4 s_found;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) / RB, rb = (threadIdx.x >> 5) % RB;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = blockIdx.x % ranks, kvh = blockIdx.y;
     const Tile tile = find_tile(c, a.group, ROWS, blockIdx.x / ranks, &s_found);
     if (tile.rows == 0) return;   // the whole cluster's tile
@@ -168,13 +163,7 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
         if (worker + it * workers < groups) {
             const int st = it % STAGES;
             const uint32_t to = ring + st * R::kStage;
-            uint32_t held;
-            if (RB == 1)
-                held = R::template load<3>(c, at, kvh, group_at(it), low, high, to);
-            else if (rb == 0)
-                held = R::template load<1>(c, at, kvh, group_at(it), low, high, to);
-            else
-                held = R::template load<2>(c, at, kvh, group_at(it), low, high, to);
+            const uint32_t held = R::load(c, at, kvh, group_at(it), low, high, to);
             held_bits = (held_bits & ~(3u << (2 * st))) | held << (2 * st);
         }
         cp_async_commit();
@@ -188,7 +177,7 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
     int pos[2];   // of this lane's rows (those past the tile's take the last row's)
 #pragma unroll
     for (int i = 0; i < 2; i++)
-        pos[i] = position_of(tile.ch, a.group, tile.row0 + min(rb * 16 + i * 8 + (lane >> 2), tile.rows - 1));
+        pos[i] = position_of(tile.ch, a.group, tile.row0 + min(i * 8 + (lane >> 2), tile.rows - 1));
     float m[2], l[2], o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -198,30 +187,25 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
 #pragma unroll
     for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
     const float factor = a.scale * kLog2e;
+    uint32_t saw = 0;   // bits as `seen`'s
 
     // ldmatrix: lane's row and piece of a 16 x 16 block
     const int lm_key = (lane & 7) + ((lane >> 4) << 3), lm_kp = (lane >> 3) & 1;     // keys: n blocks of 8
     const int lm_val = (lane & 7) + (((lane >> 3) & 1) << 3), lm_vp = lane >> 4;     // values, transposed
-    constexpr bool kQRegs = RB == 1 && D <= 128;
+    constexpr bool kQRegs = D <= 128;
     uint32_t qf[kQRegs ? D / 16 : 1][4];
     auto load_q = [&](int kk, uint32_t (&f)[4]) {
-        const int r = rb * 16 + (lane & 15), p = 2 * kk + (lane >> 4);
+        const int r = lane & 15, p = 2 * kk + (lane >> 4);
         ldmatrix4(s_q + r * R::kRow + ((p ^ (r & 7)) << 4), f);
     };
     if (kQRegs) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; kk++) load_q(kk, qf[kk]);
     }
-    auto meet = [&]() {   // the warps of the ring
-        if (RB == 1)
-            __syncwarp();
-        else
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + warp), "n"(32 * RB) : "memory");
-    };
 
     for (int it = 0; worker + it * workers < groups; it++) {
         cp_async_wait<STAGES - 2>();
-        meet();   // the group has landed, and the one before it is done with
+        __syncwarp();   // the group has landed, and the one before it is done with
         const typename R::Pages next = look(it + STAGES);
         fetch(it + STAGES - 1, pages[0]);
         pages[0] = next;
@@ -257,6 +241,7 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
                     x[n][i * 2 + e] = -INFINITY;
             }
         }
+        saw |= seen;
         float top[2];
         bool same = true;
 #pragma unroll
@@ -280,17 +265,11 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
                 }
             }
         }
+        const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[n][e] = exp2_fast(fmaf(x[n][e], factor, -m[e >> 1]));
-        if (partial) {
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (!(seen >> (4 * (e >> 1) + 2 * n + (e & 1)) & 1u)) x[n][e] = 0.0f;
-        }
+            for (int e = 0; e < 4; e++) x[n][e] = exp2_fast(fmaf(x[n][e], factor, -base[e >> 1]));
 #pragma unroll
         for (int i = 0; i < 2; i++) l[i] += (x[0][2 * i] + x[0][2 * i + 1]) + (x[1][2 * i] + x[1][2 * i + 1]);
         uint32_t pf[4];
@@ -309,7 +288,7 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
                              : "r"(values + i * 16));
                 any |= odd2(v.x) || odd2(v.y) || odd2(v.z) || odd2(v.w);
             }
-            if (__any_sync(kFull, any)) {   // the same for every warp of the ring
+            if (__any_sync(kFull, any)) {
 #pragma unroll 1
                 for (int k = 0; k < 16; k++)
 #pragma unroll
@@ -327,7 +306,7 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
                                 if (odd(v1)) o[n][i * 2 + 1] += v1;
                             }
                     }
-                meet();
+                __syncwarp();
                 for (int i = lane; i < 64 * R::kPieces; i += 32) {
                     uint32_t w;
                     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(values + i * 4));
@@ -335,7 +314,7 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
                     if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
                     asm volatile("st.shared.b32 [%0], %1;" ::"r"(values + i * 4), "r"(w) : "memory");
                 }
-                meet();
+                __syncwarp();
             }
         }
 #pragma unroll
@@ -353,8 +332,9 @@ __global__ void __launch_bounds__(32 * W * RB, D > 128 || W > 4 ? 1 : RB == 1 ? 
     for (int i = 0; i < 2; i++) {
         l[i] += __shfl_xor_sync(kFull, l[i], 1);
         l[i] += __shfl_xor_sync(kFull, l[i], 2);
-        const int r = rb * 16 + i * 8 + (lane >> 2);
-        if ((lane & 3) == 0) s_ml[warp * ROWS + r] = make_float2(m[i], l[i]);
+        const int r = i * 8 + (lane >> 2);
+        const bool any = __ballot_sync(kFull, (saw >> (4 * i) & 15u) != 0) >> (lane & ~3) & 15u;
+        if ((lane & 3) == 0) s_ml[warp * ROWS + r] = make_float2(m[i] == -INFINITY && any ? kLowest : m[i], l[i]);
 #pragma unroll
         for (int n = 0; n < D / 8; n++)
             *reinterpret_cast<float2 *>(part + (warp * ROWS + r) * D + part_piece(r, 2 * n + ((lane & 3) >> 1)) * 4 + 2 * (lane & 1)) =
@@ -425,6 +405,7 @@ __global__ void __launch_bounds__(32 * W)
     }
     const float factor = a.scale * kLog2e;
     const int key = lane >> 2, quarter = lane & 3;
+    uint32_t saw = 0;   // of this lane's key, a bit to a row
 
     uint32_t held_bits = 0;
     auto fetch = [&](int it) {
@@ -432,7 +413,7 @@ __global__ void __launch_bounds__(32 * W)
         if (g < groups) {
             const int st = it % STAGES;
             const int j0 = (first_group + g) * 8;
-            const uint32_t held = R::template load<3>(c, R::look(c, tile.ch.stream, j0, room), kvh, j0, low, high,
+            const uint32_t held = R::load(c, R::look(c, tile.ch.stream, j0, room), kvh, j0, low, high,
                                                       ring + st * R::kStage);
             held_bits = (held_bits & ~(1u << st)) | held << st;
         }
@@ -486,7 +467,8 @@ __global__ void __launch_bounds__(32 * W)
                 for (int i = 0; i < kCols; i++) o[r][i] *= keep;
                 m[r] = most;
             }
-            const float w = in ? exp2f(x[r] - m[r]) : 0.0f;
+            const float w = in ? exp2f(x[r] - (m[r] == -INFINITY ? 0.0f : m[r])) : 0.0f;
+            saw |= in ? 1u << r : 0u;
             l[r] += w;
             if (quarter == 0) s_w[warp][key][r] = w;
         }
@@ -520,7 +502,8 @@ __global__ void __launch_bounds__(32 * W)
         l[r] += __shfl_xor_sync(kFull, l[r], 4);
         l[r] += __shfl_xor_sync(kFull, l[r], 8);
         l[r] += __shfl_xor_sync(kFull, l[r], 16);
-        if (lane == 0) s_ml[warp * ROWS + r] = make_float2(m[r], l[r]);
+        const bool any = __any_sync(kFull, saw >> r & 1u);
+        if (lane == 0) s_ml[warp * ROWS + r] = make_float2(m[r] == -INFINITY && any ? kLowest : m[r], l[r]);
 #pragma unroll
         for (int i = 0; i < kCols; i++)
             part[(warp * ROWS + r) * D + part_piece(r, (lane + 32 * i) >> 2) * 4 + (lane & 3)] = o[r][i];
@@ -662,6 +645,7 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
     const float factor = a.scale * kLog2e;
     const float *q0 = s_q + (warp * 16 + g) * Sh::kPitch + 4 * t, *q1 = q0 + 8 * Sh::kPitch;
     const bool idle = warp * 16 >= tile.rows;   // none of this warp's rows is one
+    uint32_t saw = 0;   // bits as `seen`'s
 
     for (int it = 0; it < mine; it++) {
         cp_async_wait<0>();
@@ -756,6 +740,7 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
                     x[b >> 2][b & 3] = -INFINITY;
             }
         }
+        saw |= seen;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             float most = -INFINITY;
@@ -780,8 +765,8 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
         for (int n = 0; n < 4; n++) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                float w = exp2_fast(fmaf(x[n][e], factor, -m[e >> 1]));
-                if (partial && !(seen >> (4 * n + e) & 1u)) w = 0.0f;
+                const float base = m[e >> 1] == -INFINITY ? 0.0f : m[e >> 1];
+                const float w = exp2_fast(fmaf(x[n][e], factor, -base));   // 0 where not seen
                 l[e >> 1] += w;
                 x[n][e] = w;
             }
@@ -825,7 +810,8 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
         l[i] += __shfl_xor_sync(kFull, l[i], 1);
         l[i] += __shfl_xor_sync(kFull, l[i], 2);
         const int r = warp * 16 + i * 8 + g;
-        if (t == 0) s_ml[r] = make_float2(m[i], l[i]);
+        const bool any = __ballot_sync(kFull, (saw & (i ? 0xccccu : 0x3333u)) != 0) >> (lane & ~3) & 15u;
+        if (t == 0) s_ml[r] = make_float2(m[i] == -INFINITY && any ? kLowest : m[i], l[i]);
 #pragma unroll
         for (int b = 0; b < D / 32; b++)
 #pragma unroll
@@ -857,10 +843,7 @@ cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, int warps, in
     const long long work = tiles_with_rows(c, a, tile_rows) * c.n_kv;
     const long long room = ((long long)c.max_pages << c.page_shift) / (keys * warps);
     int ranks = 1;
-    while (ranks < kMostRanks && work * ranks < Z2_FILL && ranks < room) ranks *= 2;
-#ifdef Z2_RANKS
-    ranks = Z2_RANKS;
-#endif
+    while (ranks < kMostRanks && work * ranks < 148 * 4 && ranks < room) ranks *= 2;
     if (tiles * ranks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * ranks), (unsigned)c.n_kv);
@@ -878,25 +861,24 @@ cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, int warps, in
     return cudaLaunchKernelEx(&cfg, kernel, c, a, ranks);
 }
 
-template <int D, int RB, int STAGES, int W>
+template <int D, int STAGES, int W>
 cudaError_t launch_bf16(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
 {
     static std::mutex mu;
     static bool ready[64] = {false};
     typedef Ring<__nv_bfloat16, D, 16> R;
-    const size_t rings = W * STAGES * R::kStage, parts = (size_t)W * 16 * RB * D * 4;
-    const size_t smem = (rings > parts ? rings : parts) + 16 * RB * R::kRow;
-    return launch_rows(attend_rows_bf16_kernel<D, RB, STAGES, W>, smem, 16 * RB, W, 32 * W * RB, c, a, 16, mu, ready,
-                       stream);
+    const size_t rings = W * STAGES * R::kStage, parts = (size_t)W * 16 * D * 4;
+    const size_t smem = (rings > parts ? rings : parts) + 16 * R::kRow;
+    return launch_rows(attend_rows_bf16_kernel<D, STAGES, W>, smem, 16, W, 32 * W, c, a, 16, mu, ready, stream);
 }
 
-// Blocks of eight rings where a cluster of the most blocks for each tile does not fill the SMs.
-template <int D, int RB, int STAGES>
+// Blocks of eight rings where a cluster of the most blocks for each tile does not fill the SMs (one
+// stream of 6050 tokens: 12.9 us with half as many blocks, 10.4 us).
+template <int D, int STAGES>
 cudaError_t launch_bf16(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
 {
-    if (tiles_with_rows(c, a, 16 * RB) * c.n_kv * kMostRanks <= 148)
-        return launch_bf16<D, RB, 3, 8>(c, a, stream);
-    return launch_bf16<D, RB, STAGES, 4>(c, a, stream);
+    if (tiles_with_rows(c, a, 16) * c.n_kv * kMostRanks <= 148) return launch_bf16<D, 3, 8>(c, a, stream);
+    return launch_bf16<D, STAGES, 4>(c, a, stream);
 }
 
 template <int D, int ROWS, int STAGES>
@@ -927,10 +909,11 @@ cudaError_t launch_cache_attend(const CacheArgs &c, const AttendArgs &a, bool bf
     const int most_new = a.max_new > 0 && a.max_new < c.rows ? a.max_new : c.rows;
     const long long rows = (long long)most_new * a.group;
     if (bf16) {
+        // (20 or 32 rows on 64 streams: 90 and 94 us here, 92 there; 48 rows: 111 against 92; on 4
+        // streams 21 and 22 us against 25, 48 rows 32 against 25)
         if (rows > 32 && (c.dim == 64 || c.dim == 128)) return launch_cache_attend_tc(c, a, stream);
-        if (c.dim > 128) return launch_bf16<256, 1, 3, 4>(c, a, stream);
-        if (c.dim > 64) return rows > 16 ? launch_bf16<128, 2, Z2_S2>(c, a, stream) : launch_bf16<128, 1, Z2_S1>(c, a, stream);
-        return rows > 16 ? launch_bf16<64, 2, 4>(c, a, stream) : launch_bf16<64, 1, 4>(c, a, stream);
+        if (c.dim > 128) return launch_bf16<256, 3, 4>(c, a, stream);
+        return c.dim > 64 ? launch_bf16<128, 2>(c, a, stream) : launch_bf16<64, 4>(c, a, stream);
     }
     if (rows > 16)
         return c.dim > 128 ? launch_tile_f32<256>(c, a, stream)

@@ -12,6 +12,9 @@ namespace z2 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// The maximum of a part whose row saw tokens with scores of -inf alone (its sum is zero): where the
+// row has no other, the result is a NaN, as the definition has it.
+constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ float exp2_fast(float x)
 {
@@ -141,6 +144,7 @@ __device__ void join_and_store(const CacheArgs &c, const AttendArgs &a, const Ti
                                int ranks, int rank)
 {
     constexpr int kQuads = ROWS * D / 4;
+    const int quads = tile.rows * (D / 4);   // of the tile's rows
     // A part without a visible token (m = -inf) weighs nothing; a NaN sum stays one.
     auto weigh = [](float m, float most) { return m == -INFINITY ? 0.0f : exp2_fast(m - most); };
     auto add = [](float4 &sum, float f, const float4 &v) {
@@ -151,7 +155,7 @@ __device__ void join_and_store(const CacheArgs &c, const AttendArgs &a, const Ti
     };
     __syncthreads();
     // the block's own warps, into warp 0's part
-    for (int r = threadIdx.x; r < ROWS; r += THREADS) {
+    for (int r = threadIdx.x; r < tile.rows; r += THREADS) {
         float most = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; w++) most = fmaxf(most, ml[w * ROWS + r].x);
@@ -164,7 +168,7 @@ __device__ void join_and_store(const CacheArgs &c, const AttendArgs &a, const Ti
         ml[r] = make_float2(most, l);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kQuads; i += THREADS) {
+    for (int i = threadIdx.x; i < quads; i += THREADS) {
         const int r = i / (D / 4);
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -193,18 +197,18 @@ __device__ void join_and_store(const CacheArgs &c, const AttendArgs &a, const Ti
                 weight[k * ROWS + r] = f;
                 l += f * all[k * ROWS].y;
             }
-            total[r] = l;
+            total[r] = l == 0.0f && most > -INFINITY ? NAN : l;
         }
     } else {
-        for (int r = threadIdx.x; r < ROWS; r += THREADS) total[r] = ml[r].y;
+        for (int r = threadIdx.x; r < ROWS; r += THREADS) total[r] = ml[r].y == 0.0f && ml[r].x > -INFINITY ? NAN : ml[r].y;
     }
     __syncthreads();
     // this rank's share of the rows' quads
-    const int per = (kQuads + ranks - 1) / ranks;
-    const int end = min(kQuads, (rank + 1) * per);
+    const int per = (quads + ranks - 1) / ranks;
+    const int end = min(quads, (rank + 1) * per);
     for (int i = rank * per + threadIdx.x; i < end; i += THREADS) {
         const int r = i / (D / 4), d = part_piece(r, i % (D / 4)) * 4;
-        if (r >= tile.rows || d >= c.dim) continue;
+        if (d >= c.dim) continue;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (ranks > 1) {
             const uint32_t at = smem_u32(part) + i * 16;

@@ -15,6 +15,10 @@
 // pass it by more than 2^8 (P is then at most 256 instead of 1, and the sum of the same scale:
 // no rounding changes), so that O is seldom rescaled.  Stages hand over through mbarriers, every
 // wait is bounded.
+// SPLIT: where there are few rows to a key head, a block has one tile of up to 128 and its two groups
+// of softmax warps take the steps in turn, each with an accumulator of its own; a cluster of
+// blocks shares a tile's steps out where there are few tiles.  The parts are joined as in
+// cache_attend.cu.  (Warps without rows only keep the hand-over going.)
 // A value that is not finite in a step that some row does not wholly see would reach that row as
 // 0 times it: such values are set to zero in shared memory before the product and added, at the
 // end, to the rows that see them.
@@ -165,10 +169,32 @@ __device__ __forceinline__ Span span_of(const CacheArgs &c, const AttendArgs &a,
     return s;
 }
 
-template <int D>
+// Adds to a row's outputs [col, col + N) the values of step j0's tokens that are not finite, of those
+// that the row sees ([from, to)); steps that every row sees wholly went through the product as they are.
+template <int N>
+__device__ void add_odd(const CacheArgs &c, int stream, int kvh, int j0, int all_from, int all_to, int from, int to, int col,
+                        uint32_t *o)
+{
+    const int room = room_of(c);
+    bool whole = j0 >= all_from && j0 + kStep <= all_to;
+    for (int e = 0; whole && e < kStep / 8; e++) whole = j0 + 8 * e < room && page_of(c, stream, j0 + 8 * e) >= 0;
+    if (whole) return;
+    for (int j = max(from, j0); j < min(to, j0 + kStep); j++) {
+        const int p = page_of(c, stream, j);
+        if (p < 0) continue;
+        const __nv_bfloat16 *v = (const __nv_bfloat16 *)c.v + row_on_page(c, p, kvh, j) + col;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const float y = as_f(v[k]);
+            if (odd(y)) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
+        }
+    }
+}
+
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attend_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                     const CacheArgs c, const AttendArgs a, int box_rows, int turns)
+                     const CacheArgs c, const AttendArgs a, int box_rows, int turns, int ranks)
 {
     typedef TcShape<D> Sh;
     // kind::f16: D f32, A and B bf16; M = 128; S: N = 128, both K-major; O: N = D, B MN-major
@@ -183,18 +209,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     auto empty = [&](int s) { return s_bar + 8 * (kSlots + s); };
     auto s_full = [&](int q) { return s_bar + 8 * (2 * kSlots + q); };    // S, and O before it, are done
     auto p_ready = [&](int q, int h) { return s_bar + 8 * (2 * kSlots + 2 + 2 * q + h); };   // P of 64 keys
+    constexpr int kTileRows = SPLIT ? 128 : 256;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_odd;
+    __shared__ float s_gate[SPLIT ? 128 : 1];
+    // (SPLIT) the parts at the end, in the place of keys and values
+    float *part = reinterpret_cast<float *>(smem_raw + (s_kv - smem_u32(smem_raw)));
+    float2 *ml = reinterpret_cast<float2 *>(part + 2 * 128 * D);
+    float *weight = reinterpret_cast<float *>(ml + 2 * 128), *total = weight + kMostRanks * 128;
+    static_assert(!SPLIT || (2 * 128 * D + 4 * 128 + kMostRanks * 128 + 128) * 4 <= kSlots * (int)Sh::kTile, "parts fit");
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // A stream's last tiles see the most tokens: every stream's come first.  (Where a stream has
     // more tiles than it was launched for, a block takes every `turns`-th.)
-    const int kvh = blockIdx.x % c.n_kv, first_turn = blockIdx.x / c.n_kv / c.n_streams;
-    const Chunk ch = chunk_of(c, blockIdx.x / c.n_kv % c.n_streams);
+    const int rank = SPLIT ? blockIdx.x % ranks : 0, item = SPLIT ? blockIdx.x / ranks : blockIdx.x;
+    const int kvh = item % c.n_kv, first_turn = item / c.n_kv / c.n_streams;
+    const Chunk ch = chunk_of(c, item / c.n_kv % c.n_streams);
     const long long all_rows = (long long)ch.n * a.group;
-    const int n_tiles = (int)((all_rows + 255) / 256);
+    const int n_tiles = (int)((all_rows + kTileRows - 1) / kTileRows);
     if (first_turn >= n_tiles) return;
     if (threadIdx.x == 0) {
         s_abort = s_odd = 0;
@@ -220,21 +254,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint32_t tmem = 0;
     // phases of the barriers before this tile: tiles of keys and values, scores of either tile
     int kv0 = 0, scored0 = 0, scored1 = 0, weighed0 = 0, weighed1 = 0;
+    bool dead = false;   // a wait ran out
     for (int turn = first_turn; turn < n_tiles; turn += turns) {
-    const long long row_ll = (long long)(n_tiles - 1 - turn) * 256;
+    const long long row_ll = (long long)(n_tiles - 1 - turn) * kTileRows;
     const int row0 = (int)row_ll;
-    const int tile_rows = (int)(all_rows - row_ll < 256 ? all_rows - row_ll : 256);
+    const int tile_rows = (int)(all_rows - row_ll < kTileRows ? all_rows - row_ll : kTileRows);
     const int rows0 = min(tile_rows, 128), rows1 = tile_rows - rows0;
     const Span span0 = span_of(c, a, ch, row0, rows0);
     const Span span1 = rows1 > 0 ? span_of(c, a, ch, row0 + 128, rows1) : span0;
     const int low = min(span0.low, span1.low), high = max(span0.high, span1.high);
     // tokens that every row of both tiles sees: the tiles share the values, and what is done to them
     const int all_from = max(span0.all_from, span1.all_from), all_to = min(span0.all_to, span1.all_to);
-    const int step0 = low / kStep, steps = high > low ? (high + kStep - 1) / kStep - step0 : 0;
+    const int step0 = low / kStep + rank, all_steps = high > low ? (high + kStep - 1) / kStep - low / kStep : 0;
+    const int steps = all_steps > rank ? (all_steps - rank + ranks - 1) / ranks : 0;   // this rank's: step0 + i ranks
+    if (SPLIT) {
+        Tile tile;
+        tile.ch = ch;
+        tile.row0 = row0;
+        tile.rows = tile_rows;
+        load_gates<__nv_bfloat16>(a, tile, kvh, s_gate);
+    }
 
     // queries, swizzled as TMA does; zeros past the rows
 #pragma unroll 4
-    for (int i = threadIdx.x; i < 256 * (D / 8); i += kTcThreads) {
+    for (int i = threadIdx.x; i < kTileRows * (D / 8); i += kTcThreads) {
         const int r = i / (D / 8), p = i % (D / 8), row = row0 + r;
         const bool in = r < tile_rows;
         const long long at = in ? (long long)(ch.first + row / a.group) * a.q_stride +
@@ -251,7 +294,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     tmem = s_tmem;
 
-    if (steps > 0) {
+    // a row's running maximum and sum, and whether it saw a token
+    float m = -INFINITY, l = 0.0f;
+    bool saw = false;
+    if (steps > 0 && !dead) {
         if (warp == 0) {
             // ---- TMA producer: tile 2 i is step i's keys, 2 i + 1 its values
             const int boxes = kStep / box_rows;          // of a step, for each half
@@ -259,7 +305,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             bool ok = true;
             int it = kv0;
             for (int i = 0; i < steps && ok; i++) {
-                const int j0 = (step0 + i) * kStep;
+                const int j0 = (step0 + i * ranks) * kStep;
                 // lane's box of the step's boxes x halves (16 x 2 at most)
                 const int b = lane % boxes, h = lane / boxes, j = j0 + b * box_rows;
                 const bool mine = h < (int)Sh::kHalves;
@@ -302,17 +348,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int kk = 0; kk < D / 16; kk++) {
                         const uint32_t off = (kk >> 2) * (128 * 128);
-                        mma_bf16(tmem + kColS + q * 128, sw128_desc(s_q + q * Sh::kTile + off) + 2 * (kk & 3),
+                        mma_bf16(tmem + kColS + q * 128, sw128_desc(s_q + (SPLIT ? 0 : q * Sh::kTile) + off) + 2 * (kk & 3),
                                  sw128_desc(slot(t) + off) + 2 * (kk & 3), kIdescS, kk != 0);
                     }
                     mma_commit(s_full(q));
                 };
+                if (SPLIT) {
+                    for (int i = 0; i < 2 && i < steps; i++) {
+                        if (!landed(2 * i)) break;
+                        scores(i, 2 * i);
+                        done(2 * i);
+                    }
+                    for (int i = 0; i < steps && ok && !*(volatile int *)&s_abort; i++) {
+                        const int q = i & 1;
+                        if (!landed(2 * i + 1) || (i + 2 < steps && !landed(2 * i + 4))) break;
+#pragma unroll
+                        for (int k = 0; k < kStep / 16; k++) {
+                            const int kk = k ^ 4;
+                            if (k % 4 == 0 && !wait(p_ready(q, kk / 4), (uint32_t)((q ? weighed1 : weighed0) + (i >> 1)) & 1u)) break;
+                            mma_bf16_ts(tmem + kColO + q * 128, tmem + kColS + q * 128 + 32 * (kk >> 1) + 8 * (kk & 1),
+                                        sw128_desc_mn(slot(2 * i + 1) + kk * 16 * 128), kIdescO, i > 1 || k > 0);
+                        }
+                        if (!ok) break;
+                        done(2 * i + 1);
+                        if (i + 2 < steps) {
+                            scores(q, 2 * i + 4);
+                            done(2 * i + 4);
+                        } else {
+                            mma_commit(s_full(q));   // O is whole
+                        }
+                    }
+                }
                 const int tiles = rows1 > 0 ? 2 : 1;
-                if (landed(0)) {
+                if (!SPLIT && landed(0)) {
                     for (int q = 0; q < tiles; q++) scores(q, 0);
                     done(0);
                 }
-                for (int i = 0; i < steps && ok && !*(volatile int *)&s_abort; i++) {
+                for (int i = 0; !SPLIT && i < steps && ok && !*(volatile int *)&s_abort; i++) {
                     const bool more = i + 1 < steps;
                     if (!landed(2 * i + 1) || (more && !landed(2 * i + 2))) break;
                     for (int q = 0; q < tiles; q++) {
@@ -339,30 +411,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         } else if (warp >= 4) {
             // ---- softmax of tile q, this thread's row r of it
             const int q = (warp - 4) >> 2, r = threadIdx.x & 127;
-            const int rows = q ? rows1 : rows0, s_before = q ? scored1 : scored0;
-            if (rows > 0) {
+            const int rows = SPLIT ? tile_rows : q ? rows1 : rows0, s_before = q ? scored1 : scored0;
+            const int row_q = row0 + (SPLIT ? 0 : q * 128);   // the tile's first row
+            // the group's n-th step is the rank's q + 2 n, or n
+            const int count = SPLIT ? (steps - q + 1) / 2 : steps;
+            const int scanners = SPLIT ? (rows + 31) & ~31 : 128;   // threads of warps with rows
+            auto step_of = [&](int n) { return SPLIT ? q + 2 * n : n; };
+            if (SPLIT && 32 * (warp & 3) >= rows) {   // no row of this warp's
+                for (int n = 0; n < count; n++) {
+                    const bool ok = mbar_wait(s_full(q), (uint32_t)(s_before + n) & 1u) && !*(volatile int *)&s_abort;
+                    if (!__all_sync(kFull, ok)) break;
+                    if (lane == 0) {
+                        mbar_arrive(p_ready(q, 0));
+                        mbar_arrive(p_ready(q, 1));
+                    }
+                }
+            } else if (rows > 0 && count > 0) {
                 const uint32_t at = ((uint32_t)(warp & 3) * 32) << 16;   // this warp's TMEM lanes
                 const uint32_t t_s = tmem + at + kColS + q * 128, t_o = tmem + at + kColO + q * 128;
-                const int pos = position_of(ch, a.group, row0 + q * 128 + min(r, rows - 1));
+                const int pos = position_of(ch, a.group, row_q + min(r, rows - 1));
                 const int from = a.window > 0 ? max(0, pos - a.window + 1) : 0;
                 const int to = min(pos + 1, (q ? span1 : span0).high);   // this row sees [from, to)
                 const float factor = a.scale * kLog2e;
                 const int room = room_of(c);
                 // the pages of a step's runs of eight tokens, one step ahead; bit 8 e: run e is held
                 auto look = [&](int i) {
-                    const int j = (step0 + i) * kStep + 8 * lane;
+                    const int j = (step0 + i * ranks) * kStep + 8 * lane;
                     return lane < 16 && (i >= steps || (j < room && page_of(c, ch.stream, j) >= 0));
                 };
-                float m = -INFINITY, l = 0.0f;
-                bool saw = false;   // a token that the row sees
                 bool ok = true;
-                bool held_next = look(0);
-                for (int i = 0; i < steps; i++) {
+                bool held_next = look(step_of(0));
+                for (int n = 0; n < count; n++) {
+                    const int i = step_of(n);
                     const uint32_t held = __ballot_sync(kFull, held_next) & 0xffffu;
-                    held_next = look(i + 1);
-                    const int j0 = (step0 + i) * kStep;
+                    held_next = look(step_of(n + 1));
+                    const int j0 = (step0 + i * ranks) * kStep;
                     const bool partial = j0 < all_from || j0 + kStep > all_to || held != 0xffffu;
-                    ok = mbar_wait(s_full(q), (uint32_t)(s_before + i) & 1u) && !*(volatile int *)&s_abort;
+                    ok = mbar_wait(s_full(q), (uint32_t)(s_before + n) & 1u) && !*(volatile int *)&s_abort;
                     ok = __all_sync(kFull, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -404,7 +489,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         ok = __all_sync(kFull, mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u));
                         if (!ok) break;
                         const uint32_t values = s_kv + (uint32_t)(t % kSlots) * Sh::kTile;
-                        for (int k = r; k < (int)Sh::kTile / 16; k += 128) {
+                        for (int k = r; k < (int)Sh::kTile / 16; k += scanners) {
                             uint32_t w[4];
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
@@ -435,7 +520,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             m = most;
                             l *= keep;
                         }
-                        if (i > 0) {   // O is idle: S came after its last product
+                        if (n > 0) {   // O is idle: S came after its last product
 #pragma unroll 1
                             for (int b = 0; b < D / 32; b++) {
                                 uint32_t o[32];
@@ -481,11 +566,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     l += s0 + s1;
                 }
                 // ---- O / l
-                ok = ok && mbar_wait(s_full(q), (uint32_t)(s_before + steps) & 1u) && !*(volatile int *)&s_abort;
-                if (__all_sync(kFull, ok)) {
+                ok = ok && mbar_wait(s_full(q), (uint32_t)(s_before + count) & 1u) && !*(volatile int *)&s_abort;
+                if (!__all_sync(kFull, ok)) {
+                    s_abort = 1;
+                } else if (!SPLIT) {
                     tc_fence_after();
                     const bool odd_values = *(volatile int *)&s_odd;
-                    const int row = row0 + q * 128 + r, token = ch.first + row / a.group;
+                    const int row = row_q + r, token = ch.first + row / a.group;
                     const int h = kvh * a.group + row % a.group;
                     const bool live = r < rows;
                     float f = l == 0.0f ? (saw ? NAN : 0.0f) : 1.0f / l;
@@ -500,23 +587,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tmem_ld32_start(t_o + 32 * b, o);
                         tmem_wait_ld();
                         tmem_landed(o);
-                        if (odd_values && live) {
-                            for (int j = max(from, step0 * kStep); j < to; j++) {
-                                const int s0 = j & ~(kStep - 1);
-                                // steps that every row sees wholly went through the product as they are
-                                const int p = page_of(c, ch.stream, j);
-                                bool whole = s0 >= all_from && s0 + kStep <= all_to;
-                                for (int e = 0; whole && e < kStep / 8; e++)
-                                    whole = s0 + 8 * e < room && page_of(c, ch.stream, s0 + 8 * e) >= 0;
-                                if (p < 0 || whole) continue;
-                                const __nv_bfloat16 *v = (const __nv_bfloat16 *)c.v + row_on_page(c, p, kvh, j) + 32 * b;
-#pragma unroll
-                                for (int k = 0; k < 32; k++) {
-                                    const float y = as_f(v[k]);
-                                    if (odd(y)) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
-                                }
-                            }
-                        }
+                        for (int i = 0; odd_values && live && i < steps; i++)
+                            add_odd<32>(c, ch.stream, kvh, (step0 + i) * kStep, all_from, all_to, from, to, 32 * b, o);
                         __syncwarp();
                         if (live) {
 #pragma unroll
@@ -531,12 +603,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         __syncwarp();
                     }
-                } else {
-                    s_abort = 1;
                 }
             }
         }
-    } else {
+    } else if (!SPLIT && !dead) {
         // rows that see nothing
         for (int i = threadIdx.x; i < tile_rows * (D / 8); i += kTcThreads) {
             const int row = row0 + i / (D / 8);
@@ -546,21 +616,71 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     }
     tc_fence_before();
-    if (__syncthreads_or(*(volatile int *)&s_abort)) break;
+    dead = __syncthreads_or(*(volatile int *)&s_abort) || dead;
     tc_fence_after();
+    if (SPLIT) {
+        // the groups' parts (of a block that gave up, nothing: its cluster goes on), then their join
+        if (warp >= 4) {
+            const int q = (warp - 4) >> 2, r = threadIdx.x & 127;
+            const uint32_t t_o = tmem + (((uint32_t)(warp & 3) * 32) << 16) + kColO + q * 128;
+            const bool some = !dead && steps > q;
+            if (32 * (warp & 3) < tile_rows) {
+                // scores of -inf alone leave a sum of zero beside a maximum that is not -inf: a NaN
+                ml[q * 128 + r] = some ? make_float2(m == -INFINITY && saw ? kLowest : m, l) : make_float2(-INFINITY, 0.0f);
+                const int pos = position_of(ch, a.group, row0 + min(r, tile_rows - 1));
+                const int from = a.window > 0 ? max(0, pos - a.window + 1) : 0, to = min(pos + 1, span0.high);
+                const bool odd_values = *(volatile int *)&s_odd;
+#pragma unroll 1
+                for (int b = 0; b < D / 32; b++) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    if (some) {
+                        tmem_ld32_start(t_o + 32 * b, o);
+                        tmem_wait_ld();
+                        tmem_landed(o);
+                        // (bounded by the rank's own steps of this group)
+                        for (int i = q; odd_values && i < steps; i += 2)
+                            add_odd<32>(c, ch.stream, kvh, (step0 + i * ranks) * kStep, all_from, all_to, from, to, 32 * b, o);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[k] = 0;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        *reinterpret_cast<uint4 *>(part + (q * 128 + r) * D + part_piece(r, 8 * b + k) * 4) =
+                            make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                }
+            }
+        }
+        Tile tile;
+        tile.ch = ch;
+        tile.row0 = row0;
+        tile.rows = tile_rows;
+        join_and_store<__nv_bfloat16, D, 128, 2, kTcThreads>(c, a, tile, kvh, part, ml, weight, total, s_gate, ranks, rank);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();   // the next tile's keys come where the parts were
+    } else if (dead) {
+        break;
+    }
     if (threadIdx.x == 0) s_odd = 0;   // (the next tile's barrier follows)
     if (steps > 0) {
         kv0 += 2 * steps;
-        scored0 += steps + 1;
-        weighed0 += steps;
-        if (rows1 > 0) {
-            scored1 += steps + 1;
-            weighed1 += steps;
-        }
+        const int count0 = SPLIT ? (steps + 1) / 2 : steps, count1 = SPLIT ? steps / 2 : rows1 > 0 ? steps : 0;
+        scored0 += count0 + 1;
+        weighed0 += count0;
+        scored1 += count1 > 0 ? count1 + 1 : 0;
+        weighed1 += count1;
     }
     }
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Tiles of a stream, as far as the caller says (the mean where it says nothing).
+long long turns_of(const CacheArgs &c, const AttendArgs &a, int tile_rows)
+{
+    const long long most_new = a.max_new > 0 && a.max_new < c.rows ? a.max_new : c.rows / c.n_streams + 1;
+    return (most_new * a.group + tile_rows - 1) / tile_rows;
 }
 
 // Pages as a 4-D tensor (elements, tokens of a page, key heads, pages); a box is 64 elements of
@@ -579,8 +699,8 @@ bool make_page_map(CUtensorMap *m, const void *base, const CacheArgs &c, int box
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
-cudaError_t launch_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
+template <int D, bool SPLIT>
+cudaError_t launch_tc(const CacheArgs &c, const AttendArgs &a, int ranks, cudaStream_t stream)
 {
     static std::mutex mu;
     static bool ready[64] = {false};
@@ -591,37 +711,59 @@ cudaError_t launch_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stre
     {
         std::lock_guard<std::mutex> lk(mu);
         if (!ready[dev]) {
-            e = cudaFuncSetAttribute(attend_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TcShape<D>::kSmem);
+            e = cudaFuncSetAttribute(attend_tc_kernel<D, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)TcShape<D>::kSmem);
+            if (e == cudaSuccess && SPLIT)
+                e = cudaFuncSetAttribute(attend_tc_kernel<D, SPLIT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return e;
             ready[dev] = true;
         }
     }
-    const int page = 1 << c.page_shift, box_rows = page < kStep ? page : kStep;
+    const int page = 1 << c.page_shift, box_rows = page < kStep ? page : kStep, tile = SPLIT ? 128 : 256;
     CUtensorMap mk, mv;
     if (!make_page_map(&mk, c.k, c, box_rows) || !make_page_map(&mv, c.v, c, box_rows)) return cudaErrorInvalidValue;
-    // tiles of a stream, as far as the caller says (the mean where it says nothing)
-    const long long most_new = a.max_new > 0 && a.max_new < c.rows ? a.max_new : c.rows / c.n_streams + 1;
-    const long long turns = (most_new * a.group + 255) / 256;
-    const long long blocks = turns * c.n_streams * c.n_kv;
+    const long long turns = turns_of(c, a, tile), blocks = turns * c.n_streams * c.n_kv * ranks;
     if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(kTcThreads);
     cfg.dynamicSmemBytes = TcShape<D>::kSmem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)ranks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attend_tc_kernel<D>, mk, mv, c, a, box_rows, (int)turns);
+    cfg.numAttrs = ranks > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, attend_tc_kernel<D, SPLIT>, mk, mv, c, a, box_rows, (int)turns, ranks);
+}
+
+template <int D>
+cudaError_t launch_tc_any(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
+{
+    // Tiles of 128 rows while they lie on an SM each, clusters sharing a tile's steps as far as that
+    // goes on (clusters of eight such blocks only until half the SMs are taken: more do not fit at
+    // once); else tiles of 256.  Chunks on 1500 to 3000 cached tokens of 16 + 4 heads of 128, us, as 256 / 128
+    // rows by 1, 2, 4, 8 blocks, rows being tokens x 4:
+    //   1 stream,    64 rows   38.4 / 40.1  28.2  22.0  18.9      1024 rows   53.2 / 45.0  31.5  23.7  59.3
+    //   4 streams,   64 rows   47.3 / 48.2  32.8  24.3  37.0      1024 rows   64.6 / 54.7  68.2  98.5  187
+    //   16 streams,  64 rows   49.9 / 50.7  35.5  49.3  98.1       512 rows   64.6 / 97.6  127   192   370
+    //   64 streams, 128 rows   97.2 / 103   130   193   373
+    const long long tiles = turns_of(c, a, 128) * c.n_streams * c.n_kv;
+    if (tiles > 148) return launch_tc<D, false>(c, a, 1, stream);
+    const long long room = ((long long)c.max_pages << c.page_shift) / (2 * kStep);
+    int ranks = 1;
+    while (ranks < 8 && tiles * ranks * 2 <= (ranks < 4 ? 148 : 74) && ranks < room) ranks *= 2;
+    return launch_tc<D, true>(c, a, ranks, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_cache_attend_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
 {
-    return c.dim == 64 ? launch_tc<64>(c, a, stream) : launch_tc<128>(c, a, stream);
+    return c.dim == 64 ? launch_tc_any<64>(c, a, stream) : launch_tc_any<128>(c, a, stream);
 }
 
 }  // namespace z2
