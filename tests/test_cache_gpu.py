@@ -154,7 +154,8 @@ def test_attend_chunks(z2, cuda, name, heads, kv, dim, page, window):
         _check_attend(z2, c, window=window, gate=max_new != 5, max_new=max_new)
 
 
-@pytest.mark.parametrize("name,heads,kv,dim", [("bf16", 8, 2, 128), ("bf16", 4, 4, 64), ("f32", 4, 2, 128)])
+@pytest.mark.parametrize("name,heads,kv,dim", [("bf16", 8, 2, 128), ("bf16", 4, 4, 64), ("bf16", 4, 2, 24), ("bf16", 6, 3, 104),
+                                               ("bf16", 4, 2, 136), ("f32", 4, 2, 128), ("f32", 3, 1, 72)])
 def test_attend_long_chunks(z2, cuda, name, heads, kv, dim):
     """Several tiles to a stream, longer than the caller says."""
     c = _case(cuda, name, new=(300, 129), cached=(140, 0), heads=heads, kv=kv, dim=dim, page=32, seed=3)
@@ -184,7 +185,7 @@ def test_attend_pages_that_are_none(z2, cuda, name, new):
 
 
 @pytest.mark.parametrize("name", ["bf16", "f32"])
-@pytest.mark.parametrize("new,dim", [(1, 64), (5, 128), (5, 256), (40, 64), (100, 128)])
+@pytest.mark.parametrize("new,dim", [(1, 64), (5, 128), (5, 256), (40, 64), (100, 128), (40, 72), (400, 40)])
 def test_attend_odd_values_in_masked_places(z2, cuda, name, new, dim):
     """NaN and infinities past the last token, on other streams' pages, at later tokens of the chunk, left of the
     window and in slots that hold none: rows that do not see them are as without them; rows that see a NaN value have it."""

@@ -911,7 +911,7 @@ cudaError_t launch_cache_attend(const CacheArgs &c, const AttendArgs &a, bool bf
     if (bf16) {
         // (20 or 32 rows on 64 streams: 90 and 94 us here, 92 there; 48 rows: 111 against 92; on 4
         // streams 21 and 22 us against 25, 48 rows 32 against 25)
-        if (rows > 32 && (c.dim == 64 || c.dim == 128)) return launch_cache_attend_tc(c, a, stream);
+        if (rows > 32 && c.dim <= 128) return launch_cache_attend_tc(c, a, stream);
         if (c.dim > 128) return launch_bf16<256, 3, 4>(c, a, stream);
         return c.dim > 64 ? launch_bf16<128, 2>(c, a, stream) : launch_bf16<64, 4>(c, a, stream);
     }

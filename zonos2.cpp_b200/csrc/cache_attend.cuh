@@ -252,7 +252,7 @@ inline long long tiles_with_rows(const CacheArgs &c, const AttendArgs &a, int ti
 
 }  // namespace
 
-// bf16 heads of 64 or 128 elements, many rows to a key head (cache_attend_tc.cu).
+// bf16 heads of up to 128 elements, many rows to a key head (cache_attend_tc.cu).
 cudaError_t launch_cache_attend_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream);
 int read_and_clear_attend_error(int *value);
 

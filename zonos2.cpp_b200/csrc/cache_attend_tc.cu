@@ -1,5 +1,5 @@
 // cache_attend_tc.cu -- attention of chunks of new tokens over a paged cache on the tcgen05
-// tensor cores (sm_100a): bf16, heads of 64 or 128 elements.
+// tensor cores (sm_100a): bf16, heads of up to 128 elements (as 64 or 128, zeros past their end).
 //
 // A block takes 256 rows -- (token, query head) pairs that share a key head -- as two tiles of
 // 128, and the tokens they see in steps of 128 keys:
@@ -185,6 +185,7 @@ __device__ void add_odd(const CacheArgs &c, int stream, int kvh, int j0, int all
         const __nv_bfloat16 *v = (const __nv_bfloat16 *)c.v + row_on_page(c, p, kvh, j) + col;
 #pragma unroll
         for (int k = 0; k < N; k++) {
+            if (col + k >= c.dim) break;
             const float y = as_f(v[k]);
             if (odd(y)) o[k] = __float_as_uint(__uint_as_float(o[k]) + y);
         }
@@ -279,9 +280,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 4
     for (int i = threadIdx.x; i < kTileRows * (D / 8); i += kTcThreads) {
         const int r = i / (D / 8), p = i % (D / 8), row = row0 + r;
-        const bool in = r < tile_rows;
+        const bool in = r < tile_rows && p * 8 < c.dim;
         const long long at = in ? (long long)(ch.first + row / a.group) * a.q_stride +
-                                      (long long)(kvh * a.group + row % a.group) * D + p * 8
+                                      (long long)(kvh * a.group + row % a.group) * c.dim + p * 8
                                 : 0;
         cp_async16_or_zero(s_q + (r >> 7) * Sh::kTile + (p >> 3) * (128 * 128) + (r & 127) * 128 + (((p & 7) ^ (r & 7)) << 4),
                            (const __nv_bfloat16 *)a.q + at, in);
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const float g = as_f(((const __nv_bfloat16 *)a.gate)[(long long)token * a.gate_stride + h]);
                         f *= 1.0f / (1.0f + expf(-g));
                     }
-                    __nv_bfloat16 *out = (__nv_bfloat16 *)a.out + (long long)token * a.out_stride + (long long)h * D;
+                    __nv_bfloat16 *out = (__nv_bfloat16 *)a.out + (long long)token * a.out_stride + (long long)h * c.dim;
 #pragma unroll 1
                     for (int b = 0; b < D / 32; b++) {
                         uint32_t o[32];
@@ -593,6 +594,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         if (live) {
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
+                                if (32 * b + 8 * k >= c.dim) break;
                                 uint32_t w[4];
 #pragma unroll
                                 for (int e = 0; e < 4; e++)
@@ -608,10 +610,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     } else if (!SPLIT && !dead) {
         // rows that see nothing
-        for (int i = threadIdx.x; i < tile_rows * (D / 8); i += kTcThreads) {
-            const int row = row0 + i / (D / 8);
+        const int pieces = c.dim / 8;
+        for (int i = threadIdx.x; i < tile_rows * pieces; i += kTcThreads) {
+            const int row = row0 + i / pieces;
             *reinterpret_cast<uint4 *>((__nv_bfloat16 *)a.out + (long long)(ch.first + row / a.group) * a.out_stride +
-                                       (long long)(kvh * a.group + row % a.group) * D + i % (D / 8) * 8) =
+                                       (long long)(kvh * a.group + row % a.group) * c.dim + i % pieces * 8) =
                 make_uint4(0, 0, 0, 0);
         }
     }
@@ -763,7 +766,7 @@ cudaError_t launch_tc_any(const CacheArgs &c, const AttendArgs &a, cudaStream_t 
 
 cudaError_t launch_cache_attend_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
 {
-    return c.dim == 64 ? launch_tc_any<64>(c, a, stream) : launch_tc_any<128>(c, a, stream);
+    return c.dim <= 64 ? launch_tc_any<64>(c, a, stream) : launch_tc_any<128>(c, a, stream);
 }
 
 }  // namespace z2
