@@ -65,18 +65,21 @@ struct Ring {
             held |= pages.p[e] >= 0 ? 1u << e : 0u;
         }
         const uint32_t to = stage + row0 * kRow;
-        if (held == (1u << KEYS / 8) - 1 && j0 >= low && j0 + KEYS <= high && c.dim == D &&
+        if (held == (1u << KEYS / 8) - 1 && j0 >= low && j0 + KEYS <= high &&
             (KEYS == 8 || c.page_shift > 3)) {   // a whole group: its rows lie behind each other
-            const char *k = (const char *)((const T *)c.k + base[0]) + lane * 16;
-            const char *v = (const char *)((const T *)c.v + base[0]) + lane * 16;
+            const uint32_t bytes = (uint32_t)c.dim * sizeof(T);   // of a row
+            const uint32_t from = row0 * bytes + piece * 16;
+            const char *k = (const char *)((const T *)c.k + base[0]), *v = (const char *)((const T *)c.v + base[0]);
 #pragma unroll
             for (int i = 0; i < KEYS / kStep; i++)
 #pragma unroll
                 for (int x = 0; x < kAcross; x++) {
                     const int r = i * kStep;   // row0 + r; row0 < kStep
+                    if (piece * 16 + 512 * x >= (int)bytes) break;
                     const uint32_t dst = to + r * kRow + (((piece + 32 * x) ^ ((row0 + r) & 7)) << 4);
-                    cp_async16(dst, k + (i * kAcross + x) * 512);
-                    cp_async16(dst + kHalf, v + (i * kAcross + x) * 512);
+                    const uint32_t at = from + r * bytes + 512 * x;
+                    cp_async16(dst, k + at);
+                    cp_async16(dst + kHalf, v + at);
                 }
             return held;
         }
@@ -394,7 +397,8 @@ __global__ void __launch_bounds__(32 * W)
     const int first_group = low >> 3, groups = high > low ? ((high + 7) >> 3) - first_group : 0;
     const int workers = ranks * W, worker = rank * W + warp;
 
-    constexpr int kCols = D / 32;   // this lane's columns: 32 apart (piece lane / 4 + 8 i for more)
+    // this lane's columns: kRun neighbours of each 32 kRun
+    constexpr int kCols = D / 32, kRun = kCols < 4 ? kCols : 4;
     float m[ROWS], l[ROWS], o[ROWS][kCols];
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
@@ -407,27 +411,32 @@ __global__ void __launch_bounds__(32 * W)
     const int key = lane >> 2, quarter = lane & 3;
     uint32_t saw = 0;   // of this lane's key, a bit to a row
 
+    auto group_at = [&](int it) { return (first_group + worker + it * workers) * 8; };
+    auto look = [&](int it) { return R::look(c, tile.ch.stream, group_at(it), worker + it * workers < groups ? room : 0); };
     uint32_t held_bits = 0;
-    auto fetch = [&](int it) {
-        const int g = worker + it * workers;
-        if (g < groups) {
+    auto fetch = [&](int it, const typename R::Pages &at) {
+        if (worker + it * workers < groups) {
             const int st = it % STAGES;
-            const int j0 = (first_group + g) * 8;
-            const uint32_t held = R::load(c, R::look(c, tile.ch.stream, j0, room), kvh, j0, low, high,
-                                                      ring + st * R::kStage);
+            const uint32_t held = R::load(c, at, kvh, group_at(it), low, high, ring + st * R::kStage);
             held_bits = (held_bits & ~(1u << st)) | held << st;
         }
         cp_async_commit();
     };
+    typename R::Pages pages[STAGES];   // of the first turns, then [0]: of the next one to be fetched
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) fetch(i);
+    for (int i = 0; i < STAGES; i++) pages[i] = look(i);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) fetch(i, pages[i]);
+    pages[0] = pages[STAGES - 1];
     for (int it = 0; worker + it * workers < groups; it++) {
-        fetch(it + STAGES - 1);
+        const typename R::Pages next = look(it + STAGES);
+        fetch(it + STAGES - 1, pages[0]);
+        pages[0] = next;
         cp_async_wait<STAGES - 1>();
         __syncwarp();
         const int st = it % STAGES;
         const uint32_t keys = ring + st * R::kStage, values = keys + R::kHalf;
-        const int j0 = (first_group + worker + it * workers) * 8;
+        const int j0 = group_at(it);
         const bool held = held_bits >> st & 1u;
         float x[ROWS];
 #pragma unroll
@@ -450,25 +459,46 @@ __global__ void __launch_bounds__(32 * W)
             const int pos = position_of(tile.ch, a.group, tile.row0 + min(r, tile.rows - 1));
             return held && j <= pos && j < high && (a.window <= 0 || j > pos - a.window);
         };
+        float top[ROWS];
+        bool same = true;
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
             x[r] += __shfl_xor_sync(kFull, x[r], 1);
             x[r] += __shfl_xor_sync(kFull, x[r], 2);
             x[r] *= factor;
-            const bool in = !partial || sees(r, j0 + key);
-            float most = in ? x[r] : -INFINITY;
-            most = fmaxf(most, __shfl_xor_sync(kFull, most, 4));
-            most = fmaxf(most, __shfl_xor_sync(kFull, most, 8));
-            most = fmaxf(most, __shfl_xor_sync(kFull, most, 16));
-            if (most > m[r]) {   // the same in every lane
-                const float keep = m[r] == -INFINITY ? 0.0f : exp2f(m[r] - most);
+        }
+        if (partial) {
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                const bool in = sees(r, j0 + key);
+                if (!in) x[r] = -INFINITY;
+                saw |= in ? 1u << r : 0u;
+            }
+        } else {
+            saw = ~0u;
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            top[r] = x[r];
+            top[r] = fmaxf(top[r], __shfl_xor_sync(kFull, top[r], 4));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(kFull, top[r], 8));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(kFull, top[r], 16));
+            top[r] = fmaxf(top[r], m[r]);   // the same in every lane
+            same = same && top[r] == m[r];
+        }
+        if (!__all_sync(kFull, same)) {
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                const float keep = m[r] == -INFINITY ? 0.0f : exp2_fast(m[r] - top[r]);
                 l[r] *= keep;
 #pragma unroll
                 for (int i = 0; i < kCols; i++) o[r][i] *= keep;
-                m[r] = most;
+                m[r] = top[r];
             }
-            const float w = in ? exp2f(x[r] - (m[r] == -INFINITY ? 0.0f : m[r])) : 0.0f;
-            saw |= in ? 1u << r : 0u;
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            const float w = exp2_fast(x[r] - (m[r] == -INFINITY ? 0.0f : m[r]));   // 0 where not seen
             l[r] += w;
             if (quarter == 0) s_w[warp][key][r] = w;
         }
@@ -477,20 +507,40 @@ __global__ void __launch_bounds__(32 * W)
         for (int k = 0; k < 8; k++) {
             float v[kCols];
 #pragma unroll
-            for (int i = 0; i < kCols; i++) {
-                const int col = lane + 32 * i;
-                asm volatile("ld.shared.f32 %0, [%1];"
-                             : "=f"(v[i])
-                             : "r"(values + k * R::kRow + (((col >> 2) ^ k) << 4) + 4 * (col & 3)));
+            for (int i = 0; i < kCols; i += kRun) {
+                const int col = lane * kRun + 32 * i;
+                const uint32_t at = values + k * R::kRow + (((col >> 2) ^ k) << 4) + 4 * (col & 3);
+                if (kRun == 4)
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[(i + 2) % kCols]), "=f"(v[(i + 3) % kCols])
+                                 : "r"(at));
+                else
+                    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[i]), "=f"(v[i + 1]) : "r"(at));
+            }
+            float w[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; r += 4) {
+                const float4 w4 = *reinterpret_cast<const float4 *>(&s_w[warp][k][r]);
+                w[r] = w4.x;
+                w[r + 1] = w4.y;
+                w[r + 2] = w4.z;
+                w[r + 3] = w4.w;
+            }
+            if (partial) {
+                // a value that the row does not see has no part in it, not even as 0 times it
+#pragma unroll
+                for (int i = 0; i < kCols; i++) {
+                    if (!odd(v[i])) continue;
+#pragma unroll
+                    for (int r = 0; r < ROWS; r++)
+                        if (sees(r, j0 + k)) o[r][i] += v[i];
+                    v[i] = 0.0f;
+                }
             }
 #pragma unroll
-            for (int r = 0; r < ROWS; r++) {
-                const float w = s_w[warp][k][r];
+            for (int r = 0; r < ROWS; r++)
 #pragma unroll
-                for (int i = 0; i < kCols; i++)
-                    // a value that the row does not see has no part in it, not even as 0 times it
-                    if (!partial || !odd(v[i]) || sees(r, j0 + k)) o[r][i] = fmaf(w, v[i], o[r][i]);
-            }
+                for (int i = 0; i < kCols; i++) o[r][i] = fmaf(w[r], v[i], o[r][i]);
         }
         __syncwarp();
     }
@@ -505,8 +555,10 @@ __global__ void __launch_bounds__(32 * W)
         const bool any = __any_sync(kFull, saw >> r & 1u);
         if (lane == 0) s_ml[warp * ROWS + r] = make_float2(m[r] == -INFINITY && any ? kLowest : m[r], l[r]);
 #pragma unroll
-        for (int i = 0; i < kCols; i++)
-            part[(warp * ROWS + r) * D + part_piece(r, (lane + 32 * i) >> 2) * 4 + (lane & 3)] = o[r][i];
+        for (int i = 0; i < kCols; i++) {
+            const int col = lane * kRun + 32 * (i / kRun * kRun) + i % kRun;
+            part[(warp * ROWS + r) * D + part_piece(r, col >> 2) * 4 + (col & 3)] = o[r][i];
+        }
     }
     join_and_store<float, D, ROWS, W, 32 * W>(c, a, tile, kvh, part, s_ml, s_weight, s_total, s_gate, ranks, rank);
 }
@@ -881,13 +933,12 @@ cudaError_t launch_bf16(const CacheArgs &c, const AttendArgs &a, cudaStream_t st
     return launch_bf16<D, STAGES, 4>(c, a, stream);
 }
 
-template <int D, int ROWS, int STAGES>
+template <int D, int ROWS, int STAGES, int W = 4>
 cudaError_t launch_f32(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
 {
     static std::mutex mu;
     static bool ready[64] = {false};
     typedef Ring<float, D, 8> R;
-    constexpr int W = 4;
     const size_t rings = W * STAGES * R::kStage, parts = (size_t)W * ROWS * D * 4;
     const size_t smem = (rings > parts ? rings : parts) + ROWS * R::kRow;
     return launch_rows(attend_rows_f32_kernel<D, ROWS, STAGES, W>, smem, ROWS, W, 32 * W, c, a, 8, mu, ready, stream);
@@ -912,13 +963,13 @@ cudaError_t launch_cache_attend(const CacheArgs &c, const AttendArgs &a, bool bf
         // (20 or 32 rows on 64 streams: 90 and 94 us here, 92 there; 48 rows: 111 against 92; on 4
         // streams 21 and 22 us against 25, 48 rows 32 against 25)
         if (rows > 32 && c.dim <= 128) return launch_cache_attend_tc(c, a, stream);
-        if (c.dim > 128) return launch_bf16<256, 3, 4>(c, a, stream);
+        if (c.dim > 128) return launch_bf16<256, 2, 6>(c, a, stream);
         return c.dim > 64 ? launch_bf16<128, 2>(c, a, stream) : launch_bf16<64, 4>(c, a, stream);
     }
     if (rows > 16)
         return c.dim > 128 ? launch_tile_f32<256>(c, a, stream)
                            : c.dim > 64 ? launch_tile_f32<128>(c, a, stream) : launch_tile_f32<64>(c, a, stream);
-    if (c.dim > 128) return rows > 4 ? launch_f32<256, 8, 3>(c, a, stream) : launch_f32<256, 4, 3>(c, a, stream);
+    if (c.dim > 128) return rows > 4 ? launch_f32<256, 8, 2, 6>(c, a, stream) : launch_f32<256, 4, 2, 6>(c, a, stream);
     if (c.dim > 64) return rows > 4 ? launch_f32<128, 16, 3>(c, a, stream) : launch_f32<128, 4, 3>(c, a, stream);
     return rows > 4 ? launch_f32<64, 16, 4>(c, a, stream) : launch_f32<64, 4, 4>(c, a, stream);
 }
