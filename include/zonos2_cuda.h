@@ -267,7 +267,8 @@ int zonos2cu_head_i8(const int8_t *W_dev, const float *w_scale_dev, int rows_per
  *                [q_start[0], q_start[n_streams]) are not read and stay as they are.
  * k_dev and v_dev are 16-byte aligned, head_dim is a multiple of 8 up to
  * ZONOS2CU_MAX_HEAD_DIM, page_size a power of two from 8 to ZONOS2CU_MAX_PAGE, page_stride a
- * multiple of 8 (ZONOS2CU_EUNSUPPORTED elsewhere). */
+ * multiple of 8; of a stream the first 2^31 - 256 tokens count, and rows times query heads
+ * per key head stay below 2^30 (ZONOS2CU_EUNSUPPORTED elsewhere). */
 #define ZONOS2CU_MAX_HEAD_DIM 256
 #define ZONOS2CU_MAX_PAGE 4096
 typedef struct {
@@ -308,8 +309,8 @@ int zonos2cu_cache_append(const zonos2cu_cache *cache, int rows, int n_heads, co
  * (attention_forward's scores, softmax, values and head gate of src/zonos2_model.cpp, for a batch).
  * Query head h of a token at position p, with key head h / (n_heads / n_kv_heads):
  *     o = g * sum_j softmax_j(scale * q . k_j) v_j
- * over the stream's tokens j <= p (j > p - window with window > 0) that lie on a page;
- * zero where there is none.  What lies elsewhere, a NaN among it, has no part in it.
+ * over the stream's tokens j <= p (j > p - window with 0 < window < 2^30) that lie on a
+ * page; zero where there is none.  What lies elsewhere, a NaN among it, has no part in it.
  * g = 1 / (1 + exp(-gate)) (1 without gates).  Scores, sums and softmax are f32; with a
  * bf16 cache the softmax's weights are rounded to bf16 before they meet the values (each
  * is at most 1 beside the row's largest; their sum is taken unrounded).

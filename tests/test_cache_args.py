@@ -74,6 +74,10 @@ def test_attend_unsupported(z2, bad):
     assert _attend(z2, **bad) == z2.EUNSUPPORTED
 
 
+def test_too_many_rows(z2):
+    assert _attend(z2, rows=1 << 28) == z2.EUNSUPPORTED and _append(z2, rows=1 << 28) == z2.EUNSUPPORTED
+
+
 def test_no_cache(z2):
     L = z2.lib()
     assert L.zonos2cu_cache_append(None, 5, 8, P, 512, P, 128, P, 128, P, P, 1e-5, P, 64, 0, 2 * P, 512, None) == z2.EINVAL

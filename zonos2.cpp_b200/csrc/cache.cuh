@@ -52,6 +52,9 @@ cudaError_t launch_cache_attend(const CacheArgs &c, const AttendArgs &a, bool bf
 
 namespace {
 
+// (The device arrays are read by plain loads: under programmatic dependent launch a kernel may have
+// started while the one before it still wrote them, which read-only loads do not allow for.)
+
 // One stream's part of a call: its token rows and where they stand.  Whatever the device
 // arrays hold, rows stay inside the call's buffers and len is not negative.
 struct Chunk {
@@ -64,23 +67,26 @@ __device__ __forceinline__ Chunk chunk_of(const CacheArgs &c, int s)
 {
     Chunk k;
     k.stream = s;
-    k.first = min(max(__ldg(c.q_start + s), 0), c.rows);
-    k.n = min(max(__ldg(c.q_start + s + 1), k.first), c.rows) - k.first;
-    k.len = max(__ldg(c.kv_len + s), 0);
+    k.first = min(max(c.q_start[s], 0), c.rows);
+    k.n = min(max(c.q_start[s + 1], k.first), c.rows) - k.first;
+    k.len = max(c.kv_len[s], 0);
     return k;
 }
 
-// Tokens of a stream that its table has room for.
+// Tokens of a stream that its table has room for (and positions, to a step past the last, room in
+// 32 bits).
+constexpr int kMostTokens = 0x7fffff00;
+
 __device__ __forceinline__ int room_of(const CacheArgs &c)
 {
     const long long room = (long long)c.max_pages << c.page_shift;
-    return room > 0x7fffffff ? 0x7fffffff : (int)room;
+    return room > kMostTokens ? kMostTokens : (int)room;
 }
 
 // The page of a stream's token j (0 <= j < room), or -1 where there is none.
 __device__ __forceinline__ int page_of(const CacheArgs &c, int s, int j)
 {
-    const int p = __ldg(c.table + (long long)s * c.max_pages + (j >> c.page_shift));
+    const int p = c.table[(long long)s * c.max_pages + (j >> c.page_shift)];
     return p >= 0 && p < c.n_pages ? p : -1;
 }
 

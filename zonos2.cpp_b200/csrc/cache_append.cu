@@ -72,14 +72,14 @@ __device__ __forceinline__ Chunk chunk_with(const CacheArgs &c, int row)
     int low = 0, many = c.n_streams;   // the answer lies in [low, low + many), if it lies anywhere
     while (many > 32) {
         const int step = (many + 31) / 32;
-        const bool before = lane * step < many && __ldg(c.q_start + low + lane * step) <= row;
+        const bool before = lane * step < many && c.q_start[low + lane * step] <= row;
         const int last = 31 - __clz(__ballot_sync(kFull, before) | 1u);
         low += last * step;
         many = min(step, c.n_streams - low);
     }
     const bool in = lane < many;
-    const int start = in ? __ldg(c.q_start + low + lane) : 0, next = in ? __ldg(c.q_start + low + lane + 1) : 0;
-    const int len = in ? __ldg(c.kv_len + low + lane) : 0;
+    const int start = in ? c.q_start[low + lane] : 0, next = in ? c.q_start[low + lane + 1] : 0;
+    const int len = in ? c.kv_len[low + lane] : 0;
     const unsigned votes = __ballot_sync(kFull, in && start <= row);
     const int last = 31 - __clz(votes | 1u);
     Chunk k;
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kAppendThreads)
         const int e = LANE_PAIRS ? e0 + 2 * i : e0 + i;
         if (active && e < a.rot) {
             const int f = LANE_PAIRS ? e >> 1 : (e < half ? e : e - half);
-            const double turns = (double)pos * ((double)__ldg(a.freq + f) * 0.15915494309189533577);
+            const double turns = (double)pos * ((double)a.freq[f] * 0.15915494309189533577);
             sincospif(2.0f * (float)(turns - rint(turns)), &sn[i], &cs[i]);
             if (!LANE_PAIRS && e < half) sn[i] = -sn[i];   // a cos - b sin; b cos + a sin
         }
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kAppendThreads)
         float w[8];
         if (!COPY) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) w[i] = a.norm && weight && active ? __ldg(weight + e0 + i) : 1.0f;
+            for (int i = 0; i < 8; i++) w[i] = a.norm && weight && active ? weight[e0 + i] : 1.0f;
         }
         for (; round < end; round += parts * kAhead) {
             Eight<T> raws[kAhead];
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kAppendThreads)
                             if (!LANE_PAIRS) {
                                 const int e = e0 + i;
                                 if (on && e < a.rot)
-                                    other[i] *= r * (weight ? __ldg(weight + (e < half ? e + half : e - half)) : 1.0f);
+                                    other[i] *= r * (weight ? weight[e < half ? e + half : e - half] : 1.0f);
                             }
                         }
                     }

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(32 * W, D > 128 || W > 4 ? 1 : 3)
     // the rings, then the queries; at the end the parts take the rings' place
     __shared__ float2 s_ml[W * ROWS];
     __shared__ float s_weight[kMostRanks * ROWS], s_total[ROWS], s_gate[ROWS];
-    __shared__ int4 s_found;
+    __shared__ int s_found;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(32 * W)
     __shared__ float2 s_ml[W * ROWS];
     __shared__ float s_weight[kMostRanks * ROWS], s_total[ROWS], s_gate[ROWS];
     __shared__ __align__(16) float s_w[W][8][ROWS];   // a group's weights
-    __shared__ int4 s_found;
+    __shared__ int s_found;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
     __shared__ float2 s_ml[ROWS];
     __shared__ float s_weight[kMostRanks * ROWS], s_total[ROWS], s_gate[ROWS];
     __shared__ int s_held[2][4];
-    __shared__ int4 s_found;
+    __shared__ int s_found;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;

@@ -85,27 +85,24 @@ struct Tile {
     int row0, rows;    // rows == 0: none
 };
 
-__device__ Tile find_tile(const CacheArgs &c, int group, int tile_rows, long long t, int4 *s_found)
+__device__ Tile find_tile(const CacheArgs &c, int group, int tile_rows, long long t, int *s_found)
 {
-    if (threadIdx.x == 0) *s_found = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 0) *s_found = c.n_streams;
     __syncthreads();
-    auto number = [&](int s, int first) { return (long long)first * group / tile_rows + s; };
-    for (int s = threadIdx.x; s < c.n_streams; s += blockDim.x) {
-        const Chunk ch = chunk_of(c, s);
-        const int end = min(max(__ldg(c.q_start + s + 1), 0), c.rows);
-        if (number(s, ch.first) <= t && t < number(s + 1, end))   // one stream's, as the starts rise
-            *s_found = make_int4(s, ch.first, ch.n, ch.len);
-    }
+    auto number = [&](int s) {
+        const int first = min(max(c.q_start[s], 0), c.rows);
+        return (long long)first * group / tile_rows + s;
+    };
+    for (int s = threadIdx.x; s < c.n_streams; s += blockDim.x)
+        // one stream's, as the starts rise; if they do not, the same one in every block
+        if (number(s) <= t && t < number(s + 1)) atomicMin(s_found, s);
     __syncthreads();
-    const int4 f = *s_found;
+    const int s = *s_found;
     Tile tile;
     tile.rows = 0;
-    if (f.x < 0) return tile;
-    tile.ch.stream = f.x;
-    tile.ch.first = f.y;
-    tile.ch.n = f.z;
-    tile.ch.len = f.w;
-    const long long first = (t - number(f.x, f.y)) * tile_rows, all = (long long)f.z * group;
+    if (s >= c.n_streams) return tile;
+    tile.ch = chunk_of(c, s);
+    const long long first = (t - number(s)) * tile_rows, all = (long long)tile.ch.n * group;
     if (first < all) {
         tile.row0 = (int)first;
         tile.rows = (int)(all - first < tile_rows ? all - first : tile_rows);

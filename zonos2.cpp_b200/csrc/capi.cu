@@ -523,6 +523,8 @@ int check_cache(const zonos2cu_cache *c, int rows, int n_heads, z2::CacheArgs *o
     if (c->n_kv_heads > 4096 || n_heads > 65535) return ZONOS2CU_EUNSUPPORTED;
     if (c->page_stride < (long long)c->n_kv_heads * c->page_size * c->head_dim) return ZONOS2CU_EINVAL;
     if (n_heads % c->n_kv_heads) return ZONOS2CU_EINVAL;
+    // rows of a key head (tokens x its query heads) are counted in 32 bits
+    if ((long long)rows * (n_heads / c->n_kv_heads) > 0x3fffffff) return ZONOS2CU_EUNSUPPORTED;
     if (rows > 0 && c->n_streams > 0) {
         if (!c->k_dev || !c->v_dev || !c->table_dev || !c->kv_len_dev || !c->q_start_dev)
             return ZONOS2CU_EINVAL;
@@ -595,6 +597,7 @@ int zonos2cu_cache_attend(const zonos2cu_cache *cache, int rows, int n_heads, co
         (rc = check_token_rows(out_dev, out_stride, width, bytes)))
         return rc;
     if (q_dev == out_dev || (uintptr_t)gate_dev % bytes) return ZONOS2CU_EINVAL;
+    if (window < 0 || window >= 1 << 30) window = 0;   // no stream is longer than twice that
     const z2::AttendArgs a{q_dev, q_stride, n_heads, n_heads / c.n_kv, scale, window, gate_dev,
                            gate_stride, max_new, out_dev, out_stride};
     Z2_CK(z2::launch_cache_attend(c, a, cache->dtype == ZONOS2CU_BF16, (cudaStream_t)stream));

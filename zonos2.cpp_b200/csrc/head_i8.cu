@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             tile_at(tile, b0, c, v0);
             const int v = v0 + row;
             const bool live = v < args.vocab;
-            const float ws = live ? __ldg(args.w_scale + (long long)c * args.rows_per_cb + v) : 0.0f;
+            const float ws = live ? args.w_scale[(long long)c * args.rows_per_cb + v] : 0.0f;
             const int cols = min(args.nb, args.batch - b0);   // hidden rows of the tile
             // columns [from, to) in steps of 16
             const int each = (args.nb / 16 + kEpi / 4 - 1) / (kEpi / 4) * 16;
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 float l[16];
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                    const float4 s = __ldg(scale + j / 4);
+                    const float4 s = scale[j / 4];
                     l[j] = (float)(int)r[j] * s.x * ws;
                     l[j + 1] = (float)(int)r[j + 1] * s.y * ws;
                     l[j + 2] = (float)(int)r[j + 2] * s.z * ws;
