@@ -18,13 +18,17 @@ def _rounded(x):
         most = Fraction(float(np.abs(row).max()))
         if most == 0:
             continue
-        q[r] = [round(127 * Fraction(float(v)) / most) for v in row]
+        if r < 30 or r % 100 == 0:
+            q[r] = [round(127 * Fraction(float(v)) / most) for v in row]
+        else:   # (in 64 bits: no random row has a tie that they would not show)
+            q[r] = np.rint(127 * row.astype(np.float64) / float(most))
         scale[r] = float(most / 127)
     return q, scale
 
 
 @pytest.mark.parametrize("name", ["bf16", "f32"])
-@pytest.mark.parametrize("rows,dim,pad", [(1, 16, 0), (7, 33, 0), (5, 130, 3), (3, 1024, 8), (2, 6001, 0), (2, 8192, 16)])
+@pytest.mark.parametrize("rows,dim,pad", [(1, 16, 0), (7, 33, 0), (5, 130, 3), (3, 1024, 8), (2, 6001, 0), (2, 8192, 16), (1300, 40, 0),
+                                          (1185, 2600, 8)])
 def test_quantize_rows(z2, cuda, name, rows, dim, pad):
     import torch
     t = torch.bfloat16 if name == "bf16" else torch.float32
