@@ -283,7 +283,7 @@ typedef struct {
 } zonos2cu_cache;
 
 /* The new tokens' queries and keys normalised and rotated, their keys and values written to
- * the pages (attention_forward's QK-norm, rotation and cache write of src/zonos2_model.cpp, for a batch).
+ * the pages (the QK-norm, rotation and cache write of the attention, src/zonos2_model.cpp:221, for a batch).
  * Per token at position p and per head:
  *     x' = x * weight / sqrt(mean(x^2) + eps)      (eps >= 0; x' = x below 0)
  *     (a, b) -> (a cos(p f) - b sin(p f), b cos(p f) + a sin(p f))
@@ -306,7 +306,7 @@ int zonos2cu_cache_append(const zonos2cu_cache *cache, int rows, int n_heads, co
                           int rot_halves, void *q_out_dev, long long q_out_stride, void *stream);
 
 /* Attention of the new tokens over the pages, after zonos2cu_cache_append on the same stream
- * (attention_forward's scores, softmax, values and head gate of src/zonos2_model.cpp, for a batch).
+ * (the attention's scores, softmax, values and head gate, src/zonos2_model.cpp:221, for a batch).
  * Query head h of a token at position p, with key head h / (n_heads / n_kv_heads):
  *     o = g * sum_j softmax_j(scale * q . k_j) v_j
  * over the stream's tokens j <= p (j > p - window with 0 < window < 2^30) that lie on a

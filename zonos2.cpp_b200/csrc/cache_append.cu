@@ -10,9 +10,13 @@
 // and only then rounded to f32 for the sine: f32 alone would lose every digit of a far
 // position's angle.  Each result is rounded once.
 //
-// Bound: memory for prompts (every element is read once and written once), launch latency for
-// a few tokens.  A warp takes a token's heads one after another with the angles' sines kept, or
-// for few tokens one round of them, the token's heads shared out over warps.
+// A warp takes a token's heads one after another with the angles' sines kept, or for few tokens one
+// round of them, the token's heads shared out over warps.
+//
+// Bound: memory for prompts (every element is read once and written once) and beside it the issue
+// slots; launch latency for a few tokens.  8200 tokens of 16 + 2 x 4 bf16 heads of 128 (101 MB): 26.6 us,
+// 3.8 TB/s, the issue slots 61 % taken; 34 us with one loop over all heads, which chose each head's
+// address and kind again.  One token: 3.2 us in a captured stream of them, 9.3 us as called from Python.
 #include <type_traits>
 
 #include "cache.cuh"

@@ -13,8 +13,12 @@
 // shared memory: the result depends on the sizes alone, and no scratch memory is needed.
 //
 // Bound: memory for one token or a few per stream (keys and values are read once), so each warp
-// has a ring of groups of its own in flight by asynchronous copies and no block-wide barrier
-// before the join.
+// has a ring of groups of its own in flight by asynchronous copies, the pages looked up a turn
+// ahead, and no block-wide barrier before the join.  16 + 4 bf16 heads of 128:
+//   256 streams of 256 to 4096 tokens, one new (1.14 GB)       187 us, 6.1 TB/s
+//   64 streams of 64 to 6144, up to five new (408 MB)           78 us, 5.2 TB/s
+//   1 stream of 6050, one new (12.4 MB)                         10 us: a chain of latencies (1.5 the
+//       tile, 2.5 its pages and queries, 3.6 the keys and the work on them, 4.5 the join)
 #include <math.h>
 
 #include <mutex>
@@ -348,7 +352,9 @@ __global__ void __launch_bounds__(32 * W, D > 128 || W > 4 ? 1 : 3)
 
 // ---- f32, on the FMA pipe ----------------------------------------------------
 // ROWS rows to a tile, groups of 8 keys.  A lane takes a quarter of a key's elements for
-// the scores of all rows (key lane / 4), then D / 32 of the output's columns.
+// the scores of all rows (key lane / 4), then D / 32 of the output's columns.  8 + 2 heads of 128, 64
+// streams of 1500 tokens, one new (197 MB): 75 us, 2.6 TB/s; 175 us with each group's page looked up
+// in its turn and the values read four bytes at a time.
 template <int D, int ROWS, int STAGES, int W>
 __global__ void __launch_bounds__(32 * W)
     attend_rows_f32_kernel(const CacheArgs c, const AttendArgs a, int ranks)
@@ -568,7 +574,8 @@ __global__ void __launch_bounds__(32 * W)
 // products run on the tensor cores in tf32 (11 bits of a significand), each operand as the sum
 // of two such parts, hi = its upper bits and lo = the rest:
 //     a b = hi_a hi_b + hi_a lo_b + lo_a hi_b + (2^-22 of it)
-// which leaves errors of the size of f32's own in a sum of 128 products.  The tensor cores add
+// (6 streams, up to 333 new tokens of 16 + 4 heads of 128, a window of 512: 135 us, 2150 us by the
+// kernel above), which leaves errors of the size of f32's own in a sum of 128 products.  The tensor cores add
 // to an accumulator by truncation, a bias that grows with the number of additions: the upper
 // parts' products, the mixed ones (2^-11 of them, and so their bias) and each 64 elements of the
 // depth or 32 keys have accumulators of their own, which are added with rounding to nearest (with
