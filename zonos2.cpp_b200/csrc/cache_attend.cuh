@@ -69,11 +69,14 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Bits 15 and 31: an exponent of ones in the lower and the upper bf16 (one more carries out of it).
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
+
 __device__ __forceinline__ bool odd(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
 // A NaN or an infinity among the two bf16 values of a word.
 __device__ __forceinline__ bool odd2(uint32_t w)
 {
-    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+    return (odd_bits(w) & 0x80008000u) != 0;
 }
 
 // The tile of this block: rows [row0, row0 + rows) of stream chunk ch, counted in (token, head

@@ -467,13 +467,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tmem_landed(x[piece & 1]);
                     };
                     auto mask = [&](int piece) {
-                        const int begin = from - j0 - 32 * piece, end = to - j0 - 32 * piece;
+                        const int begin = max(0, min(32, from - j0 - 32 * piece)), end = max(0, min(32, to - j0 - 32 * piece));
+                        // the runs' bits to bytes: bit e comes to 8 e
+                        uint32_t in = (((held >> (4 * piece) & 15u) * 0x00204081u) & 0x01010101u) * 255u;
+                        in &= (uint32_t)((1ull << end) - (1ull << min(begin, end)));
 #pragma unroll
-                        for (int k = 0; k < 32; k++) {
-                            const bool in = k >= begin && k < end && (held >> (4 * piece + (k >> 3)) & 1u);
-                            if (!in) x[piece & 1][k] = 0xff800000u;
-                            saw |= in;
-                        }
+                        for (int k = 0; k < 32; k++)
+                            if (!(in >> k & 1u)) x[piece & 1][k] = 0xff800000u;
+                        saw |= in != 0;
                     };
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     start(0);
@@ -495,14 +496,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         ok = __all_sync(kFull, mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u));
                         if (!ok) break;
                         const uint32_t values = s_kv + (uint32_t)(t % kSlots) * Sh::kTile;
-                        for (int k = r; k < (int)Sh::kTile / 16; k += scanners) {
-                            uint32_t w[4];
+                        uint32_t w[4], any = 0;
+                        auto piece_at = [&](int k) {
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                                          : "r"(values + k * 16));
-                            if (odd2(w[0]) || odd2(w[1]) || odd2(w[2]) || odd2(w[3])) {
-                                s_odd = 1;   // ahead of the zeros that the other tile's threads may find
-                                __threadfence_block();
+                        };
+#pragma unroll 4
+                        for (int k = r; k < (int)Sh::kTile / 16; k += scanners) {
+                            piece_at(k);
+                            any |= odd_bits(w[0]) | odd_bits(w[1]) | odd_bits(w[2]) | odd_bits(w[3]);
+                        }
+                        if (any & 0x80008000u) {
+                            s_odd = 1;   // ahead of the zeros that the other tile's threads may find
+                            __threadfence_block();
+#pragma unroll 1
+                            for (int k = r; k < (int)Sh::kTile / 16; k += scanners) {
+                                piece_at(k);
 #pragma unroll
                                 for (int e = 0; e < 4; e++) {
                                     if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
