@@ -226,6 +226,34 @@ def test_attend_odd_values_in_masked_places(z2, cuda, name, new, dim):
             assert torch.isfinite(last[:, rest]).all()
 
 
+@pytest.mark.parametrize("name,new,heads", [("bf16", 1, 4), ("bf16", 40, 4), ("bf16", 300, 4), ("f32", 1, 4), ("f32", 3, 2), ("f32", 40, 4)])
+def test_last_positions(z2, cuda, name, new, heads):
+    """The last tokens that a stream can have, 2^31 - 256 of them, all others on no page: as the same tokens on a
+    stream's first page."""
+    import torch
+    page, last = 4096, 2 ** 31 - 256
+    c = _case(cuda, name, new=(new,), cached=(page - 256 - new,), heads=heads, kv=2, dim=64, page=page, seed=new)
+    c["table"] = c["table"][:, :1]
+    host = R.Cache(c["k"], c["v"], c["table"], c["kv_len"], c["q_start"])
+    want, tol = R.attend(host, c["rows"], c["q"].cpu(), c["out"], None, 40, c["gate"].cpu())
+    table = torch.full((1, 2 ** 31 // page), -1, dtype=torch.int32)
+    table[0, -1] = int(c["table"][0, 0])
+    c["table"], c["kv_len"] = table.to(cuda), torch.tensor([last], dtype=torch.int32).to(cuda)
+    for max_new in (0, new):
+        c["out"].fill_(7.0)
+        z2.cache_attend(_cache(z2, c), c["q"], c["out"], window=40, gate=c["gate"], max_new=max_new)
+        _near(c["out"], want, tol)
+    freq = (10000.0 ** (-torch.arange(32) / 32) / 8).float()
+    host = R.Cache(c["k"], c["v"], c["table"], c["kv_len"], c["q_start"])
+    want, tol, keys, k_tol, values = R.append(host, new, c["q"].cpu(), c["new_k"].cpu(), c["new_v"].cpu(), None, None, 1e-5,
+                                              freq, False)
+    z2.cache_append(_cache(z2, c), c["q"], c["new_k"], c["new_v"], c["out"], freq=freq.to(cuda))
+    _near(c["out"], want, tol)
+    _near(c["k"], keys, k_tol)
+    assert torch.equal(c["v"].cpu(), values)
+    assert z2.device_error() == 0
+
+
 @pytest.mark.parametrize("name", ["bf16", "f32"])
 @pytest.mark.parametrize("new", [1, 4, 50])
 def test_attend_large_scores(z2, cuda, name, new):

@@ -39,15 +39,16 @@ struct Ring {
     static constexpr int kStage = 2 * kHalf;
     static constexpr int kPieces = kRow / 16;
 
-    // The pages of a group's runs of eight keys.
+    // The pages of a group's runs of eight keys.  (on: the group is one; j0 of others, past the last,
+    // may have left 32 bits.)
     struct Pages {
         int p[KEYS / 8];
     };
-    __device__ static Pages look(const CacheArgs &c, int s, int j0, int room)
+    __device__ static Pages look(const CacheArgs &c, int s, int j0, int room, bool on)
     {
         Pages pages;
 #pragma unroll
-        for (int e = 0; e < KEYS / 8; e++) pages.p[e] = j0 + 8 * e < room ? page_of(c, s, j0 + 8 * e) : -1;
+        for (int e = 0; e < KEYS / 8; e++) pages.p[e] = on && j0 + 8 * e < room ? page_of(c, s, j0 + 8 * e) : -1;
         return pages;
     }
 
@@ -137,8 +138,8 @@ __global__ void __launch_bounds__(32 * W, D > 128 || W > 4 ? 1 : 3)
     const int sees_all_from = a.window > 0 ? max(0, pos_last - a.window + 1) : 0;   // .. to pos_first
     const int first_group = low >> 4, groups = high > low ? ((high + 15) >> 4) - first_group : 0;
     const int workers = ranks * W, worker = rank * W + warp;
-    auto group_at = [&](int it) { return (first_group + worker + it * workers) * 16; };
-    auto look = [&](int it) { return R::look(c, tile.ch.stream, group_at(it), worker + it * workers < groups ? room : 0); };
+    auto group_at = [&](int it) { return (int)((uint32_t)(first_group + worker + it * workers) * 16u); };
+    auto look = [&](int it) { return R::look(c, tile.ch.stream, group_at(it), room, worker + it * workers < groups); };
     typename R::Pages pages[STAGES];   // of the first turns, then [0]: of the next one to be fetched
 #pragma unroll
     for (int i = 0; i < STAGES; i++) pages[i] = look(i);
@@ -417,8 +418,8 @@ __global__ void __launch_bounds__(32 * W)
     const int key = lane >> 2, quarter = lane & 3;
     uint32_t saw = 0;   // of this lane's key, a bit to a row
 
-    auto group_at = [&](int it) { return (first_group + worker + it * workers) * 8; };
-    auto look = [&](int it) { return R::look(c, tile.ch.stream, group_at(it), worker + it * workers < groups ? room : 0); };
+    auto group_at = [&](int it) { return (int)((uint32_t)(first_group + worker + it * workers) * 8u); };
+    auto look = [&](int it) { return R::look(c, tile.ch.stream, group_at(it), room, worker + it * workers < groups); };
     uint32_t held_bits = 0;
     auto fetch = [&](int it, const typename R::Pages &at) {
         if (worker + it * workers < groups) {
@@ -644,7 +645,7 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
     const int sees_all_from = a.window > 0 ? max(0, pos_last - a.window + 1) : 0;   // .. to pos_first
     const int first_step = low / kTileKeys, steps = high > low ? (high + kTileKeys - 1) / kTileKeys - first_step : 0;
     const int mine = steps > rank ? (steps - rank + ranks - 1) / ranks : 0;   // this rank's steps
-    auto step_at = [&](int it) { return (first_step + rank + it * ranks) * kTileKeys; };
+    auto step_at = [&](int it) { return (int)((uint32_t)(first_step + rank + it * ranks) * kTileKeys); };
     // a warp loads the step's run of eight keys that has its number
     auto look = [&](int it) {
         const int j = step_at(it) + 8 * warp;

@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int room = room_of(c);
                 // the pages of a step's runs of eight tokens, one step ahead; bit 8 e: run e is held
                 auto look = [&](int i) {
-                    const int j = (step0 + i * ranks) * kStep + 8 * lane;
+                    const int j = (int)((uint32_t)(step0 + i * ranks) * kStep) + 8 * lane;
                     return lane < 16 && (i >= steps || (j < room && page_of(c, ch.stream, j) >= 0));
                 };
                 bool ok = true;
