@@ -226,6 +226,39 @@ def test_attend_odd_values_in_masked_places(z2, cuda, name, new, dim):
             assert torch.isfinite(last[:, rest]).all()
 
 
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("new,dim", [(1, 64), (3, 128), (5, 256), (40, 64), (40, 128), (90, 256), (400, 128), (70, 40)])
+def test_attend_seen_infinities(z2, cuda, name, new, dim):
+    """Tokens that every row sees: a key whose score is -inf has no weight, an infinite value makes its element infinite,
+    and a row's infinite query makes that row alone a NaN."""
+    import torch
+    c = _case(cuda, name, new=(new,), cached=(150,), heads=4, kv=2, dim=dim, page=16, seed=new + dim)
+    c["q"].view(new, 4, dim)[..., 1] = c["q"].view(new, 4, dim)[..., 1].abs() + 0.25
+    host = R.Cache(c["k"], c["v"], c["table"], c["kv_len"], c["q_start"])
+    place = host.place
+    host.place = lambda s, j: None if j in (30, 101) else place(s, j)
+    want, tol = R.attend(host, new, c["q"].cpu(), c["out"], None, 0, c["gate"].cpu())
+    for j in (30, 101):
+        p, slot = place(0, j)
+        c["k"][p, :, slot, 1] = -float("inf")
+        c["v"][p, :, slot] = 1e30
+    (p, slot), (p1, slot1) = place(0, 20), place(0, 149)
+    c["v"][p, :, slot, 3], c["v"][p1, :, slot1, 4] = float("inf"), -float("inf")
+    z2.cache_attend(_cache(z2, c), c["q"], c["out"], gate=c["gate"])
+    got, rest = c["out"].view(new, 4, dim).cpu(), torch.ones(dim, dtype=torch.bool)
+    assert bool((got[..., 3] == float("inf")).all()) and bool((got[..., 4] == -float("inf")).all())
+    rest[3] = rest[4] = False
+    _near(got[..., rest], want.view(new, 4, dim)[..., rest], tol.view(new, 4, dim)[..., rest])
+    c["q"].view(new, 4, dim)[new - 1, 2, 5] = float("inf")
+    z2.cache_attend(_cache(z2, c), c["q"], c["out"], gate=c["gate"])
+    again = c["out"].view(new, 4, dim).cpu()
+    assert bool(again[new - 1, 2].isnan().all())
+    keep = torch.ones(new, 4, dtype=torch.bool)
+    keep[new - 1, 2] = False
+    _near(again[keep][:, rest], want.view(new, 4, dim)[keep][:, rest], tol.view(new, 4, dim)[keep][:, rest])
+    assert z2.device_error() == 0
+
+
 @pytest.mark.parametrize("name,new,heads", [("bf16", 1, 4), ("bf16", 40, 4), ("bf16", 300, 4), ("f32", 1, 4), ("f32", 3, 2), ("f32", 40, 4)])
 def test_last_positions(z2, cuda, name, new, heads):
     """The last tokens that a stream can have, 2^31 - 256 of them, all others on no page: as the same tokens on a

@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(32 * W)
 // products run on the tensor cores in tf32 (11 bits of a significand), each operand as the sum
 // of two such parts, hi = its upper bits and lo = the rest:
 //     a b = hi_a hi_b + hi_a lo_b + lo_a hi_b + (2^-22 of it)
-// (6 streams, up to 333 new tokens of 16 + 4 heads of 128, a window of 512: 135 us, 2150 us by the
+// (6 streams, up to 333 new tokens of 16 + 4 heads of 128, a window of 512: 136 us, 2150 us by the
 // kernel above), which leaves errors of the size of f32's own in a sum of 128 products.  The tensor cores add
 // to an accumulator by truncation, a bias that grows with the number of additions: the upper
 // parts' products, the mixed ones (2^-11 of them, and so their bias) and each 64 elements of the
@@ -618,6 +618,15 @@ struct TileF32 {
     static constexpr size_t kSmem = (size_t)(kTileRows * kPitch + 2 * kStage) * 4;
 };
 
+// A score by f32 arithmetic alone.
+__device__ __noinline__ float plain_score(const float *q, const float *k, int n)
+{
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < n; i++) sum = fmaf(q[i], k[i], sum);
+    return sum;
+}
+
 template <int D>
 __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
     attend_tile_f32_kernel(const CacheArgs c, const AttendArgs a, int ranks)
@@ -651,7 +660,7 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
         const int j = step_at(it) + 8 * warp;
         return it < mine && j < room ? page_of(c, tile.ch.stream, j) : -1;
     };
-    int page = look(0);
+    int page;
     const int live = c.dim / 4;
     for (int i = threadIdx.x; i < ROWS * (D / 4); i += 128) {
         const int r = i / (D / 4), p = i % (D / 4), row = tile.row0 + r;
@@ -693,20 +702,31 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
         cp_async_commit();
         page = look(it + 1);
     };
-    fetch(0);
 
     int pos[2];
 #pragma unroll
     for (int i = 0; i < 2; i++)
         pos[i] = position_of(tile.ch, a.group, tile.row0 + min(warp * 16 + i * 8 + g, tile.rows - 1));
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    float m[2], l[2], o[D / 8][4];
     const float factor = a.scale * kLog2e;
     const float *q0 = s_q + (warp * 16 + g) * Sh::kPitch + 4 * t, *q1 = q0 + 8 * Sh::kPitch;
     const bool idle = warp * 16 >= tile.rows;   // none of this warp's rows is one
-    uint32_t saw = 0;   // bits as `seen`'s
+    uint32_t saw;   // bits as `seen`'s
 
+    // An infinity has no two parts: where the first pass leaves a NaN, a second one takes all that is not
+    // finite by itself, as a NaN or an infinity of the result may be one of the inputs'.
+    for (int careful = 0; careful < 2; careful++) {
+    saw = 0;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+    }
+#pragma unroll
+    for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    page = look(0);
+    fetch(0);
+#pragma unroll 1
     for (int it = 0; it < mine; it++) {
         cp_async_wait<0>();
         __syncthreads();   // the step has landed, and the one before it is done with
@@ -717,7 +737,7 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
         uint32_t held = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) held |= s_held[it & 1][e] ? 1u << e : 0u;
-        const bool partial = j0 < sees_all_from || j0 + kTileKeys - 1 > pos_first || j0 + kTileKeys > high || held != 15u;
+        const bool partial = j0 < sees_all_from || j0 + kTileKeys - 1 > pos_first || j0 + kTileKeys > high || held != 15u || careful;
         auto sees = [&](int i, int j) {   // row slot i of this lane, token j
             return j <= pos[i] && j < high && (a.window <= 0 || j > pos[i] - a.window) && (held >> ((j - j0) >> 3) & 1u);
         };
@@ -789,6 +809,16 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
 #pragma unroll
             for (int e = 0; e < 4; e++) x[n][e] += hi[n][e] + lo[n][e];
         }
+        if (careful) {
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (isnan(x[n][e]))
+                        x[n][e] = plain_score(s_q + (warp * 16 + 8 * (e >> 1) + g) * Sh::kPitch,
+                                              keys + (8 * n + 2 * t + (e & 1)) * Sh::kPitch, c.dim);
+            __syncwarp();
+        }
         uint32_t seen = 0xffffu;   // bit 4 n + element
         if (partial) {
             seen = 0;
@@ -809,7 +839,8 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
             most = fmaxf(most, __shfl_xor_sync(kFull, most, 1));
             most = fmaxf(most, __shfl_xor_sync(kFull, most, 2)) * factor;
             if (most > m[i]) {
-                const float keep = m[i] == -INFINITY ? 0.0f : exp2_fast(m[i] - most);
+                // (before the first weight O is zero, or what is not finite and added by itself)
+                const float keep = m[i] == -INFINITY ? 1.0f : exp2_fast(m[i] - most);
                 m[i] = most;
                 l[i] *= keep;
 #pragma unroll
@@ -863,7 +894,16 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
         }
     }
     cp_async_wait<0>();
-    __syncthreads();   // every warp is done with the stages: the part takes their place
+    bool odd_result = false;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        float sum = l[i];   // a NaN, if one of these is, or infinities of both signs are
+#pragma unroll
+        for (int n = 0; n < D / 8; n++) sum += o[n][2 * i] + o[n][2 * i + 1];
+        odd_result |= isnan(sum) && warp * 16 + i * 8 + g < tile.rows;
+    }
+    if (!__syncthreads_or(odd_result)) break;   // (and every warp is done with the stages: the part takes their place)
+    }
     float *part = s_q;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
