@@ -217,7 +217,8 @@ int zonos2cu_block_norm(const void *resid_dev, const void *block_dev, zonos2cu_d
 /* Rows of x (bf16 or f32, their starts x_stride elements apart) rounded to 8 bits with a
  * scale each (no counterpart in the reference):
  *     scale[r] = max_k |x[r][k]| / 127,   q[r][k] = x[r][k] * 127 / max_k |x[r][k]|,
- * q rounded once to the nearest integer, ties to even, so that |q| <= 127.  A row of
+ * q rounded once to the nearest integer, ties to even, so that |q| <= 127.  Rows have fewer
+ * than 2^30 elements (ZONOS2CU_EUNSUPPORTED elsewhere).  A row of
  * zeros has scale 0; a row that holds a NaN or an infinity has q = 0 and scale NaN.
  *   q_dev        [rows][dim] i8; scale_dev [rows] f32.
  * For the weights of zonos2cu_head_i8 once, at set-up. */
@@ -237,8 +238,8 @@ int zonos2cu_quantize_rows(const void *x_dev, zonos2cu_dtype dtype, int rows, in
  *   work_dev     work_bytes of scratch, 16-byte aligned, at least
  *                zonos2cu_head_i8_work(batch, dim).  Calls that may overlap need scratch of
  *                their own.
- * dim must be a multiple of 16 (ZONOS2CU_EUNSUPPORTED elsewhere), at most
- * ZONOS2CU_MAX_I8_DIM (no sum of products then passes 32 bits). */
+ * dim must be a multiple of 16, and batch and n_cb * rows_per_cb lie below 2^30
+ * (ZONOS2CU_EUNSUPPORTED elsewhere); dim is at most ZONOS2CU_MAX_I8_DIM (no sum of products then passes 32 bits). */
 #define ZONOS2CU_MAX_I8_DIM 131072
 long long zonos2cu_head_i8_work(int batch, int dim);
 int zonos2cu_head_i8(const int8_t *W_dev, const float *w_scale_dev, int rows_per_cb, int n_cb,
@@ -257,7 +258,7 @@ int zonos2cu_head_i8(const int8_t *W_dev, const float *w_scale_dev, int rows_per
  *                and values may share one buffer, page by page).
  *   table_dev     [n_streams][max_pages] i32.  An entry outside [0, n_pages) is no page:
  *                nothing is written there, and its tokens are not attended (entries
- *                behind a stream's last token are not read; pages that a window has left
+ *                behind a stream's last token have no effect; pages that a window has left
  *                behind may be given back and marked -1).
  *   kv_len_dev    [n_streams] i32, the stream's tokens, the new ones of the call among
  *                them (tokens past max_pages * page_size are nowhere).
@@ -267,8 +268,8 @@ int zonos2cu_head_i8(const int8_t *W_dev, const float *w_scale_dev, int rows_per
  *                [q_start[0], q_start[n_streams]) are not read and stay as they are.
  * k_dev and v_dev are 16-byte aligned, head_dim is a multiple of 8 up to
  * ZONOS2CU_MAX_HEAD_DIM, page_size a power of two from 8 to ZONOS2CU_MAX_PAGE, page_stride a
- * multiple of 8; of a stream the first 2^31 - 256 tokens count, and rows times query heads
- * per key head stay below 2^30 (ZONOS2CU_EUNSUPPORTED elsewhere). */
+ * multiple of 8, n_kv_heads at most 4096 and n_heads 65535; of a stream the first 2^31 - 256
+ * tokens count, and n_streams and rows times query heads per key head stay below 2^30 (ZONOS2CU_EUNSUPPORTED elsewhere). */
 #define ZONOS2CU_MAX_HEAD_DIM 256
 #define ZONOS2CU_MAX_PAGE 4096
 typedef struct {
@@ -321,7 +322,8 @@ int zonos2cu_cache_append(const zonos2cu_cache *cache, int rows, int n_heads, co
  *   max_new      the most new tokens that a stream has, as far as the caller knows (0:
  *                not at all).  It chooses between kernels; chunks longer than it says are
  *                still attended.
- * n_heads is a multiple of n_kv_heads; scale is positive and finite.  Sums are taken in an
+ * n_heads is a multiple of n_kv_heads; scale is positive and finite.  The sum of the values'
+ * sizes, times 256, must lie within f32.  Sums are taken in an
  * order that the sizes alone give. */
 int zonos2cu_cache_attend(const zonos2cu_cache *cache, int rows, int n_heads, const void *q_dev,
                           long long q_stride, float scale, int window, const void *gate_dev,

@@ -76,6 +76,8 @@ def test_attend_unsupported(z2, bad):
 
 def test_too_many_rows(z2):
     assert _attend(z2, rows=1 << 28) == z2.EUNSUPPORTED and _append(z2, rows=1 << 28) == z2.EUNSUPPORTED
+    many = dict(n_streams=1 << 30)
+    assert _attend(z2, many) == z2.EUNSUPPORTED and _append(z2, many) == z2.EUNSUPPORTED
 
 
 def test_no_cache(z2):
@@ -107,6 +109,7 @@ def test_head_i8_refuses(z2, bad):
 def test_head_i8_unsupported_and_work(z2):
     assert _head(z2, dim=2040) == z2.EUNSUPPORTED
     assert _head(z2, n_cb=1 << 20, rows_per_cb=1024) == z2.EUNSUPPORTED
+    assert _head(z2, dim=16, batch=1 << 30, work_bytes=1 << 40) == z2.EUNSUPPORTED
     assert _head(z2, batch=0) == 0
     for batch, dim in ((1, 16), (7, 48), (4096, 2048), (2 ** 20, 131072)):
         need = z2.head_i8_work(batch, dim)
@@ -125,6 +128,7 @@ def test_quantize_refuses(z2):
     for bad in (dict(x=None), dict(q=None), dict(scale=None), dict(dtype=4), dict(rows=-1), dict(dim=0), dict(stride=19), dict(x=P + 2),
                 dict(scale=P + 1), dict(x=P + 1, dtype=z2.BF16)):
         assert call(**bad) == z2.EINVAL
+    assert call(dim=1 << 30, stride=1 << 30) == z2.EUNSUPPORTED
     assert call(rows=0) == 0
 
 

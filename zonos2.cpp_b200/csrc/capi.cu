@@ -464,6 +464,7 @@ int zonos2cu_quantize_rows(const void *x_dev, zonos2cu_dtype dtype, int rows, in
 {
     if (dtype != ZONOS2CU_F32 && dtype != ZONOS2CU_BF16) return ZONOS2CU_EINVAL;
     if (rows < 0 || dim < 1 || x_stride < dim) return ZONOS2CU_EINVAL;
+    if (dim > 0x3fffffff) return ZONOS2CU_EUNSUPPORTED;   // elements of a row are counted in 32 bits
     if (rows == 0) return ZONOS2CU_OK;
     if (!x_dev || !q_dev || !scale_dev) return ZONOS2CU_EINVAL;
     if ((uintptr_t)x_dev % (dtype == ZONOS2CU_F32 ? 4 : 2) || (uintptr_t)scale_dev % 4)
@@ -490,7 +491,7 @@ int zonos2cu_head_i8(const int8_t *W_dev, const float *w_scale_dev, int rows_per
     if (dim > ZONOS2CU_MAX_I8_DIM) return ZONOS2CU_EINVAL;
     if (dim % 16) return ZONOS2CU_EUNSUPPORTED;
     // rows, logits of a row and blocks of either are counted in 32 bits
-    if ((long long)n_cb * rows_per_cb > 0x3fffffff) return ZONOS2CU_EUNSUPPORTED;
+    if ((long long)n_cb * rows_per_cb > 0x3fffffff || batch > 0x3fffffff) return ZONOS2CU_EUNSUPPORTED;
     if (batch == 0) return ZONOS2CU_OK;
     if (!w_scale_dev || !work_dev) return ZONOS2CU_EINVAL;
     if ((uintptr_t)W_dev % 16 || (uintptr_t)w_scale_dev % 4 || (uintptr_t)work_dev % 16 ||
@@ -520,7 +521,7 @@ int check_cache(const zonos2cu_cache *c, int rows, int n_heads, z2::CacheArgs *o
         c->page_size > ZONOS2CU_MAX_PAGE || (c->page_size & (c->page_size - 1)) || c->page_stride % 8)
         return ZONOS2CU_EUNSUPPORTED;
     // heads lie on a launch grid's third axis, or are counted beside a token's
-    if (c->n_kv_heads > 4096 || n_heads > 65535) return ZONOS2CU_EUNSUPPORTED;
+    if (c->n_kv_heads > 4096 || n_heads > 65535 || c->n_streams > 0x3fffffff) return ZONOS2CU_EUNSUPPORTED;
     if (c->page_stride < (long long)c->n_kv_heads * c->page_size * c->head_dim) return ZONOS2CU_EINVAL;
     if (n_heads % c->n_kv_heads) return ZONOS2CU_EINVAL;
     // rows of a key head (tokens x its query heads) are counted in 32 bits
