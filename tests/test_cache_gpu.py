@@ -155,12 +155,21 @@ def test_attend_chunks(z2, cuda, name, heads, kv, dim, page, window):
 
 
 @pytest.mark.parametrize("name,heads,kv,dim", [("bf16", 8, 2, 128), ("bf16", 4, 4, 64), ("bf16", 4, 2, 24), ("bf16", 6, 3, 104),
-                                               ("bf16", 4, 2, 136), ("f32", 4, 2, 128), ("f32", 3, 1, 72)])
+                                               ("bf16", 4, 2, 136), ("bf16", 4, 1, 256), ("bf16", 5, 5, 192), ("f32", 4, 2, 128), ("f32", 3, 1, 72)])
 def test_attend_long_chunks(z2, cuda, name, heads, kv, dim):
     """Several tiles to a stream, longer than the caller says."""
     c = _case(cuda, name, new=(300, 129), cached=(140, 0), heads=heads, kv=kv, dim=dim, page=32, seed=3)
     for max_new in (300, 40):
         _check_attend(z2, c, max_new=max_new)
+
+
+@pytest.mark.parametrize("streams,new,cached", [(1, 40, 3000), (3, 17, 1000), (40, 9, 200), (90, 9, 30)])
+def test_attend_wide_heads(z2, cuda, streams, new, cached):
+    """Heads past 128 elements in chunks: clusters of eight blocks to a tile, of two, one, and more tiles than SMs."""
+    c = _case(cuda, "bf16", new=(new,) * streams, cached=(cached,) * streams, heads=8, kv=2, dim=232, page=8, holes=((0, 1),), seed=2)
+    for max_new in (0, new):
+        _check_attend(z2, c, max_new=max_new)
+    _check_attend(z2, c, window=150, gate=False, scale=0.3)
 
 
 @pytest.mark.parametrize("name", ["bf16", "f32"])

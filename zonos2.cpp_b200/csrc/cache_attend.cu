@@ -922,9 +922,16 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
     join_and_store<float, D, ROWS, 1, 128>(c, a, tile, kvh, part, s_ml, s_weight, s_total, s_gate, ranks, rank);
 }
 
+// The blocks of a tile's cluster: doubled while all blocks fit the SMs at once (`slots`: a block an SM, and then
+// clusters of eight and more only until half of them are taken, as more do not fit; or several blocks), and for
+// streams of unlike lengths to four while there are fewer than `few`.  16 + 4 bf16 heads of 128, one token, us:
+//   16 streams of 1500 tokens   by 16, 8, 4 blocks     38.2  22.2  15.7
+//   64 streams of 1500          by 4, 2, 1             47.9  49.8  37.7
+//   64 streams of 64 to 6144    by 4, 2, 1             81.7  86.1  110
+// heads of 256, 2 streams of 1500, by 16 and 8: 18.7 and 10.7; 16 streams, by 16 and 2: 97 and 23.7.
 template <typename Kernel>
 cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, int warps, int threads, const CacheArgs &c,
-                        const AttendArgs &a, int keys, std::mutex &mu, bool (&ready)[64], cudaStream_t stream)
+                        const AttendArgs &a, int keys, int few, int slots, std::mutex &mu, bool (&ready)[64], cudaStream_t stream)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -940,10 +947,10 @@ cudaError_t launch_rows(Kernel kernel, size_t smem, int tile_rows, int warps, in
         }
     }
     const long long tiles = (long long)c.rows * a.group / tile_rows + c.n_streams;
-    const long long work = tiles_with_rows(c, a, tile_rows) * c.n_kv;
+    const long long work = likely_tiles(c, a, tile_rows) * c.n_kv;
     const long long room = ((long long)c.max_pages << c.page_shift) / (keys * warps);
     int ranks = 1;
-    while (ranks < kMostRanks && work * ranks < 148 * 4 && ranks < room) ranks *= 2;
+    while (ranks < kMostRanks && ranks < room && (work * ranks * 2 <= (slots == 148 && ranks >= 4 ? 74 : slots) || (ranks < 4 && work * ranks < few))) ranks *= 2;
     if (tiles * ranks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * ranks), (unsigned)c.n_kv);
@@ -969,15 +976,16 @@ cudaError_t launch_bf16(const CacheArgs &c, const AttendArgs &a, cudaStream_t st
     typedef Ring<__nv_bfloat16, D, 16> R;
     const size_t rings = W * STAGES * R::kStage, parts = (size_t)W * 16 * D * 4;
     const size_t smem = (rings > parts ? rings : parts) + 16 * R::kRow;
-    return launch_rows(attend_rows_bf16_kernel<D, STAGES, W>, smem, 16, W, 32 * W, c, a, 16, mu, ready, stream);
+    return launch_rows(attend_rows_bf16_kernel<D, STAGES, W>, smem, 16, W, 32 * W, c, a, 16, D > 128 ? 0 : 592, D > 128 ? 148 : 444, mu, ready, stream);
 }
 
 // Blocks of eight rings where a cluster of the most blocks for each tile does not fill the SMs (one
-// stream of 6050 tokens: 12.9 us with half as many blocks, 10.4 us).
+// stream of 6050 tokens: 12.9 us with half as many blocks, 10.4 us; past half the SMs clusters of sixteen such
+// blocks do not all fit at once: 2 streams of up to 6144 tokens 16.9 us, 10.8 by blocks of four).
 template <int D, int STAGES>
 cudaError_t launch_bf16(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
 {
-    if (tiles_with_rows(c, a, 16) * c.n_kv * kMostRanks <= 148) return launch_bf16<D, 3, 8>(c, a, stream);
+    if (tiles_with_rows(c, a, 16) * c.n_kv * kMostRanks <= 74) return launch_bf16<D, 3, 8>(c, a, stream);
     return launch_bf16<D, STAGES, 4>(c, a, stream);
 }
 
@@ -989,7 +997,7 @@ cudaError_t launch_f32(const CacheArgs &c, const AttendArgs &a, cudaStream_t str
     typedef Ring<float, D, 8> R;
     const size_t rings = W * STAGES * R::kStage, parts = (size_t)W * ROWS * D * 4;
     const size_t smem = (rings > parts ? rings : parts) + ROWS * R::kRow;
-    return launch_rows(attend_rows_f32_kernel<D, ROWS, STAGES, W>, smem, ROWS, W, 32 * W, c, a, 8, mu, ready, stream);
+    return launch_rows(attend_rows_f32_kernel<D, ROWS, STAGES, W>, smem, ROWS, W, 32 * W, c, a, 8, D > 128 ? 148 : 592, D > 128 ? 148 : D > 64 ? 296 : 444, mu, ready, stream);
 }
 
 template <int D>
@@ -997,7 +1005,9 @@ cudaError_t launch_tile_f32(const CacheArgs &c, const AttendArgs &a, cudaStream_
 {
     static std::mutex mu;
     static bool ready[64] = {false};
-    return launch_rows(attend_tile_f32_kernel<D>, TileF32<D>::kSmem, kTileRows, 1, 128, c, a, kTileKeys, mu, ready, stream);
+    // (a window makes the tiles alike: 6 streams of up to 333 tokens, a window of 512: 136 us by two blocks, 124 by one)
+    const bool even = a.window > 0 && a.window < ((long long)c.max_pages << c.page_shift) / 4;
+    return launch_rows(attend_tile_f32_kernel<D>, TileF32<D>::kSmem, kTileRows, 1, 128, c, a, kTileKeys, even ? 0 : D > 128 ? 148 : 592, D > 128 ? 148 : even ? 296 : 444, mu, ready, stream);
 }
 
 }  // namespace
@@ -1009,8 +1019,9 @@ cudaError_t launch_cache_attend(const CacheArgs &c, const AttendArgs &a, bool bf
     const long long rows = (long long)most_new * a.group;
     if (bf16) {
         // (20 or 32 rows on 64 streams: 90 and 94 us here, 92 there; 48 rows: 111 against 92; on 4
-        // streams 21 and 22 us against 25, 48 rows 32 against 25)
-        if (rows > 32 && c.dim <= 128) return launch_cache_attend_tc(c, a, stream);
+        // streams 21 and 22 us against 25, 48 rows 32 against 25.  Heads of 256, 32 and 64 rows on 16 streams:
+        // 34 and 65 us here, 41 and 44 there; on 4 streams 18 and 23 against 25 and 26)
+        if (rows > 32) return launch_cache_attend_tc(c, a, stream);
         if (c.dim > 128) return launch_bf16<256, 2, 6>(c, a, stream);
         return c.dim > 64 ? launch_bf16<128, 2>(c, a, stream) : launch_bf16<64, 4>(c, a, stream);
     }

@@ -250,9 +250,17 @@ inline long long tiles_with_rows(const CacheArgs &c, const AttendArgs &a, int ti
     return filled < tiles ? filled : tiles;
 }
 
+// .. and as many as there may well be: the token rows', and half a tile more to each stream.
+inline long long likely_tiles(const CacheArgs &c, const AttendArgs &a, int tile_rows)
+{
+    const long long most = tiles_with_rows(c, a, tile_rows), least = c.rows < c.n_streams ? c.rows : c.n_streams;
+    const long long tiles = ((long long)c.rows * a.group + tile_rows - 1) / tile_rows + c.n_streams / 2;
+    return tiles > most ? most : tiles < least ? least : tiles;
+}
+
 }  // namespace
 
-// bf16 heads of up to 128 elements, many rows to a key head (cache_attend_tc.cu).
+// bf16, many rows to a key head (cache_attend_tc.cu).
 cudaError_t launch_cache_attend_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream);
 int read_and_clear_attend_error(int *value);
 

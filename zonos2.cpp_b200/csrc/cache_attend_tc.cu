@@ -1,5 +1,5 @@
 // cache_attend_tc.cu -- attention of chunks of new tokens over a paged cache on the tcgen05
-// tensor cores (sm_100a): bf16, heads of up to 128 elements (as 64 or 128, zeros past their end).
+// tensor cores (sm_100a): bf16, heads of up to 256 elements (as 64, 128 or 256, zeros past their end).
 //
 // A block takes 256 rows -- (token, query head) pairs that share a key head -- as two tiles of
 // 128, and the tokens they see in steps of 128 keys:
@@ -12,7 +12,7 @@
 // While one tile's softmax runs, the tensor core works for the other.  A step of both tiles
 // is 4 x 512 cycles of MMAs and 2 x 128 x 128 exponentials, 2048 cycles of the SM's 16 a
 // cycle: neither may wait for the other.  4 chunks of 2048 tokens on 2048 to 4096 cached ones, 16 + 4
-// heads of 128 (275 GFLOP): 306 us, 0.90 PFLOP/s, the tensor pipe 46 % active; a step takes 3900
+// heads of 128 (275 GFLOP): 297 us, 0.93 PFLOP/s, the tensor pipe 46 % active; a step takes 3800
 // cycles, 2300 of them a tile's softmax (1550 the exponentials) and the rest its products and
 // hand-overs.  A quarter of the exponentials by a polynomial on the FMA pipe was slower (324 us),
 // the tiles taking turns at them too (419 us against 394 then), and two threads to a row (475 us).
@@ -24,6 +24,10 @@
 // of softmax warps take the steps in turn, each with an accumulator of its own; a cluster of
 // blocks shares a tile's steps out where there are few tiles.  The parts are joined as in
 // cache_attend.cu.  (Warps without rows only keep the hand-over going.)
+// Heads past 128 are always SPLIT, with one group of softmax warps and one accumulator: TMEM holds that, 256
+// columns, and the scores of two steps, so that the next step's scores are there when a step's softmax ends;
+// shared memory holds one tile of keys and one of values beside the queries.  The chunks above with heads
+// of 256 (550 GFLOP): 823 us, 0.67 PFLOP/s; 3694 us by 16 rows to a tile on mma.sync.
 // A value that is not finite in a step that some row does not wholly see would reach that row as
 // 0 times it: such values are set to zero in shared memory before the product and added, at the
 // end, to the rows that see them.
@@ -39,17 +43,25 @@ int read_and_clear_attend_error(int *value) { return take_device_error(value); }
 
 namespace {
 
-constexpr int kTcThreads = 384;
 constexpr int kStep = 128;       // keys of a step
-constexpr int kSlots = 5;        // tiles of keys or values in shared memory
+constexpr int kTcRanks = 8;      // blocks of a cluster, at most
 constexpr float kSlack = 8.0f;   // how far scores may pass the running maximum, in powers of two
 
 template <int D>
 struct TcShape {
     static constexpr uint32_t kHalves = D / 64;              // 128-byte columns of a tile
     static constexpr uint32_t kTile = 128 * D * 2;           // bytes of 128 rows
-    static constexpr uint32_t kQ = 2 * kTile;
-    static constexpr size_t kSmem = kQ + kSlots * kTile + 1024 + 256;
+    static constexpr bool kOne = D > 128;                    // one group of softmax warps
+    static constexpr int kGroups = kOne ? 1 : 2, kThreads = 128 + 128 * kGroups;
+    static constexpr int kSlots = kOne ? 2 : 5;              // tiles of keys or values in shared memory
+    static constexpr uint32_t kQ = kOne ? kTile : 2 * kTile;
+    // the parts at the end: outputs in the place of keys and values, and what lies behind them (of kOne the
+    // ranks' maxima and sums first, which otherwise take the second part's place), in floats
+    static constexpr uint32_t kParts = kGroups * 128 * D + (kOne ? kTcRanks * 128 * 2 : 0);
+    static constexpr uint32_t kJoin = (kParts + kGroups * 128 * 2 + kMostRanks * 128 + 128) * 4;
+    static constexpr uint32_t kRing = kOne ? kJoin : kSlots * kTile;
+    static_assert(kJoin <= kRing && kSlots * kTile <= kRing && kRing % 8 == 0, "both fit");
+    static constexpr size_t kSmem = kQ + kRing + 1024 + 256;
 };
 
 // Shared-memory matrix descriptor, MN-major (rows of K, the product's columns behind each
@@ -198,32 +210,35 @@ __device__ void add_odd(const CacheArgs &c, int stream, int kvh, int j0, int all
 }
 
 template <int D, bool SPLIT>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
     attend_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const CacheArgs c, const AttendArgs a, int box_rows, int turns, int ranks)
 {
     typedef TcShape<D> Sh;
+    constexpr bool kOne = Sh::kOne;
+    constexpr int kGroups = Sh::kGroups, kSlots = Sh::kSlots, kTcThreads = Sh::kThreads;
+    static_assert(SPLIT || !kOne, "no room for two tiles");
     // kind::f16: D f32, A and B bf16; M = 128; S: N = 128, both K-major; O: N = D, B MN-major
     constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (128u >> 3 << 17) | (128u >> 4 << 24);
     constexpr uint32_t kIdescO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)D >> 3 << 17) | (128u >> 4 << 24);
-    constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns: S (then P) of both tiles, O of both
+    constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns: S (then P) of both tiles, O of both (kOne: of the one)
 
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-    const uint32_t s_q = smem, s_kv = smem + Sh::kQ, s_bar = s_kv + kSlots * Sh::kTile;
+    const uint32_t s_q = smem, s_kv = smem + Sh::kQ, s_bar = s_kv + Sh::kRing;
     auto full = [&](int s) { return s_bar + 8 * s; };
     auto empty = [&](int s) { return s_bar + 8 * (kSlots + s); };
     auto s_full = [&](int q) { return s_bar + 8 * (2 * kSlots + q); };    // S, and O before it, are done
     auto p_ready = [&](int q, int h) { return s_bar + 8 * (2 * kSlots + 2 + 2 * q + h); };   // P of 64 keys
+    const uint32_t o_done = s_bar + 8 * (2 * kSlots + 6);   // (kOne) a step's product
     constexpr int kTileRows = SPLIT ? 128 : 256;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_odd;
     __shared__ float s_gate[SPLIT ? 128 : 1];
     // (SPLIT) the parts at the end, in the place of keys and values
     float *part = reinterpret_cast<float *>(smem_raw + (s_kv - smem_u32(smem_raw)));
-    float2 *ml = reinterpret_cast<float2 *>(part + 2 * 128 * D);
-    float *weight = reinterpret_cast<float *>(ml + 2 * 128), *total = weight + kMostRanks * 128;
-    static_assert(!SPLIT || (2 * 128 * D + 4 * 128 + kMostRanks * 128 + 128) * 4 <= kSlots * (int)Sh::kTile, "parts fit");
+    float2 *ml = reinterpret_cast<float2 *>(part + Sh::kParts);
+    float *weight = reinterpret_cast<float *>(ml + kGroups * 128), *total = weight + kMostRanks * 128;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -247,6 +262,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(p_ready(q, 0), 4);   // the tile's warps
             mbar_init(p_ready(q, 1), 4);
         }
+        mbar_init(o_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_map(&map_k);
         prefetch_map(&map_v);
@@ -259,7 +275,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     uint32_t tmem = 0;
     // phases of the barriers before this tile: tiles of keys and values, scores of either tile
-    int kv0 = 0, scored0 = 0, scored1 = 0, weighed0 = 0, weighed1 = 0;
+    int kv0 = 0, scored0 = 0, scored1 = 0, weighed0 = 0, weighed1 = 0, summed = 0;
     bool dead = false;   // a wait ran out
     for (int turn = first_turn; turn < n_tiles; turn += turns) {
     const long long row_ll = (long long)(n_tiles - 1 - turn) * kTileRows;
@@ -312,11 +328,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             int it = kv0;
             for (int i = 0; i < steps && ok; i++) {
                 const int j0 = (step0 + i * ranks) * kStep;
-                // lane's box of the step's boxes x halves (16 x 2 at most)
-                const int b = lane % boxes, h = lane / boxes, j = j0 + b * box_rows;
-                const bool mine = h < (int)Sh::kHalves;
+                // lane's box of the step's boxes (16 at most), and of the halves every 32 / boxes-th
+                const int b = lane % boxes, h0 = lane / boxes, j = j0 + b * box_rows;
                 int page = -1;
-                if (mine && j < room) page = page_of(c, ch.stream, j);
+                if (j < room) page = page_of(c, ch.stream, j);
                 if (page < 0) page = c.n_pages;          // out of the map: zeros
                 const int slot_in_page = j & ((1 << c.page_shift) - 1);
                 for (int kv = 0; kv < 2; kv++, it++) {
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (!ok) break;
                     if (lane == 0) mbar_expect_tx(full(s), Sh::kTile);
                     __syncwarp();
-                    if (mine)
+                    for (int h = h0; h < (int)Sh::kHalves; h += 32 / boxes)
                         tma_load_4d(s_kv + s * Sh::kTile + h * (128 * 128) + b * box_rows * 128, kv ? &map_v : &map_k,
                                     h * 64, slot_in_page, kvh, page, full(s));
                 }
@@ -365,19 +380,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         scores(i, 2 * i);
                         done(2 * i);
                     }
+                    // (kOne: there is one accumulator; the keys after next come when the values leave, behind the
+                    // next ones)
                     for (int i = 0; i < steps && ok && !*(volatile int *)&s_abort; i++) {
                         const int q = i & 1;
-                        if (!landed(2 * i + 1) || (i + 2 < steps && !landed(2 * i + 4))) break;
+                        if (!landed(2 * i + 1) || (!kOne && i + 2 < steps && !landed(2 * i + 4))) break;
 #pragma unroll
                         for (int k = 0; k < kStep / 16; k++) {
                             const int kk = k ^ 4;
                             if (k % 4 == 0 && !wait(p_ready(q, kk / 4), (uint32_t)((q ? weighed1 : weighed0) + (i >> 1)) & 1u)) break;
-                            mma_bf16_ts(tmem + kColO + q * 128, tmem + kColS + q * 128 + 32 * (kk >> 1) + 8 * (kk & 1),
-                                        sw128_desc_mn(slot(2 * i + 1) + kk * 16 * 128), kIdescO, i > 1 || k > 0);
+                            mma_bf16_ts(tmem + kColO + (kOne ? 0 : q * 128), tmem + kColS + q * 128 + 32 * (kk >> 1) + 8 * (kk & 1),
+                                        sw128_desc_mn(slot(2 * i + 1) + kk * 16 * 128), kIdescO, i >= kGroups || k > 0);
                         }
                         if (!ok) break;
                         done(2 * i + 1);
-                        if (i + 2 < steps) {
+                        if (kOne) {
+                            mma_commit(o_done);
+                            if (i + 2 < steps) {
+                                if (!landed(2 * i + 4)) break;
+                                scores(q, 2 * i + 4);
+                                done(2 * i + 4);
+                            }
+                        } else if (i + 2 < steps) {
                             scores(q, 2 * i + 4);
                             done(2 * i + 4);
                         } else {
@@ -417,24 +441,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         } else if (warp >= 4) {
             // ---- softmax of tile q, this thread's row r of it
             const int q = (warp - 4) >> 2, r = threadIdx.x & 127;
-            const int rows = SPLIT ? tile_rows : q ? rows1 : rows0, s_before = q ? scored1 : scored0;
+            const int rows = SPLIT ? tile_rows : q ? rows1 : rows0;
             const int row_q = row0 + (SPLIT ? 0 : q * 128);   // the tile's first row
             // the group's n-th step is the rank's q + 2 n, or n
-            const int count = SPLIT ? (steps - q + 1) / 2 : steps;
+            const int count = SPLIT ? (steps - q + kGroups - 1) / kGroups : steps;
+            // S, P and their barriers' phase of it: the group's, or (kOne) the two in turn
+            auto buffer = [&](int n) { return kOne ? n & 1 : q; };
+            auto turn_of = [&](int before0, int before1, int n) {
+                return (uint32_t)(kOne ? (n & 1 ? before1 : before0) + (n >> 1) : (q ? before1 : before0) + n) & 1u;
+            };
             const int scanners = SPLIT ? (rows + 31) & ~31 : 128;   // threads of warps with rows
-            auto step_of = [&](int n) { return SPLIT ? q + 2 * n : n; };
+            auto step_of = [&](int n) { return SPLIT ? q + kGroups * n : n; };
             if (SPLIT && 32 * (warp & 3) >= rows) {   // no row of this warp's
                 for (int n = 0; n < count; n++) {
-                    const bool ok = mbar_wait(s_full(q), (uint32_t)(s_before + n) & 1u) && !*(volatile int *)&s_abort;
+                    const bool ok = mbar_wait(s_full(buffer(n)), turn_of(scored0, scored1, n)) && !*(volatile int *)&s_abort;
                     if (!__all_sync(kFull, ok)) break;
                     if (lane == 0) {
-                        mbar_arrive(p_ready(q, 0));
-                        mbar_arrive(p_ready(q, 1));
+                        mbar_arrive(p_ready(buffer(n), 0));
+                        mbar_arrive(p_ready(buffer(n), 1));
                     }
                 }
             } else if (rows > 0 && count > 0) {
                 const uint32_t at = ((uint32_t)(warp & 3) * 32) << 16;   // this warp's TMEM lanes
-                const uint32_t t_s = tmem + at + kColS + q * 128, t_o = tmem + at + kColO + q * 128;
+                const uint32_t t_o = tmem + at + kColO + q * 128;
                 const int pos = position_of(ch, a.group, row_q + min(r, rows - 1));
                 const int from = a.window > 0 ? max(0, pos - a.window + 1) : 0;
                 const int to = min(pos + 1, (q ? span1 : span0).high);   // this row sees [from, to)
@@ -453,7 +482,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     held_next = look(step_of(n + 1));
                     const int j0 = (step0 + i * ranks) * kStep;
                     const bool partial = j0 < all_from || j0 + kStep > all_to || held != 0xffffu;
-                    ok = mbar_wait(s_full(q), (uint32_t)(s_before + n) & 1u) && !*(volatile int *)&s_abort;
+                    const uint32_t t_s = tmem + at + kColS + buffer(n) * 128;
+                    ok = mbar_wait(s_full(buffer(n)), turn_of(scored0, scored1, n)) && !*(volatile int *)&s_abort;
                     ok = __all_sync(kFull, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -536,7 +566,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             m = most;
                             l *= keep;
                         }
-                        if (n > 0) {   // O is idle: S came after its last product
+                        if (kOne && n > 0) ok = __all_sync(kFull, mbar_wait(o_done, (uint32_t)(summed + n - 1) & 1u));
+                        if (!ok) break;
+                        if (n > 0) {   // O is idle: S came after its last product (kOne: that is done)
 #pragma unroll 1
                             for (int b = 0; b < D / 32; b++) {
                                 uint32_t o[32];
@@ -574,7 +606,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             tmem_wait_st();
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) mbar_arrive(p_ready(q, piece >> 1));
+                            if (lane == 0) mbar_arrive(p_ready(buffer(n), piece >> 1));
                         }
                     }
                     float s0, s1;
@@ -582,7 +614,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     l += s0 + s1;
                 }
                 // ---- O / l
-                ok = ok && mbar_wait(s_full(q), (uint32_t)(s_before + count) & 1u) && !*(volatile int *)&s_abort;
+                ok = ok && (kOne ? mbar_wait(o_done, (uint32_t)(summed + count - 1) & 1u)
+                                 : mbar_wait(s_full(q), turn_of(scored0, scored1, count))) && !*(volatile int *)&s_abort;
                 if (!__all_sync(kFull, ok)) {
                     s_abort = 1;
                 } else if (!SPLIT) {
@@ -657,7 +690,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tmem_wait_ld();
                         tmem_landed(o);
                         // (bounded by the rank's own steps of this group)
-                        for (int i = q; odd_values && i < steps; i += 2)
+                        for (int i = q; odd_values && i < steps; i += kGroups)
                             add_odd<32>(c, ch.stream, kvh, (step0 + i * ranks) * kStep, all_from, all_to, from, to, 32 * b, o);
                     } else {
 #pragma unroll
@@ -674,7 +707,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tile.ch = ch;
         tile.row0 = row0;
         tile.rows = tile_rows;
-        join_and_store<__nv_bfloat16, D, 128, 2, kTcThreads>(c, a, tile, kvh, part, ml, weight, total, s_gate, ranks, rank);
+        join_and_store<__nv_bfloat16, D, 128, kGroups, kTcThreads>(c, a, tile, kvh, part, ml, weight, total, s_gate, ranks, rank);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();   // the next tile's keys come where the parts were
     } else if (dead) {
@@ -684,10 +717,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (steps > 0) {
         kv0 += 2 * steps;
         const int count0 = SPLIT ? (steps + 1) / 2 : steps, count1 = SPLIT ? steps / 2 : rows1 > 0 ? steps : 0;
-        scored0 += count0 + 1;
+        scored0 += kOne ? count0 : count0 + 1;
         weighed0 += count0;
-        scored1 += count1 > 0 ? count1 + 1 : 0;
+        scored1 += kOne ? count1 : count1 > 0 ? count1 + 1 : 0;
         weighed1 += count1;
+        summed += steps;
     }
     }
     if (warp == 1)
@@ -744,7 +778,7 @@ cudaError_t launch_tc(const CacheArgs &c, const AttendArgs &a, int ranks, cudaSt
     if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(kTcThreads);
+    cfg.blockDim = dim3(TcShape<D>::kThreads);
     cfg.dynamicSmemBytes = TcShape<D>::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -770,10 +804,10 @@ cudaError_t launch_tc_any(const CacheArgs &c, const AttendArgs &a, cudaStream_t 
     //   16 streams,  64 rows   49.9 / 50.7  35.5  49.3  98.1       512 rows   64.6 / 97.6  127   192   370
     //   64 streams, 128 rows   97.2 / 103   130   193   373
     const long long tiles = turns_of(c, a, 128) * c.n_streams * c.n_kv;
-    if (tiles > 148) return launch_tc<D, false>(c, a, 1, stream);
+    if (!TcShape<D>::kOne && tiles > 148) return launch_tc<D, TcShape<D>::kOne>(c, a, 1, stream);
     const long long room = ((long long)c.max_pages << c.page_shift) / (2 * kStep);
     int ranks = 1;
-    while (ranks < 8 && tiles * ranks * 2 <= (ranks < 4 ? 148 : 74) && ranks < room) ranks *= 2;
+    while (ranks < kTcRanks && tiles * ranks * 2 <= (ranks < 4 ? 148 : 74) && ranks < room) ranks *= 2;
     return launch_tc<D, true>(c, a, ranks, stream);
 }
 
@@ -781,6 +815,7 @@ cudaError_t launch_tc_any(const CacheArgs &c, const AttendArgs &a, cudaStream_t 
 
 cudaError_t launch_cache_attend_tc(const CacheArgs &c, const AttendArgs &a, cudaStream_t stream)
 {
+    if (c.dim > 128) return launch_tc_any<256>(c, a, stream);
     return c.dim <= 64 ? launch_tc_any<64>(c, a, stream) : launch_tc_any<128>(c, a, stream);
 }
 
