@@ -474,7 +474,10 @@ class PagedCache:
             raise TypeError(f"{what}: {self._dtype} expected, got {t.dtype}")
         if t.get_device() != self._dev:
             raise ValueError(f"{what}: tensors on the cache's device expected")
-        return width if t.is_contiguous() else _rows(t, what)
+        stride, unit = t.stride()
+        if unit != 1 and width > 1:
+            raise ValueError(f"{what}: expected [rows, dim] with contiguous rows")
+        return stride if rows > 1 else width
 
 
 def cache_append(cache: PagedCache, q, k, v, q_out, *, freq=None, halves: bool = False, q_weight=None,
