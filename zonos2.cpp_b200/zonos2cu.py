@@ -460,11 +460,19 @@ class PagedCache:
         self.k_pages, self.v_pages, self.table = k_pages, v_pages, table
         self.kv_len, self.q_start = kv_len, q_start
         self.kv_heads, self.head_dim = kv, dim
-        self._dtype, self._dev = k_pages.dtype, k_pages.get_device()
+        self._dtype, self._dev, self._f32 = k_pages.dtype, k_pages.get_device(), torch.float32
         self._c = _Cache(k_pages.data_ptr(), v_pages.data_ptr(), _dtype(k_pages), n_pages, page, kv, dim,
                          k_pages.stride(0) if n_pages > 1 else kv * page * dim, table.data_ptr(), S, wide,
                          kv_len.data_ptr(), q_start.data_ptr())
         self._at = C.addressof(self._c)
+
+    def _f32_vector(self, what: str, t, n: int) -> int:
+        """The address of n f32 values in a row on the cache's device."""
+        if t.dtype is not self._f32:
+            raise TypeError(f"{what}: {self._f32} expected, got {t.dtype}")
+        if t.get_device() != self._dev or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{what}: a contiguous tensor of {n} elements on the cache's device expected")
+        return t.data_ptr()
 
     def _tokens(self, what: str, t, rows: int, width: int) -> int:
         """The row stride of token rows [rows, width] of the cache's type and device."""
@@ -501,12 +509,11 @@ def cache_append(cache: PagedCache, q, k, v, q_out, *, freq=None, halves: bool =
     elif q_out is not None:
         raise ValueError("cache_append: q_out without q")
     pairs = 0 if freq is None else freq.numel()
-    import torch
-    f32 = (torch.float32,)
-    _whole("cache_append", k, (freq, pairs, f32), (q_weight, dim, f32), (k_weight, dim, f32))
-    _launch("zonos2cu_cache_append", k, stream, cache._at, rows, heads, _ptr(q), qs, k.data_ptr(), ks,
-            v.data_ptr(), vs, _ptr(q_weight), _ptr(k_weight), eps, _ptr(freq), 2 * pairs, int(halves),
-            _ptr(q_out), os_)
+    at = [None if t is None else cache._f32_vector("cache_append", t, n)
+          for t, n in ((freq, pairs), (q_weight, dim), (k_weight, dim))]
+    _launch("zonos2cu_cache_append", k, stream, cache._at, rows, heads, None if q is None else q.data_ptr(), qs,
+            k.data_ptr(), ks, v.data_ptr(), vs, at[1], at[2], eps, at[0], 2 * pairs, int(halves),
+            None if q is None else q_out.data_ptr(), os_)
 
 
 def cache_attend(cache: PagedCache, q, out, *, scale: float | None = None, window: int = 0, gate=None,
