@@ -320,12 +320,14 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
     float m = -INFINITY, l = 0.0f;
     bool saw = false;
     if (steps > 0 && !dead) {
-        if (warp == 0) {
-            // ---- TMA producer: tile 2 i is step i's keys, 2 i + 1 its values
+        if (warp == 0 || (kOne && warp == 2)) {
+            // ---- TMA producer: tile 2 i is step i's keys, 2 i + 1 its values (kOne: warp 2's, so that keys need
+            // not wait for the values before them)
             const int boxes = kStep / box_rows;          // of a step, for each half
             const int room = room_of(c);
             bool ok = true;
             int it = kv0;
+            constexpr int kStride = kOne ? 2 : 1;   // of a producer's tiles
             for (int i = 0; i < steps && ok; i++) {
                 const int j0 = (step0 + i * ranks) * kStep;
                 // lane's box of the step's boxes (16 at most), and of the halves every 32 / boxes-th
@@ -334,7 +336,8 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                 if (j < room) page = page_of(c, ch.stream, j);
                 if (page < 0) page = c.n_pages;          // out of the map: zeros
                 const int slot_in_page = j & ((1 << c.page_shift) - 1);
-                for (int kv = 0; kv < 2; kv++, it++) {
+                for (int kv = kOne ? warp >> 1 : 0; kv < (kOne ? (warp >> 1) + 1 : 2); kv++) {
+                    it = kv0 + 2 * i + kv;
                     const int s = it % kSlots;
                     ok = mbar_wait(empty(s), (((uint32_t)(it / kSlots)) & 1u) ^ 1u) && !*(volatile int *)&s_abort;
                     ok = __all_sync(kFull, ok);
@@ -348,8 +351,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
             }
             if (!ok) {
                 s_abort = 1;
-                for (int k = 0; k < kSlots && k < it - kv0; k++) {   // copies still in flight land first
-                    const int t = it - 1 - k;
+                for (int t = it - kStride; t >= kv0 && t >= it - kSlots; t -= kStride) {   // copies still in flight land first
                     mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u);
                 }
             }
