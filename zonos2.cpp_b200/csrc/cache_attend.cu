@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(32 * W, D > 128 || W > 4 ? 1 : 3)
 // ---- f32, on the FMA pipe ----------------------------------------------------
 // ROWS rows to a tile, groups of 8 keys.  A lane takes a quarter of a key's elements for
 // the scores of all rows (key lane / 4), then D / 32 of the output's columns.  8 + 2 heads of 128, 64
-// streams of 1500 tokens, one new (197 MB): 75 us, 2.6 TB/s; 175 us with each group's page looked up
+// streams of 1500 tokens, one new (197 MB): 63 us, 3.1 TB/s; 175 us with more blocks to a cluster than it takes, each group's page looked up
 // in its turn and the values read four bytes at a time.
 template <int D, int ROWS, int STAGES, int W>
 __global__ void __launch_bounds__(32 * W)
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(32 * W)
 // products run on the tensor cores in tf32 (11 bits of a significand), each operand as the sum
 // of two such parts, hi = its upper bits and lo = the rest:
 //     a b = hi_a hi_b + hi_a lo_b + lo_a hi_b + (2^-22 of it)
-// (6 streams, up to 333 new tokens of 16 + 4 heads of 128, a window of 512: 136 us, 2150 us by the
+// (6 streams, up to 333 new tokens of 16 + 4 heads of 128, a window of 512: 124 us, 2150 us by the
 // kernel above), which leaves errors of the size of f32's own in a sum of 128 products.  The tensor cores add
 // to an accumulator by truncation, a bias that grows with the number of additions: the upper
 // parts' products, the mixed ones (2^-11 of them, and so their bias) and each 64 elements of the

@@ -3,7 +3,8 @@
 //
 // A block takes 256 rows -- (token, query head) pairs that share a key head -- as two tiles of
 // 128, and the tokens they see in steps of 128 keys:
-//   warp 0        TMA producer: a step's keys and values, page by page (a box is a page or 128 of
+//   warp 0        TMA producer: a step's keys and values (keys alone past heads of 128, where warp 2
+//                 has the values), page by page (a box is a page or 128 of
 //                 its tokens), 128-byte swizzled, into a ring of 128 x D tiles;
 //   warp 1        allocates TMEM and issues tcgen05.mma: S = Q K^T (128 x 128, f32) and
 //                 O += P V (P in TMEM as bf16 in place of S, V read as it lies, rows of D);
@@ -12,7 +13,7 @@
 // While one tile's softmax runs, the tensor core works for the other.  A step of both tiles
 // is 4 x 512 cycles of MMAs and 2 x 128 x 128 exponentials, 2048 cycles of the SM's 16 a
 // cycle: neither may wait for the other.  4 chunks of 2048 tokens on 2048 to 4096 cached ones, 16 + 4
-// heads of 128 (275 GFLOP): 297 us, 0.93 PFLOP/s, the tensor pipe 46 % active; a step takes 3800
+// heads of 128 (275 GFLOP): 297 us, 0.93 PFLOP/s, the tensor pipe 48 % active; a step takes 3800
 // cycles, 2300 of them a tile's softmax (1550 the exponentials) and the rest its products and
 // hand-overs.  A quarter of the exponentials by a polynomial on the FMA pipe was slower (324 us),
 // the tiles taking turns at them too (419 us against 394 then), and two threads to a row (475 us).
@@ -26,8 +27,10 @@
 // cache_attend.cu.  (Warps without rows only keep the hand-over going.)
 // Heads past 128 are always SPLIT, with one group of softmax warps and one accumulator: TMEM holds that, 256
 // columns, and the scores of two steps, so that the next step's scores are there when a step's softmax ends;
-// shared memory holds one tile of keys and one of values beside the queries.  The chunks above with heads
-// of 256 (550 GFLOP): 823 us, 0.67 PFLOP/s; 3694 us by 16 rows to a tile on mma.sync.
+// shared memory holds one tile of keys and one of values beside the queries, each asked for by a warp of its own
+// as soon as the one before it is done with.  The chunks above with heads of 256 (550 GFLOP): 550 us, 1.0 PFLOP/s;
+// 823 us with one warp for both, whose keys wait for the values before them; 3694 us by 16 rows to a tile on mma.sync.
+// Values in two halves of 64 tokens, each freed by itself, took 538 us here and 3 us more of 43 on shorter chunks.
 // A value that is not finite in a step that some row does not wholly see would reach that row as
 // 0 times it: such values are set to zero in shared memory before the product and added, at the
 // end, to the rows that see them.
