@@ -153,7 +153,7 @@ def test_python_checks(z2):
 
     c, x, kv = cache(), torch.zeros(5, 32, dtype=bf), torch.zeros(5, 16, dtype=bf)
     for args, kw in (((x, kv[:4], kv, x), {}), ((x, kv, kv[:, :8], x), {}), ((x[:, :20], kv, kv, x), {}), ((x, kv, kv, x[:4]), {}),
-                     ((None, kv, kv, x), {}), ((x, kv, kv, x), dict(k_weight=torch.zeros(7))),
+                     ((None, kv, kv, x), {}), ((x, kv, kv, None), {}), ((x, kv, kv, x), dict(k_weight=torch.zeros(7))),
                      ((x, kv, kv, torch.zeros(32, 5, dtype=bf).t()), {})):
         with pytest.raises(ValueError):
             z2.cache_append(c, *args, **kw)

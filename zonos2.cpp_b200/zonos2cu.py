@@ -503,6 +503,8 @@ def cache_append(cache: PagedCache, q, k, v, q_out, *, freq=None, halves: bool =
     qs = os_ = 0
     heads = cache.kv_heads
     if q is not None:
+        if q_out is None:
+            raise ValueError("cache_append: q without q_out")
         heads = q.shape[1] // dim
         qs = cache._tokens("cache_append", q, rows, heads * dim)
         os_ = cache._tokens("cache_append", q_out, rows, heads * dim)
