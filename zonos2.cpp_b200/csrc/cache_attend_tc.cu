@@ -233,7 +233,9 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
     auto empty = [&](int s) { return s_bar + 8 * (kSlots + s); };
     auto s_full = [&](int q) { return s_bar + 8 * (2 * kSlots + q); };    // S, and O before it, are done
     auto p_ready = [&](int q, int h) { return s_bar + 8 * (2 * kSlots + 2 + 2 * q + h); };   // P of 64 keys
-    const uint32_t o_done = s_bar + 8 * (2 * kSlots + 6);   // (kOne) a step's product
+    // (kOne) a step's product, even and odd steps' apart; and odd steps' values, which share a slot with the even ones'
+    auto o_done = [&](int n) { return s_bar + 8 * (2 * kSlots + 6 + (n & 1)); };
+    const uint32_t odd_values_full = s_bar + 8 * (2 * kSlots + 8);
     constexpr int kTileRows = SPLIT ? 128 : 256;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_odd;
@@ -265,7 +267,9 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
             mbar_init(p_ready(q, 0), 4);   // the tile's warps
             mbar_init(p_ready(q, 1), 4);
         }
-        mbar_init(o_done, 1);
+        mbar_init(o_done(0), 1);
+        mbar_init(o_done(1), 1);
+        mbar_init(odd_values_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_map(&map_k);
         prefetch_map(&map_v);
@@ -278,7 +282,18 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
     }
     uint32_t tmem = 0;
     // phases of the barriers before this tile: tiles of keys and values, scores of either tile
-    int kv0 = 0, scored0 = 0, scored1 = 0, weighed0 = 0, weighed1 = 0, summed = 0;
+    int kv0 = 0, scored0 = 0, scored1 = 0, weighed0 = 0, weighed1 = 0;
+    // The barrier that step i's keys (kv = 0) or values (kv = 1) land on, and the phase's parity.
+    // A wait tells a phase by its parity alone, so that whoever waits must know the phase before it to be
+    // done.  Softmax warps do not wait for every step's values or products: all they know at step i is that
+    // its scores are there, S(i), and what the issuer's thread had started before them.  Up to heads of 128 the slot's tile before
+    // values V(i) is K(i-2), which S(i-2) has used.  Past 128 S(i) comes after PV(i-2), so that V(i-2) has landed
+    // and PV(i-2) is done, but neither holds for step i - 1: a barrier for even and one for odd steps each.
+    auto landing = [&](int i, int kv) {
+        return kOne && kv && (i & 1) ? odd_values_full : full((kv0 + 2 * i + kv) % kSlots);
+    };
+    auto in_turn = [&](int i) { return (uint32_t)((i & 1 ? weighed1 : weighed0) + (i >> 1)) & 1u; };   // (kOne)
+    auto landing_parity = [&](int i, int kv) { return kOne && kv ? in_turn(i) : (uint32_t)((kv0 + 2 * i + kv) / kSlots) & 1u; };
     bool dead = false;   // a wait ran out
     for (int turn = first_turn; turn < n_tiles; turn += turns) {
     const long long row_ll = (long long)(n_tiles - 1 - turn) * kTileRows;
@@ -329,9 +344,9 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
             const int boxes = kStep / box_rows;          // of a step, for each half
             const int room = room_of(c);
             bool ok = true;
-            int it = kv0;
-            constexpr int kStride = kOne ? 2 : 1;   // of a producer's tiles
-            for (int i = 0; i < steps && ok; i++) {
+            const int kv_first = kOne ? warp >> 1 : 0, kv_end = kOne ? kv_first + 1 : 2;   // this producer's
+            int i = 0, kv = kv_first;
+            for (; i < steps && ok; i++) {
                 const int j0 = (step0 + i * ranks) * kStep;
                 // lane's box of the step's boxes (16 at most), and of the halves every 32 / boxes-th
                 const int b = lane % boxes, h0 = lane / boxes, j = j0 + b * box_rows;
@@ -339,24 +354,25 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                 if (j < room) page = page_of(c, ch.stream, j);
                 if (page < 0) page = c.n_pages;          // out of the map: zeros
                 const int slot_in_page = j & ((1 << c.page_shift) - 1);
-                for (int kv = kOne ? warp >> 1 : 0; kv < (kOne ? (warp >> 1) + 1 : 2); kv++) {
-                    it = kv0 + 2 * i + kv;
-                    const int s = it % kSlots;
+                for (kv = kv_first; kv < kv_end; kv++) {
+                    const int it = kv0 + 2 * i + kv, s = it % kSlots;
+                    const uint32_t bar = landing(i, kv);
                     ok = mbar_wait(empty(s), (((uint32_t)(it / kSlots)) & 1u) ^ 1u) && !*(volatile int *)&s_abort;
                     ok = __all_sync(kFull, ok);
                     if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(full(s), Sh::kTile);
+                    if (lane == 0) mbar_expect_tx(bar, Sh::kTile);
                     __syncwarp();
                     for (int h = h0; h < (int)Sh::kHalves; h += 32 / boxes)
                         tma_load_4d(s_kv + s * Sh::kTile + h * (128 * 128) + b * box_rows * 128, kv ? &map_v : &map_k,
-                                    h * 64, slot_in_page, kvh, page, full(s));
+                                    h * 64, slot_in_page, kvh, page, bar);
                 }
+                if (!ok) break;
             }
             if (!ok) {
                 s_abort = 1;
-                for (int t = it - kStride; t >= kv0 && t >= it - kSlots; t -= kStride) {   // copies still in flight land first
-                    mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u);
-                }
+                // copies still in flight land first (the last kSlots tiles', none of which is step i's kv-th)
+                for (int t = 2 * i + kv - 1; t >= 0 && t >= 2 * i + kv - kSlots; t--)
+                    if (!kOne || (t & 1) == kv) mbar_wait(landing(t >> 1, t & 1), landing_parity(t >> 1, t & 1));
             }
         } else if (warp == 1) {
             // ---- MMA issuer
@@ -368,7 +384,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                     return ok;
                 };
                 auto slot = [&](int t) { return s_kv + (uint32_t)((kv0 + t) % kSlots) * Sh::kTile; };
-                auto landed = [&](int t) { return wait(full((kv0 + t) % kSlots), (uint32_t)((kv0 + t) / kSlots) & 1u); };
+                auto landed = [&](int t) { return wait(landing(t >> 1, t & 1), landing_parity(t >> 1, t & 1)); };
                 auto done = [&](int t) { mma_commit(empty((kv0 + t) % kSlots)); };
                 auto scores = [&](int q, int t) {   // S of tile q by the keys in tile t
 #pragma unroll
@@ -385,8 +401,8 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                         scores(i, 2 * i);
                         done(2 * i);
                     }
-                    // (kOne: there is one accumulator; the keys after next come when the values leave, behind the
-                    // next ones)
+                    // (kOne: there is one accumulator, and S(i + 2) is issued behind PV(i); its keys have been asked for
+                    // since S(i + 1) was done with the slot.)
                     for (int i = 0; i < steps && ok && !*(volatile int *)&s_abort; i++) {
                         const int q = i & 1;
                         if (!landed(2 * i + 1) || (!kOne && i + 2 < steps && !landed(2 * i + 4))) break;
@@ -400,7 +416,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                         if (!ok) break;
                         done(2 * i + 1);
                         if (kOne) {
-                            mma_commit(o_done);
+                            mma_commit(o_done(i));
                             if (i + 2 < steps) {
                                 if (!landed(2 * i + 4)) break;
                                 scores(q, 2 * i + 4);
@@ -527,10 +543,9 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                     }
                     if (partial) {
                         // values that are not finite: out of the product
-                        const int t = kv0 + 2 * i + 1;
-                        ok = __all_sync(kFull, mbar_wait(full(t % kSlots), (uint32_t)(t / kSlots) & 1u));
+                        ok = __all_sync(kFull, mbar_wait(landing(i, 1), landing_parity(i, 1)));
                         if (!ok) break;
-                        const uint32_t values = s_kv + (uint32_t)(t % kSlots) * Sh::kTile;
+                        const uint32_t values = s_kv + (uint32_t)((kv0 + 2 * i + 1) % kSlots) * Sh::kTile;
                         uint32_t w[4], any = 0;
                         auto piece_at = [&](int k) {
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -571,7 +586,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                             m = most;
                             l *= keep;
                         }
-                        if (kOne && n > 0) ok = __all_sync(kFull, mbar_wait(o_done, (uint32_t)(summed + n - 1) & 1u));
+                        if (kOne && n > 0) ok = __all_sync(kFull, mbar_wait(o_done(n - 1), in_turn(n - 1)));
                         if (!ok) break;
                         if (n > 0) {   // O is idle: S came after its last product (kOne: that is done)
 #pragma unroll 1
@@ -619,7 +634,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                     l += s0 + s1;
                 }
                 // ---- O / l
-                ok = ok && (kOne ? mbar_wait(o_done, (uint32_t)(summed + count - 1) & 1u)
+                ok = ok && (kOne ? mbar_wait(o_done(count - 1), in_turn(count - 1))
                                  : mbar_wait(s_full(q), turn_of(scored0, scored1, count))) && !*(volatile int *)&s_abort;
                 if (!__all_sync(kFull, ok)) {
                     s_abort = 1;
@@ -726,7 +741,6 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
         weighed0 += count0;
         scored1 += kOne ? count1 : count1 > 0 ? count1 + 1 : 0;
         weighed1 += count1;
-        summed += steps;
     }
     }
     if (warp == 1)
