@@ -191,8 +191,10 @@ __global__ void __launch_bounds__(kAppendThreads)
                     if (LANE_PAIRS) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
-                            y[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+                            // (elements past the rotated ones are no pairs: 0 times an infinite neighbour would be a NaN)
+                            const bool pair = e0 + 2 * i < a.rot;
+                            y[2 * i] = pair ? x[2 * i] * cs[i] - x[2 * i + 1] * sn[i] : x[2 * i];
+                            y[2 * i + 1] = pair ? x[2 * i + 1] * cs[i] + x[2 * i] * sn[i] : x[2 * i + 1];
                         }
                     } else {
 #pragma unroll
