@@ -123,3 +123,36 @@ def attend(c, rows, q, out, scale=None, window=0, gate=None):
                 e = g[i] * size * off
                 tol[a + i, cols] = e + HALF[t] * (y[a + i, cols].abs() + e)
     return y, tol
+
+
+def attend_whole(c, rows, q, out, scale=None, window=0, gate=None):
+    """attend() by one product for all rows of a stream and query head: for many rows."""
+    t = c.k.dtype
+    scale = c.dim ** -0.5 if scale is None else float(np.float32(scale))
+    y, tol = out.cpu().double().clone(), torch.zeros(out.shape, dtype=torch.float64)
+    heads = q.shape[1] // c.dim
+    group = heads // c.heads
+    for s, a, n, length in c.streams(rows):
+        room = min(length, c.table.shape[1] * c.page)
+        at = [j for j in range(room) if c.place(s, j) is not None]
+        if not at:
+            y[a:a + n, :heads * c.dim] = 0
+            continue
+        where = torch.tensor([c.place(s, j) for j in at], dtype=torch.long)
+        j, pos = torch.tensor(at), torch.arange(length - n, length)[:, None]
+        sees = (j <= pos) & (j > pos - window) if window > 0 else j <= pos
+        some = sees.any(1, keepdim=True)
+        for h in range(heads):
+            cols = slice(h * c.dim, (h + 1) * c.dim)
+            k, v = (x[where[:, 0], h // group, where[:, 1]].double() for x in (c.k, c.v))
+            qr = q[a:a + n, cols].double()
+            x = (qr @ k.t() * scale).masked_fill(~sees, -math.inf)
+            p = torch.softmax(torch.where(some, x, 0.0), 1) * sees
+            g = 1.0 if gate is None else 1 / (1 + torch.exp(-gate[a:a + n, h:h + 1].double()))
+            terms = ((qr.abs() @ k.abs().t()) * scale * sees).amax(1, keepdim=True)
+            off = 2 * torch.expm1(2 * 2.0 ** -16 * terms + 2.0 ** -18) + (HALF[t] if t == torch.bfloat16 else 0.0)
+            off = off + 2.0 ** -24 * sees.sum(1, keepdim=True) + 2.0 ** -18
+            y[a:a + n, cols] = g * (p @ v)
+            e = g * (p @ v.abs()) * off
+            tol[a:a + n, cols] = e + HALF[t] * (y[a:a + n, cols].abs() + e)
+    return y, tol
