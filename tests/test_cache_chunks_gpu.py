@@ -119,3 +119,31 @@ def test_blocks_of_256_rows_longer_than_said(z2, cuda):
             first = c["out"].clone() if first is None else first
             assert torch.equal(first, c["out"])
     assert z2.device_error() == 0
+
+
+@pytest.mark.parametrize("name,dim,streams,new,cached", [("bf16", 64, 26, 150, 100), ("bf16", 128, 26, 150, 0), ("bf16", 128, 1, 150, 300), ("bf16", 256, 2, 60, 200),
+                                                         ("bf16", 128, 3, 1, 200), ("f32", 64, 2, 1, 90), ("f32", 128, 2, 40, 90)])
+def test_closed_gates(z2, cuda, name, dim, streams, new, cached):
+    """Gates of zero: zeros, but not in the place of an infinite value that the row sees (zero times it is no number), and
+    rows that see nothing are zeros whatever their gate."""
+    import torch
+    heads, kv = 12, 6
+    c = _case(cuda, name, new=(new,) * streams, cached=(cached,) * streams, heads=heads, kv=kv, dim=dim, page=16)
+    c["table"][streams - 1] = -1 if streams > 1 else c["table"][0]
+    c["gate"].fill_(-200.0)
+    c["gate"][:, 3] = float("nan")
+    c["v"][int(c["table"][0, 0]), :, 0, 5] = float("inf")   # stream 0's first token: seen by all of its rows
+    for max_new in (new, 0):
+        c["out"].fill_(7.0)
+        z2.cache_attend(_cache(z2, c), c["q"], c["out"], gate=c["gate"], max_new=max_new)
+        got = c["out"].view(-1, heads, dim).cpu()
+        if streams > 1:
+            assert bool((got[(streams - 1) * new:] == 0).all())
+            got = got[:(streams - 1) * new]
+        assert bool(got[:, 3].isnan().all())
+        rest = torch.ones(len(got), heads, dim, dtype=torch.bool)
+        rest[:, 3] = False
+        rest[:new, :, 5] = False
+        assert bool((got[rest] == 0).all())
+        assert bool(got[:new, :, 5].isnan().all())
+    assert z2.device_error() == 0

@@ -644,8 +644,9 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                     const int row = row_q + r, token = ch.first + row / a.group;
                     const int h = kvh * a.group + row % a.group;
                     const bool live = r < rows;
+                    // (rows that saw nothing are zeros whatever their gate; their O is)
                     float f = l == 0.0f ? (saw ? NAN : 0.0f) : 1.0f / l;
-                    if (a.gate && live) {
+                    if (a.gate && live && l != 0.0f) {
                         const float g = as_f(((const __nv_bfloat16 *)a.gate)[(long long)token * a.gate_stride + h]);
                         f *= 1.0f / (1.0f + expf(-g));
                     }
@@ -666,8 +667,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
                                 uint32_t w[4];
 #pragma unroll
                                 for (int e = 0; e < 4; e++)
-                                    w[e] = pack_bf16(f == 0.0f ? 0.0f : __uint_as_float(o[8 * k + 2 * e]) * f,
-                                                     f == 0.0f ? 0.0f : __uint_as_float(o[8 * k + 2 * e + 1]) * f);
+                                    w[e] = pack_bf16(__uint_as_float(o[8 * k + 2 * e]) * f, __uint_as_float(o[8 * k + 2 * e + 1]) * f);
                                 *reinterpret_cast<uint4 *>(out + 32 * b + 8 * k) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
                         }
