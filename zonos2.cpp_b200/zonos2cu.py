@@ -448,7 +448,8 @@ class PagedCache:
             raise ValueError("PagedCache: keys and values [n_pages, n_kv_heads, page_size, head_dim]")
         n_pages, kv, page, dim = k_pages.shape
         for t in (k_pages, v_pages):
-            if t.stride()[1:] != (page * dim, dim, 1) or t.stride(0) != k_pages.stride(0):
+            want = (k_pages.stride(0), page * dim, dim, 1)
+            if any(n > 1 and have != w for n, have, w in zip(t.shape, t.stride(), want)):   # (one element: any)
                 raise ValueError("PagedCache: whole pages at one stride expected")
         if table.dim() != 2:
             raise ValueError("PagedCache: table [n_streams, max_pages]")
