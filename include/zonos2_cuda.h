@@ -322,7 +322,7 @@ int zonos2cu_cache_append(const zonos2cu_cache *cache, int rows, int n_heads, co
  *   max_new      the most new tokens that a stream has, as far as the caller knows (0:
  *                not at all).  It chooses between kernels; chunks longer than it says are
  *                still attended.
- * n_heads is a multiple of n_kv_heads; scale is positive and finite.  The sum of the values'
+ * n_heads is a multiple of n_kv_heads; scale is positive, and finite also times log2(e).  The sum of the values'
  * sizes, times 256, must lie within f32.  Sums are taken in an
  * order that the sizes alone give. */
 int zonos2cu_cache_attend(const zonos2cu_cache *cache, int rows, int n_heads, const void *q_dev,

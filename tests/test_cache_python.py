@@ -24,3 +24,12 @@ def test_strides_of_axes_of_one(z2):
             z2.PagedCache(bad, bad, *_rest())
     with pytest.raises(ValueError):
         z2.PagedCache(torch.zeros(5, 2, 16, 64), torch.zeros(5, 4, 16, 64)[:, :2], *_rest())
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 3.4e38, -1.0, 0.0, float("inf"), float("nan")])
+def test_scales_that_leave_f32(z2, scale):
+    """The kernels take scores times log2(e): a scale whose product with it is not finite is refused, before CUDA is touched."""
+    import ctypes as C
+    P = 1 << 20
+    c = z2._Cache(P, 2 * P, z2.BF16, 10, 16, 2, 64, 2048, P, 3, 4, P, P)
+    assert z2.lib().zonos2cu_cache_attend(C.addressof(c), 5, 8, P, 512, scale, 0, P, 8, 0, 2 * P, 512, None) == z2.EINVAL

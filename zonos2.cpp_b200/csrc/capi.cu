@@ -589,7 +589,7 @@ int zonos2cu_cache_attend(const zonos2cu_cache *cache, int rows, int n_heads, co
     z2::CacheArgs c{};
     int rc = check_cache(cache, rows, n_heads, &c);
     if (rc) return rc;
-    if (!(scale > 0.0f) || !isfinite(scale)) return ZONOS2CU_EINVAL;
+    if (!(scale > 0.0f) || !isfinite(scale * z2::kLog2e)) return ZONOS2CU_EINVAL;   // the kernels' exponentials are of 2
     if (gate_dev && gate_stride < n_heads) return ZONOS2CU_EINVAL;
     if (rows == 0 || c.n_streams == 0) return ZONOS2CU_OK;
     const int bytes = cache->dtype == ZONOS2CU_F32 ? 4 : 2;
