@@ -311,10 +311,13 @@ int zonos2cu_cache_append(const zonos2cu_cache *cache, int rows, int n_heads, co
  * Query head h of a token at position p, with key head h / (n_heads / n_kv_heads):
  *     o = g * sum_j softmax_j(scale * q . k_j) v_j
  * over the stream's tokens j <= p (j > p - window with 0 < window < 2^30) that lie on a
- * page; zero where there is none.  What lies elsewhere, a NaN among it, has no part in it.
- * g = 1 / (1 + exp(-gate)) (1 without gates).  Scores, sums and softmax are f32; with a
+ * page; zero where there is none, whatever the gate.  What lies elsewhere, a NaN among it, has no part
+ * in it; an infinite value that the row sees makes its element infinite, or a NaN where its weight or the gate is zero in f32.
+ * g = 1 / (1 + exp(-gate)) (1 without gates).  Scores, sums and softmax are f32.  With a
  * bf16 cache the softmax's weights are rounded to bf16 before they meet the values (each
- * is at most 1 beside the row's largest; their sum is taken unrounded).
+ * is at most 1 beside the row's largest; their sum is taken unrounded): for normal values the error is then 2.0e-3 to 2.3e-3 in
+ * the 2-norm, 1.7e-3 of it the result's own rounding.  With an f32 cache and more than 16 rows (tokens times query heads of a key
+ * head) products are taken in three parts of 11 bits, to 2^-20 of each: 9e-7 in the 2-norm, 5.7e-7 in f32 throughout.
  *   q_dev, out_dev  [rows] token rows of n_heads heads of head_dim elements of the cache's
  *                type, q_stride and out_stride elements apart, 16-byte aligned
  *                (ZONOS2CU_EUNSUPPORTED elsewhere).  out_dev must not overlap the others.

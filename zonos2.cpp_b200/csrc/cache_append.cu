@@ -14,8 +14,8 @@
 // round of them, the token's heads shared out over warps.
 //
 // Bound: memory for prompts (every element is read once and written once) and beside it the issue
-// slots; launch latency for a few tokens.  8200 tokens of 16 + 2 x 4 bf16 heads of 128 (101 MB): 26.6 us,
-// 3.8 TB/s, the issue slots 61 % taken; 34 us with one loop over all heads, which chose each head's
+// slots; launch latency for a few tokens.  8200 tokens of 16 + 2 x 4 bf16 heads of 128 (101 MB): 23 to 30 us,
+// 3.4 to 4.4 TB/s, the issue slots 61 % taken; 34 us with one loop over all heads, which chose each head's
 // address and kind again.  One token: 3.2 us in a captured stream of them, 8.8 us as called from Python.
 #include <type_traits>
 

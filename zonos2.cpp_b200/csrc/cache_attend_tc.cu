@@ -10,10 +10,11 @@
 //                 O += P V (P in TMEM as bf16 in place of S, V read as it lies, rows of D);
 //   warps 4..7, 8..11  softmax of one tile each, a row to a thread: S from TMEM, its
 //                 maximum, 2^(x - m), P back to TMEM, and at the end O / l to global memory.
+// (P is rounded to bf16, the values' type, as cache_attend.cu says; its sum l is taken before.)
 // While one tile's softmax runs, the tensor core works for the other.  A step of both tiles
 // is 4 x 512 cycles of MMAs and 2 x 128 x 128 exponentials, 2048 cycles of the SM's 16 a
 // cycle: neither may wait for the other.  4 chunks of 2048 tokens on 2048 to 4096 cached ones, 16 + 4
-// heads of 128 (275 GFLOP): 297 us, 0.93 PFLOP/s, the tensor pipe 48 % active; a step takes 3800
+// heads of 128 (275 GFLOP): 297 to 340 us as the power limit has it, up to 0.93 PFLOP/s, the tensor pipe 48 % active; a step takes 3800
 // cycles, 2300 of them a tile's softmax (1550 the exponentials) and the rest its products and
 // hand-overs.  A quarter of the exponentials by a polynomial on the FMA pipe was slower (324 us),
 // the tiles taking turns at them too (419 us against 394 then), and two threads to a row (475 us).
@@ -65,6 +66,9 @@ struct TcShape {
     static constexpr uint32_t kRing = kOne ? kJoin : kSlots * kTile;
     static_assert(kJoin <= kRing && kSlots * kTile <= kRing && kRing % 8 == 0, "both fit");
     static constexpr size_t kSmem = kQ + kRing + 1024 + 256;
+    // A block takes all of TMEM and, in a cluster, keeps it until the others have come as far: no two blocks of these kernels may share
+    // an SM (1 KB of static shared memory, 1 KB that each block takes beside it), or two clusters could wait for each other.
+    static_assert(2 * (kSmem + 2048) > 228 * 1024, "one block to an SM");
 };
 
 // Shared-memory matrix descriptor, MN-major (rows of K, the product's columns behind each

@@ -7,8 +7,8 @@
 //
 // The products are summed exactly, in 32-bit integers, so that nothing is rounded but the rows
 // themselves and, at the end, the logits.
-// 9 x 1024 x 2048, with the rounding: 1 row 9.3 us, 64 rows 10.8 us, 333 rows 14.8 us, 4096 rows 78 us
-// (1.98 POP/s; the product alone 73 us with the tensor pipe 58 % active, the rounding 14 us of
+// 9 x 1024 x 2048, with the rounding: 1 row 9.3 us, 64 rows 10.8 us, 333 rows 14.8 us, 4096 rows 78 us (92 us for
+// seconds on end, at the power limit; 1.98 POP/s; the product alone 73 us with the tensor pipe 58 % active, the rounding 14 us of
 // which the product's start hides part).
 #include <cuda_bf16.h>
 #include <math.h>
