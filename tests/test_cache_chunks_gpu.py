@@ -147,3 +147,27 @@ def test_closed_gates(z2, cuda, name, dim, streams, new, cached):
         assert bool((got[rest] == 0).all())
         assert bool(got[:new, :, 5].isnan().all())
     assert z2.device_error() == 0
+
+
+def test_two_calls_at_once(z2, cuda):
+    """Chunks of heads of 64, 128 and 256 on two streams side by side, clusters of blocks and blocks alone: the bits of each
+    call by itself."""
+    import torch
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    cases = []
+    for i, (dim, streams, new) in enumerate([(64, 2, 60), (64, 12, 100), (128, 3, 40), (256, 2, 90), (256, 20, 30), (64, 40, 130)]):
+        c = _case(cuda, "bf16", new=(new,) * streams, cached=(700,) * streams, heads=8, kv=4, dim=dim, page=16, seed=i)
+        c["cache"], c["outs"] = _cache(z2, c), [torch.empty_like(c["out"]) for _ in range(2)]
+        z2.cache_attend(c["cache"], c["q"], c["out"], gate=c["gate"], max_new=new)
+        cases.append((c, new))
+    torch.cuda.synchronize()
+    for turn in range(10):
+        for i in range(len(cases)):
+            for k, side in enumerate(sides):
+                c, new = cases[(i * (2 * k + 1) + 3 * k + turn) % len(cases)]
+                z2.cache_attend(c["cache"], c["q"], c["outs"][k], gate=c["gate"], max_new=new, stream=side)
+    torch.cuda.synchronize()
+    assert z2.device_error() == 0
+    for c, _ in cases:
+        for out in c["outs"]:
+            assert torch.equal(c["out"], out)
