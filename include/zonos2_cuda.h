@@ -312,7 +312,8 @@ int zonos2cu_cache_append(const zonos2cu_cache *cache, int rows, int n_heads, co
  *     o = g * sum_j softmax_j(scale * q . k_j) v_j
  * over the stream's tokens j <= p (j > p - window with 0 < window < 2^30) that lie on a
  * page; zero where there is none, whatever the gate.  What lies elsewhere, a NaN among it, has no part
- * in it; an infinite value that the row sees makes its element infinite, or a NaN where its weight or the gate is zero in f32.
+ * in it.  An infinite value that the row sees makes its element infinite, or a NaN (as 0 times it) where its weight or the gate
+ * is zero in f32.
  * g = 1 / (1 + exp(-gate)) (1 without gates).  Scores, sums and softmax are f32.  With a
  * bf16 cache the softmax's weights are rounded to bf16 before they meet the values (each
  * is at most 1 beside the row's largest; their sum is taken unrounded): for normal values the error is then 2.0e-3 to 2.3e-3 in
